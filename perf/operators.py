@@ -176,9 +176,15 @@ def run(s: dict):
 
 
 def _run_own(s, case):
-    from engraft_ngram_amd import losses, muon
-
     kind = case["kind"]
+    if kind == "muon":
+        from engraft_ngram_amd import muon
+
+        muon.muon_step(s["params"], s["grads"], s["momenta"], lr=LR, weight_decay=DECAY, momentum=MOMENTUM, nesterov=True,
+                       steps=STEPS, coefficients=QUINTIC, eps=EPS)
+        return dict(params=s["params"], momenta=s["momenta"])
+    from engraft_ngram_amd import losses
+
     if kind == "logprobs":
         return losses.token_logprobs(s["logits"], s["targets"], temperature=case["temperature"])
     if kind == "policy":
@@ -186,14 +192,10 @@ def _run_own(s, case):
                                        segment_ids=s["segment_ids"], n_segments=case["segments"], clip=CLIP, kl_coef=KL_COEF,
                                        temperature=case["temperature"], reduction=case["reduction"], grad_scale=GRAD_SCALE[case["dtype"]])
         return dict(loss=r.loss, kl=r.kl, clip_fraction=r.clip_fraction, logprobs=r.logprobs, d_logits=d)
-    if kind == "preference":
-        r, d = losses.preference_loss_grad(s["logits"], s["targets"], s["segment_ids"], s["ref_logprobs"], beta=BETA,
-                                           label_smoothing=SMOOTHING, temperature=case["temperature"],
-                                           grad_scale=GRAD_SCALE[case["dtype"]])
-        return dict(loss=r.loss, margins=r.margins, sequence_logprobs=r.sequence_logprobs, logprobs=r.logprobs, d_logits=d)
-    muon.muon_step(s["params"], s["grads"], s["momenta"], lr=LR, weight_decay=DECAY, momentum=MOMENTUM, nesterov=True,
-                   steps=STEPS, coefficients=QUINTIC, eps=EPS)
-    return dict(params=s["params"], momenta=s["momenta"])
+    r, d = losses.preference_loss_grad(s["logits"], s["targets"], s["segment_ids"], s["ref_logprobs"], beta=BETA,
+                                       label_smoothing=SMOOTHING, temperature=case["temperature"],
+                                       grad_scale=GRAD_SCALE[case["dtype"]])
+    return dict(loss=r.loss, margins=r.margins, sequence_logprobs=r.sequence_logprobs, logprobs=r.logprobs, d_logits=d)
 
 
 def _softmax_stats(s, case):
