@@ -139,6 +139,69 @@ class EgF16Matrix(ctypes.Structure):
                 ("exps", c_void_p)]
 
 
+class EgLogits(ctypes.Structure):
+    _fields_ = [
+        ("data", c_void_p),
+        ("dtype", c_int32),
+        ("targets_i32", c_int32),
+        ("n", c_int64),
+        ("v", c_int64),
+        ("row_stride", c_int64),
+        ("targets", c_void_p),
+        ("temperature", ctypes.c_float),
+    ]
+
+
+class EgPolicy(ctypes.Structure):
+    _fields_ = [
+        ("advantages", c_void_p),
+        ("old_logprobs", c_void_p),
+        ("ref_logprobs", c_void_p),
+        ("segment_ids", c_void_p),
+        ("n_segments", c_int64),
+        ("segment_ids_i32", c_int32),
+        ("reduction", c_int32),
+        ("clip_low", ctypes.c_float),
+        ("clip_high", ctypes.c_float),
+        ("kl_coef", ctypes.c_float),
+    ]
+
+
+class EgPreference(ctypes.Structure):
+    _fields_ = [
+        ("segment_ids", c_void_p),
+        ("ref_logprobs", c_void_p),
+        ("n_pairs", c_int64),
+        ("segment_ids_i32", c_int32),
+        ("beta", ctypes.c_float),
+        ("label_smoothing", ctypes.c_float),
+    ]
+
+
+class EgMuon(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64),
+        ("cols", c_int64),
+        ("count", c_int32),
+        ("planes", c_int32),
+        ("params", c_void_p),
+        ("grads", c_void_p),
+        ("momenta", c_void_p),
+        ("param_dtype", c_int32),
+        ("grad_dtype", c_int32),
+        ("param_stride", c_int64 * 2),
+        ("grad_stride", c_int64 * 2),
+        ("momentum_stride", c_int64 * 2),
+        ("coefficients", c_void_p),
+        ("steps", c_int32),
+        ("nesterov", c_int32),
+        ("momentum", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("keep", ctypes.c_float),
+        ("rate", ctypes.c_float),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES = {
     "eg_last_error": (c_char_p, []),
@@ -232,6 +295,15 @@ SIGNATURES = {
                                   c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "eg_build_id_bitmap": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
     "eg_id_bitmap_words": (c_int64, [c_int64]),
+    "eg_loss_workspace_size": (c_int64, [c_int64, c_int64, c_int32, c_int64]),
+    "eg_token_logprobs": (c_int32, [POINTER(EgLogits), c_void_p, c_void_p, c_int64, c_void_p]),
+    "eg_policy_loss": (c_int32, [POINTER(EgLogits), POINTER(EgPolicy), c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                 ctypes.c_float, c_void_p, c_int64, c_void_p]),
+    "eg_preference_loss": (c_int32, [POINTER(EgLogits), POINTER(EgPreference), c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_int64, ctypes.c_float, c_void_p, c_int64, c_void_p]),
+    "eg_logits_grad": (c_int32, [POINTER(EgLogits), c_void_p, c_void_p, ctypes.c_float, c_void_p, c_int64, c_void_p]),
+    "eg_muon_workspace_size": (c_int64, [c_int64, c_int64, c_int32, c_int32]),
+    "eg_muon_step": (c_int32, [POINTER(EgMuon), c_void_p, c_int64, c_void_p]),
 }
 
 _LIB = None

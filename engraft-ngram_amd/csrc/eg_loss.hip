@@ -1,0 +1,726 @@
+// Losses of next-token logits and the gradient of the logits: what a descent's
+// d_out comes from (engraft/replica/distill.py:283-325 holds the reference's
+// own loss, a torch expression over log_softmax).
+//
+// With z a row of n_vocab logits, c = log2(e) / temperature and M = max z,
+//
+//   S = sum_j 2^(c (z_j - M)),   lp = ln2 c (z_t - M) - ln S,
+//   d_j = g ([j == t] - 2^(c (z_j - M)) / S) / temperature,   g = dL / d lp:
+//
+// a pass over the logits gives M and S of every row (row_stats_kernel, the running
+// maximum and sum of each thread joined in a fixed order), a kernel of one
+// workgroup turns them into the rows' lp, the loss and every row's g
+// (logprobs_finish, policy_finish, preference_finish), and a second pass reads the
+// logits and writes d (logits_grad_kernel).  The differences z - M are taken
+// before the multiplication by c, so a row of the type's lowest value gives a
+// uniform softmax and -inf gives exact zeros.  A row whose target is negative is left
+// out: its logits are not read (NaN there is harmless), its lp is 0 and its gradient
+// zero.  A target beyond the vocabulary gives NaN (lp and gradient), never a
+// read out of range.
+//
+// Sums are fp32 per thread and workgroup (a thread adds at most a few hundred terms),
+// sums over rows and sequences fp64; no floating atomics, so a call gives the same
+// bits every time.
+#include "eg_common.h"
+
+#include <algorithm>
+
+namespace eg {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;
+
+// 16 bytes at any element's alignment: rows of an odd vocabulary start anywhere
+// (global accesses need no alignment beyond the element's on gfx950).
+struct __attribute__((packed, aligned(2))) Chunk {
+  uint32_t w[4];
+};
+
+template <typename T>
+struct Logit;  // values per chunk, chunk -> fp32, fp32 -> chunk
+
+template <>
+struct Logit<float> {
+  static constexpr int kVec = 4;
+  static __device__ inline void unpack(const Chunk& c, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __builtin_bit_cast(float, c.w[i]);
+  }
+  static __device__ inline Chunk pack(const float (&f)[4]) {
+    Chunk c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c.w[i] = __builtin_bit_cast(uint32_t, f[i]);
+    return c;
+  }
+};
+
+template <>
+struct Logit<__bf16> {
+  static constexpr int kVec = 8;
+  static __device__ inline void unpack(const Chunk& c, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __builtin_bit_cast(float, c.w[i] << 16);
+      f[2 * i + 1] = __builtin_bit_cast(float, c.w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ inline Chunk pack(const float (&f)[8]) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    Chunk c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const pair p = {(__bf16)f[2 * i], (__bf16)f[2 * i + 1]};
+      c.w[i] = __builtin_bit_cast(uint32_t, p);
+    }
+    return c;
+  }
+};
+
+template <>
+struct Logit<_Float16> {
+  static constexpr int kVec = 8;
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+  static __device__ inline void unpack(const Chunk& c, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const pair p = __builtin_bit_cast(pair, c.w[i]);
+      f[2 * i] = (float)p[0];
+      f[2 * i + 1] = (float)p[1];
+    }
+  }
+  static __device__ inline Chunk pack(const float (&f)[8]) {
+    Chunk c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const pair p = {(_Float16)f[2 * i], (_Float16)f[2 * i + 1]};
+      c.w[i] = __builtin_bit_cast(uint32_t, p);
+    }
+    return c;
+  }
+};
+
+// What every kernel here knows of the rows.
+struct Rows {
+  const void* z;
+  int64_t n, stride;  // rows, elements from one to the next
+  const void* targets;
+  int32_t v;
+  int targets32;      // targets are int32, otherwise int64
+  float c;            // log2(e) / temperature
+  double inv_temp;
+};
+
+__device__ inline int64_t target_of(const Rows& r, int64_t i) {
+  return r.targets32 ? (int64_t)((const int32_t*)r.targets)[i] : ((const int64_t*)r.targets)[i];
+}
+
+// The running maximum and sum of 2^(c (z - m)).
+struct Stat {
+  float m, s;
+};
+
+__device__ inline float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ inline Stat join(const Stat& a, const Stat& b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  return {m, a.s * pow2((a.m - m) * c) + b.s * pow2((b.m - m) * c)};
+}
+
+// The larger of three, NaNs dropped (they come back through the sum).
+__device__ inline float max3(float a, float b, float x) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(x));
+  return r;
+}
+
+template <typename T, int K>
+__device__ inline void add_chunks(const Chunk (&q)[K], float c, Stat& st) {
+  constexpr int VEC = Logit<T>::kVec;
+  float f[K][VEC];
+  float m = st.m;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    Logit<T>::unpack(q[k], f[k]);
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) m = max3(m, f[k][i], f[k][i + 1]);
+  }
+  float s = st.s * pow2((st.m - m) * c);
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s += pow2((f[k][i] - m) * c);
+  st = {m, s};
+}
+
+// A thread's statistics of elements [e0, e1) of a row, e0 a multiple of the chunk.
+template <typename T, int THREADS>
+__device__ inline Stat thread_stats(const T* row, int e0, int e1, float c) {
+  constexpr int VEC = Logit<T>::kVec, K = 4;
+  Stat st = {kLowest, 0.0f};
+  int e = e0 + (int)threadIdx.x * VEC;
+  for (; e + (K - 1) * THREADS * VEC + VEC <= e1; e += K * THREADS * VEC) {
+    Chunk q[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) q[k] = *(const Chunk*)(row + e + k * THREADS * VEC);
+    add_chunks<T, K>(q, c, st);
+  }
+  for (; e + VEC <= e1; e += THREADS * VEC) {
+    const Chunk q[1] = {*(const Chunk*)(row + e)};
+    add_chunks<T, 1>(q, c, st);
+  }
+  for (; e < e1; ++e) {  // the one thread whose chunk passes the end
+    const float f = (float)row[e];
+    const float m = fmaxf(st.m, f);
+    st = {m, st.s * pow2((st.m - m) * c) + pow2((f - m) * c)};
+  }
+  return st;
+}
+
+template <int THREADS>
+__device__ inline Stat block_stats(Stat st, float c, Stat* red) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) st = join(st, Stat{__shfl_xor(st.m, o), __shfl_xor(st.s, o)}, c);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) red[wave] = st;
+  __syncthreads();
+  st = red[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) st = join(st, red[w], c);
+  return st;
+}
+
+// Elements [e0, e1) of part `p` of a row of v elements in `parts` parts.
+__device__ inline void part_range(int v, int parts, int part_len, int p, int& e0, int& e1) {
+  e0 = p * part_len;
+  e1 = p + 1 == parts ? v : e0 + part_len;
+}
+
+// Grid (parts, rows): the statistics of a part of a row -> stats[row][part].
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void row_stats_kernel(const Rows r, int parts, int part_len, Stat* stats) {
+  __shared__ Stat red[THREADS / 64];
+  const int64_t i = blockIdx.y + (int64_t)gridDim.y * blockIdx.z;
+  if (i >= r.n || target_of(r, i) < 0) return;
+  int e0, e1;
+  part_range(r.v, parts, part_len, (int)blockIdx.x, e0, e1);
+  Stat st = thread_stats<T, THREADS>((const T*)r.z + i * r.stride, e0, e1, r.c);
+  st = block_stats<THREADS>(st, r.c, red);
+  if (threadIdx.x == 0) stats[i * parts + blockIdx.x] = st;
+}
+
+// What the gradient pass needs of a row: g (dL / d lp), M and 1 / S.
+struct RowState {
+  float g, m, inv_s;
+};
+
+// Grid (parts, rows): a part of a row's gradient; scale holds 1 / temperature.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void logits_grad_kernel(const Rows r, int parts, int part_len,
+                                                              const RowState* state, const float* upstream,
+                                                              float scale, T* d, int64_t d_stride) {
+  constexpr int VEC = Logit<T>::kVec, K = 4;
+  const int64_t i = r.n - 1 - (blockIdx.y + (int64_t)gridDim.y * blockIdx.z);  // the rows read last first
+  if (i < 0) return;
+  int e0, e1;
+  part_range(r.v, parts, part_len, (int)blockIdx.x, e0, e1);
+  const int64_t t = target_of(r, i);
+  T* out = d + i * d_stride;
+  const T* row = (const T*)r.z + i * r.stride;
+  int e = e0 + (int)threadIdx.x * VEC;
+  if (t < 0) {
+    const Chunk zero = {{0, 0, 0, 0}};
+    for (; e + VEC <= e1; e += THREADS * VEC) *(Chunk*)(out + e) = zero;
+    for (; e < e1; ++e) out[e] = (T)0.0f;
+    return;
+  }
+  // the target's element is this thread's: read before anything is written (d may be the logits)
+  const bool owner = t >= e0 && t < e1 && (int)((t - e0) / VEC) % THREADS == (int)threadIdx.x;
+  const float f_t = owner ? (float)row[t] : 0.0f;
+  const RowState st = state[i];
+  const float g = st.g * (upstream != nullptr ? scale * *upstream : scale);
+  const float k = -g * st.inv_s, c = r.c, m = st.m;
+  auto value = [&](float f) { return k * pow2((f - m) * c); };
+  for (; e + (K - 1) * THREADS * VEC + VEC <= e1; e += K * THREADS * VEC) {
+    Chunk q[K];
+#pragma unroll
+    for (int j = 0; j < K; ++j) q[j] = *(const Chunk*)(row + e + j * THREADS * VEC);
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      float f[VEC];
+      Logit<T>::unpack(q[j], f);
+#pragma unroll
+      for (int x = 0; x < VEC; ++x) f[x] = value(f[x]);
+      *(Chunk*)(out + e + j * THREADS * VEC) = Logit<T>::pack(f);
+    }
+  }
+  for (; e + VEC <= e1; e += THREADS * VEC) {
+    float f[VEC];
+    Logit<T>::unpack(*(const Chunk*)(row + e), f);
+#pragma unroll
+    for (int x = 0; x < VEC; ++x) f[x] = value(f[x]);
+    *(Chunk*)(out + e) = Logit<T>::pack(f);
+  }
+  for (; e < e1; ++e) out[e] = (T)value((float)row[e]);
+  if (owner) out[t] = (T)(g + value(f_t));  // again, by the thread that wrote it
+}
+
+// ---- one workgroup over all rows ------------------------------------------------------------
+
+constexpr int kFinish = 1024;
+
+__device__ inline double block_sum64(double x, double* red) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+  __syncthreads();
+  double t = 0.0;
+  for (int w = 0; w < kFinish / 64; ++w) t += red[w];
+  return t;
+}
+
+// A row's statistics joined over its parts, in order.
+__device__ inline Stat row_stat(const Stat* stats, int64_t i, int parts, float c) {
+  Stat st = stats[i * parts];
+  for (int p = 1; p < parts; ++p) st = join(st, stats[i * parts + p], c);
+  return st;
+}
+
+// In 64 bits, for a row's terms: a loss is a sum of terms that nearly cancel, and an
+// fp32 lp's rounding (half a unit in the last place, 2^-21 at -10) would be most of its error.
+template <typename T>
+__device__ inline double row_logprob(const Rows& r, int64_t i, int64_t t, const Stat& st) {
+  if (t >= r.v) return __builtin_nan("");
+  const float f = (float)((const T*)r.z)[i * r.stride + t];
+  return (double)(f - st.m) * r.inv_temp - log((double)st.s);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void logprobs_finish(const Rows r, int parts, const Stat* stats, float* lp) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= r.n) return;
+  const int64_t t = target_of(r, i);
+  lp[i] = t < 0 ? 0.0f : (float)row_logprob<T>(r, i, t, row_stat(stats, i, parts, r.c));
+}
+
+// Segment of a row: a value outside [0, n) for none.
+struct Segments {
+  const void* ids;
+  int64_t n;
+  int ids32;
+};
+
+__device__ inline int64_t segment_of(const Segments& s, int64_t i) {
+  return s.ids32 ? (int64_t)((const int32_t*)s.ids)[i] : ((const int64_t*)s.ids)[i];
+}
+
+struct Policy {
+  const float* advantages;
+  const float* old_lp;  // NULL: the policy's own (a ratio of 1)
+  const float* ref_lp;  // NULL: no KL term
+  Segments seg;         // mean over segments of the mean over their tokens
+  int reduction;        // eg_reduction
+  float clip_low, clip_high, kl_coef;
+};
+
+struct PolicyTerms {
+  double loss, kl, clipped, g;
+};
+
+// A row's loss, KL and clip terms, and dL / d lp, all unweighted.
+__device__ inline PolicyTerms policy_terms(const Policy& p, int64_t i, double lp) {
+  const double a = (double)p.advantages[i];
+  const double ratio = p.old_lp != nullptr ? exp(lp - (double)p.old_lp[i]) : (lp == lp ? 1.0 : lp);
+  const double lo = 1.0 - (double)p.clip_low, hi = 1.0 + (double)p.clip_high;
+  const double held_ratio = ratio < lo ? lo : ratio > hi ? hi : ratio;  // NaN stays
+  const double free = ratio * a, held = held_ratio * a;
+  const bool active = free <= held;
+  PolicyTerms t = {active ? -free : -held, 0.0, free > held ? 1.0 : 0.0, active || free != free ? -free : 0.0};
+  if (p.ref_lp != nullptr) {
+    const double diff = (double)p.ref_lp[i] - lp, up = expm1(diff);
+    t.kl = up - diff;
+    t.loss += (double)p.kl_coef * t.kl;
+    t.g -= (double)p.kl_coef * up;
+  }
+  return t;
+}
+
+// One workgroup: the rows' weights, lp, terms and state; sums[3] = loss, KL, clipped share.
+// counts: [segments] scratch where the reduction is by segment.
+template <typename T>
+__global__ __launch_bounds__(kFinish) void policy_finish(const Rows r, const Policy p, int parts, const Stat* stats,
+                                                         int* counts, float* lp_out, RowState* state, float* sums) {
+  __shared__ double red[kFinish / 64];
+  __shared__ int total;
+  const int tid = threadIdx.x;
+  if (tid == 0) total = 0;
+  double w_all = 1.0;  // a row's weight where it is the same for all; by segment the share of a segment
+  if (p.reduction == EG_REDUCE_SEQUENCE) {
+    for (int64_t s = tid; s < p.seg.n; s += kFinish) counts[s] = 0;
+    __syncthreads();
+    for (int64_t i = tid; i < r.n; i += kFinish) {
+      const int64_t s = segment_of(p.seg, i);
+      if (s >= 0 && s < p.seg.n && target_of(r, i) >= 0) atomicAdd(counts + s, 1);
+    }
+    __syncthreads();
+    int some = 0;
+    for (int64_t s = tid; s < p.seg.n; s += kFinish) some += counts[s] > 0;
+    atomicAdd(&total, some);
+    __syncthreads();
+    w_all = 1.0 / (double)max(total, 1);
+  } else {
+    __syncthreads();
+    if (p.reduction == EG_REDUCE_TOKEN) {
+      int some = 0;
+      for (int64_t i = tid; i < r.n; i += kFinish) some += target_of(r, i) >= 0;
+      atomicAdd(&total, some);
+      __syncthreads();
+      w_all = 1.0 / (double)max(total, 1);
+    }
+  }
+  double loss = 0.0, kl = 0.0, clipped = 0.0;
+  for (int64_t i = tid; i < r.n; i += kFinish) {
+    const int64_t t = target_of(r, i);
+    double lp = 0.0;
+    RowState st = {0.0f, 0.0f, 0.0f};
+    if (t >= 0) {
+      const Stat rs = row_stat(stats, i, parts, r.c);
+      lp = row_logprob<T>(r, i, t, rs);
+      double w = w_all;
+      if (p.reduction == EG_REDUCE_SEQUENCE) {
+        const int64_t s = segment_of(p.seg, i);
+        w = s >= 0 && s < p.seg.n ? w_all / (double)counts[s] : 0.0;
+      }
+      st = {0.0f, rs.m, 1.0f / rs.s};
+      if (w != 0.0) {
+        const PolicyTerms q = policy_terms(p, i, lp);
+        loss += w * q.loss;
+        kl += w * q.kl;
+        clipped += w * q.clipped;
+        st.g = (float)(w * q.g);
+      }
+    }
+    lp_out[i] = (float)lp;
+    state[i] = st;
+  }
+  loss = block_sum64(loss, red);
+  kl = block_sum64(kl, red);
+  clipped = block_sum64(clipped, red);
+  if (tid == 0) {
+    sums[0] = (float)loss;
+    sums[1] = (float)kl;
+    sums[2] = (float)clipped;
+  }
+}
+
+struct Preference {
+  Segments seg;          // 2 pairs segments, non-decreasing over the rows: chosen 2 p, rejected 2 p + 1
+  const float* ref_lp;   // [2 pairs]
+  float beta, smoothing;
+};
+
+// One workgroup: lp, the sequences' sums, margins, loss and state.  starts [2 pairs + 1],
+// d_seq and seq_sum [2 pairs] and lp64 [n] are scratch.
+template <typename T>
+__global__ __launch_bounds__(kFinish) void preference_finish(const Rows r, const Preference p, int parts,
+                                                             const Stat* stats, int64_t* starts, float* d_seq,
+                                                             double* seq_sum, double* lp64, float* lp_out, float* seq_out,
+                                                             float* margins, RowState* state, float* loss_out) {
+  __shared__ double red[kFinish / 64];
+  __shared__ int unordered;
+  const int tid = threadIdx.x;
+  const int64_t count = p.seg.n, pairs = count / 2;
+  if (tid == 0) unordered = 0;
+  __syncthreads();
+  auto held = [&](int64_t s) { return s < 0 ? (int64_t)-1 : s > count ? count : s; };
+  for (int64_t i = tid; i < r.n; i += kFinish) {
+    const int64_t t = target_of(r, i);
+    // starts[s]: the first row of segment s or a later one
+    const int64_t s = held(segment_of(p.seg, i)), before = i > 0 ? held(segment_of(p.seg, i - 1)) : -1;
+    for (int64_t q = before + 1; q <= s; ++q) starts[q] = i;
+    if (before > s) unordered = 1;
+    if (i == r.n - 1)
+      for (int64_t q = s + 1; q <= count; ++q) starts[q] = r.n;
+    double lp = 0.0;
+    RowState st = {0.0f, 0.0f, 0.0f};
+    if (t >= 0) {
+      const Stat rs = row_stat(stats, i, parts, r.c);
+      lp = row_logprob<T>(r, i, t, rs);
+      st = {0.0f, rs.m, 1.0f / rs.s};
+    }
+    lp64[i] = lp;
+    lp_out[i] = (float)lp;
+    state[i] = st;
+  }
+  if (r.n == 0)
+    for (int64_t q = tid; q <= count; q += kFinish) starts[q] = 0;
+  __syncthreads();
+  for (int64_t s = tid >> 6; s < count; s += kFinish / 64) {
+    double sum = 0.0;
+    for (int64_t i = starts[s] + (tid & 63); i < starts[s + 1]; i += 64) sum += lp64[i];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((tid & 63) == 0) {
+      seq_sum[s] = sum;
+      seq_out[s] = (float)sum;
+    }
+  }
+  __syncthreads();
+  double loss = 0.0;
+  for (int64_t q = tid; q < pairs; q += kFinish) {
+    // segments out of order have no sums: NaN
+    const double h = unordered ? __builtin_nan("") : (double)p.beta * ((seq_sum[2 * q] - (double)p.ref_lp[2 * q]) -
+                                                                    (seq_sum[2 * q + 1] - (double)p.ref_lp[2 * q + 1]));
+    const double e = exp(-fabs(h)), tail = log1p(e);  // -log sigma(h) = tail + max(-h, 0)
+    const double small = e / (1.0 + e), large = 1.0 / (1.0 + e);
+    const double up = h >= 0.0 ? large : small, down = h >= 0.0 ? small : large;  // sigma(h), sigma(-h)
+    const double eps = (double)p.smoothing;
+    loss += (tail + (1.0 - eps) * fmax(-h, 0.0) + eps * fmax(h, 0.0)) + (h != h ? h : 0.0);
+    const float g = (float)((double)p.beta * (eps * up - (1.0 - eps) * down) / (double)pairs);
+    d_seq[2 * q] = g;
+    d_seq[2 * q + 1] = -g;
+    margins[q] = (float)h;
+  }
+  loss = block_sum64(loss, red);
+  if (tid == 0) loss_out[0] = (float)(loss / (double)max(pairs, (int64_t)1));
+  __syncthreads();
+  for (int64_t i = tid; i < r.n; i += kFinish) {
+    const int64_t s = segment_of(p.seg, i);
+    if (s >= 0 && s < count && target_of(r, i) >= 0) state[i].g = d_seq[s];
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------------
+
+int value_bytes(int dtype) { return dtype == EG_DTYPE_F32 ? 4 : 2; }
+
+// How a pass over the logits is cut: threads a workgroup, and parts of a row.
+struct Cut {
+  int threads, parts, part_len;
+};
+
+constexpr int64_t kGroupsWanted = 512;  // two workgroups a CU
+constexpr int kPartBytes = 16384;       // the shortest part worth a workgroup
+
+Cut make_cut(int64_t n, int64_t v, int dtype) {
+  const int64_t size = value_bytes(dtype), vec = 16 / size;
+  int64_t parts = n > 0 ? std::min(kGroupsWanted / n, v * size / kPartBytes) : 1;
+  parts = std::max<int64_t>(parts, 1);
+  const int64_t len = ((v + parts - 1) / parts + vec - 1) / vec * vec;
+  parts = (v + len - 1) / len;
+  return {len * size > 32768 ? 1024 : 256, (int)parts, (int)len};
+}
+
+int check_logits(const eg_logits* l, Rows* r) {
+  EG_CHECK_ARG(l != nullptr, "logits is NULL");
+  EG_CHECK_ARG(l->dtype == EG_DTYPE_F32 || l->dtype == EG_DTYPE_BF16 || l->dtype == EG_DTYPE_F16,
+               "logits dtype=%d must be f32, bf16 or f16", l->dtype);
+  EG_CHECK_ARG(l->n >= 0, "n=%lld rows must not be negative", (long long)l->n);
+  EG_CHECK_ARG(l->v >= 1 && l->v <= 0x7fffffff - 65536, "vocabulary v=%lld must be in [1, 2^31 - 65536)",
+               (long long)l->v);
+  EG_CHECK_ARG(l->n <= 1 || l->row_stride >= l->v, "row_stride=%lld must be at least v=%lld",
+               (long long)l->row_stride, (long long)l->v);
+  EG_CHECK_ARG(l->temperature > 0.0f && l->temperature < 3.0e38f, "temperature=%g must be positive and finite",
+               (double)l->temperature);
+  EG_CHECK_ARG(l->n == 0 || (l->data != nullptr && l->targets != nullptr), "logits data or targets is NULL");
+  EG_CHECK_ARG((uintptr_t)l->data % value_bytes(l->dtype) == 0, "logits data is not aligned to its type");
+  *r = {l->data, l->n, l->row_stride, l->targets, (int32_t)l->v, l->targets_i32 != 0, kLog2e / l->temperature,
+        1.0 / (double)l->temperature};
+  return EG_OK;
+}
+
+int check_segments(const void* ids, int32_t i32, int64_t n, Segments* s) {
+  EG_CHECK_ARG(n >= 0, "n_segments=%lld must not be negative", (long long)n);
+  *s = {ids, n, i32 != 0};
+  return EG_OK;
+}
+
+// Workspace of a loss: the parts' statistics, then scratch of the segments (24 bytes each)
+// and of the rows (8 bytes each).
+int64_t stats_bytes(int64_t n, const Cut& cut) { return (n * cut.parts * (int64_t)sizeof(Stat) + 15) / 16 * 16; }
+
+dim3 row_grid(const Cut& cut, int64_t n) {
+  const int64_t y = std::min<int64_t>(n, 32768);
+  return dim3((unsigned)cut.parts, (unsigned)y, (unsigned)((n + y - 1) / y));
+}
+
+template <typename F>
+int by_dtype(int dtype, F&& f) {
+  switch (dtype) {
+    case EG_DTYPE_F32: return f(float{});
+    case EG_DTYPE_BF16: return f(__bf16{});
+    default: return f(_Float16{});
+  }
+}
+
+int launch_stats(const Rows& r, int dtype, const Cut& cut, Stat* stats, hipStream_t stream) {
+  if (r.n == 0) return EG_OK;
+  return by_dtype(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const dim3 grid = row_grid(cut, r.n);
+    if (cut.threads == 1024)
+      row_stats_kernel<T, 1024><<<grid, 1024, 0, stream>>>(r, cut.parts, cut.part_len, stats);
+    else
+      row_stats_kernel<T, 256><<<grid, 256, 0, stream>>>(r, cut.parts, cut.part_len, stats);
+    return launch_status("row_stats_kernel");
+  });
+}
+
+int launch_grad(const Rows& r, int dtype, const Cut& cut, const RowState* state, const float* upstream, float scale,
+                void* d, int64_t d_stride, hipStream_t stream) {
+  if (r.n == 0) return EG_OK;
+  return by_dtype(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const dim3 grid = row_grid(cut, r.n);
+    if (cut.threads == 1024)
+      logits_grad_kernel<T, 1024><<<grid, 1024, 0, stream>>>(r, cut.parts, cut.part_len, state, upstream, scale,
+                                                             (T*)d, d_stride);
+    else
+      logits_grad_kernel<T, 256><<<grid, 256, 0, stream>>>(r, cut.parts, cut.part_len, state, upstream, scale, (T*)d,
+                                                           d_stride);
+    return launch_status("logits_grad_kernel");
+  });
+}
+
+int check_grad(const eg_logits* l, const void* d, int64_t d_stride) {
+  EG_CHECK_ARG(l->n == 0 || d != nullptr, "d_logits is NULL");
+  EG_CHECK_ARG(l->n <= 1 || d_stride >= l->v, "d_stride=%lld must be at least v=%lld", (long long)d_stride,
+               (long long)l->v);
+  EG_CHECK_ARG((uintptr_t)d % value_bytes(l->dtype) == 0, "d_logits is not aligned to its type");
+  EG_CHECK_ARG(d != l->data || d_stride == l->row_stride || l->n <= 1,
+               "d_logits in place of the logits must have their row stride");
+  return EG_OK;
+}
+
+}  // namespace
+}  // namespace eg
+
+using namespace eg;
+
+extern "C" {
+
+int64_t eg_loss_workspace_size(int64_t n, int64_t v, int32_t dtype, int64_t n_segments) {
+  if (n < 0 || v < 1 || n_segments < 0) return -1;
+  return stats_bytes(n, make_cut(n, v, dtype)) + (n_segments + 1) * 24 + n * 8;
+}
+
+#define EG_CHECK_WORKSPACE(need)                                                                              \
+  do {                                                                                                        \
+    if ((need) > 0 && (workspace == nullptr || workspace_bytes < (need)))                                     \
+      return ::eg::set_error(EG_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, \
+                             (long long)(need));                                                              \
+    EG_CHECK_ARG((uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");                        \
+  } while (0)
+
+int eg_token_logprobs(const eg_logits* logits, float* logprobs, void* workspace, int64_t workspace_bytes,
+                      void* stream) {
+  Rows r;
+  if (int rc = check_logits(logits, &r); rc != EG_OK) return rc;
+  EG_CHECK_ARG(r.n == 0 || logprobs != nullptr, "logprobs is NULL");
+  if (r.n == 0) return EG_OK;
+  const Cut cut = make_cut(r.n, r.v, logits->dtype);
+  EG_CHECK_WORKSPACE(stats_bytes(r.n, cut));
+  Stat* stats = (Stat*)workspace;
+  if (int rc = launch_stats(r, logits->dtype, cut, stats, (hipStream_t)stream); rc != EG_OK) return rc;
+  return by_dtype(logits->dtype, [&](auto zero) {
+    using T = decltype(zero);
+    logprobs_finish<T><<<dim3((unsigned)((r.n + 255) / 256)), 256, 0, (hipStream_t)stream>>>(r, cut.parts, stats,
+                                                                                            logprobs);
+    return launch_status("logprobs_finish");
+  });
+}
+
+int eg_policy_loss(const eg_logits* logits, const eg_policy* policy, float* logprobs, float* sums, float* state,
+                   void* d_logits, int64_t d_stride, float grad_scale, void* workspace, int64_t workspace_bytes,
+                   void* stream) {
+  Rows r;
+  if (int rc = check_logits(logits, &r); rc != EG_OK) return rc;
+  EG_CHECK_ARG(policy != nullptr && sums != nullptr, "policy or sums is NULL");
+  EG_CHECK_ARG(r.n == 0 || (logprobs != nullptr && state != nullptr && policy->advantages != nullptr),
+               "logprobs, state or advantages is NULL");
+  EG_CHECK_ARG(policy->reduction >= EG_REDUCE_SUM && policy->reduction <= EG_REDUCE_SEQUENCE, "reduction=%d",
+               policy->reduction);
+  EG_CHECK_ARG(policy->clip_low >= 0.0f && policy->clip_low <= 1.0f && policy->clip_high >= 0.0f,
+               "clip (%g, %g): 0 <= low <= 1 and high >= 0 are needed", (double)policy->clip_low,
+               (double)policy->clip_high);
+  Policy p = {policy->advantages, policy->old_logprobs, policy->ref_logprobs, {nullptr, 0, 0}, policy->reduction,
+              policy->clip_low, policy->clip_high, policy->kl_coef};
+  if (p.reduction == EG_REDUCE_SEQUENCE) {
+    if (int rc = check_segments(policy->segment_ids, policy->segment_ids_i32, policy->n_segments, &p.seg); rc != EG_OK)
+      return rc;
+    EG_CHECK_ARG(r.n == 0 || policy->segment_ids != nullptr, "segment_ids is NULL");
+  }
+  if (d_logits != nullptr)
+    if (int rc = check_grad(logits, d_logits, d_stride); rc != EG_OK) return rc;
+  const Cut cut = make_cut(r.n, r.v, logits->dtype);
+  const int64_t first = stats_bytes(r.n, cut);
+  EG_CHECK_WORKSPACE(first + (p.seg.n + 1) * 24);
+  Stat* stats = (Stat*)workspace;
+  int* counts = (int*)((char*)workspace + first);
+  if (int rc = launch_stats(r, logits->dtype, cut, stats, (hipStream_t)stream); rc != EG_OK) return rc;
+  int rc = by_dtype(logits->dtype, [&](auto zero) {
+    using T = decltype(zero);
+    policy_finish<T><<<1, kFinish, 0, (hipStream_t)stream>>>(r, p, cut.parts, stats, counts, logprobs,
+                                                             (RowState*)state, sums);
+    return launch_status("policy_finish");
+  });
+  if (rc != EG_OK || d_logits == nullptr) return rc;
+  return launch_grad(r, logits->dtype, cut, (const RowState*)state, nullptr, grad_scale / logits->temperature,
+                     d_logits, d_stride, (hipStream_t)stream);
+}
+
+int eg_preference_loss(const eg_logits* logits, const eg_preference* preference, float* logprobs,
+                       float* sequence_logprobs, float* margins, float* loss, float* state, void* d_logits,
+                       int64_t d_stride, float grad_scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  Rows r;
+  if (int rc = check_logits(logits, &r); rc != EG_OK) return rc;
+  EG_CHECK_ARG(preference != nullptr && loss != nullptr, "preference or loss is NULL");
+  EG_CHECK_ARG(preference->n_pairs >= 1, "n_pairs=%lld must be at least 1", (long long)preference->n_pairs);
+  EG_CHECK_ARG(preference->ref_logprobs != nullptr && sequence_logprobs != nullptr && margins != nullptr,
+               "ref_logprobs, sequence_logprobs or margins is NULL");
+  EG_CHECK_ARG(r.n == 0 || (logprobs != nullptr && state != nullptr && preference->segment_ids != nullptr),
+               "logprobs, state or segment_ids is NULL");
+  EG_CHECK_ARG(preference->label_smoothing >= 0.0f && preference->label_smoothing <= 1.0f,
+               "label_smoothing=%g must be in [0, 1]", (double)preference->label_smoothing);
+  if (d_logits != nullptr)
+    if (int rc = check_grad(logits, d_logits, d_stride); rc != EG_OK) return rc;
+  Preference p;
+  if (int rc = check_segments(preference->segment_ids, preference->segment_ids_i32, 2 * preference->n_pairs, &p.seg);
+      rc != EG_OK)
+    return rc;
+  p.ref_lp = preference->ref_logprobs;
+  p.beta = preference->beta;
+  p.smoothing = preference->label_smoothing;
+  const Cut cut = make_cut(r.n, r.v, logits->dtype);
+  const int64_t first = stats_bytes(r.n, cut);
+  EG_CHECK_WORKSPACE(first + (p.seg.n + 1) * 24 + r.n * 8);
+  Stat* stats = (Stat*)workspace;
+  int64_t* starts = (int64_t*)((char*)workspace + first);
+  double* seq_sum = (double*)(starts + p.seg.n + 1);
+  double* lp64 = seq_sum + p.seg.n;
+  float* d_seq = (float*)(lp64 + r.n);
+  if (int rc = launch_stats(r, logits->dtype, cut, stats, (hipStream_t)stream); rc != EG_OK) return rc;
+  int rc = by_dtype(logits->dtype, [&](auto zero) {
+    using T = decltype(zero);
+    preference_finish<T><<<1, kFinish, 0, (hipStream_t)stream>>>(r, p, cut.parts, stats, starts, d_seq, seq_sum,
+                                                                 lp64, logprobs, sequence_logprobs, margins,
+                                                                 (RowState*)state, loss);
+    return launch_status("preference_finish");
+  });
+  if (rc != EG_OK || d_logits == nullptr) return rc;
+  return launch_grad(r, logits->dtype, cut, (const RowState*)state, nullptr, grad_scale / logits->temperature,
+                     d_logits, d_stride, (hipStream_t)stream);
+}
+
+int eg_logits_grad(const eg_logits* logits, const float* state, const float* upstream, float grad_scale,
+                   void* d_logits, int64_t d_stride, void* stream) {
+  Rows r;
+  if (int rc = check_logits(logits, &r); rc != EG_OK) return rc;
+  EG_CHECK_ARG(r.n == 0 || state != nullptr, "state is NULL");
+  if (int rc = check_grad(logits, d_logits, d_stride); rc != EG_OK) return rc;
+  return launch_grad(r, logits->dtype, make_cut(r.n, r.v, logits->dtype), (const RowState*)state, upstream,
+                     grad_scale / logits->temperature, d_logits, d_stride, (hipStream_t)stream);
+}
+
+}  // extern "C"

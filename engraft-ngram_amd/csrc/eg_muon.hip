@@ -1,0 +1,610 @@
+// A momentum step whose update is orthogonalised by Newton-Schulz products: the
+// optimizer of the PLE block's projection weights (whose gradients ple_forward's
+// backward gives; the reference's own descent trains table rows alone).
+//
+//   m = mu m + g,  u = g + mu m (nesterov) or m,  X = u / (|u|_F + eps),
+//   `steps` times:  A = X X^T,  B = b A + c A^2,  X = a X + B X,
+//   w = (1 - lr decay) w - lr scale X.
+//
+// X is taken with its shorter side as rows (an orthogonalised transpose is the
+// transposed result), m x n with m <= n.  A and B are symmetric: only the tiles
+// on and above the diagonal are computed, so an iteration costs
+// m^2 n + m^3 + 2 m^2 n multiply-adds x 2 / 2.
+//
+// Arithmetic.  fp16 matrix cores, sums in fp32.  |X|_2 <= |X|_F <= 1 and the
+// polynomial keeps the singular values below a bound the host follows from step
+// to step, so every element of X, A and B has a known bound and one power of two
+// an iteration puts it below 60,000: fp16's 11 bits (three more than bf16's at
+// the same rate) over a range whose smallest normal is 2^-30 of that bound.  Two
+// planes (PLANES 2: hi = rne(x), lo = rne(x - hi), 22 bits, products hi hi + hi lo
+// + lo hi) keep fp32's accuracy, for fp32 weights; one plane costs a third of
+// the matrix work and leaves 2^-12 a rounding, below what a 16-bit weight keeps.
+//
+// Layout.  An operand is kept fragment-major: 32 rows x 16 k are one 1 KB run
+// (lane l holds row l % 32, k 8 (l / 32) .. + 7: one MFMA operand), [row block]
+// [k / 16][plane].  A product needs X by rows (A = X X^T) and X^T by rows (B X =
+// B (X^T)^T), so an iteration writes both; the MFMA's output registers hold
+// four consecutive rows of a column, which is how X^T's runs are laid out, and X's
+// go through LDS.  Rows and columns are padded with zeros to multiples of 64.
+#include "eg_common.h"
+
+#include <math.h>
+
+#include <algorithm>
+
+namespace eg {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kRun = 1024;       // bytes of a fragment: 32 rows x 16 k of fp16
+constexpr int kStepBytes = 4 * kRun;  // a row block's part of a K step: 64 k of one plane, 32 k of two
+constexpr int kMaxBatch = 64;    // matrices a launch
+
+// Byte offset of fragment (row block, k / 16, plane) in an operand of k16 fragments a row block.
+template <int PLANES>
+__device__ inline int64_t run_at(int64_t row_block, int64_t k16s, int64_t k16, int plane) {
+  return ((row_block * k16s + k16) * PLANES + plane) * kRun;
+}
+
+// ---- momentum, norm, planes -------------------------------------------------------------------
+
+struct Strides {
+  int64_t row, col;
+};
+
+struct Matrices {
+  void* param[kMaxBatch];
+  const void* grad[kMaxBatch];
+  float* momentum[kMaxBatch];
+};
+
+__device__ inline float load_value(const void* p, int dtype, int64_t i) {
+  if (dtype == EG_DTYPE_F32) return ((const float*)p)[i];
+  if (dtype == EG_DTYPE_BF16) return (float)((const __bf16*)p)[i];
+  return (float)((const _Float16*)p)[i];
+}
+
+__device__ inline void store_value(void* p, int dtype, int64_t i, float v) {
+  if (dtype == EG_DTYPE_F32) ((float*)p)[i] = v;
+  else if (dtype == EG_DTYPE_BF16) ((__bf16*)p)[i] = (__bf16)v;
+  else ((_Float16*)p)[i] = (_Float16)v;
+}
+
+struct UpdateArgs {
+  int64_t rows, cols;
+  Strides grad, momentum;
+  int grad_dtype, has_momentum, nesterov;
+  float mu;
+  int tiles_c, tiles;  // 64 x 64 tiles along a row, and in all
+  float* partials;     // [matrix][tile]: sums of u^2
+};
+
+// u of an element, from the gradient and the momentum after its update.
+__device__ inline float update_of(const UpdateArgs& a, float g, float m) {
+  if (!a.has_momentum) return g;
+  return a.nesterov ? g + a.mu * m : m;
+}
+
+// Grid (tiles, matrices): a 64 x 64 tile's momentum, and its part of |u|^2.
+__global__ __launch_bounds__(256) void muon_momentum_kernel(const UpdateArgs a, const Matrices mats) {
+  __shared__ float red[4];
+  const int64_t r0 = (int64_t)(blockIdx.x / a.tiles_c) * 64, c0 = (int64_t)(blockIdx.x % a.tiles_c) * 64;
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const void* grad = mats.grad[b];
+  float* mom = mats.momentum[b];
+  float sum = 0.0f;
+  const int64_t c = c0 + lane;
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const int64_t r = r0 + wave * 16 + i;
+    if (r < a.rows && c < a.cols) {
+      const float g = load_value(grad, a.grad_dtype, r * a.grad.row + c * a.grad.col);
+      float m = 0.0f;
+      if (a.has_momentum) {
+        float* q = mom + r * a.momentum.row + c * a.momentum.col;
+        m = a.mu * *q + g;
+        *q = m;
+      }
+      const float u = update_of(a, g, m);
+      sum += u * u;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) red[wave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) a.partials[(int64_t)b * a.tiles + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+struct PlanesArgs {
+  UpdateArgs u;
+  float eps, scale;     // x = u / (|u| + eps), kept times scale
+  char *by_row, *by_col;  // fragments of u and of u^T
+  int64_t batch_row, batch_col;  // bytes from one matrix to the next
+  int64_t k16_row, k16_col;      // fragments along a row of u, of u^T
+};
+
+// v's planes.  v is one fp32 value to the compiler: rounded to fp16 as part of the
+// multiplication that made it (v_fma_mixlo_f16) in one place and by itself in the
+// other, hi and the hi that lo is taken from differ at ties.
+__device__ inline void split(float v, _Float16& hi, _Float16& lo) {
+  asm("" : "+v"(v));
+  hi = (_Float16)v;
+  lo = (_Float16)(v - (float)hi);
+}
+
+template <int PLANES>
+__device__ inline void store_run(char* at, int lane, const float (&v)[8]) {
+  f16x8 hi, lo;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    _Float16 h, l;
+    split(v[i], h, l);
+    hi[i] = h;
+    lo[i] = l;
+  }
+  *(f16x8*)(at + lane * 16) = hi;
+  if (PLANES == 2) *(f16x8*)(at + kRun + lane * 16) = lo;
+}
+
+// Grid (padded tiles, matrices): a 64 x 64 tile of x as fragments of both orders.
+template <int PLANES>
+__global__ __launch_bounds__(256) void muon_planes_kernel(const PlanesArgs p, const Matrices mats) {
+  __shared__ float tile[64][65];
+  __shared__ double red[4];
+  const UpdateArgs& a = p.u;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.y;
+  const int64_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x % a.tiles_c, r0 = tr * 64, c0 = tc * 64;
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < a.tiles; i += 256) sum += (double)a.partials[(int64_t)b * a.tiles + i];
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) red[wave] = sum;
+  const void* grad = mats.grad[b];
+  const float* mom = mats.momentum[b];
+  const int64_t c = c0 + lane;
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const int64_t r = r0 + wave * 16 + i;
+    float u = 0.0f;
+    if (r < a.rows && c < a.cols) {
+      const float g = load_value(grad, a.grad_dtype, r * a.grad.row + c * a.grad.col);
+      u = update_of(a, g, a.has_momentum ? mom[r * a.momentum.row + c * a.momentum.col] : 0.0f);
+    }
+    tile[wave * 16 + i][lane] = u;
+  }
+  __syncthreads();
+  const float norm = sqrtf((float)(red[0] + red[1] + red[2] + red[3]));
+  const float s = p.scale / (norm + p.eps);
+  char* by_row = p.by_row + (int64_t)b * p.batch_row;
+  char* by_col = p.by_col + (int64_t)b * p.batch_col;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int run = wave * 2 + q, blk = run >> 2, k = run & 3;  // row block and k / 16 within the tile
+    const int row = blk * 32 + (lane & 31), col = k * 16 + 8 * (lane >> 5);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = tile[row][col + i] * s;
+    store_run<PLANES>(by_row + run_at<PLANES>(tr * 2 + blk, p.k16_row, tc * 4 + k, 0), lane, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = tile[col + i][row] * s;
+    store_run<PLANES>(by_col + run_at<PLANES>(tc * 2 + blk, p.k16_col, tr * 4 + k, 0), lane, v);
+  }
+}
+
+// ---- the products -----------------------------------------------------------------------------
+
+// What becomes of D = P Q^T:
+//   kGram   alpha D, symmetric: its fragments (D^T's and, off the diagonal tiles, D's)
+//   kPoly   alpha D + beta C with C symmetric: the same
+//   kStep   alpha D + beta C: the fragments of it and of its transpose
+//   kLast   o = alpha D + beta C: param = keep param - rate o
+enum Epilogue { kGram, kPoly, kStep, kLast };
+
+struct ProductArgs {
+  const char *p, *q;          // operands, fragment-major
+  int64_t batch_p, batch_q;   // bytes from one matrix to the next
+  int p_blocks, q_blocks;     // row blocks of 32
+  int steps;                  // K steps
+  int tiles_q;                // tiles along Q's rows (kStep, kLast); tiles a side (kGram, kPoly)
+  const char* c;              // C^T by rows: [q block][p rows as k]
+  int64_t batch_c;
+  char *out_t, *out;          // D^T and D by rows (kStep: X^T, X; the symmetric ones: the same buffer)
+  int64_t batch_out_t, batch_out;
+  float alpha, beta;
+  // kLast
+  int64_t rows, cols;         // D's real size
+  Strides param;
+  int param_dtype, read_param;
+  float keep, rate;
+};
+
+__device__ inline void wait_loads() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }  // vmcnt(0) alone
+
+// Grid (tiles, matrices).  BM x BN outputs of WM x WN wavefronts, a two-stage LDS
+// ring of K steps filled by direct-to-LDS loads, one barrier a step.
+template <int PLANES, int BM, int BN, int WM, int WN, Epilogue EPI>
+__global__ __launch_bounds__(WM * WN * 64) void muon_product_kernel(const ProductArgs a, const Matrices mats) {
+  constexpr int NW = WM * WN, AB = BM / 32, BB = BN / 32, TI = AB / WM, TJ = BB / WN;
+  constexpr int STAGE = (AB + BB) * kStepBytes, LOADS = 4 * (AB + BB) / NW, SUB = 4 / PLANES;
+  static_assert(4 * (AB + BB) % NW == 0, "whole runs a wavefront");
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  const int b = blockIdx.y;
+  int ti, tj;
+  if (EPI == kGram || EPI == kPoly) {  // tile t of the upper triangle, column by column
+    const int t = blockIdx.x;
+    tj = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
+    while (tj * (tj + 1) / 2 > t) --tj;
+    while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
+    ti = t - tj * (tj + 1) / 2;
+  } else {
+    ti = blockIdx.x / a.tiles_q;
+    tj = blockIdx.x % a.tiles_q;
+  }
+  const int i0 = ti * AB, j0 = tj * BB;  // first row blocks
+  const char* p = a.p + b * a.batch_p;
+  const char* q = a.q + b * a.batch_q;
+  const int64_t block_bytes = (int64_t)a.steps * kStepBytes;
+
+  // this wavefront's loads: runs wave, wave + NW, ... of a stage.  Blocks past the
+  // last re-read the last: their products only reach outputs that are not stored.
+  const char* src[LOADS];
+#pragma unroll
+  for (int l = 0; l < LOADS; ++l) {
+    const int run = l * NW + wave, blk = run / 4;
+    src[l] = (blk < AB ? p + (int64_t)min(i0 + blk, a.p_blocks - 1) * block_bytes
+                       : q + (int64_t)min(j0 + blk - AB, a.q_blocks - 1) * block_bytes) +
+             (run % 4) * kRun + lane * 16;
+  }
+  auto issue = [&](int step) {
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l)
+      __builtin_amdgcn_global_load_lds(
+          (const void*)(src[l] + (int64_t)step * kStepBytes),
+          (__attribute__((address_space(3))) void*)(lds + (step & 1) * STAGE + (l * NW + wave) * kRun), 16, 0, 0);
+  };
+
+  f32x16 acc[TI][TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+  issue(0);
+  for (int step = 0; step < a.steps; ++step) {
+    wait_loads();     // this wavefront's part of the step is in LDS
+    __syncthreads();  // everyone's, and nobody still reads the stage filled next
+    if (step + 1 < a.steps) issue(step + 1);
+    const char* st = lds + (step & 1) * STAGE + lane * 16;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      f16x8 pa[PLANES][TI], qb[PLANES][TJ];
+#pragma unroll
+      for (int x = 0; x < PLANES; ++x) {
+#pragma unroll
+        for (int i = 0; i < TI; ++i) pa[x][i] = *(const f16x8*)(st + (wm * TI + i) * kStepBytes + (s * PLANES + x) * kRun);
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+          qb[x][j] = *(const f16x8*)(st + (AB + wn * TJ + j) * kStepBytes + (s * PLANES + x) * kRun);
+      }
+#pragma unroll
+      for (int pass = PLANES == 2 ? 0 : 2; pass < 3; ++pass)  // lo hi, hi lo, hi hi
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+          for (int j = 0; j < TJ; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pa[pass == 0 ? PLANES - 1 : 0][i],
+                                                               qb[pass == 1 ? PLANES - 1 : 0][j], acc[i][j], 0, 0, 0);
+    }
+  }
+  __syncthreads();  // the ring is the epilogue's transpose buffer now
+
+  // lane l of a 32 x 32 block holds column l % 32, rows 8 g + 4 (l / 32) + r
+  constexpr int PITCH = 80;  // bytes of a row of 32 fp16 in the transpose buffer, 16-byte aligned
+  char* turn = lds + wave * (32 * PITCH);
+  const int col = lane & 31, half = lane >> 5;
+  const int64_t p16 = (int64_t)a.p_blocks * 2, q16 = (int64_t)a.q_blocks * 2;  // k / 16 along D^T's and D's rows
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      const int bi = i0 + wm * TI + i, bj = j0 + wn * TJ + j;
+      if (bi >= a.p_blocks || bj >= a.q_blocks) continue;
+      float v[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] = a.alpha * acc[i][j][r];
+      if (EPI != kGram) {
+        const char* c = a.c + b * a.batch_c;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int64_t at = run_at<PLANES>(bj, p16, bi * 2 + (g >> 1), 0) + (col + 32 * (g & 1)) * 16 + 8 * half;
+          const f16x4 hi = *(const f16x4*)(c + at);
+          f16x4 lo = {0, 0, 0, 0};
+          if (PLANES == 2) lo = *(const f16x4*)(c + at + kRun);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[4 * g + r] += a.beta * ((float)hi[r] + (float)lo[r]);
+        }
+      }
+      if (EPI == kLast) {
+        void* w = mats.param[b];
+        const int64_t y = (int64_t)bj * 32 + col;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int64_t x = (int64_t)bi * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+          if (x < a.rows && y < a.cols) {
+            const int64_t at = x * a.param.row + y * a.param.col;
+            const float old = a.read_param ? a.keep * load_value(w, a.param_dtype, at) : 0.0f;
+            store_value(w, a.param_dtype, at, old - a.rate * v[r]);
+          }
+        }
+        continue;
+      }
+      _Float16 hi[16], lo[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) split(v[r], hi[r], lo[r]);
+      char* out_t = a.out_t + b * a.batch_out_t;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        char* at = out_t + run_at<PLANES>(bj, p16, bi * 2 + (g >> 1), 0) + (col + 32 * (g & 1)) * 16 + 8 * half;
+        *(f16x4*)at = f16x4{hi[4 * g], hi[4 * g + 1], hi[4 * g + 2], hi[4 * g + 3]};
+        if (PLANES == 2) *(f16x4*)(at + kRun) = f16x4{lo[4 * g], lo[4 * g + 1], lo[4 * g + 2], lo[4 * g + 3]};
+      }
+      if (EPI != kStep && ti == tj) continue;  // a diagonal tile's blocks cover its transpose
+      char* out = a.out + b * a.batch_out;
+#pragma unroll
+      for (int x = 0; x < PLANES; ++x) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          *(_Float16*)(turn + (8 * (r >> 2) + 4 * half + (r & 3)) * PITCH + col * 2) = x == 0 ? hi[r] : lo[r];
+        __builtin_amdgcn_wave_barrier();  // a wavefront's LDS operations are in order
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const f16x8 run = *(const f16x8*)(turn + col * PITCH + s * 32 + half * 16);
+          *(f16x8*)(out + run_at<PLANES>(bi, q16, bj * 2 + s, x) + lane * 16) = run;
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------
+
+int64_t pad64(int64_t x) { return (x + 63) / 64 * 64; }
+
+// The buffers of one matrix, m x n padded: X, two X^T, A, B.
+struct Layout {
+  int64_t m, n;          // padded, m <= n
+  int64_t x, a;          // bytes of X (or X^T), of A (or B)
+  int64_t tiles;         // 64 x 64 tiles of the padded matrix
+  int64_t partials;      // bytes of all matrices' partial sums
+  int64_t total;
+};
+
+Layout make_layout(int64_t rows, int64_t cols, int64_t count, int planes) {
+  Layout l;
+  l.m = pad64(std::min(rows, cols));
+  l.n = pad64(std::max(rows, cols));
+  l.x = l.m * l.n * 2 * planes;
+  l.a = l.m * l.m * 2 * planes;
+  l.tiles = (l.m / 64) * (l.n / 64);
+  l.partials = (count * l.tiles * 4 + 255) / 256 * 256;
+  l.total = l.partials + count * (3 * l.x + 2 * l.a);
+  return l;
+}
+
+template <int PLANES, int BM, int BN, int WM, int WN, Epilogue EPI>
+int launch_product_as(const ProductArgs& args, const Matrices& mats, int count, hipStream_t stream) {
+  ProductArgs a = args;
+  constexpr int AB = BM / 32, BB = BN / 32, bytes = 2 * (AB + BB) * kStepBytes;
+  static_assert(bytes >= WM * WN * 32 * 80, "the transpose buffers fit the ring");
+  const int tp = (a.p_blocks + AB - 1) / AB, tq = (a.q_blocks + BB - 1) / BB;
+  a.tiles_q = tq;
+  const int tiles = EPI == kGram || EPI == kPoly ? tq * (tq + 1) / 2 : tp * tq;
+  auto kernel = muon_product_kernel<PLANES, BM, BN, WM, WN, EPI>;
+  if (bytes > 65536) {
+    static const hipError_t set =
+        hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    EG_CHECK_HIP(set);
+  }
+  kernel<<<dim3((unsigned)tiles, (unsigned)count), WM * WN * 64, bytes, stream>>>(a, mats);
+  return launch_status("muon_product_kernel");
+}
+
+template <int PLANES, Epilogue EPI>
+int launch_product(const ProductArgs& a, const Matrices& mats, int count, hipStream_t stream) {
+  return launch_product_as<PLANES, 128, 128, 2, 2, EPI>(a, mats, count, stream);
+}
+
+// Powers of two by which X, A and B of an iteration are kept, from the bound of X's
+// singular values; false where the coefficients leave no finite ones.
+struct Bounds {
+  double sigma;         // X's singular values are at most this
+  int x, gram, poly;    // exponents
+};
+
+int exponent_for(double bound) { return (int)floor(log2(60000.0 / std::max(bound, 1e-30))); }
+
+// max over [0, s] of |f|, on a grid fine against a cubic's curvature there, with a margin.
+template <typename F>
+double largest(double s, F&& f) {
+  double top = 0.0;
+  for (int i = 0; i <= 4096; ++i) top = std::max(top, fabs(f(s * i / 4096.0)));
+  return top * 1.01;
+}
+
+Bounds bounds_of(double sigma, const float* k) {
+  const double a = k[0], b = k[1], c = k[2], s2 = sigma * sigma;
+  Bounds r;
+  r.sigma = sigma;
+  r.x = exponent_for(sigma);
+  r.gram = exponent_for(s2);
+  r.poly = exponent_for(largest(s2, [&](double y) { return b * y + c * y * y; }));
+  (void)a;
+  return r;
+}
+
+double next_sigma(double sigma, const float* k) {
+  return largest(sigma, [&](double s) { const double y = s * s; return s * (k[0] + k[1] * y + k[2] * y * y); });
+}
+
+template <int PLANES>
+int run_muon(const eg_muon* o, int first, int count, const Layout& l, char* ws, hipStream_t stream) {
+  Matrices mats = {};
+  for (int i = 0; i < count; ++i) {
+    mats.param[i] = o->params[first + i];
+    mats.grad[i] = o->grads[first + i];
+    mats.momentum[i] = o->momenta != nullptr ? o->momenta[first + i] : nullptr;
+  }
+  const bool tall = o->rows > o->cols;
+  char* base = ws + l.partials;
+  char* x = base;
+  char* xt[2] = {x + count * l.x, x + 2 * count * l.x};
+  char* gram = x + 3 * count * l.x;
+  char* poly = gram + count * l.a;
+  const int m32 = (int)(l.m / 32), n32 = (int)(l.n / 32);
+  const int m_steps = (int)(l.m * PLANES / 64), n_steps = (int)(l.n * PLANES / 64);
+  Bounds bd = bounds_of(1.0, o->coefficients);
+
+  PlanesArgs pa;
+  pa.u = {o->rows, o->cols, {o->grad_stride[0], o->grad_stride[1]}, {o->momentum_stride[0], o->momentum_stride[1]},
+          o->grad_dtype, o->momenta != nullptr, o->nesterov, o->momentum, (int)(pad64(o->cols) / 64), (int)l.tiles,
+          (float*)ws};
+  pa.eps = o->eps;
+  pa.scale = ldexpf(1.0f, bd.x);
+  pa.by_row = tall ? xt[0] : x;
+  pa.by_col = tall ? x : xt[0];
+  pa.batch_row = pa.batch_col = l.x;
+  pa.k16_row = pad64(o->cols) / 16;
+  pa.k16_col = pad64(o->rows) / 16;
+  muon_momentum_kernel<<<dim3((unsigned)l.tiles, (unsigned)count), 256, 0, stream>>>(pa.u, mats);
+  if (int rc = launch_status("muon_momentum_kernel"); rc != EG_OK) return rc;
+  muon_planes_kernel<PLANES><<<dim3((unsigned)l.tiles, (unsigned)count), 256, 0, stream>>>(pa, mats);
+  if (int rc = launch_status("muon_planes_kernel"); rc != EG_OK) return rc;
+
+  for (int s = 0; s < o->steps; ++s) {
+    const float* k = o->coefficients + 3 * s;
+    const bool last = s + 1 == o->steps;
+    char* xt_now = xt[s & 1];
+    ProductArgs a = {};
+    // A = X X^T
+    a.p = a.q = x;
+    a.batch_p = a.batch_q = l.x;
+    a.p_blocks = a.q_blocks = m32;
+    a.steps = n_steps;
+    a.out_t = a.out = gram;
+    a.batch_out_t = a.batch_out = l.a;
+    a.alpha = ldexpf(1.0f, bd.gram - 2 * bd.x);
+    if (int rc = launch_product<PLANES, kGram>(a, mats, count, stream); rc != EG_OK) return rc;
+    // B = b A + c A A
+    a.p = a.q = a.c = gram;
+    a.batch_p = a.batch_q = a.batch_c = l.a;
+    a.steps = m_steps;
+    a.out_t = a.out = poly;
+    a.alpha = ldexpf(k[2], bd.poly - 2 * bd.gram);
+    a.beta = ldexpf(k[1], bd.poly - bd.gram);
+    if (int rc = launch_product<PLANES, kPoly>(a, mats, count, stream); rc != EG_OK) return rc;
+    // X = a X + B X
+    if (!last) {
+      const double sigma = next_sigma(bd.sigma, k);
+      const Bounds nx = bounds_of(sigma, k + 3);
+      a.p = poly;
+      a.q = xt_now;
+      a.batch_q = l.x;
+      a.q_blocks = n32;
+      a.c = xt_now;
+      a.batch_c = l.x;
+      a.out_t = xt[1 - (s & 1)];
+      a.out = x;
+      a.batch_out_t = a.batch_out = l.x;
+      a.alpha = ldexpf(1.0f, nx.x - bd.poly - bd.x);
+      a.beta = ldexpf(k[0], nx.x - bd.x);
+      if (int rc = launch_product<PLANES, kStep>(a, mats, count, stream); rc != EG_OK) return rc;
+      bd = nx;
+    } else {
+      // D is X, or X^T for a tall matrix: a lane's column runs along the matrix's rows
+      a.p = tall ? xt_now : poly;
+      a.q = tall ? poly : xt_now;
+      a.batch_p = tall ? l.x : l.a;
+      a.batch_q = tall ? l.a : l.x;
+      a.p_blocks = tall ? n32 : m32;
+      a.q_blocks = tall ? m32 : n32;
+      a.c = tall ? x : xt_now;
+      a.batch_c = l.x;
+      a.alpha = ldexpf(1.0f, -bd.poly - bd.x);
+      a.beta = ldexpf(k[0], -bd.x);
+      a.rows = o->rows;
+      a.cols = o->cols;
+      a.param = {o->param_stride[0], o->param_stride[1]};
+      a.param_dtype = o->param_dtype;
+      a.read_param = o->keep != 0.0f;
+      a.keep = o->keep;
+      a.rate = o->rate;
+      if (int rc = launch_product<PLANES, kLast>(a, mats, count, stream); rc != EG_OK) return rc;
+    }
+  }
+  return EG_OK;
+}
+
+int check_muon(const eg_muon* o) {
+  EG_CHECK_ARG(o != nullptr, "muon is NULL");
+  EG_CHECK_ARG(o->rows >= 1 && o->cols >= 1 && o->rows <= (1 << 20) && o->cols <= (1 << 20),
+               "a matrix of %lld x %lld: 1 to 2^20 rows and columns", (long long)o->rows, (long long)o->cols);
+  EG_CHECK_ARG(o->count >= 0, "count=%d must not be negative", o->count);
+  EG_CHECK_ARG(o->count == 0 || (o->params != nullptr && o->grads != nullptr), "params or grads is NULL");
+  EG_CHECK_ARG(o->planes == 1 || o->planes == 2, "planes=%d must be 1 or 2", o->planes);
+  for (const int d : {o->param_dtype, o->grad_dtype})
+    EG_CHECK_ARG(d == EG_DTYPE_F32 || d == EG_DTYPE_BF16 || d == EG_DTYPE_F16, "dtype=%d must be f32, bf16 or f16", d);
+  EG_CHECK_ARG(o->steps >= 1 && o->steps <= 100 && o->coefficients != nullptr, "steps=%d must be in [1, 100]", o->steps);
+  EG_CHECK_ARG(o->eps > 0.0f && o->eps <= 1.0f, "eps=%g must be in (0, 1]", (double)o->eps);
+  EG_CHECK_ARG(isfinite(o->keep) && isfinite(o->rate) && isfinite(o->momentum), "a factor is not finite");
+  double sigma = 1.0;
+  for (int s = 0; s < o->steps; ++s) {
+    const float* k = o->coefficients + 3 * s;
+    EG_CHECK_ARG(isfinite(k[0]) && isfinite(k[1]) && isfinite(k[2]) && sigma < 16.0 && sigma > 1.0 / 16.0,
+                 "coefficients of step %d: singular values of up to %g (1/16 to 16 are kept)", s, sigma);
+    sigma = next_sigma(sigma, k);
+  }
+  for (int i = 0; i < o->count; ++i)
+    EG_CHECK_ARG(o->params[i] != nullptr && o->grads[i] != nullptr && (o->momenta == nullptr || o->momenta[i] != nullptr),
+                 "matrix %d: a pointer is NULL", i);
+  return EG_OK;
+}
+
+}  // namespace
+}  // namespace eg
+
+using namespace eg;
+
+extern "C" {
+
+int64_t eg_muon_workspace_size(int64_t rows, int64_t cols, int32_t count, int32_t planes) {
+  if (rows < 1 || cols < 1 || count < 0 || rows > (1 << 20) || cols > (1 << 20) || planes < 1 || planes > 2) return -1;
+  return make_layout(rows, cols, std::min(count, (int32_t)kMaxBatch), planes).total;
+}
+
+int eg_muon_step(const eg_muon* muon, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = check_muon(muon); rc != EG_OK) return rc;
+  if (muon->count == 0) return EG_OK;
+  const int64_t need = eg_muon_workspace_size(muon->rows, muon->cols, muon->count, muon->planes);
+  if (workspace == nullptr || workspace_bytes < need)
+    return set_error(EG_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                     (long long)need);
+  EG_CHECK_ARG((uintptr_t)workspace % 256 == 0, "workspace must be 256-byte aligned");
+  for (int first = 0; first < muon->count; first += kMaxBatch) {
+    const int count = std::min(muon->count - first, kMaxBatch);
+    const Layout l = make_layout(muon->rows, muon->cols, count, muon->planes);
+    const int rc = muon->planes == 2 ? run_muon<2>(muon, first, count, l, (char*)workspace, (hipStream_t)stream)
+                                     : run_muon<1>(muon, first, count, l, (char*)workspace, (hipStream_t)stream);
+    if (rc != EG_OK) return rc;
+  }
+  return EG_OK;
+}
+
+}  // extern "C"

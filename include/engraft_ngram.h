@@ -701,6 +701,121 @@ int eg_split_f16(const eg_f16_matrix* x, void* stream);
 int eg_gemm_f16x3(const eg_f16_matrix* a, const eg_f16_matrix* b, const eg_f16_matrix* b2, float* c, int64_t ldc,
                   float* c2, int64_t ldc2, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Losses of next-token logits, and the gradient of the logits ------------------
+ *
+ * What a descent's d_out comes from; the reference's own loss is a torch
+ * expression over log_softmax (kd_loss, engraft/replica/distill.py:283-325). */
+
+enum eg_dtype { EG_DTYPE_F32 = 0, EG_DTYPE_BF16 = 1, EG_DTYPE_F16 = 2 };
+
+/* Logits z [n, v], element (i, j) at data[i * row_stride + j], divided by
+ * `temperature`; targets [n] int64 (or int32): a row whose target is negative is
+ * left out (its logits are not read, its log-probability and gradient are 0), a
+ * target of v or more gives NaN there.  No alignment beyond the type's. */
+typedef struct eg_logits {
+  const void* data;
+  int32_t dtype; /* eg_dtype */
+  int32_t targets_i32;
+  int64_t n, v, row_stride;
+  const void* targets;
+  float temperature;
+} eg_logits;
+
+/* How the rows of a loss are weighted: 1 each; 1 / the rows with a target; or 1 /
+ * (segments with such a row x the segment's rows with a target). */
+enum eg_reduction { EG_REDUCE_SUM = 0, EG_REDUCE_TOKEN = 1, EG_REDUCE_SEQUENCE = 2 };
+
+/* The clipped policy loss: with r = exp(lp - old), A = advantages and d = ref - lp,
+ *   sum_i w_i (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1)).
+ * old_logprobs NULL: the policy's own, r = 1 (its gradient stays); ref_logprobs
+ * NULL: no KL term.  segment_ids [n] int64 (or int32), any order, for
+ * EG_REDUCE_SEQUENCE alone: a value outside [0, n_segments) gives its row the weight 0. */
+typedef struct eg_policy {
+  const float* advantages;
+  const float* old_logprobs;
+  const float* ref_logprobs;
+  const void* segment_ids;
+  int64_t n_segments;
+  int32_t segment_ids_i32;
+  int32_t reduction;
+  float clip_low, clip_high, kl_coef;
+} eg_policy;
+
+/* The preference loss of paired log ratios: with s_k the sum of segment k's
+ * log-probabilities and h_p = beta ((s_2p - ref_2p) - (s_2p+1 - ref_2p+1)),
+ *   mean_p(-(1 - label_smoothing) log sigma(h_p) - label_smoothing log sigma(-h_p)).
+ * segment_ids [n] int64 (or int32), not decreasing (otherwise margins, loss and
+ * gradient are NaN); rows outside [0, 2 n_pairs) belong to no sequence.
+ * ref_logprobs [2 n_pairs]. */
+typedef struct eg_preference {
+  const void* segment_ids;
+  const float* ref_logprobs;
+  int64_t n_pairs;
+  int32_t segment_ids_i32;
+  float beta, label_smoothing;
+} eg_preference;
+
+/* Bytes of workspace of the entry points below (16-byte aligned); n_segments: 0,
+ * the policy loss's n_segments under EG_REDUCE_SEQUENCE, or 2 n_pairs. */
+int64_t eg_loss_workspace_size(int64_t n, int64_t v, int32_t dtype, int64_t n_segments);
+
+/* logprobs f32 [n]: the targets' log-probabilities. */
+int eg_token_logprobs(const eg_logits* logits, float* logprobs, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/* sums f32 [3]: the loss, the weighted KL term (without kl_coef) and the weighted
+ * share of clipped rows; logprobs f32 [n]; state f32 [n, 3], what eg_logits_grad
+ * takes.  With d_logits (the logits' type, rows d_stride apart; may be the logits
+ * themselves) also the gradient of grad_scale times the loss. */
+int eg_policy_loss(const eg_logits* logits, const eg_policy* policy, float* logprobs, float* sums, float* state,
+                   void* d_logits, int64_t d_stride, float grad_scale, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
+/* loss f32 [1], margins f32 [n_pairs] (h), sequence_logprobs f32 [2 n_pairs];
+ * logprobs, state and d_logits as eg_policy_loss. */
+int eg_preference_loss(const eg_logits* logits, const eg_preference* preference, float* logprobs,
+                       float* sequence_logprobs, float* margins, float* loss, float* state, void* d_logits,
+                       int64_t d_stride, float grad_scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* d_logits from a loss's state: grad_scale times *upstream (device; NULL: 1) times
+ * the gradient of the loss that wrote it from the same logits. */
+int eg_logits_grad(const eg_logits* logits, const float* state, const float* upstream, float grad_scale,
+                   void* d_logits, int64_t d_stride, void* stream);
+
+/* ---- Orthogonalised weight updates -------------------------------------------------
+ *
+ * The optimizer step of matrices whose gradients eg_ple's backward gives; no
+ * counterpart in the reference (its descent trains table rows alone). */
+
+/* `count` matrices of one shape, types and strides (elements; params[i] etc. are
+ * HOST arrays of device pointers):
+ *   momenta[i] = momentum momenta[i] + grads[i]         (f32; momenta NULL: none kept)
+ *   u = grads[i] + momentum momenta[i] (nesterov), momenta[i], or grads[i]
+ *   X = u / (|u|_F + eps); steps times, with coefficients [steps][3] = (a, b, c) (host):
+ *     X = a X + (b A + c A^2) X,  A = X X^T   (rows <= cols; transposed otherwise)
+ *   params[i] = keep params[i] - rate X         (keep 0: params[i] is not read)
+ * on the fp16 matrix cores with fp32 sums: planes 2 (22-bit operands, three
+ * products) or 1 (11-bit operands).  The coefficients must keep the bound of the
+ * singular values, 1 at first, between 1/16 and 16. */
+typedef struct eg_muon {
+  int64_t rows, cols;
+  int32_t count;
+  int32_t planes;
+  void* const* params;
+  const void* const* grads;
+  float* const* momenta;
+  int32_t param_dtype, grad_dtype; /* eg_dtype */
+  int64_t param_stride[2], grad_stride[2], momentum_stride[2];
+  const float* coefficients;
+  int32_t steps, nesterov;
+  float momentum, eps, keep, rate;
+} eg_muon;
+
+/* Bytes of eg_muon_step's workspace (256-byte aligned); -1 for a bad argument. */
+int64_t eg_muon_workspace_size(int64_t rows, int64_t cols, int32_t count, int32_t planes);
+
+int eg_muon_step(const eg_muon* muon, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,73 @@
+"""What the orthogonalised step refuses, on the host and before any launch."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+
+def _muon(**kw):
+    from engraft_ngram_amd import _lib
+    one = (ctypes.c_void_p * 1)(256)
+    coef = (ctypes.c_float * 3)(3.4445, -4.7750, 2.0315)
+    o = _lib.EgMuon()
+    o.rows, o.cols, o.count, o.planes = 100, 200, 1, 2
+    o.params = o.grads = o.momenta = ctypes.cast(one, ctypes.c_void_p)
+    o.coefficients, o.steps = ctypes.cast(coef, ctypes.c_void_p), 1
+    o.momentum, o.eps, o.keep, o.rate = 0.9, 1e-7, 1.0, 0.1
+    o._kept = (one, coef)
+    for k, x in kw.items():
+        setattr(o, k, x)
+    return o
+
+
+@pytest.mark.parametrize("needle,bad", [
+    ("0 x 200", dict(rows=0)), ("2^20", dict(cols=(1 << 20) + 1)), ("count=-1", dict(count=-1)),
+    ("NULL", dict(params=None)), ("planes=3", dict(planes=3)), ("dtype=9", dict(grad_dtype=9)),
+    ("steps=0", dict(steps=0)), ("steps=101", dict(steps=101)), ("eps=0", dict(eps=0.0)),
+    ("not finite", dict(rate=float("nan"))),
+])
+def test_arguments_are_checked(needle, bad):
+    from engraft_ngram_amd import _lib
+    lib = _lib.load()
+    o = _muon(**bad)
+    rc = lib.eg_muon_step(ctypes.byref(o), 256, 1 << 40, None)
+    assert rc == _lib.EG_ERR_ARG and needle in lib.eg_last_error().decode()
+
+
+def test_workspace_is_checked():
+    from engraft_ngram_amd import _lib
+    lib = _lib.load()
+    need = lib.eg_muon_workspace_size(100, 200, 1, 2)
+    assert need > 0 and lib.eg_muon_workspace_size(100, 200, 2, 2) > need > lib.eg_muon_workspace_size(100, 200, 1, 1)
+    assert lib.eg_muon_workspace_size(100, 200, 1, 3) == -1
+    o = _muon()
+    assert lib.eg_muon_step(ctypes.byref(o), 256, need - 1, None) == _lib.EG_ERR_WORKSPACE
+    assert lib.eg_muon_step(ctypes.byref(o), 8, need, None) == _lib.EG_ERR_ARG
+    o = _muon(count=0)
+    assert lib.eg_muon_step(ctypes.byref(o), None, 0, None) == _lib.EG_OK
+    # a NULL among the matrices
+    none = (ctypes.c_void_p * 1)(None)
+    o = _muon(grads=ctypes.cast(none, ctypes.c_void_p))
+    assert lib.eg_muon_step(ctypes.byref(o), 256, need, None) == _lib.EG_ERR_ARG
+
+
+def test_coefficients_that_leave_the_range():
+    from engraft_ngram_amd import _lib
+    lib = _lib.load()
+    coef = (ctypes.c_float * 6)(100.0, 0.0, 0.0, 1.0, 0.0, 0.0)  # singular values of up to 100 after a step
+    o = _muon(coefficients=ctypes.cast(coef, ctypes.c_void_p), steps=2)
+    assert lib.eg_muon_step(ctypes.byref(o), 256, 1 << 40, None) == _lib.EG_ERR_ARG
+    assert "singular values" in lib.eg_last_error().decode()
+
+
+def test_host_tensors_are_refused():
+    from engraft_ngram_amd import muon
+    w = torch.zeros((3, 4))
+    with pytest.raises(ValueError, match="on the GPU"):
+        muon.muon_step([w], [w], [w], lr=0.1)
+    with pytest.raises(ValueError, match="on the GPU"):
+        muon.orthogonalize(w)
+    with pytest.raises(ValueError, match="on the GPU"):
+        muon.MuonState([w])
