@@ -37,10 +37,10 @@ namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kRun = 1024;       // bytes of a fragment: 32 rows x 16 k of fp16
-constexpr int kStepBytes = 4 * kRun;  // a row block's part of a K step: 64 k of one plane, 32 k of two
 constexpr int kMaxBatch = 64;    // matrices a launch
 
 // Byte offset of fragment (row block, k / 16, plane) in an operand of k16 fragments a row block.
@@ -208,7 +208,7 @@ struct ProductArgs {
   const char *p, *q;          // operands, fragment-major
   int64_t batch_p, batch_q;   // bytes from one matrix to the next
   int p_blocks, q_blocks;     // row blocks of 32
-  int steps;                  // K steps
+  int k16;                    // K / 16
   int tiles_q;                // tiles along Q's rows (kStep, kLast); tiles a side (kGram, kPoly)
   const char* c;              // C^T by rows: [q block][p rows as k]
   int64_t batch_c;
@@ -222,133 +222,221 @@ struct ProductArgs {
   float keep, rate;
 };
 
-__device__ inline void wait_loads() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }  // vmcnt(0) alone
+constexpr int kGroup = 8;  // row tiles that are walked together, column by column
 
-// Grid (tiles, matrices).  BM x BN outputs of WM x WN wavefronts, a two-stage LDS
-// ring of K steps filled by direct-to-LDS loads, one barrier a step.
-template <int PLANES, int BM, int BN, int WM, int WN, Epilogue EPI>
-__global__ __launch_bounds__(WM * WN * 64) void muon_product_kernel(const ProductArgs a, const Matrices mats) {
-  constexpr int NW = WM * WN, AB = BM / 32, BB = BN / 32, TI = AB / WM, TJ = BB / WN;
-  constexpr int STAGE = (AB + BB) * kStepBytes, LOADS = 4 * (AB + BB) / NW, SUB = 4 / PLANES;
-  static_assert(4 * (AB + BB) % NW == 0, "whole runs a wavefront");
+// Workgroups are dealt to the 8 XCDs in turn; block b's tile is such that each XCD
+// takes a contiguous run of tiles, whose panels its own L2 shares.
+__device__ inline int xcd_order(int b, int n) {
+  const int x = b % 8, k = b / 8, each = n / 8, more = n % 8;
+  return x * each + min(x, more) + k;
+}
+
+// LDS of a product's workgroup: the parts of the tile that leave their sums at a time.
+template <int T, int NW>
+struct ProductShape {
+  static constexpr int kParts = NW < 4 ? NW : 4;
+  static constexpr int kAll = T * T * 4096 / kParts * (NW - 1);  // bytes of one part's sums
+  static constexpr int kRound = kParts * kAll <= 147456 ? kParts : kParts == 4 && 3 * kAll <= 147456 ? 3 : 1;
+  static constexpr int kBytes = kRound * kAll > kParts * 32 * 80 ? kRound * kAll : kParts * 32 * 80;
+};
+
+// Grid (tiles, matrices): an output tile of T x T blocks of 32 x 32 a workgroup.  Its NW
+// wavefronts each compute the whole tile over their share of K, fragments loaded
+// straight into registers DEPTH k16 ahead (a fragment is 1 KB of consecutive memory):
+// no LDS and no barrier until the wavefronts' sums are added at the end.
+template <int PLANES, int T, int NW, int DEPTH, Epilogue EPI>
+__global__ __launch_bounds__(NW * 64, NW / 4) void muon_product_kernel(const ProductArgs a, const Matrices mats) {
+  constexpr int PARTS = NW < 4 ? NW : 4;  // wavefronts that finish a part of the tile each
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.y;
   int ti, tj;
+  const int t = xcd_order(blockIdx.x, gridDim.x);
   if (EPI == kGram || EPI == kPoly) {  // tile t of the upper triangle, column by column
-    const int t = blockIdx.x;
     tj = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
     while (tj * (tj + 1) / 2 > t) --tj;
     while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
     ti = t - tj * (tj + 1) / 2;
   } else {
-    ti = blockIdx.x / a.tiles_q;
-    tj = blockIdx.x % a.tiles_q;
+    const int tiles_p = gridDim.x / a.tiles_q, group = t / (kGroup * a.tiles_q), first = group * kGroup;
+    const int deep = min(kGroup, tiles_p - first), u = t - first * a.tiles_q;
+    ti = first + u % deep;
+    tj = u / deep;
   }
-  const int i0 = ti * AB, j0 = tj * BB;  // first row blocks
-  const char* p = a.p + b * a.batch_p;
-  const char* q = a.q + b * a.batch_q;
-  const int64_t block_bytes = (int64_t)a.steps * kStepBytes;
-
-  // this wavefront's loads: runs wave, wave + NW, ... of a stage.  Blocks past the
-  // last re-read the last: their products only reach outputs that are not stored.
-  const char* src[LOADS];
+  const int i0 = ti * T, j0 = tj * T;  // first row blocks
+  const int64_t block_bytes = (int64_t)a.k16 * PLANES * kRun;
+  // blocks past the last re-read the last: their products only reach outputs that are not stored
+  const char *ps[T], *qs[T];
 #pragma unroll
-  for (int l = 0; l < LOADS; ++l) {
-    const int run = l * NW + wave, blk = run / 4;
-    src[l] = (blk < AB ? p + (int64_t)min(i0 + blk, a.p_blocks - 1) * block_bytes
-                       : q + (int64_t)min(j0 + blk - AB, a.q_blocks - 1) * block_bytes) +
-             (run % 4) * kRun + lane * 16;
+  for (int i = 0; i < T; ++i) {
+    ps[i] = a.p + b * a.batch_p + (int64_t)min(i0 + i, a.p_blocks - 1) * block_bytes;
+    qs[i] = a.q + b * a.batch_q + (int64_t)min(j0 + i, a.q_blocks - 1) * block_bytes;
   }
-  auto issue = [&](int step) {
-#pragma unroll
-    for (int l = 0; l < LOADS; ++l)
-      __builtin_amdgcn_global_load_lds(
-          (const void*)(src[l] + (int64_t)step * kStepBytes),
-          (__attribute__((address_space(3))) void*)(lds + (step & 1) * STAGE + (l * NW + wave) * kRun), 16, 0, 0);
-  };
+  const int k_first = a.k16 * wave / NW, k_count = a.k16 * (wave + 1) / NW - k_first;
 
-  f32x16 acc[TI][TJ];
+  f32x16 acc[T][T];
 #pragma unroll
-  for (int i = 0; i < TI; ++i)
+  for (int i = 0; i < T; ++i)
 #pragma unroll
-    for (int j = 0; j < TJ; ++j)
+    for (int j = 0; j < T; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-  issue(0);
-  for (int step = 0; step < a.steps; ++step) {
-    wait_loads();     // this wavefront's part of the step is in LDS
-    __syncthreads();  // everyone's, and nobody still reads the stage filled next
-    if (step + 1 < a.steps) issue(step + 1);
-    const char* st = lds + (step & 1) * STAGE + lane * 16;
-#pragma unroll
-    for (int s = 0; s < SUB; ++s) {
-      f16x8 pa[PLANES][TI], qb[PLANES][TJ];
+  if (k_count > 0) {
+    f16x8 pa[DEPTH][PLANES][T], qb[DEPTH][PLANES][T];
+    const uint32_t lane16 = (uint32_t)lane * 16;
+    auto load = [&](int f, int k) {
+      const int64_t at = (int64_t)(k_first + min(k, k_count - 1)) * (PLANES * kRun);
 #pragma unroll
       for (int x = 0; x < PLANES; ++x) {
 #pragma unroll
-        for (int i = 0; i < TI; ++i) pa[x][i] = *(const f16x8*)(st + (wm * TI + i) * kStepBytes + (s * PLANES + x) * kRun);
-#pragma unroll
-        for (int j = 0; j < TJ; ++j)
-          qb[x][j] = *(const f16x8*)(st + (AB + wn * TJ + j) * kStepBytes + (s * PLANES + x) * kRun);
+        for (int i = 0; i < T; ++i) {
+          pa[f][x][i] = *(const f16x8*)(ps[i] + at + lane16 + x * kRun);
+          qb[f][x][i] = *(const f16x8*)(qs[i] + at + lane16 + x * kRun);
+        }
       }
+    };
+    auto multiply = [&](int f) {
 #pragma unroll
       for (int pass = PLANES == 2 ? 0 : 2; pass < 3; ++pass)  // lo hi, hi lo, hi hi
 #pragma unroll
-        for (int i = 0; i < TI; ++i)
+        for (int i = 0; i < T; ++i)
 #pragma unroll
-          for (int j = 0; j < TJ; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pa[pass == 0 ? PLANES - 1 : 0][i],
-                                                               qb[pass == 1 ? PLANES - 1 : 0][j], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < T; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pa[f][pass == 0 ? PLANES - 1 : 0][i],
+                                                               qb[f][pass == 1 ? PLANES - 1 : 0][j], acc[i][j], 0, 0, 0);
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) load(d, d);
+    __builtin_amdgcn_sched_barrier(0);
+    int k = 0;
+    for (; k + DEPTH <= k_count; k += DEPTH) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        multiply(d);
+        __builtin_amdgcn_sched_barrier(0);
+        load(d, k + d + DEPTH);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d)
+      if (k + d < k_count) multiply(d);
+  }
+
+  // The wavefronts' sums.  Part w of the tile (of PARTS: its quarters, or halves by rows) goes to
+  // wavefront w; the others leave theirs in LDS, as many parts at a time as fit.
+  constexpr int SI = PARTS == 4 ? T / 2 : T / PARTS, SJ = PARTS == 4 ? T / 2 : T;  // blocks of a part
+  constexpr int PART_BYTES = SI * SJ * 4096, ROUND = ProductShape<T, NW>::kRound;
+  f32x16 sum[SI][SJ];
+#pragma unroll
+  for (int w0 = 0; w0 < PARTS; w0 += ROUND) {
+    if (NW > 1 && w0 > 0) __syncthreads();
+#pragma unroll
+    for (int w = w0; w < w0 + ROUND && w < PARTS; ++w) {
+      const int pi = PARTS == 4 ? w / 2 * SI : w * SI, pj = PARTS == 4 ? w % 2 * SJ : 0;
+      if (wave == w) {
+#pragma unroll
+        for (int i = 0; i < SI; ++i)
+#pragma unroll
+          for (int j = 0; j < SJ; ++j) sum[i][j] = acc[pi + i][pj + j];
+      } else {
+        char* at = lds + ((w - w0) * (NW - 1) + (wave > w ? wave - 1 : wave)) * PART_BYTES + lane * 16;
+#pragma unroll
+        for (int i = 0; i < SI; ++i)
+#pragma unroll
+          for (int j = 0; j < SJ; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              *(f32x4*)(at + ((i * SJ + j) * 4 + g) * 1024) = f32x4{acc[pi + i][pj + j][4 * g], acc[pi + i][pj + j][4 * g + 1],
+                                                                   acc[pi + i][pj + j][4 * g + 2], acc[pi + i][pj + j][4 * g + 3]};
+      }
+    }
+    if (NW > 1) __syncthreads();
+    if (wave >= w0 && wave < w0 + ROUND && wave < PARTS) {
+#pragma unroll 1
+      for (int other = 0; other < NW - 1; ++other) {
+        const char* at = lds + ((wave - w0) * (NW - 1) + other) * PART_BYTES + lane * 16;
+#pragma unroll
+        for (int i = 0; i < SI; ++i)
+#pragma unroll
+          for (int j = 0; j < SJ; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const f32x4 v = *(const f32x4*)(at + ((i * SJ + j) * 4 + g) * 1024);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) sum[i][j][4 * g + r] += v[r];
+            }
+      }
     }
   }
-  __syncthreads();  // the ring is the epilogue's transpose buffer now
+  if (NW > 1) __syncthreads();  // the transpose buffers are where sums were
+  if (wave >= PARTS) return;
+  const int bi0 = i0 + (PARTS == 4 ? wave / 2 * SI : wave * SI), bj0 = j0 + (PARTS == 4 ? wave % 2 * SJ : 0);
 
   // lane l of a 32 x 32 block holds column l % 32, rows 8 g + 4 (l / 32) + r
   constexpr int PITCH = 80;  // bytes of a row of 32 fp16 in the transpose buffer, 16-byte aligned
   char* turn = lds + wave * (32 * PITCH);
   const int col = lane & 31, half = lane >> 5;
   const int64_t p16 = (int64_t)a.p_blocks * 2, q16 = (int64_t)a.q_blocks * 2;  // k / 16 along D^T's and D's rows
+  // all of C (and of the weights) is read before anything is stored: a load does not wait
+  // for the stores before it
 #pragma unroll
-  for (int i = 0; i < TI; ++i)
+  for (int i = 0; i < SI; ++i)
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) {
-      const int bi = i0 + wm * TI + i, bj = j0 + wn * TJ + j;
-      if (bi >= a.p_blocks || bj >= a.q_blocks) continue;
-      float v[16];
+    for (int j = 0; j < SJ; ++j) {
+      const int bi = min(bi0 + i, a.p_blocks - 1), bj = min(bj0 + j, a.q_blocks - 1);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = a.alpha * acc[i][j][r];
-      if (EPI != kGram) {
-        const char* c = a.c + b * a.batch_c;
+      for (int r = 0; r < 16; ++r) sum[i][j][r] *= a.alpha;
+      if (EPI == kGram) continue;
+      const char* c = a.c + b * a.batch_c;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int64_t at = run_at<PLANES>(bj, p16, bi * 2 + (g >> 1), 0) + (col + 32 * (g & 1)) * 16 + 8 * half;
-          const f16x4 hi = *(const f16x4*)(c + at);
-          f16x4 lo = {0, 0, 0, 0};
-          if (PLANES == 2) lo = *(const f16x4*)(c + at + kRun);
+      for (int g = 0; g < 4; ++g) {
+        const int64_t at = run_at<PLANES>(bj, p16, bi * 2 + (g >> 1), 0) + (col + 32 * (g & 1)) * 16 + 8 * half;
+        const f16x4 hi = *(const f16x4*)(c + at);
+        f16x4 lo = {0, 0, 0, 0};
+        if (PLANES == 2) lo = *(const f16x4*)(c + at + kRun);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[4 * g + r] += a.beta * ((float)hi[r] + (float)lo[r]);
-        }
+        for (int r = 0; r < 4; ++r) sum[i][j][4 * g + r] += a.beta * ((float)hi[r] + (float)lo[r]);
       }
-      if (EPI == kLast) {
-        void* w = mats.param[b];
-        const int64_t y = (int64_t)bj * 32 + col;
+    }
+  if (EPI == kLast) {
+    void* w = mats.param[b];
+    if (a.read_param) {
+#pragma unroll
+      for (int i = 0; i < SI; ++i)
+#pragma unroll
+        for (int j = 0; j < SJ; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int64_t x = (int64_t)(bi0 + i) * 32 + 8 * (r >> 2) + 4 * half + (r & 3), y = (int64_t)(bj0 + j) * 32 + col;
+            const float old = load_value(w, a.param_dtype, min(x, a.rows - 1) * a.param.row + min(y, a.cols - 1) * a.param.col);
+            sum[i][j][r] = a.keep * old - a.rate * sum[i][j][r];
+          }
+    }
+#pragma unroll
+    for (int i = 0; i < SI; ++i)
+#pragma unroll
+      for (int j = 0; j < SJ; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int64_t x = (int64_t)bi * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-          if (x < a.rows && y < a.cols) {
-            const int64_t at = x * a.param.row + y * a.param.col;
-            const float old = a.read_param ? a.keep * load_value(w, a.param_dtype, at) : 0.0f;
-            store_value(w, a.param_dtype, at, old - a.rate * v[r]);
-          }
+          const int64_t x = (int64_t)(bi0 + i) * 32 + 8 * (r >> 2) + 4 * half + (r & 3), y = (int64_t)(bj0 + j) * 32 + col;
+          if (x < a.rows && y < a.cols)
+            store_value(w, a.param_dtype, x * a.param.row + y * a.param.col,
+                        a.read_param ? sum[i][j][r] : -a.rate * sum[i][j][r]);
         }
-        continue;
-      }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < SI; ++i)
+#pragma unroll
+    for (int j = 0; j < SJ; ++j) {
+      const int bi = bi0 + i, bj = bj0 + j;
+      if (bi >= a.p_blocks || bj >= a.q_blocks) continue;
       _Float16 hi[16], lo[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) split(v[r], hi[r], lo[r]);
+      for (int r = 0; r < 16; ++r) split(sum[i][j][r], hi[r], lo[r]);
       char* out_t = a.out_t + b * a.batch_out_t;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -399,27 +487,32 @@ Layout make_layout(int64_t rows, int64_t cols, int64_t count, int planes) {
   return l;
 }
 
-template <int PLANES, int BM, int BN, int WM, int WN, Epilogue EPI>
+template <int PLANES, int T, int NW, int DEPTH, Epilogue EPI>
 int launch_product_as(const ProductArgs& args, const Matrices& mats, int count, hipStream_t stream) {
   ProductArgs a = args;
-  constexpr int AB = BM / 32, BB = BN / 32, bytes = 2 * (AB + BB) * kStepBytes;
-  static_assert(bytes >= WM * WN * 32 * 80, "the transpose buffers fit the ring");
-  const int tp = (a.p_blocks + AB - 1) / AB, tq = (a.q_blocks + BB - 1) / BB;
+  constexpr int bytes = ProductShape<T, NW>::kBytes;
+  const int tp = (a.p_blocks + T - 1) / T, tq = (a.q_blocks + T - 1) / T;
   a.tiles_q = tq;
   const int tiles = EPI == kGram || EPI == kPoly ? tq * (tq + 1) / 2 : tp * tq;
-  auto kernel = muon_product_kernel<PLANES, BM, BN, WM, WN, EPI>;
+  auto kernel = muon_product_kernel<PLANES, T, NW, DEPTH, EPI>;
   if (bytes > 65536) {
     static const hipError_t set =
         hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     EG_CHECK_HIP(set);
   }
-  kernel<<<dim3((unsigned)tiles, (unsigned)count), WM * WN * 64, bytes, stream>>>(a, mats);
+  kernel<<<dim3((unsigned)tiles, (unsigned)count), NW * 64, bytes, stream>>>(a, mats);
   return launch_status("muon_product_kernel");
 }
 
+#ifndef EG_T
+#define EG_T 4
+#define EG_NW 4
+#define EG_D1 6
+#define EG_D2 3
+#endif
 template <int PLANES, Epilogue EPI>
 int launch_product(const ProductArgs& a, const Matrices& mats, int count, hipStream_t stream) {
-  return launch_product_as<PLANES, 128, 128, 2, 2, EPI>(a, mats, count, stream);
+  return launch_product_as<PLANES, EG_T, EG_NW, PLANES == 2 ? EG_D2 : EG_D1, EPI>(a, mats, count, stream);
 }
 
 // Powers of two by which X, A and B of an iteration are kept, from the bound of X's
@@ -469,7 +562,7 @@ int run_muon(const eg_muon* o, int first, int count, const Layout& l, char* ws, 
   char* gram = x + 3 * count * l.x;
   char* poly = gram + count * l.a;
   const int m32 = (int)(l.m / 32), n32 = (int)(l.n / 32);
-  const int m_steps = (int)(l.m * PLANES / 64), n_steps = (int)(l.n * PLANES / 64);
+  const int m16 = (int)(l.m / 16), n16 = (int)(l.n / 16);
   Bounds bd = bounds_of(1.0, o->coefficients);
 
   PlanesArgs pa;
@@ -497,7 +590,7 @@ int run_muon(const eg_muon* o, int first, int count, const Layout& l, char* ws, 
     a.p = a.q = x;
     a.batch_p = a.batch_q = l.x;
     a.p_blocks = a.q_blocks = m32;
-    a.steps = n_steps;
+    a.k16 = n16;
     a.out_t = a.out = gram;
     a.batch_out_t = a.batch_out = l.a;
     a.alpha = ldexpf(1.0f, bd.gram - 2 * bd.x);
@@ -505,7 +598,7 @@ int run_muon(const eg_muon* o, int first, int count, const Layout& l, char* ws, 
     // B = b A + c A A
     a.p = a.q = a.c = gram;
     a.batch_p = a.batch_q = a.batch_c = l.a;
-    a.steps = m_steps;
+    a.k16 = m16;
     a.out_t = a.out = poly;
     a.alpha = ldexpf(k[2], bd.poly - 2 * bd.gram);
     a.beta = ldexpf(k[1], bd.poly - bd.gram);
