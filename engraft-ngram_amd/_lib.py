@@ -361,6 +361,9 @@ def autograd_ext():
     lib = load()
     mod.init(*(ctypes.cast(getattr(lib, f), c_void_p).value
                for f in ("eg_gather_slots", "eg_scatter_grad_apply", "eg_last_error")))
+    mod.init_ops({f: ctypes.cast(getattr(lib, f), c_void_p).value
+                  for f in ("eg_loss_workspace_size", "eg_token_logprobs", "eg_policy_loss", "eg_preference_loss",
+                            "eg_logits_grad", "eg_muon_workspace_size", "eg_muon_step", "eg_last_error")}, EgError)
     _EXT = mod
     return mod
 

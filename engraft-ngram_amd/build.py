@@ -4,8 +4,9 @@ it the host-only C++ autograd module ``_eg_autograd.so``.
 ``python engraft-ngram_amd/build.py`` or ``build()``: one ``hipcc`` invocation
 over every ``csrc/*.hip`` file.  The packed-fp32 target feature is switched off
 for all device code (``-Xclang -target-feature -Xclang -packed-fp32-ops``):
-hipcc then never emits v_pk_{add,mul,fma}_f32.  ``csrc/eg_autograd.cpp`` is
-compiled by ``g++`` against torch's headers and libraries at the same time.
+hipcc then never emits v_pk_{add,mul,fma}_f32.  ``csrc/eg_autograd.cpp`` and
+``csrc/eg_torch_ops.cpp`` are compiled by ``g++`` against torch's headers and
+libraries at the same time.
 """
 from __future__ import annotations
 
@@ -33,11 +34,11 @@ def hipcc() -> str:
 
 
 EXT_PATH = PKG / "_eg_autograd.so"
-EXT_SOURCE = PKG / "csrc" / "eg_autograd.cpp"
+EXT_SOURCES = [PKG / "csrc" / "eg_autograd.cpp", PKG / "csrc" / "eg_torch_ops.cpp"]
 
 
 def ext_command(out: Path) -> list[str]:
-    """g++ over ``csrc/eg_autograd.cpp``: a CPython module linked to torch."""
+    """g++ over the host sources: a CPython module linked to torch."""
     import sysconfig
 
     from torch.utils import cpp_extension
@@ -49,7 +50,7 @@ def ext_command(out: Path) -> list[str]:
            "-DTORCH_EXTENSION_NAME=_eg_autograd"]
     for inc in [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(ROOT / "include")]:
         cmd += ["-I", inc]
-    cmd += ["-o", str(out), str(EXT_SOURCE)]
+    cmd += ["-o", str(out), *map(str, EXT_SOURCES)]
     for lib_dir in cpp_extension.library_paths():
         cmd += ["-L", lib_dir, f"-Wl,-rpath,{lib_dir}"]
     return cmd + ["-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]

@@ -108,7 +108,10 @@ void init(int64_t gather, int64_t scatter, int64_t error) {
 
 }  // namespace
 
+void bind_ops(pybind11::module_& m);  // eg_torch_ops.cpp
+
 PYBIND11_MODULE(_eg_autograd, m) {
+  bind_ops(m);
   m.def("init", &init, "the library's eg_gather_slots, eg_scatter_grad_apply and eg_last_error addresses");
   m.def("gather_slots", &gather_slots, "OverlayEmb's differentiable gather (see the file's header)");
 }

@@ -462,6 +462,250 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void muon_product_kernel(const Pro
     }
 }
 
+// ---- a matrix in one workgroup's LDS ------------------------------------------------------------
+
+constexpr int kSmallWaves = 16;
+constexpr int kSmallSteps = 32;
+constexpr int kSmallBytes = 160 * 1024;
+
+// A step's factors: A = gram D; B = poly D + poly_c A; X = step D + step_c X.
+struct Factors {
+  float gram, poly, poly_c, step, step_c;
+};
+
+struct SmallArgs {
+  UpdateArgs u;
+  float eps, scale;
+  int pr, pc;                  // rows and columns padded to 64
+  int steps;
+  Strides param;
+  int param_dtype, read_param;
+  float keep, rate;
+  Factors f[kSmallSteps];
+};
+
+// Sum over k of a block's product, its operands in LDS: 32 rows of P (row block bp) by 32 of Q.
+// TURNED adds the cross products in the other order: the transposed block's very sums.
+template <int PLANES, bool TURNED>
+__device__ inline f32x16 block_product(const char* p, int bp, const char* q, int bq, int k16s, int lane) {
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+  const char* pa = p + run_at<PLANES>(bp, k16s, 0, 0) + lane * 16;
+  const char* qa = q + run_at<PLANES>(bq, k16s, 0, 0) + lane * 16;
+  for (int k0 = 0; k0 < k16s; k0 += 4)  // K is padded to 64
+#pragma unroll
+    for (int k = k0; k < k0 + 4; ++k) {
+      const f16x8 ph = *(const f16x8*)(pa + k * PLANES * kRun), qh = *(const f16x8*)(qa + k * PLANES * kRun);
+      if (PLANES == 2) {
+        const f16x8 pl = *(const f16x8*)(pa + (k * 2 + 1) * kRun), ql = *(const f16x8*)(qa + (k * 2 + 1) * kRun);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(TURNED ? ph : pl, TURNED ? ql : qh, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(TURNED ? pl : ph, TURNED ? qh : ql, acc, 0, 0, 0);
+      }
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+    }
+  return acc;
+}
+
+// A block's planes as its transpose's fragments hold them: 4 x 4 values a lane.
+template <int PLANES>
+struct BlockPlanes {
+  f16x4 v[PLANES][4];
+};
+
+// alpha acc + beta C, C's transpose by rows at c (row block bq, k block bp).
+template <int PLANES>
+__device__ inline void add_c(f32x16& acc, float alpha, float beta, const char* c, int bp, int bq, int k16s, int lane) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const char* at = c + run_at<PLANES>(bq, k16s, bp * 2 + (g >> 1), 0) + ((lane & 31) + 32 * (g & 1)) * 16 + 8 * (lane >> 5);
+    const f16x4 hi = *(const f16x4*)at;
+    f16x4 lo = {0, 0, 0, 0};
+    if (PLANES == 2) lo = *(const f16x4*)(at + kRun);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[4 * g + r] = alpha * acc[4 * g + r] + beta * ((float)hi[r] + (float)lo[r]);
+  }
+}
+
+template <int PLANES>
+__device__ inline BlockPlanes<PLANES> planes_of(const f32x16& v) {
+  BlockPlanes<PLANES> o;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      _Float16 hi, lo;
+      split(v[4 * g + r], hi, lo);
+      o.v[0][g][r] = hi;
+      if (PLANES == 2) o.v[PLANES - 1][g][r] = lo;
+    }
+  return o;
+}
+
+// Into the transpose's rows at `to` (row block bq, k block bp).
+template <int PLANES>
+__device__ inline void store_planes(char* to, const BlockPlanes<PLANES>& o, int bp, int bq, int k16s, int lane) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    char* at = to + run_at<PLANES>(bq, k16s, bp * 2 + (g >> 1), 0) + ((lane & 31) + 32 * (g & 1)) * 16 + 8 * (lane >> 5);
+#pragma unroll
+    for (int x = 0; x < PLANES; ++x) *(f16x4*)(at + x * kRun) = o.v[x][g];
+  }
+}
+
+// Grid (matrices): the whole step of one matrix.  X, X^T, A and B stay in LDS as fragments; every
+// block of a product is one wavefront's, X's and X^T's blocks both computed (B X and X^T B) rather
+// than turned.  The two have to be the same values to the last bit, hence TURNED: a
+// difference between X and X^T is not damped as X's own errors are, it grows by a step's a.
+template <int PLANES>
+__global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const SmallArgs a, const Matrices mats) {
+  constexpr int MAX_ELEMENTS = kSmallBytes / (4 * PLANES);       // of X, both orders
+  constexpr int UNITS = (MAX_ELEMENTS / 512 + kSmallWaves - 1) / kSmallWaves;  // 8 x 64 elements
+  constexpr int BLOCKS = (2 * MAX_ELEMENTS / 1024 + kSmallWaves - 1) / kSmallWaves;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, b = blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool tall = a.u.rows > a.u.cols;
+  const int m = tall ? a.pc : a.pr, n = tall ? a.pr : a.pc, m16 = m / 16, n16 = n / 16, mb = m / 32, nb = n / 32;
+  char* x = lds;                                // X by rows: m x n
+  char* xt = x + m * n * 2 * PLANES;            // X^T by rows
+  char* gram = xt + m * n * 2 * PLANES;
+  char* poly = gram + m * m * 2 * PLANES;
+  float* red = (float*)gram;
+
+  // momentum; a thread has 8 rows of a column in each of its units
+  const void* grad = mats.grad[b];
+  float* mom = mats.momentum[b];
+  const int chunks = a.pc / 64, units = a.pr / 8 * chunks;
+  float u[UNITS][8], sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int unit = wave + i * kSmallWaves;
+    if (unit >= units) break;
+    const int r0 = unit / chunks * 8, c = unit % chunks * 64 + lane;
+    float g[8], old[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const bool in = r0 + r < a.u.rows && c < a.u.cols;
+      g[r] = in ? load_value(grad, a.u.grad_dtype, (r0 + r) * a.u.grad.row + c * a.u.grad.col) : 0.0f;
+      old[r] = in && a.u.has_momentum ? mom[(r0 + r) * a.u.momentum.row + c * a.u.momentum.col] : 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float now = a.u.mu * old[r] + g[r];
+      if (a.u.has_momentum && r0 + r < a.u.rows && c < a.u.cols)
+        mom[(r0 + r) * a.u.momentum.row + c * a.u.momentum.col] = now;
+      u[i][r] = update_of(a.u, g[r], now);
+      sum += u[i][r] * u[i][r];
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) red[wave] = sum;
+  __syncthreads();
+  float total = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kSmallWaves; ++w) total += red[w];
+  const float s = a.scale / (sqrtf(total) + a.eps);
+  char* by_row = tall ? xt : x;
+  char* by_col = tall ? x : xt;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int unit = wave + i * kSmallWaves;
+    if (unit >= units) break;
+    const int r0 = unit / chunks * 8, c = unit % chunks * 64 + lane;
+    f16x8 hi, lo;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      _Float16 h, l;
+      split(u[i][r] * s, h, l);
+      hi[r] = h;
+      lo[r] = l;
+      char* at = by_row + run_at<PLANES>((r0 + r) / 32, a.pc / 16, c / 16, 0) + ((r0 + r) % 32 + 32 * (c % 16 / 8)) * 16 + c % 8 * 2;
+      *(_Float16*)at = h;
+      if (PLANES == 2) *(_Float16*)(at + kRun) = l;
+    }
+    char* at = by_col + run_at<PLANES>(c / 32, a.pr / 16, r0 / 16, 0) + (c % 32 + 32 * (r0 % 16 / 8)) * 16;
+    *(f16x8*)at = hi;
+    if (PLANES == 2) *(f16x8*)(at + kRun) = lo;
+  }
+  __syncthreads();
+
+  for (int step = 0; step < a.steps; ++step) {
+    const Factors f = a.f[step];
+    for (int k = wave; k < mb * mb; k += kSmallWaves) {  // A = X X^T
+      f32x16 acc = block_product<PLANES, false>(x, k / mb, x, k % mb, n16, lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] *= f.gram;
+      store_planes<PLANES>(gram, planes_of<PLANES>(acc), k / mb, k % mb, m16, lane);
+    }
+    __syncthreads();
+    for (int k = wave; k < mb * mb; k += kSmallWaves) {  // B = b A + c A A
+      f32x16 acc = block_product<PLANES, false>(gram, k / mb, gram, k % mb, m16, lane);
+      add_c<PLANES>(acc, f.poly, f.poly_c, gram, k / mb, k % mb, m16, lane);
+      store_planes<PLANES>(poly, planes_of<PLANES>(acc), k / mb, k % mb, m16, lane);
+    }
+    __syncthreads();
+    if (step + 1 == a.steps) break;
+    // X = a X + B X, and its transpose: blocks [0, mb nb) are X's, whose transpose goes to xt
+    BlockPlanes<PLANES> out[BLOCKS];
+    const int all = 2 * mb * nb;
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+      const int k = wave + i * kSmallWaves;
+      if (k >= all) break;
+      const bool turned = k >= mb * nb;
+      const int e = turned ? k - mb * nb : k, bm = e / nb, bn = e % nb;
+      f32x16 acc = turned ? block_product<PLANES, true>(xt, bn, poly, bm, m16, lane)
+                          : block_product<PLANES, false>(poly, bm, xt, bn, m16, lane);
+      if (turned)
+        add_c<PLANES>(acc, f.step, f.step_c, x, bn, bm, n16, lane);
+      else
+        add_c<PLANES>(acc, f.step, f.step_c, xt, bm, bn, m16, lane);
+      out[i] = planes_of<PLANES>(acc);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+      const int k = wave + i * kSmallWaves;
+      if (k >= all) break;
+      const bool turned = k >= mb * nb;
+      const int e = turned ? k - mb * nb : k, bm = e / nb, bn = e % nb;
+      if (turned)
+        store_planes<PLANES>(x, out[i], bn, bm, n16, lane);
+      else
+        store_planes<PLANES>(xt, out[i], bm, bn, m16, lane);
+    }
+    __syncthreads();
+  }
+
+  // the last step's X goes to the weights, in the order whose lanes run along their rows
+  const Factors f = a.f[a.steps - 1];
+  void* w = mats.param[b];
+  for (int k = wave; k < mb * nb; k += kSmallWaves) {
+    const int bm = k / nb, bn = k % nb;
+    f32x16 acc = tall ? block_product<PLANES, true>(xt, bn, poly, bm, m16, lane) : block_product<PLANES, false>(poly, bm, xt, bn, m16, lane);
+    if (tall)
+      add_c<PLANES>(acc, f.step, f.step_c, x, bn, bm, n16, lane);
+    else
+      add_c<PLANES>(acc, f.step, f.step_c, xt, bm, bn, m16, lane);
+    const int r0 = (tall ? bn : bm) * 32 + 4 * (lane >> 5), c = (tall ? bm : bn) * 32 + (lane & 31);
+    float old[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = r0 + 8 * (r >> 2) + (r & 3);
+      old[r] = a.read_param && row < a.u.rows && c < a.u.cols
+                   ? a.keep * load_value(w, a.param_dtype, row * a.param.row + c * a.param.col) : 0.0f;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = r0 + 8 * (r >> 2) + (r & 3);
+      if (row < a.u.rows && c < a.u.cols)
+        store_value(w, a.param_dtype, row * a.param.row + c * a.param.col, old[r] - a.rate * acc[r]);
+    }
+  }
+}
+
 // ---- host side --------------------------------------------------------------------------------
 
 int64_t pad64(int64_t x) { return (x + 63) / 64 * 64; }
@@ -524,27 +768,73 @@ struct Bounds {
 
 int exponent_for(double bound) { return (int)floor(log2(60000.0 / std::max(bound, 1e-30))); }
 
-// max over [0, s] of |f|, on a grid fine against a cubic's curvature there, with a margin.
-template <typename F>
-double largest(double s, F&& f) {
-  double top = 0.0;
-  for (int i = 0; i <= 4096; ++i) top = std::max(top, fabs(f(s * i / 4096.0)));
-  return top * 1.01;
-}
+constexpr double kMargin = 1.01;  // over what the bounds ignore: fp32 and fp16 roundings
 
 Bounds bounds_of(double sigma, const float* k) {
-  const double a = k[0], b = k[1], c = k[2], s2 = sigma * sigma;
-  Bounds r;
-  r.sigma = sigma;
-  r.x = exponent_for(sigma);
-  r.gram = exponent_for(s2);
-  r.poly = exponent_for(largest(s2, [&](double y) { return b * y + c * y * y; }));
-  (void)a;
-  return r;
+  const double b = k[1], c = k[2], s2 = sigma * sigma;
+  // |b y + c y^2| over [0, s2]: at the end, or where the slope b + 2 c y is zero
+  double top = fabs(b * s2 + c * s2 * s2);
+  const double y = c != 0.0 ? -b / (2.0 * c) : 0.0;
+  if (y > 0.0 && y < s2) top = std::max(top, fabs(b * y + c * y * y));
+  return {sigma, exponent_for(sigma), exponent_for(s2), exponent_for(kMargin * top)};
 }
 
+// The largest |a s + b s^3 + c s^5| over [0, sigma]: at the end, or where the slope, a quadratic
+// a + 3 b y + 5 c y^2 of y = s^2, is zero.
 double next_sigma(double sigma, const float* k) {
-  return largest(sigma, [&](double s) { const double y = s * s; return s * (k[0] + k[1] * y + k[2] * y * y); });
+  const double a = k[0], b = k[1], c = k[2], s2 = sigma * sigma;
+  double top = 0.0;
+  auto at = [&](double y) {
+    if (y > 0.0 && y <= s2) top = std::max(top, fabs(sqrt(y) * (a + y * (b + y * c))));
+  };
+  at(s2);
+  if (c != 0.0) {
+    const double d = 9.0 * b * b - 20.0 * a * c;
+    if (d >= 0.0) {
+      at((-3.0 * b + sqrt(d)) / (10.0 * c));
+      at((-3.0 * b - sqrt(d)) / (10.0 * c));
+    }
+  } else if (b != 0.0) {
+    at(-a / (3.0 * b));
+  }
+  return kMargin * top;
+}
+
+// Bytes of LDS that X, X^T, A and B take.
+int64_t small_bytes(const Layout& l) { return 2 * (l.x + l.a); }
+
+template <int PLANES>
+int run_small(const eg_muon* o, const Matrices& mats, int count, const Layout& l, const UpdateArgs& u,
+              hipStream_t stream) {
+  SmallArgs a;
+  a.u = u;
+  a.eps = o->eps;
+  a.pr = (int)pad64(o->rows);
+  a.pc = (int)pad64(o->cols);
+  a.steps = o->steps;
+  a.param = {o->param_stride[0], o->param_stride[1]};
+  a.param_dtype = o->param_dtype;
+  a.read_param = o->keep != 0.0f;
+  a.keep = o->keep;
+  a.rate = o->rate;
+  Bounds bd = bounds_of(1.0, o->coefficients);
+  a.scale = ldexpf(1.0f, bd.x);
+  for (int s = 0; s < o->steps; ++s) {
+    const float* k = o->coefficients + 3 * s;
+    const bool last = s + 1 == o->steps;
+    const Bounds nx = last ? bd : bounds_of(next_sigma(bd.sigma, k), k + 3);
+    const int x = last ? 0 : nx.x;  // the last X is itself
+    a.f[s] = {ldexpf(1.0f, bd.gram - 2 * bd.x), ldexpf(k[2], bd.poly - 2 * bd.gram), ldexpf(k[1], bd.poly - bd.gram),
+              ldexpf(1.0f, x - bd.poly - bd.x), ldexpf(k[0], x - bd.x)};
+    bd = nx;
+  }
+  const int bytes = (int)small_bytes(l);
+  auto kernel = muon_small_kernel<PLANES>;
+  static const hipError_t set =
+      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kSmallBytes);
+  EG_CHECK_HIP(set);
+  kernel<<<dim3((unsigned)count), kSmallWaves * 64, bytes, stream>>>(a, mats);
+  return launch_status("muon_small_kernel");
 }
 
 template <int PLANES>
@@ -555,6 +845,11 @@ int run_muon(const eg_muon* o, int first, int count, const Layout& l, char* ws, 
     mats.grad[i] = o->grads[first + i];
     mats.momentum[i] = o->momenta != nullptr ? o->momenta[first + i] : nullptr;
   }
+  const UpdateArgs update = {o->rows, o->cols, {o->grad_stride[0], o->grad_stride[1]},
+                             {o->momentum_stride[0], o->momentum_stride[1]}, o->grad_dtype, o->momenta != nullptr,
+                             o->nesterov, o->momentum, (int)(pad64(o->cols) / 64), (int)l.tiles, (float*)ws};
+  if (small_bytes(l) <= kSmallBytes && o->steps <= kSmallSteps)
+    return run_small<PLANES>(o, mats, count, l, update, stream);
   const bool tall = o->rows > o->cols;
   char* base = ws + l.partials;
   char* x = base;
@@ -566,9 +861,7 @@ int run_muon(const eg_muon* o, int first, int count, const Layout& l, char* ws, 
   Bounds bd = bounds_of(1.0, o->coefficients);
 
   PlanesArgs pa;
-  pa.u = {o->rows, o->cols, {o->grad_stride[0], o->grad_stride[1]}, {o->momentum_stride[0], o->momentum_stride[1]},
-          o->grad_dtype, o->momenta != nullptr, o->nesterov, o->momentum, (int)(pad64(o->cols) / 64), (int)l.tiles,
-          (float*)ws};
+  pa.u = update;
   pa.eps = o->eps;
   pa.scale = ldexpf(1.0f, bd.x);
   pa.by_row = tall ? xt[0] : x;

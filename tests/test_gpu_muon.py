@@ -11,6 +11,7 @@ result)."""
 from __future__ import annotations
 
 import math
+import types
 
 import pytest
 import torch
@@ -217,3 +218,29 @@ def test_python_arguments_are_checked_on_the_gpu(cuda):
     before = w.clone()
     muon.muon_step([w[:0]], [w[:0]], [m[:0]], lr=0.1)  # nothing to do
     assert torch.equal(w, before)
+
+
+def test_block_sees_the_step(cuda):
+    """ple_forward keeps planes of its weights between calls: after a step of the weights (w_key as one matrix a
+    stream, a view) it computes with the new ones, and autograd refuses a graph that saved the old."""
+    from engraft_ngram_amd import muon, ple
+    n, hc, t = 64, 4, 40
+    w = ple.PleWeights(w_key=random((hc * n, n), torch.float32, 1, 0.1), w_value=random((n, n), torch.float32, 2, 0.1),
+                       norm_key=torch.ones(hc * n, device=cuda), norm_query=torch.ones(hc * n, device=cuda),
+                       norm_conv=torch.ones(hc * n, device=cuda), conv1d=random((hc * n, 4), torch.float32, 3, 0.1))
+    w.w_key.requires_grad_()
+    w.w_value.requires_grad_()
+    emb, hidden = random((t, n), torch.float32, 4), random((t, hc, n), torch.float32, 5)
+    hist = torch.zeros((9, hc, n), device=cuda)
+
+    hp = types.SimpleNamespace(hc_mult=hc, n_embd=n, f_norm_rms_eps=1e-6, ple_ngram_size=3)
+    before = ple.ple_forward(emb, hidden, w, hist, hp)[0]
+    grads = torch.autograd.grad(before.square().sum(), [w.w_key, w.w_value], retain_graph=True)
+    state = muon.MuonState([w.w_key.view(hc, n, n), w.w_value])
+    state.step([grads[0].view(hc, n, n), grads[1]], lr=0.1)
+    after = ple.ple_forward(emb, hidden, w, hist, hp)[0]
+    fresh = ple.PleWeights(w.w_key.detach().clone(), w.w_value.detach().clone(), w.norm_key, w.norm_query, w.norm_conv,
+                           w.conv1d)
+    assert torch.equal(after, ple.ple_forward(emb, hidden, fresh, hist, hp)[0]) and not torch.equal(after, before)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        before.square().sum().backward()
