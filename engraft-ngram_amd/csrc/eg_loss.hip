@@ -214,33 +214,25 @@ struct RowState {
   float g, m, inv_s;
 };
 
-// Grid (parts, rows): a part of a row's gradient; scale holds 1 / temperature.
+// Elements [e0, e1) of a row that is left out.
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void logits_grad_kernel(const Rows r, int parts, int part_len,
-                                                              const RowState* state, const float* upstream,
-                                                              float scale, T* d, int64_t d_stride) {
-  constexpr int VEC = Logit<T>::kVec, K = 4;
-  const int64_t i = r.n - 1 - (blockIdx.y + (int64_t)gridDim.y * blockIdx.z);  // the rows read last first
-  if (i < 0) return;
-  int e0, e1;
-  part_range(r.v, parts, part_len, (int)blockIdx.x, e0, e1);
-  const int64_t t = target_of(r, i);
-  T* out = d + i * d_stride;
-  const T* row = (const T*)r.z + i * r.stride;
+__device__ inline void write_zeros(T* out, int e0, int e1) {
+  constexpr int VEC = Logit<T>::kVec;
   int e = e0 + (int)threadIdx.x * VEC;
-  if (t < 0) {
-    const Chunk zero = {{0, 0, 0, 0}};
-    for (; e + VEC <= e1; e += THREADS * VEC) *(Chunk*)(out + e) = zero;
-    for (; e < e1; ++e) out[e] = (T)0.0f;
-    return;
-  }
-  // the target's element is this thread's: read before anything is written (d may be the logits)
-  const bool owner = t >= e0 && t < e1 && (int)((t - e0) / VEC) % THREADS == (int)threadIdx.x;
-  const float f_t = owner ? (float)row[t] : 0.0f;
-  const RowState st = state[i];
-  const float g = st.g * (upstream != nullptr ? scale * *upstream : scale);
-  const float k = -g * st.inv_s, c = r.c, m = st.m;
+  const Chunk zero = {{0, 0, 0, 0}};
+  for (; e + VEC <= e1; e += THREADS * VEC) *(Chunk*)(out + e) = zero;
+  for (; e < e1; ++e) out[e] = (T)0.0f;
+}
+
+// Elements [e0, e1) of g ([j == t] - 2^(c (z_j - m)) inv_s); f_t is z_t, read before anything
+// is written (out may be the row itself).
+template <typename T, int THREADS>
+__device__ inline void write_gradient(const T* row, T* out, int e0, int e1, int64_t t, float f_t, float g, float m,
+                                      float inv_s, float c) {
+  constexpr int VEC = Logit<T>::kVec, K = 4;
+  const float k = -g * inv_s;
   auto value = [&](float f) { return k * pow2((f - m) * c); };
+  int e = e0 + (int)threadIdx.x * VEC;
   for (; e + (K - 1) * THREADS * VEC + VEC <= e1; e += K * THREADS * VEC) {
     Chunk q[K];
 #pragma unroll
@@ -262,13 +254,38 @@ __global__ __launch_bounds__(THREADS) void logits_grad_kernel(const Rows r, int 
     *(Chunk*)(out + e) = Logit<T>::pack(f);
   }
   for (; e < e1; ++e) out[e] = (T)value((float)row[e]);
-  if (owner) out[t] = (T)(g + value(f_t));  // again, by the thread that wrote it
+  // the target's element again, by the thread that wrote it
+  if (t >= e0 && t < e1 && (int)((t - e0) / VEC) % THREADS == (int)threadIdx.x) out[t] = (T)(g + value(f_t));
+}
+
+// Grid (parts, rows): a part of a row's gradient; scale holds 1 / temperature.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void logits_grad_kernel(const Rows r, int parts, int part_len,
+                                                              const RowState* state, const float* upstream,
+                                                              float scale, T* d, int64_t d_stride) {
+  const int64_t i = r.n - 1 - (blockIdx.y + (int64_t)gridDim.y * blockIdx.z);  // the rows read last first
+  if (i < 0) return;
+  int e0, e1;
+  part_range(r.v, parts, part_len, (int)blockIdx.x, e0, e1);
+  const int64_t t = target_of(r, i);
+  T* out = d + i * d_stride;
+  if (t < 0) {
+    write_zeros<T, THREADS>(out, e0, e1);
+    return;
+  }
+  const T* row = (const T*)r.z + i * r.stride;
+  const float f_t = t >= e0 && t < e1 ? (float)row[t] : 0.0f;
+  const RowState st = state[i];
+  const float g = st.g * (upstream != nullptr ? scale * *upstream : scale);
+  if (row == out) __syncthreads();  // everyone has read f_t
+  write_gradient<T, THREADS>(row, out, e0, e1, t, f_t, g, st.m, st.inv_s, r.c);
 }
 
 // ---- one workgroup over all rows ------------------------------------------------------------
 
 constexpr int kFinish = 1024;
 
+template <int THREADS>
 __device__ inline double block_sum64(double x, double* red) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
@@ -276,7 +293,7 @@ __device__ inline double block_sum64(double x, double* red) {
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
   __syncthreads();
   double t = 0.0;
-  for (int w = 0; w < kFinish / 64; ++w) t += red[w];
+  for (int w = 0; w < THREADS / 64; ++w) t += red[w];
   return t;
 }
 
@@ -289,11 +306,14 @@ __device__ inline Stat row_stat(const Stat* stats, int64_t i, int parts, float c
 
 // In 64 bits, for a row's terms: a loss is a sum of terms that nearly cancel, and an
 // fp32 lp's rounding (half a unit in the last place, 2^-21 at -10) would be most of its error.
+__device__ inline double logprob_of(const Rows& r, float z_below_m, float s) {
+  return (double)z_below_m * r.inv_temp - log((double)s);
+}
+
+// z_t - M, NaN for a target beyond the vocabulary.
 template <typename T>
-__device__ inline double row_logprob(const Rows& r, int64_t i, int64_t t, const Stat& st) {
-  if (t >= r.v) return __builtin_nan("");
-  const float f = (float)((const T*)r.z)[i * r.stride + t];
-  return (double)(f - st.m) * r.inv_temp - log((double)st.s);
+__device__ inline float z_below_m(const Rows& r, int64_t i, int64_t t, float m) {
+  return t < r.v ? (float)((const T*)r.z)[i * r.stride + t] - m : __builtin_nanf("");
 }
 
 template <typename T>
@@ -301,7 +321,12 @@ __global__ __launch_bounds__(256) void logprobs_finish(const Rows r, int parts, 
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= r.n) return;
   const int64_t t = target_of(r, i);
-  lp[i] = t < 0 ? 0.0f : (float)row_logprob<T>(r, i, t, row_stat(stats, i, parts, r.c));
+  float x = 0.0f;
+  if (t >= 0) {
+    const Stat st = row_stat(stats, i, parts, r.c);
+    x = (float)logprob_of(r, z_below_m<T>(r, i, t, st.m), st.s);
+  }
+  lp[i] = x;
 }
 
 // Segment of a row: a value outside [0, n) for none.
@@ -325,92 +350,204 @@ struct Policy {
 };
 
 struct PolicyTerms {
-  double loss, kl, clipped, g;
+  double loss, kl, clipped;
 };
 
-// A row's loss, KL and clip terms, and dL / d lp, all unweighted.
+// A row's loss, KL and clip terms, unweighted.
 __device__ inline PolicyTerms policy_terms(const Policy& p, int64_t i, double lp) {
   const double a = (double)p.advantages[i];
   const double ratio = p.old_lp != nullptr ? exp(lp - (double)p.old_lp[i]) : (lp == lp ? 1.0 : lp);
   const double lo = 1.0 - (double)p.clip_low, hi = 1.0 + (double)p.clip_high;
   const double held_ratio = ratio < lo ? lo : ratio > hi ? hi : ratio;  // NaN stays
   const double free = ratio * a, held = held_ratio * a;
-  const bool active = free <= held;
-  PolicyTerms t = {active ? -free : -held, 0.0, free > held ? 1.0 : 0.0, active || free != free ? -free : 0.0};
+  PolicyTerms t = {free <= held ? -free : -held, 0.0, free > held ? 1.0 : 0.0};
   if (p.ref_lp != nullptr) {
-    const double diff = (double)p.ref_lp[i] - lp, up = expm1(diff);
-    t.kl = up - diff;
+    const double diff = (double)p.ref_lp[i] - lp;
+    t.kl = expm1(diff) - diff;
     t.loss += (double)p.kl_coef * t.kl;
-    t.g -= (double)p.kl_coef * up;
   }
   return t;
 }
 
-// One workgroup: the rows' weights, lp, terms and state; sums[3] = loss, KL, clipped share.
-// counts: [segments] scratch where the reduction is by segment.
-template <typename T>
-__global__ __launch_bounds__(kFinish) void policy_finish(const Rows r, const Policy p, int parts, const Stat* stats,
-                                                         int* counts, float* lp_out, RowState* state, float* sums) {
-  __shared__ double red[kFinish / 64];
+// dL / d lp of a row of weight w.  The differences of log-probabilities are taken in 64 bits
+// (ln S from fp32's, corrected once: S e^-y - 1), their exponentials in fp32: every thread
+// of a workgroup computes it, in a few dozen operations.
+__device__ inline float policy_g(const Policy& p, int64_t i, float z_below_m, const Rows& r, float s, float w) {
+  const float y = logf(s);
+  const double lp = (double)z_below_m * r.inv_temp - ((double)y + (double)fmaf(s, expf(-y), -1.0f));
+  const float a = p.advantages[i];
+  const float ratio = p.old_lp != nullptr ? expf((float)(lp - (double)p.old_lp[i])) : (lp == lp ? 1.0f : (float)lp);
+  const float lo = 1.0f - p.clip_low, hi = 1.0f + p.clip_high;
+  const float held_ratio = ratio < lo ? lo : ratio > hi ? hi : ratio;
+  const float free = ratio * a, held = held_ratio * a;
+  float g = free > held ? 0.0f : -free;  // NaN stays
+  if (p.ref_lp != nullptr) g -= p.kl_coef * expm1f((float)((double)p.ref_lp[i] - lp));
+  return w * g;
+}
+
+// One workgroup of kFinish threads: the weight of a row with a target, weights[segment] by
+// segment, otherwise weights[0].  Counts are kept in the same place.
+__device__ inline void policy_weights(const Rows& r, const Policy& p, float* weights) {
   __shared__ int total;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  int* counts = (int*)weights;
+  const bool by_segment = p.reduction == EG_REDUCE_SEQUENCE;
   if (tid == 0) total = 0;
-  double w_all = 1.0;  // a row's weight where it is the same for all; by segment the share of a segment
-  if (p.reduction == EG_REDUCE_SEQUENCE) {
+  if (by_segment)
     for (int64_t s = tid; s < p.seg.n; s += kFinish) counts[s] = 0;
-    __syncthreads();
+  __syncthreads();
+  int some = 0;
+  if (p.reduction == EG_REDUCE_TOKEN)
+#pragma unroll 4
+    for (int64_t i = tid; i < r.n; i += kFinish) some += target_of(r, i) >= 0;
+  if (by_segment)
     for (int64_t i = tid; i < r.n; i += kFinish) {
+      const bool in = target_of(r, i) >= 0;
       const int64_t s = segment_of(p.seg, i);
-      if (s >= 0 && s < p.seg.n && target_of(r, i) >= 0) atomicAdd(counts + s, 1);
+      // one addition for the rows of a wavefront that share a segment
+      uint64_t left = __ballot(in && s >= 0 && s < p.seg.n);
+      while (left != 0) {
+        const int64_t one = __shfl(s, __ffsll((unsigned long long)left) - 1);
+        const uint64_t same = __ballot(s == one) & left;
+        if (lane == __ffsll((unsigned long long)same) - 1) atomicAdd(counts + one, __popcll(same));
+        left &= ~same;
+      }
     }
-    __syncthreads();
-    int some = 0;
-    for (int64_t s = tid; s < p.seg.n; s += kFinish) some += counts[s] > 0;
-    atomicAdd(&total, some);
-    __syncthreads();
-    w_all = 1.0 / (double)max(total, 1);
+  __syncthreads();
+  if (by_segment)
+    for (int64_t s = tid; s < p.seg.n; s += kFinish) some += __hip_atomic_load(counts + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) > 0;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) some += __shfl_xor(some, o);
+  if (lane == 0) atomicAdd(&total, some);
+  __syncthreads();
+  const double all = p.reduction == EG_REDUCE_SUM ? 1.0 : 1.0 / (double)max(total, 1);
+  if (!by_segment) {
+    if (tid == 0) weights[0] = (float)all;
   } else {
-    __syncthreads();
-    if (p.reduction == EG_REDUCE_TOKEN) {
-      int some = 0;
-      for (int64_t i = tid; i < r.n; i += kFinish) some += target_of(r, i) >= 0;
-      atomicAdd(&total, some);
-      __syncthreads();
-      w_all = 1.0 / (double)max(total, 1);
+    for (int64_t s = tid; s < p.seg.n; s += kFinish) {
+      const int c = __hip_atomic_load(counts + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      weights[s] = (float)(all / (double)max(c, 1));
     }
   }
-  double loss = 0.0, kl = 0.0, clipped = 0.0;
-  for (int64_t i = tid; i < r.n; i += kFinish) {
+}
+
+__device__ inline float weight_of(const Policy& p, int64_t i, const float* weights) {
+  if (p.reduction != EG_REDUCE_SEQUENCE) return weights[0];
+  const int64_t s = segment_of(p.seg, i);
+  return s >= 0 && s < p.seg.n ? weights[s] : 0.0f;
+}
+
+// The rows from tid on, THREADS apart within [i0, i1): lp, state and the thread's sums.  DONE: the
+// gradient is written (perhaps over the logits), z_t - M is in the place of the state's g.
+template <typename T, int THREADS, bool DONE>
+__device__ inline void policy_rows(const Rows& r, const Policy& p, int64_t i0, int64_t i1, int parts,
+                                   const Stat* stats, const float* weights, float* lp_out, RowState* state,
+                                   double (&sum)[3]) {
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += THREADS) {
     const int64_t t = target_of(r, i);
     double lp = 0.0;
     RowState st = {0.0f, 0.0f, 0.0f};
     if (t >= 0) {
       const Stat rs = row_stat(stats, i, parts, r.c);
-      lp = row_logprob<T>(r, i, t, rs);
-      double w = w_all;
-      if (p.reduction == EG_REDUCE_SEQUENCE) {
-        const int64_t s = segment_of(p.seg, i);
-        w = s >= 0 && s < p.seg.n ? w_all / (double)counts[s] : 0.0;
-      }
+      const float below = DONE ? state[i].g : z_below_m<T>(r, i, t, rs.m);
+      lp = logprob_of(r, below, rs.s);
+      const float w = weight_of(p, i, weights);
       st = {0.0f, rs.m, 1.0f / rs.s};
-      if (w != 0.0) {
+      if (w != 0.0f) {
         const PolicyTerms q = policy_terms(p, i, lp);
-        loss += w * q.loss;
-        kl += w * q.kl;
-        clipped += w * q.clipped;
-        st.g = (float)(w * q.g);
+        sum[0] += (double)w * q.loss;
+        sum[1] += (double)w * q.kl;
+        sum[2] += (double)w * q.clipped;
+        if (!DONE) st.g = policy_g(p, i, below, r, rs.s, w);
       }
     }
     lp_out[i] = (float)lp;
-    state[i] = st;
+    if (!DONE) state[i] = st;
   }
-  loss = block_sum64(loss, red);
-  kl = block_sum64(kl, red);
-  clipped = block_sum64(clipped, red);
-  if (tid == 0) {
-    sums[0] = (float)loss;
-    sums[1] = (float)kl;
-    sums[2] = (float)clipped;
+}
+
+// One workgroup over all rows: weights, lp, state; sums[3] = loss, KL, clipped share.
+template <typename T>
+__global__ __launch_bounds__(kFinish) void policy_finish(const Rows r, const Policy p, int parts, const Stat* stats,
+                                                         float* weights, float* lp_out, RowState* state, float* sums) {
+  __shared__ double red[kFinish / 64];
+  policy_weights(r, p, weights);
+  __syncthreads();
+  double sum[3] = {0.0, 0.0, 0.0};
+  policy_rows<T, kFinish, false>(r, p, 0, r.n, parts, stats, weights, lp_out, state, sum);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const double x = block_sum64<kFinish>(sum[k], red);
+    if (threadIdx.x == 0) sums[k] = (float)x;
+  }
+}
+
+// Many rows: the weights first,
+__global__ __launch_bounds__(kFinish) void policy_weights_kernel(const Rows r, const Policy p, float* weights,
+                                                                 int* finished) {
+  if (threadIdx.x == 0) *finished = 0;
+  policy_weights(r, p, weights);
+}
+
+// then a workgroup a row, its statistics and its gradient: the second reading of the row (300 KB
+// of a 150,000-word vocabulary in bf16) comes from the caches,
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void policy_row_kernel(const Rows r, const Policy p, const float* weights,
+                                                             Stat* stats, RowState* state, float scale, T* d,
+                                                             int64_t d_stride) {
+  __shared__ Stat red[THREADS / 64];
+  const int64_t i = blockIdx.y + (int64_t)gridDim.y * blockIdx.z;
+  if (i >= r.n) return;
+  const int64_t t = target_of(r, i);
+  T* out = d + i * d_stride;
+  if (t < 0) {
+    write_zeros<T, THREADS>(out, 0, r.v);
+    return;
+  }
+  const T* row = (const T*)r.z + i * r.stride;
+  const float f_t = t < r.v ? (float)row[t] : __builtin_nanf("");
+  Stat st = thread_stats<T, THREADS>(row, 0, r.v, r.c);
+  st = block_stats<THREADS>(st, r.c, red);
+  if (threadIdx.x == 0) {
+    stats[i] = st;
+    state[i].g = f_t - st.m;
+  }
+  const float w = weight_of(p, i, weights);
+  const float g = w != 0.0f ? policy_g(p, i, f_t - st.m, r, st.s, w) : 0.0f;
+  write_gradient<T, THREADS>(row, out, 0, r.v, t, f_t, g * scale, st.m, 1.0f / st.s, r.c);
+}
+
+// and the rows' terms, 256 rows a workgroup; the last workgroup to finish adds the workgroups' sums,
+// in order.
+template <typename T, bool DONE>
+__global__ __launch_bounds__(256) void policy_terms_kernel(const Rows r, const Policy p, const Stat* stats,
+                                                           const float* weights, float* lp_out, RowState* state,
+                                                           double* partial, int* finished, float* sums) {
+  __shared__ double red[4];
+  __shared__ int last;
+  double sum[3] = {0.0, 0.0, 0.0};
+  const int64_t i0 = (int64_t)blockIdx.x * 256;
+  policy_rows<T, 256, DONE>(r, p, i0, min(i0 + 256, r.n), 1, stats, weights, lp_out, state, sum);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const double x = block_sum64<256>(sum[k], red);
+    if (threadIdx.x == 0)
+      __hip_atomic_store(partial + blockIdx.x * 3 + k, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(finished, 1) == (int)gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    double x = 0.0;
+    for (unsigned q = threadIdx.x; q < gridDim.x; q += 256)
+      x += __hip_atomic_load(partial + q * 3 + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    x = block_sum64<256>(x, red);
+    if (threadIdx.x == 0) sums[k] = (float)x;
   }
 }
 
@@ -446,7 +583,7 @@ __global__ __launch_bounds__(kFinish) void preference_finish(const Rows r, const
     RowState st = {0.0f, 0.0f, 0.0f};
     if (t >= 0) {
       const Stat rs = row_stat(stats, i, parts, r.c);
-      lp = row_logprob<T>(r, i, t, rs);
+      lp = logprob_of(r, z_below_m<T>(r, i, t, rs.m), rs.s);
       st = {0.0f, rs.m, 1.0f / rs.s};
     }
     lp64[i] = lp;
@@ -482,7 +619,7 @@ __global__ __launch_bounds__(kFinish) void preference_finish(const Rows r, const
     d_seq[2 * q + 1] = -g;
     margins[q] = (float)h;
   }
-  loss = block_sum64(loss, red);
+  loss = block_sum64<kFinish>(loss, red);
   if (tid == 0) loss_out[0] = (float)(loss / (double)max(pairs, (int64_t)1));
   __syncthreads();
   for (int64_t i = tid; i < r.n; i += kFinish) {
@@ -536,8 +673,8 @@ int check_segments(const void* ids, int32_t i32, int64_t n, Segments* s) {
   return EG_OK;
 }
 
-// Workspace of a loss: the parts' statistics, then scratch of the segments (24 bytes each)
-// and of the rows (8 bytes each).
+// Workspace of a loss: the parts' statistics, then scratch of the rows (8 bytes each) and of the
+// segments (24 bytes each).
 int64_t stats_bytes(int64_t n, const Cut& cut) { return (n * cut.parts * (int64_t)sizeof(Stat) + 15) / 16 * 16; }
 
 dim3 row_grid(const Cut& cut, int64_t n) {
@@ -602,7 +739,7 @@ extern "C" {
 
 int64_t eg_loss_workspace_size(int64_t n, int64_t v, int32_t dtype, int64_t n_segments) {
   if (n < 0 || v < 1 || n_segments < 0) return -1;
-  return stats_bytes(n, make_cut(n, v, dtype)) + (n_segments + 1) * 24 + n * 8;
+  return stats_bytes(n, make_cut(n, v, dtype)) + (n_segments + 1) * 24 + n * 8 + 64;
 }
 
 #define EG_CHECK_WORKSPACE(need)                                                                              \
@@ -655,19 +792,47 @@ int eg_policy_loss(const eg_logits* logits, const eg_policy* policy, float* logp
     if (int rc = check_grad(logits, d_logits, d_stride); rc != EG_OK) return rc;
   const Cut cut = make_cut(r.n, r.v, logits->dtype);
   const int64_t first = stats_bytes(r.n, cut);
-  EG_CHECK_WORKSPACE(first + (p.seg.n + 1) * 24);
+  EG_CHECK_WORKSPACE(first + (p.seg.n + 1) * 24 + r.n * 8 + 64);
   Stat* stats = (Stat*)workspace;
-  int* counts = (int*)((char*)workspace + first);
-  if (int rc = launch_stats(r, logits->dtype, cut, stats, (hipStream_t)stream); rc != EG_OK) return rc;
-  int rc = by_dtype(logits->dtype, [&](auto zero) {
+  double* partial = (double*)((char*)workspace + first);  // 3 of every 256 rows
+  float* weights = (float*)(partial + r.n);
+  int* finished = (int*)(weights + p.seg.n + 1);
+  const hipStream_t st = (hipStream_t)stream;
+  RowState* kept = (RowState*)state;
+  const bool many = cut.parts == 1 && r.n >= kGroupsWanted;
+  if (many) {
+    policy_weights_kernel<<<1, kFinish, 0, st>>>(r, p, weights, finished);
+    if (int rc = launch_status("policy_weights_kernel"); rc != EG_OK) return rc;
+  }
+  if (many && d_logits != nullptr) {
+    const int rc = by_dtype(logits->dtype, [&](auto zero) {
+      using T = decltype(zero);
+      const dim3 grid = row_grid(cut, r.n);
+      const float scale = grad_scale / logits->temperature;
+      if (cut.threads == 1024)
+        policy_row_kernel<T, 1024><<<grid, 1024, 0, st>>>(r, p, weights, stats, kept, scale, (T*)d_logits, d_stride);
+      else
+        policy_row_kernel<T, 256><<<grid, 256, 0, st>>>(r, p, weights, stats, kept, scale, (T*)d_logits, d_stride);
+      return launch_status("policy_row_kernel");
+    });
+    if (rc != EG_OK) return rc;
+  } else if (int rc = launch_stats(r, logits->dtype, cut, stats, st); rc != EG_OK) {
+    return rc;
+  }
+  const int rc = by_dtype(logits->dtype, [&](auto zero) {
     using T = decltype(zero);
-    policy_finish<T><<<1, kFinish, 0, (hipStream_t)stream>>>(r, p, cut.parts, stats, counts, logprobs,
-                                                             (RowState*)state, sums);
+    const dim3 grid((unsigned)((r.n + 255) / 256));
+    if (many && d_logits != nullptr)
+      policy_terms_kernel<T, true><<<grid, 256, 0, st>>>(r, p, stats, weights, logprobs, kept, partial, finished, sums);
+    else if (many)
+      policy_terms_kernel<T, false><<<grid, 256, 0, st>>>(r, p, stats, weights, logprobs, kept, partial, finished, sums);
+    else
+      policy_finish<T><<<1, kFinish, 0, st>>>(r, p, cut.parts, stats, weights, logprobs, kept, sums);
     return launch_status("policy_finish");
   });
-  if (rc != EG_OK || d_logits == nullptr) return rc;
-  return launch_grad(r, logits->dtype, cut, (const RowState*)state, nullptr, grad_scale / logits->temperature,
-                     d_logits, d_stride, (hipStream_t)stream);
+  if (rc != EG_OK || d_logits == nullptr || many) return rc;
+  return launch_grad(r, logits->dtype, cut, (const RowState*)state, nullptr, grad_scale / logits->temperature, d_logits,
+                     d_stride, st);
 }
 
 int eg_preference_loss(const eg_logits* logits, const eg_preference* preference, float* logprobs,
