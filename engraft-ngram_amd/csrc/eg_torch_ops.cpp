@@ -128,11 +128,25 @@ Scratch make_scratch(const Logits& l, int64_t segments, bool state, const Tensor
 
 Tensor empty_floats(int64_t n, const Tensor& like) { return torch::empty({n}, like.options().dtype(torch::kFloat32)); }
 
-void* rows_of(const MaybeTensor& d, int64_t n) { return d && n > 0 ? d->data_ptr() : nullptr; }
+// Where a gradient is written: `out`, or a new tensor; undefined without one.
+Tensor gradient(const Tensor& z, bool wanted, const MaybeTensor& out) {
+  if (!wanted) return Tensor();
+  if (!out) return torch::empty(z.sizes(), z.options());
+  if (out->sizes() != z.sizes() || out->scalar_type() != z.scalar_type() || out->device() != z.device() ||
+      (out->size(1) > 1 && out->stride(1) != 1))
+    refuse("out must be ", z.scalar_type(), " ", z.sizes(), " on ", z.device(), " with unit stride within a row");
+  return *out;
+}
+
+void* rows_of(const Tensor& d, int64_t n) { return d.defined() && n > 0 ? d.data_ptr() : nullptr; }
+
+Tensor part(const Tensor& t, int64_t first, int64_t count) { return t.as_strided({count}, {1}, first); }
+Tensor scalar(const Tensor& t, int64_t at) { return t.as_strided({}, {}, at); }
 
 const float* values(const Tensor& t) { return (const float*)t.data_ptr(); }
 
 Tensor token_logprobs(const Tensor& logits, const Tensor& targets, double temperature, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
   const Logits l = make_logits(logits, targets, temperature);
   Tensor lp = empty_floats(l.c.n, logits);
   const Scratch s = make_scratch(l, 0, false, logits);
@@ -140,12 +154,13 @@ Tensor token_logprobs(const Tensor& logits, const Tensor& targets, double temper
   return lp;
 }
 
-// (state and workspace, sums, log-probabilities)
-std::tuple<Tensor, Tensor, Tensor> policy(const Tensor& logits, const Tensor& targets, const Tensor& advantages,
+// (state and workspace, loss, KL, clipped share, log-probabilities, d_logits)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, MaybeTensor> policy(const Tensor& logits, const Tensor& targets, const Tensor& advantages,
                                           const MaybeTensor& old_lp, const MaybeTensor& ref_lp, const MaybeTensor& ids,
                                           int64_t segments, double low, double high, double kl_coef,
-                                          double temperature, int64_t reduction, const MaybeTensor& d,
-                                          double grad_scale, int64_t stream) {
+                                          double temperature, int64_t reduction, bool grad,
+                                          const MaybeTensor& out, double grad_scale, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
   const Logits l = make_logits(logits, targets, temperature);
   const int64_t n = l.c.n;
   const auto dev = logits.device();
@@ -166,17 +181,19 @@ std::tuple<Tensor, Tensor, Tensor> policy(const Tensor& logits, const Tensor& ta
   p.clip_high = (float)high;
   p.kl_coef = (float)kl_coef;
   const Scratch s = make_scratch(l, std::max<int64_t>(p.n_segments, 0), true, logits);
+  const Tensor d = gradient(logits, grad, out);
   Tensor sums = empty_floats(3, logits), lp = empty_floats(n, logits);
   check(g.policy(&l.c, &p, (float*)lp.data_ptr(), (float*)sums.data_ptr(), (float*)s.at, rows_of(d, n),
-                 d ? row_stride(*d) : 0, (float)grad_scale, s.at + s.first, s.size, (void*)stream));
-  if (d) written(*d);
-  return {s.buffer, sums, lp};
+                 d.defined() ? row_stride(d) : 0, (float)grad_scale, s.at + s.first, s.size, (void*)stream));
+  if (out) written(d);
+  return {s.buffer, scalar(sums, 0), scalar(sums, 1), scalar(sums, 2), lp, d.defined() ? MaybeTensor(d) : std::nullopt};
 }
 
-// (state and workspace, loss then margins then the sequences' sums, log-probabilities)
-std::tuple<Tensor, Tensor, Tensor> preference(const Tensor& logits, const Tensor& targets, const Tensor& ids,
+// (state and workspace, loss, margins, the sequences' sums, log-probabilities, d_logits)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, MaybeTensor> preference(const Tensor& logits, const Tensor& targets, const Tensor& ids,
                                               const Tensor& ref_lp, double beta, double smoothing, double temperature,
-                                              const MaybeTensor& d, double grad_scale, int64_t stream) {
+                                              bool grad, const MaybeTensor& out, double grad_scale, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
   const Logits l = make_logits(logits, targets, temperature);
   const int64_t n = l.c.n;
   const auto dev = logits.device();
@@ -187,19 +204,24 @@ std::tuple<Tensor, Tensor, Tensor> preference(const Tensor& logits, const Tensor
   const eg_preference p = {i.data_ptr(), values(r), pairs, i.scalar_type() == torch::kInt32, (float)beta,
                            (float)smoothing};
   const Scratch s = make_scratch(l, count, true, logits);
+  const Tensor d = gradient(logits, grad, out);
   Tensor sums = empty_floats(1 + pairs + count, logits), lp = empty_floats(n, logits);
   float* to = (float*)sums.data_ptr();
   check(g.preference(&l.c, &p, (float*)lp.data_ptr(), to + 1 + pairs, to + 1, to, (float*)s.at, rows_of(d, n),
-                     d ? row_stride(*d) : 0, (float)grad_scale, s.at + s.first, s.size, (void*)stream));
-  if (d) written(*d);
-  return {s.buffer, sums, lp};
+                     d.defined() ? row_stride(d) : 0, (float)grad_scale, s.at + s.first, s.size, (void*)stream));
+  if (out) written(d);
+  return {s.buffer, scalar(sums, 0), part(sums, 1, pairs), part(sums, 1 + pairs, count), lp,
+          d.defined() ? MaybeTensor(d) : std::nullopt};
 }
 
-void logits_grad(const Tensor& logits, const Tensor& targets, double temperature, const Tensor& state,
-                 const Tensor& upstream, const Tensor& d, int64_t stream) {
+Tensor logits_grad(const Tensor& logits, const Tensor& targets, double temperature, const Tensor& state,
+                   const Tensor& upstream, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const Tensor d = gradient(logits, true, std::nullopt);
   const Logits l = make_logits(logits, targets, temperature);
   const Tensor up = upstream.to(torch::kFloat32);
   check(g.logits_grad(&l.c, values(state), values(up), 1.0f, rows_of(d, l.c.n), row_stride(d), (void*)stream));
+  return d;
 }
 
 // ---- the orthogonalised step --------------------------------------------------------------------
@@ -223,6 +245,7 @@ void check_writable(const Tensor& t, const char* name) {
 void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& momenta,
           const std::vector<float>& coefficients, int64_t steps, int64_t planes, bool nesterov, double momentum,
           double eps, double keep, double lr, bool update, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
   if (params.size() != grads.size() || (update && params.size() != momenta.size()))
     refuse(params.size(), " params, ", grads.size(), " grads and ", momenta.size(), " momenta");
   // matrices of one shape, types and strides share their launches

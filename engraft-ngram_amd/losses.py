@@ -56,16 +56,6 @@ class PreferenceLoss:
     logprobs: torch.Tensor
 
 
-def _gradient(logits: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
-    if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or \
-            (out.shape[1] > 1 and out.stride(1) != 1):
-        raise ValueError(f"out must be {logits.dtype} {list(logits.shape)} on {logits.device} with unit stride within "
-                         "a row")
-    return out
-
-
 def _stream(t: torch.Tensor) -> int:
     return _lib.stream_ptr(t.device) if t.is_cuda else 0  # a host tensor is refused by the call
 
@@ -77,8 +67,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, temperature: 
 
 
 def _policy(logits, targets, advantages, old_logprobs, ref_logprobs, segment_ids, n_segments, clip, kl_coef,
-            temperature, reduction, d_logits, grad_scale):
-    """``(state, sums, logprobs)`` of one ``eg_policy_loss`` call."""
+            temperature, reduction, grad=False, out=None, grad_scale=1.0):
+    """``(state, loss, kl, clip_fraction, logprobs, d_logits)`` of one ``eg_policy_loss`` call."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {tuple(_REDUCTIONS)}, got {reduction!r}")
     if ref_logprobs is None and kl_coef != 0.0:
@@ -87,32 +77,28 @@ def _policy(logits, targets, advantages, old_logprobs, ref_logprobs, segment_ids
         raise ValueError("reduction='sequence' needs segment_ids and n_segments")
     return _lib.autograd_ext().policy(logits, targets, advantages, old_logprobs, ref_logprobs, segment_ids,
                                       n_segments or 0, clip[0], clip[1], kl_coef, temperature, _REDUCTIONS[reduction],
-                                      d_logits, grad_scale, _stream(logits))
+                                      grad, out, grad_scale, _stream(logits))
 
 
-def _preference(logits, targets, segment_ids, ref_logprobs, beta, label_smoothing, temperature, d_logits, grad_scale):
-    """``(state, loss, margins, sequence_logprobs, logprobs)`` of one ``eg_preference_loss`` call."""
-    state, sums, lp = _lib.autograd_ext().preference(logits, targets, segment_ids, ref_logprobs, beta, label_smoothing,
-                                                     temperature, d_logits, grad_scale, _stream(logits))
-    pairs = ref_logprobs.shape[0] // 2
-    return state, sums[0], sums[1:1 + pairs], sums[1 + pairs:], lp
+def _preference(logits, targets, segment_ids, ref_logprobs, beta, label_smoothing, temperature, grad=False, out=None,
+                grad_scale=1.0):
+    """``(state, loss, margins, sequence_logprobs, logprobs, d_logits)`` of one ``eg_preference_loss`` call."""
+    return _lib.autograd_ext().preference(logits, targets, segment_ids, ref_logprobs, beta, label_smoothing, temperature,
+                                          grad, out, grad_scale, _stream(logits))
 
 
 def _logits_grad(ctx, upstream):
     """The gradient pass from a loss's saved state, times the loss's own gradient."""
     logits, targets, state = ctx.saved_tensors
-    d = _gradient(logits, None)
-    _lib.autograd_ext().logits_grad(logits, targets, ctx.temperature, state, upstream, d, _stream(logits))
-    return d
+    return _lib.autograd_ext().logits_grad(logits, targets, ctx.temperature, state, upstream, _stream(logits))
 
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, *args):
-        state, sums, lp = _policy(logits, targets, *args, None, 1.0)
+        state, loss, kl, clipped, lp, _ = _policy(logits, targets, *args)
         ctx.save_for_backward(logits, targets, state)
         ctx.temperature = args[7]
-        loss, kl, clipped = sums[0].clone(), sums[1], sums[2]
         ctx.mark_non_differentiable(kl, clipped, lp)
         return loss, kl, clipped, lp
 
@@ -125,10 +111,9 @@ class _PolicyLoss(torch.autograd.Function):
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, *args):
-        state, loss, margins, seqs, lp = _preference(logits, targets, *args, None, 1.0)
+        state, loss, margins, seqs, lp, _ = _preference(logits, targets, *args)
         ctx.save_for_backward(logits, targets, state)
         ctx.temperature = args[4]
-        loss = loss.clone()
         ctx.mark_non_differentiable(margins, seqs, lp)
         return loss, margins, seqs, lp
 
@@ -169,11 +154,9 @@ def policy_loss_grad(logits: torch.Tensor, targets: torch.Tensor, advantages: to
     """:func:`policy_loss` and the gradient of ``grad_scale`` times it, as
     ``(PolicyLoss, d_logits)`` without autograd.  ``out``: where the gradient is
     written (the logits themselves for in place)."""
-    with torch.no_grad():
-        d = _gradient(logits, out)
-        _, sums, lp = _policy(logits, targets, advantages, old_logprobs, ref_logprobs, segment_ids, n_segments,
-                                    clip, kl_coef, temperature, reduction, d, grad_scale)
-    return PolicyLoss(sums[0], sums[1], sums[2], lp), d
+    _, loss, kl, clipped, lp, d = _policy(logits, targets, advantages, old_logprobs, ref_logprobs, segment_ids, n_segments,
+                                          clip, kl_coef, temperature, reduction, True, out, grad_scale)
+    return PolicyLoss(loss, kl, clipped, lp), d
 
 
 def preference_loss(logits: torch.Tensor, targets: torch.Tensor, segment_ids: torch.Tensor,
@@ -202,8 +185,6 @@ def preference_loss_grad(logits: torch.Tensor, targets: torch.Tensor, segment_id
     """:func:`preference_loss` and the gradient of ``grad_scale`` times it, as
     ``(PreferenceLoss, d_logits)`` without autograd.  ``out``: where the gradient is
     written (the logits themselves for in place)."""
-    with torch.no_grad():
-        d = _gradient(logits, out)
-        _, loss, margins, seqs, lp = _preference(logits, targets, segment_ids, ref_logprobs, beta,
-                                                       label_smoothing, temperature, d, grad_scale)
+    _, loss, margins, seqs, lp, d = _preference(logits, targets, segment_ids, ref_logprobs, beta, label_smoothing,
+                                                temperature, True, out, grad_scale)
     return PreferenceLoss(loss, margins, seqs, lp), d
