@@ -61,16 +61,27 @@ struct Matrices {
   float* momentum[kMaxBatch];
 };
 
-__device__ inline float load_value(const void* p, int dtype, int64_t i) {
-  if (dtype == EG_DTYPE_F32) return ((const float*)p)[i];
-  if (dtype == EG_DTYPE_BF16) return (float)((const __bf16*)p)[i];
-  return (float)((const _Float16*)p)[i];
+template <typename F>
+__device__ inline void by_type(int dtype, F&& f) {
+  if (dtype == EG_DTYPE_F32) f(0.0f);
+  else if (dtype == EG_DTYPE_BF16) f((__bf16)0.0f);
+  else f((_Float16)0.0f);
 }
 
-__device__ inline void store_value(void* p, int dtype, int64_t i, float v) {
-  if (dtype == EG_DTYPE_F32) ((float*)p)[i] = v;
-  else if (dtype == EG_DTYPE_BF16) ((__bf16*)p)[i] = (__bf16)v;
-  else ((_Float16*)p)[i] = (_Float16)v;
+// Four values of a row from column c on (zeros past the end).
+template <typename T>
+__device__ inline void load4(const T* row, Strides s, int64_t c, int64_t cols, float (&v)[4]) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Four {
+    T x[4];
+  };
+  if (s.col == 1 && c + 4 <= cols) {
+    const Four q = *(const Four*)(row + c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (float)q.x[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = c + k < cols ? (float)row[(c + k) * s.col] : 0.0f;
+  }
 }
 
 struct UpdateArgs {
@@ -88,30 +99,61 @@ __device__ inline float update_of(const UpdateArgs& a, float g, float m) {
   return a.nesterov ? g + a.mu * m : m;
 }
 
-// Grid (tiles, matrices): a 64 x 64 tile's momentum, and its part of |u|^2.
-__global__ __launch_bounds__(256) void muon_momentum_kernel(const UpdateArgs a, const Matrices mats) {
-  __shared__ float red[4];
-  const int64_t r0 = (int64_t)(blockIdx.x / a.tiles_c) * 64, c0 = (int64_t)(blockIdx.x % a.tiles_c) * 64;
-  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const void* grad = mats.grad[b];
-  float* mom = mats.momentum[b];
-  float sum = 0.0f;
-  const int64_t c = c0 + lane;
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int64_t r = r0 + wave * 16 + i;
-    if (r < a.rows && c < a.cols) {
-      const float g = load_value(grad, a.grad_dtype, r * a.grad.row + c * a.grad.col);
-      float m = 0.0f;
-      if (a.has_momentum) {
-        float* q = mom + r * a.momentum.row + c * a.momentum.col;
-        m = a.mu * *q + g;
-        *q = m;
-      }
-      const float u = update_of(a, g, m);
+// A thread's part of a 64 x 64 tile: four columns from c on of the rows r0 + 16 i, i < 4.
+struct TilePart {
+  int64_t r0, c;
+};
+__device__ inline TilePart tile_part(const UpdateArgs& a, unsigned tile) {
+  return {(int64_t)(tile / a.tiles_c) * 64 + threadIdx.x / 16, (int64_t)(tile % a.tiles_c) * 64 + threadIdx.x % 16 * 4};
+}
+
+// Grid (tiles, matrices): a 64 x 64 tile's momentum, and its part of |u|^2.  Bound by HBM: the
+// gradient and the momentum read, the momentum written.
+template <typename G>
+__device__ inline float momentum_tile(const UpdateArgs& a, const G* grad, float* mom) {
+  const TilePart p = tile_part(a, blockIdx.x);
+  float g[4][4], m[4][4], sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = min(p.r0 + 16 * i, a.rows - 1);
+    load4(grad + r * a.grad.row, a.grad, p.c, a.cols, g[i]);
+    if (a.has_momentum) load4((const float*)mom + r * a.momentum.row, a.momentum, p.c, a.cols, m[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = p.r0 + 16 * i;
+    if (r >= a.rows) continue;
+    float now[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      now[k] = a.has_momentum ? a.mu * m[i][k] + g[i][k] : 0.0f;
+      const float u = update_of(a, g[i][k], now[k]);
       sum += u * u;
     }
+    if (!a.has_momentum) continue;
+    float* to = mom + r * a.momentum.row;
+    struct __attribute__((packed, aligned(4))) Four {
+      float x[4];
+    };
+    if (a.momentum.col == 1 && p.c + 4 <= a.cols) {
+      *(Four*)(to + p.c) = {now[0], now[1], now[2], now[3]};
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (p.c + k < a.cols) to[(p.c + k) * a.momentum.col] = now[k];
+    }
   }
+  return sum;
+}
+
+__global__ __launch_bounds__(256) void muon_momentum_kernel(const UpdateArgs a, const Matrices mats) {
+  __shared__ float red[4];
+  const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float sum = 0.0f;
+  by_type(a.grad_dtype, [&](auto zero) {
+    using G = decltype(zero);
+    sum = momentum_tile(a, (const G*)mats.grad[b], mats.momentum[b]);
+  });
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane == 0) red[wave] = sum;
@@ -157,25 +199,33 @@ __global__ __launch_bounds__(256) void muon_planes_kernel(const PlanesArgs p, co
   __shared__ double red[4];
   const UpdateArgs& a = p.u;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.y;
-  const int64_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x % a.tiles_c, r0 = tr * 64, c0 = tc * 64;
+  // the tiles the momentum kernel did last first: they are still cached
+  const unsigned at_tile = gridDim.x - 1 - blockIdx.x;
+  const int64_t tr = at_tile / a.tiles_c, tc = at_tile % a.tiles_c;
   double sum = 0.0;
   for (int i = threadIdx.x; i < a.tiles; i += 256) sum += (double)a.partials[(int64_t)b * a.tiles + i];
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane == 0) red[wave] = sum;
-  const void* grad = mats.grad[b];
-  const float* mom = mats.momentum[b];
-  const int64_t c = c0 + lane;
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int64_t r = r0 + wave * 16 + i;
-    float u = 0.0f;
-    if (r < a.rows && c < a.cols) {
-      const float g = load_value(grad, a.grad_dtype, r * a.grad.row + c * a.grad.col);
-      u = update_of(a, g, a.has_momentum ? mom[r * a.momentum.row + c * a.momentum.col] : 0.0f);
+  by_type(a.grad_dtype, [&](auto zero) {
+    using G = decltype(zero);
+    const G* grad = (const G*)mats.grad[b];
+    const float* mom = mats.momentum[b];
+    const TilePart at = tile_part(a, at_tile);
+    float g[4][4], m[4][4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = min(at.r0 + 16 * i, a.rows - 1);
+      load4(grad + r * a.grad.row, a.grad, at.c, a.cols, g[i]);
+      if (a.has_momentum) load4(mom + r * a.momentum.row, a.momentum, at.c, a.cols, m[i]);
     }
-    tile[wave * 16 + i][lane] = u;
-  }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        tile[threadIdx.x / 16 + 16 * i][threadIdx.x % 16 * 4 + k] =
+            at.r0 + 16 * i < a.rows && at.c + k < a.cols ? update_of(a, g[i][k], m[i][k]) : 0.0f;
+  });
   __syncthreads();
   const float norm = sqrtf((float)(red[0] + red[1] + red[2] + red[3]));
   const float s = p.scale / (norm + p.eps);
@@ -231,13 +281,17 @@ __device__ inline int xcd_order(int b, int n) {
   return x * each + min(x, more) + k;
 }
 
-// LDS of a product's workgroup: the parts of the tile that leave their sums at a time.
+// How a product's wavefronts finish: part w of the tile (its quarters, halves by rows, or all of it) is
+// wavefront w's, SI x SJ blocks, and the others' sums of it come through LDS, kTurns at a time.
 template <int T, int NW>
 struct ProductShape {
   static constexpr int kParts = NW < 4 ? NW : 4;
-  static constexpr int kAll = T * T * 4096 / kParts * (NW - 1);  // bytes of one part's sums
-  static constexpr int kRound = kParts * kAll <= 147456 ? kParts : kParts == 4 && 3 * kAll <= 147456 ? 3 : 1;
-  static constexpr int kBytes = kRound * kAll > kParts * 32 * 80 ? kRound * kAll : kParts * 32 * 80;
+  static constexpr int SI = kParts == 4 ? T / 2 : T / kParts, SJ = kParts == 4 ? T / 2 : T;
+  static constexpr int kTurns = kParts * SI * SJ * 4096 * (NW - 1) > 163840 ? 2 : 1;  // SI / kTurns block rows each
+  static constexpr int kSlot = SI / kTurns * SJ * 4096;                             // one wavefront's sums of one part
+  static constexpr int kSums = kParts * (NW - 1) * kSlot;
+  static constexpr int kBytes = kSums > kParts * 32 * 80 ? kSums : kParts * 32 * 80;
+  static_assert(SI % kTurns == 0 && kSums <= 163840, "the sums fit");
 };
 
 // Grid (tiles, matrices): an output tile of T x T blocks of 32 x 32 a workgroup.  Its NW
@@ -245,8 +299,9 @@ struct ProductShape {
 // straight into registers DEPTH k16 ahead (a fragment is 1 KB of consecutive memory):
 // no LDS and no barrier until the wavefronts' sums are added at the end.
 template <int PLANES, int T, int NW, int DEPTH, Epilogue EPI>
-__global__ __launch_bounds__(NW * 64, NW / 4) void muon_product_kernel(const ProductArgs a, const Matrices mats) {
-  constexpr int PARTS = NW < 4 ? NW : 4;  // wavefronts that finish a part of the tile each
+__global__ __launch_bounds__(NW * 64, NW < 4 ? 1 : NW / 4) void muon_product_kernel(const ProductArgs a, const Matrices mats) {
+  using Shape = ProductShape<T, NW>;
+  constexpr int PARTS = Shape::kParts, SI = Shape::SI, SJ = Shape::SJ;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -325,55 +380,57 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void muon_product_kernel(const Pro
       if (k + d < k_count) multiply(d);
   }
 
-  // The wavefronts' sums.  Part w of the tile (of PARTS: its quarters, or halves by rows) goes to
-  // wavefront w; the others leave theirs in LDS, as many parts at a time as fit.
-  constexpr int SI = PARTS == 4 ? T / 2 : T / PARTS, SJ = PARTS == 4 ? T / 2 : T;  // blocks of a part
-  constexpr int PART_BYTES = SI * SJ * 4096, ROUND = ProductShape<T, NW>::kRound;
   f32x16 sum[SI][SJ];
+  auto part_i = [](int w) { return PARTS == 4 ? w / 2 * SI : w * SI; };
+  auto part_j = [](int w) { return PARTS == 4 ? w % 2 * SJ : 0; };
 #pragma unroll
-  for (int w0 = 0; w0 < PARTS; w0 += ROUND) {
-    if (NW > 1 && w0 > 0) __syncthreads();
+  for (int w = 0; w < PARTS; ++w)
+    if (wave == w) {
 #pragma unroll
-    for (int w = w0; w < w0 + ROUND && w < PARTS; ++w) {
-      const int pi = PARTS == 4 ? w / 2 * SI : w * SI, pj = PARTS == 4 ? w % 2 * SJ : 0;
-      if (wave == w) {
+      for (int i = 0; i < SI; ++i)
 #pragma unroll
-        for (int i = 0; i < SI; ++i)
+        for (int j = 0; j < SJ; ++j) sum[i][j] = acc[part_i(w) + i][part_j(w) + j];
+    }
+  if (NW > 1) {
+    constexpr int RI = SI / Shape::kTurns;
 #pragma unroll
-          for (int j = 0; j < SJ; ++j) sum[i][j] = acc[pi + i][pj + j];
-      } else {
-        char* at = lds + ((w - w0) * (NW - 1) + (wave > w ? wave - 1 : wave)) * PART_BYTES + lane * 16;
+    for (int turn = 0; turn < Shape::kTurns; ++turn) {
+      if (turn > 0) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < SI; ++i)
+      for (int w = 0; w < PARTS; ++w) {
+        if (wave == w) continue;
+        char* at = lds + (w * (NW - 1) + (wave > w ? wave - 1 : wave)) * Shape::kSlot + lane * 16;
 #pragma unroll
-          for (int j = 0; j < SJ; ++j)
+        for (int i = 0; i < RI; ++i)
+#pragma unroll
+          for (int j = 0; j < SJ; ++j) {
+            const f32x16& v = acc[part_i(w) + turn * RI + i][part_j(w) + j];
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-              *(f32x4*)(at + ((i * SJ + j) * 4 + g) * 1024) = f32x4{acc[pi + i][pj + j][4 * g], acc[pi + i][pj + j][4 * g + 1],
-                                                                   acc[pi + i][pj + j][4 * g + 2], acc[pi + i][pj + j][4 * g + 3]};
+              *(f32x4*)(at + ((i * SJ + j) * 4 + g) * 1024) = f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+          }
       }
-    }
-    if (NW > 1) __syncthreads();
-    if (wave >= w0 && wave < w0 + ROUND && wave < PARTS) {
-#pragma unroll 1
-      for (int other = 0; other < NW - 1; ++other) {
-        const char* at = lds + ((wave - w0) * (NW - 1) + other) * PART_BYTES + lane * 16;
+      __syncthreads();
+      if (wave < PARTS)
 #pragma unroll
-        for (int i = 0; i < SI; ++i)
+        for (int i = 0; i < RI; ++i)
 #pragma unroll
-          for (int j = 0; j < SJ; ++j)
+          for (int j = 0; j < SJ; ++j) {
+            const char* at = lds + wave * (NW - 1) * Shape::kSlot + (i * SJ + j) * 4096 + lane * 16;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const f32x4 v = *(const f32x4*)(at + ((i * SJ + j) * 4 + g) * 1024);
+            for (int other = 0; other < NW - 1; ++other)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) sum[i][j][4 * g + r] += v[r];
-            }
-      }
+              for (int g = 0; g < 4; ++g) {
+                const f32x4 v = *(const f32x4*)(at + other * Shape::kSlot + g * 1024);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum[turn * RI + i][j][4 * g + r] += v[r];
+              }
+          }
     }
   }
   if (NW > 1) __syncthreads();  // the transpose buffers are where sums were
   if (wave >= PARTS) return;
-  const int bi0 = i0 + (PARTS == 4 ? wave / 2 * SI : wave * SI), bj0 = j0 + (PARTS == 4 ? wave % 2 * SJ : 0);
+  const int bi0 = i0 + part_i(wave), bj0 = j0 + part_j(wave);
 
   // lane l of a 32 x 32 block holds column l % 32, rows 8 g + 4 (l / 32) + r
   constexpr int PITCH = 80;  // bytes of a row of 32 fp16 in the transpose buffer, 16-byte aligned
@@ -402,30 +459,44 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void muon_product_kernel(const Pro
       }
     }
   if (EPI == kLast) {
-    void* w = mats.param[b];
-    if (a.read_param) {
+    by_type(a.param_dtype, [&](auto zero) {
+      using W = decltype(zero);
+      W* w = (W*)mats.param[b];
+      auto place = [&](int i, int j, int r, int64_t& x, int64_t& y) {
+        x = (int64_t)(bi0 + i) * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+        y = (int64_t)(bj0 + j) * 32 + col;
+      };
+      if (a.read_param) {
+        W old[SI][SJ][16];
+#pragma unroll
+        for (int i = 0; i < SI; ++i)
+#pragma unroll
+          for (int j = 0; j < SJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              int64_t x, y;
+              place(i, j, r, x, y);
+              old[i][j][r] = w[min(x, a.rows - 1) * a.param.row + min(y, a.cols - 1) * a.param.col];
+            }
+#pragma unroll
+        for (int i = 0; i < SI; ++i)
+#pragma unroll
+          for (int j = 0; j < SJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[i][j][r] = a.keep * (float)old[i][j][r] - a.rate * sum[i][j][r];
+      }
+      const float scale = a.read_param ? 1.0f : -a.rate;
 #pragma unroll
       for (int i = 0; i < SI; ++i)
 #pragma unroll
         for (int j = 0; j < SJ; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int64_t x = (int64_t)(bi0 + i) * 32 + 8 * (r >> 2) + 4 * half + (r & 3), y = (int64_t)(bj0 + j) * 32 + col;
-            const float old = load_value(w, a.param_dtype, min(x, a.rows - 1) * a.param.row + min(y, a.cols - 1) * a.param.col);
-            sum[i][j][r] = a.keep * old - a.rate * sum[i][j][r];
+            int64_t x, y;
+            place(i, j, r, x, y);
+            if (x < a.rows && y < a.cols) w[x * a.param.row + y * a.param.col] = (W)(scale * sum[i][j][r]);
           }
-    }
-#pragma unroll
-    for (int i = 0; i < SI; ++i)
-#pragma unroll
-      for (int j = 0; j < SJ; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int64_t x = (int64_t)(bi0 + i) * 32 + 8 * (r >> 2) + 4 * half + (r & 3), y = (int64_t)(bj0 + j) * 32 + col;
-          if (x < a.rows && y < a.cols)
-            store_value(w, a.param_dtype, x * a.param.row + y * a.param.col,
-                        a.read_param ? sum[i][j][r] : -a.rate * sum[i][j][r]);
-        }
+    });
     return;
   }
 #pragma unroll
@@ -574,31 +645,40 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
   float* red = (float*)gram;
 
   // momentum; a thread has 8 rows of a column in each of its units
-  const void* grad = mats.grad[b];
-  float* mom = mats.momentum[b];
   const int chunks = a.pc / 64, units = a.pr / 8 * chunks;
   float u[UNITS][8], sum = 0.0f;
+  by_type(a.u.grad_dtype, [&](auto zero) {
+    using G = decltype(zero);
+    const G* grad = (const G*)mats.grad[b];
+    float* mom = mats.momentum[b];
+    G g[UNITS][8];
+    float old[UNITS][8];
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) {
-    const int unit = wave + i * kSmallWaves;
-    if (unit >= units) break;
-    const int r0 = unit / chunks * 8, c = unit % chunks * 64 + lane;
-    float g[8], old[8];
+    for (int i = 0; i < UNITS; ++i) {
+      const int unit = min(wave + i * kSmallWaves, units - 1);
+      const int r0 = unit / chunks * 8, c = min(unit % chunks * 64 + lane, (int)a.u.cols - 1);
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const bool in = r0 + r < a.u.rows && c < a.u.cols;
-      g[r] = in ? load_value(grad, a.u.grad_dtype, (r0 + r) * a.u.grad.row + c * a.u.grad.col) : 0.0f;
-      old[r] = in && a.u.has_momentum ? mom[(r0 + r) * a.u.momentum.row + c * a.u.momentum.col] : 0.0f;
+      for (int r = 0; r < 8; ++r) {
+        const int row = min(r0 + r, (int)a.u.rows - 1);
+        g[i][r] = grad[row * a.u.grad.row + c * a.u.grad.col];
+        old[i][r] = a.u.has_momentum ? mom[row * a.u.momentum.row + c * a.u.momentum.col] : 0.0f;
+      }
     }
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const float now = a.u.mu * old[r] + g[r];
-      if (a.u.has_momentum && r0 + r < a.u.rows && c < a.u.cols)
-        mom[(r0 + r) * a.u.momentum.row + c * a.u.momentum.col] = now;
-      u[i][r] = update_of(a.u, g[r], now);
-      sum += u[i][r] * u[i][r];
+    for (int i = 0; i < UNITS; ++i) {
+      const int unit = wave + i * kSmallWaves;
+      if (unit >= units) break;
+      const int r0 = unit / chunks * 8, c = unit % chunks * 64 + lane;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const bool in = r0 + r < a.u.rows && c < a.u.cols;
+        const float now = a.u.mu * old[i][r] + (float)g[i][r];
+        if (a.u.has_momentum && in) mom[(r0 + r) * a.u.momentum.row + c * a.u.momentum.col] = now;
+        u[i][r] = in ? update_of(a.u, (float)g[i][r], now) : 0.0f;
+        sum += u[i][r] * u[i][r];
+      }
     }
-  }
+  });
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane == 0) red[wave] = sum;
@@ -681,7 +761,6 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
 
   // the last step's X goes to the weights, in the order whose lanes run along their rows
   const Factors f = a.f[a.steps - 1];
-  void* w = mats.param[b];
   for (int k = wave; k < mb * nb; k += kSmallWaves) {
     const int bm = k / nb, bn = k % nb;
     f32x16 acc = tall ? block_product<PLANES, true>(xt, bn, poly, bm, m16, lane) : block_product<PLANES, false>(poly, bm, xt, bn, m16, lane);
@@ -690,19 +769,23 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
     else
       add_c<PLANES>(acc, f.step, f.step_c, xt, bm, bn, m16, lane);
     const int r0 = (tall ? bn : bm) * 32 + 4 * (lane >> 5), c = (tall ? bm : bn) * 32 + (lane & 31);
-    float old[16];
+    by_type(a.param_dtype, [&](auto zero) {
+      using W = decltype(zero);
+      W* w = (W*)mats.param[b];
+      W old[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = r0 + 8 * (r >> 2) + (r & 3);
-      old[r] = a.read_param && row < a.u.rows && c < a.u.cols
-                   ? a.keep * load_value(w, a.param_dtype, row * a.param.row + c * a.param.col) : 0.0f;
-    }
+      for (int r = 0; r < 16; ++r) {
+        const int row = min(r0 + 8 * (r >> 2) + (r & 3), (int)a.u.rows - 1);
+        old[r] = a.read_param ? w[row * a.param.row + min(c, (int)a.u.cols - 1) * a.param.col] : (W)0.0f;
+      }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = r0 + 8 * (r >> 2) + (r & 3);
-      if (row < a.u.rows && c < a.u.cols)
-        store_value(w, a.param_dtype, row * a.param.row + c * a.param.col, old[r] - a.rate * acc[r]);
-    }
+      for (int r = 0; r < 16; ++r) {
+        const int row = r0 + 8 * (r >> 2) + (r & 3);
+        if (row < a.u.rows && c < a.u.cols)
+          w[row * a.param.row + c * a.param.col] =
+              (W)((a.read_param ? a.keep * (float)old[r] : 0.0f) - a.rate * acc[r]);
+      }
+    });
   }
 }
 
@@ -748,15 +831,23 @@ int launch_product_as(const ProductArgs& args, const Matrices& mats, int count, 
   return launch_status("muon_product_kernel");
 }
 
-#ifndef EG_T
-#define EG_T 4
-#define EG_NW 4
-#define EG_D1 6
-#define EG_D2 3
-#endif
+// The tile by the number of 128 x 128 ones, whose rounds over the 256 CUs (one a CU) cost what
+// they cost however full they are:
+//   few (kFewTiles): 64 x 64, four times the workgroups: a 1024 x 1024 fp32 step 174 us against 354, 1536 x
+//     1536 420 against 468; 2048 x 2048 775 against 642;
+//   one plane and four rounds' worth: a wavefront a tile with nothing to add up, since the sums of four
+//     cost as much as a tile's products at K 2,560: 137 us a product of 1,600 tiles against 164
+//     (two planes, 2,000 tiles: 470 against 442).
+constexpr int kFewTiles = 128, kManyTiles = 1024;
+
 template <int PLANES, Epilogue EPI>
 int launch_product(const ProductArgs& a, const Matrices& mats, int count, hipStream_t stream) {
-  return launch_product_as<PLANES, EG_T, EG_NW, PLANES == 2 ? EG_D2 : EG_D1, EPI>(a, mats, count, stream);
+  const int64_t tp = (a.p_blocks + 3) / 4, tq = (a.q_blocks + 3) / 4;
+  const int64_t tiles = count * (EPI == kGram || EPI == kPoly ? tq * (tq + 1) / 2 : tp * tq);
+  if (tiles <= kFewTiles) return launch_product_as<PLANES, 2, 4, PLANES == 2 ? 4 : 6, EPI>(a, mats, count, stream);
+  if (PLANES == 1 && EPI == kStep && tiles >= kManyTiles)
+    return launch_product_as<PLANES, 4, 1, 6, EPI>(a, mats, count, stream);
+  return launch_product_as<PLANES, 4, 4, PLANES == 2 ? 3 : 6, EPI>(a, mats, count, stream);
 }
 
 // Powers of two by which X, A and B of an iteration are kept, from the bound of X's
