@@ -539,18 +539,29 @@ constexpr int kSmallWaves = 16;
 constexpr int kSmallSteps = 32;
 constexpr int kSmallBytes = 160 * 1024;
 
+// run_at within LDS.
+template <int PLANES>
+__device__ inline int lds_run(int row_block, int k16s, int k16, int plane) {
+  return ((row_block * k16s + k16) * PLANES + plane) * kRun;
+}
+
+// A matrix of which every element's offset fits 31 bits (the host sees to it).
+struct Strides32 {
+  int row, col;
+};
+
 // A step's factors: A = gram D; B = poly D + poly_c A; X = step D + step_c X.
 struct Factors {
   float gram, poly, poly_c, step, step_c;
 };
 
 struct SmallArgs {
-  UpdateArgs u;
-  float eps, scale;
+  int rows, cols;
+  Strides32 grad, momentum, param;
+  int grad_dtype, has_momentum, nesterov, param_dtype, read_param;
+  float mu, eps, scale;
   int pr, pc;                  // rows and columns padded to 64
   int steps;
-  Strides param;
-  int param_dtype, read_param;
   float keep, rate;
   Factors f[kSmallSteps];
 };
@@ -562,8 +573,8 @@ __device__ inline f32x16 block_product(const char* p, int bp, const char* q, int
   f32x16 acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-  const char* pa = p + run_at<PLANES>(bp, k16s, 0, 0) + lane * 16;
-  const char* qa = q + run_at<PLANES>(bq, k16s, 0, 0) + lane * 16;
+  const char* pa = p + lds_run<PLANES>(bp, k16s, 0, 0) + lane * 16;
+  const char* qa = q + lds_run<PLANES>(bq, k16s, 0, 0) + lane * 16;
   for (int k0 = 0; k0 < k16s; k0 += 4)  // K is padded to 64
 #pragma unroll
     for (int k = k0; k < k0 + 4; ++k) {
@@ -589,7 +600,7 @@ template <int PLANES>
 __device__ inline void add_c(f32x16& acc, float alpha, float beta, const char* c, int bp, int bq, int k16s, int lane) {
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const char* at = c + run_at<PLANES>(bq, k16s, bp * 2 + (g >> 1), 0) + ((lane & 31) + 32 * (g & 1)) * 16 + 8 * (lane >> 5);
+    const char* at = c + lds_run<PLANES>(bq, k16s, bp * 2 + (g >> 1), 0) + ((lane & 31) + 32 * (g & 1)) * 16 + 8 * (lane >> 5);
     const f16x4 hi = *(const f16x4*)at;
     f16x4 lo = {0, 0, 0, 0};
     if (PLANES == 2) lo = *(const f16x4*)(at + kRun);
@@ -618,7 +629,7 @@ template <int PLANES>
 __device__ inline void store_planes(char* to, const BlockPlanes<PLANES>& o, int bp, int bq, int k16s, int lane) {
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    char* at = to + run_at<PLANES>(bq, k16s, bp * 2 + (g >> 1), 0) + ((lane & 31) + 32 * (g & 1)) * 16 + 8 * (lane >> 5);
+    char* at = to + lds_run<PLANES>(bq, k16s, bp * 2 + (g >> 1), 0) + ((lane & 31) + 32 * (g & 1)) * 16 + 8 * (lane >> 5);
 #pragma unroll
     for (int x = 0; x < PLANES; ++x) *(f16x4*)(at + x * kRun) = o.v[x][g];
   }
@@ -636,7 +647,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, b = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool tall = a.u.rows > a.u.cols;
+  const bool tall = a.rows > a.cols;
   const int m = tall ? a.pc : a.pr, n = tall ? a.pr : a.pc, m16 = m / 16, n16 = n / 16, mb = m / 32, nb = n / 32;
   char* x = lds;                                // X by rows: m x n
   char* xt = x + m * n * 2 * PLANES;            // X^T by rows
@@ -647,7 +658,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
   // momentum; a thread has 8 rows of a column in each of its units
   const int chunks = a.pc / 64, units = a.pr / 8 * chunks;
   float u[UNITS][8], sum = 0.0f;
-  by_type(a.u.grad_dtype, [&](auto zero) {
+  by_type(a.grad_dtype, [&](auto zero) {
     using G = decltype(zero);
     const G* grad = (const G*)mats.grad[b];
     float* mom = mats.momentum[b];
@@ -656,25 +667,38 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) {
       const int unit = min(wave + i * kSmallWaves, units - 1);
-      const int r0 = unit / chunks * 8, c = min(unit % chunks * 64 + lane, (int)a.u.cols - 1);
+      const int r0 = unit / chunks * 8, c = min(unit % chunks * 64 + lane, a.cols - 1);
+      const int gc = c * a.grad.col, mc = c * a.momentum.col;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const int row = min(r0 + r, (int)a.u.rows - 1);
-        g[i][r] = grad[row * a.u.grad.row + c * a.u.grad.col];
-        old[i][r] = a.u.has_momentum ? mom[row * a.u.momentum.row + c * a.u.momentum.col] : 0.0f;
+      for (int r = 0; r < 8; ++r) g[i][r] = (grad + min(r0 + r, a.rows - 1) * a.grad.row)[gc];
+      if (a.has_momentum) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) old[i][r] = (mom + min(r0 + r, a.rows - 1) * a.momentum.row)[mc];
       }
     }
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) {
       const int unit = wave + i * kSmallWaves;
       if (unit >= units) break;
-      const int r0 = unit / chunks * 8, c = unit % chunks * 64 + lane;
+      const int r0 = unit / chunks * 8, c = unit % chunks * 64 + lane, mc = c * a.momentum.col;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) u[i][r] = (float)g[i][r];
+      if (a.has_momentum) {
+        float now[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          now[r] = a.mu * old[i][r] + u[i][r];
+          u[i][r] = a.nesterov ? u[i][r] + a.mu * now[r] : now[r];
+        }
+        if (c < a.cols) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r0 + r < a.rows) (mom + (r0 + r) * a.momentum.row)[mc] = now[r];
+        }
+      }
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        const bool in = r0 + r < a.u.rows && c < a.u.cols;
-        const float now = a.u.mu * old[i][r] + (float)g[i][r];
-        if (a.u.has_momentum && in) mom[(r0 + r) * a.u.momentum.row + c * a.u.momentum.col] = now;
-        u[i][r] = in ? update_of(a.u, (float)g[i][r], now) : 0.0f;
+        u[i][r] = r0 + r < a.rows && c < a.cols ? u[i][r] : 0.0f;
         sum += u[i][r] * u[i][r];
       }
     }
@@ -701,11 +725,11 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
       split(u[i][r] * s, h, l);
       hi[r] = h;
       lo[r] = l;
-      char* at = by_row + run_at<PLANES>((r0 + r) / 32, a.pc / 16, c / 16, 0) + ((r0 + r) % 32 + 32 * (c % 16 / 8)) * 16 + c % 8 * 2;
+      char* at = by_row + lds_run<PLANES>((r0 + r) / 32, a.pc / 16, c / 16, 0) + ((r0 + r) % 32 + 32 * (c % 16 / 8)) * 16 + c % 8 * 2;
       *(_Float16*)at = h;
       if (PLANES == 2) *(_Float16*)(at + kRun) = l;
     }
-    char* at = by_col + run_at<PLANES>(c / 32, a.pr / 16, r0 / 16, 0) + (c % 32 + 32 * (r0 % 16 / 8)) * 16;
+    char* at = by_col + lds_run<PLANES>(c / 32, a.pr / 16, r0 / 16, 0) + (c % 32 + 32 * (r0 % 16 / 8)) * 16;
     *(f16x8*)at = hi;
     if (PLANES == 2) *(f16x8*)(at + kRun) = lo;
   }
@@ -772,18 +796,22 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
     by_type(a.param_dtype, [&](auto zero) {
       using W = decltype(zero);
       W* w = (W*)mats.param[b];
-      W old[16];
+      const int cs = min(c, a.cols - 1) * a.param.col;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = min(r0 + 8 * (r >> 2) + (r & 3), (int)a.u.rows - 1);
-        old[r] = a.read_param ? w[row * a.param.row + min(c, (int)a.u.cols - 1) * a.param.col] : (W)0.0f;
+      for (int r = 0; r < 16; ++r) acc[r] *= -a.rate;
+      if (a.read_param) {
+        W old[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) old[r] = w[min(r0 + 8 * (r >> 2) + (r & 3), a.rows - 1) * a.param.row + cs];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] += a.keep * (float)old[r];
       }
+      if (c < a.cols) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = r0 + 8 * (r >> 2) + (r & 3);
-        if (row < a.u.rows && c < a.u.cols)
-          w[row * a.param.row + c * a.param.col] =
-              (W)((a.read_param ? a.keep * (float)old[r] : 0.0f) - a.rate * acc[r]);
+        for (int r = 0; r < 16; ++r) {
+          const int row = r0 + 8 * (r >> 2) + (r & 3);
+          if (row < a.rows) w[row * a.param.row + cs] = (W)acc[r];
+        }
       }
     });
   }
@@ -891,21 +919,33 @@ double next_sigma(double sigma, const float* k) {
   return kMargin * top;
 }
 
+// Whether every element lies within 2^29 elements of the first.
+bool near(const eg_muon* o, const int64_t* stride) {
+  auto span = [](int64_t n, int64_t s) { return n == 1 ? 0.0 : (double)(n - 1) * fabs((double)s); };
+  return span(o->rows, stride[0]) + span(o->cols, stride[1]) < (double)(1 << 29);
+}
+
 // Bytes of LDS that X, X^T, A and B take.
 int64_t small_bytes(const Layout& l) { return 2 * (l.x + l.a); }
 
 template <int PLANES>
-int run_small(const eg_muon* o, const Matrices& mats, int count, const Layout& l, const UpdateArgs& u,
-              hipStream_t stream) {
+int run_small(const eg_muon* o, const Matrices& mats, int count, const Layout& l, hipStream_t stream) {
   SmallArgs a;
-  a.u = u;
+  a.rows = (int)o->rows;
+  a.cols = (int)o->cols;
+  a.grad = {(int)o->grad_stride[0], (int)o->grad_stride[1]};
+  a.momentum = {(int)o->momentum_stride[0], (int)o->momentum_stride[1]};
+  a.param = {(int)o->param_stride[0], (int)o->param_stride[1]};
+  a.grad_dtype = o->grad_dtype;
+  a.has_momentum = o->momenta != nullptr;
+  a.nesterov = o->nesterov;
+  a.param_dtype = o->param_dtype;
+  a.read_param = o->keep != 0.0f;
+  a.mu = o->momentum;
   a.eps = o->eps;
   a.pr = (int)pad64(o->rows);
   a.pc = (int)pad64(o->cols);
   a.steps = o->steps;
-  a.param = {o->param_stride[0], o->param_stride[1]};
-  a.param_dtype = o->param_dtype;
-  a.read_param = o->keep != 0.0f;
   a.keep = o->keep;
   a.rate = o->rate;
   Bounds bd = bounds_of(1.0, o->coefficients);
@@ -939,8 +979,9 @@ int run_muon(const eg_muon* o, int first, int count, const Layout& l, char* ws, 
   const UpdateArgs update = {o->rows, o->cols, {o->grad_stride[0], o->grad_stride[1]},
                              {o->momentum_stride[0], o->momentum_stride[1]}, o->grad_dtype, o->momenta != nullptr,
                              o->nesterov, o->momentum, (int)(pad64(o->cols) / 64), (int)l.tiles, (float*)ws};
-  if (small_bytes(l) <= kSmallBytes && o->steps <= kSmallSteps)
-    return run_small<PLANES>(o, mats, count, l, update, stream);
+  if (small_bytes(l) <= kSmallBytes && o->steps <= kSmallSteps && near(o, o->param_stride) && near(o, o->grad_stride) &&
+      near(o, o->momentum_stride))
+    return run_small<PLANES>(o, mats, count, l, stream);
   const bool tall = o->rows > o->cols;
   char* base = ws + l.partials;
   char* x = base;
