@@ -25,6 +25,7 @@
 
 #include <algorithm>
 
+
 namespace eg {
 namespace {
 
@@ -168,9 +169,8 @@ __device__ inline void add_chunks(const Chunk (&q)[K], float c, Stat& st) {
 
 // A thread's statistics of elements [e0, e1) of a row, e0 a multiple of the chunk.
 template <typename T, int THREADS>
-__device__ inline Stat thread_stats(const T* row, int e0, int e1, float c) {
+__device__ inline Stat thread_stats(const T* row, int e0, int e1, float c, Stat st = {kLowest, 0.0f}) {
   constexpr int VEC = Logit<T>::kVec, K = 4;
-  Stat st = {kLowest, 0.0f};
   int e = e0 + (int)threadIdx.x * VEC;
   for (; e + (K - 1) * THREADS * VEC + VEC <= e1; e += K * THREADS * VEC) {
     Chunk q[K];
@@ -560,12 +560,12 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const Rows r, const
   write_gradient<T, THREADS>(row, out, 0, r.v, t, f_t, g * scale, st.m, 1.0f / st.s, r.c);
 }
 
-// or, where a row's chunks fit the registers of a workgroup of 1,024 threads (NV a thread), with the
-// row read once and held,
+// or, of longer rows, with the first NV chunks a thread held in registers from the one to the other
+// (16 KB a chunk of 1,024 threads: NV 20 is a whole CU's and holds all of 151,936 bf16),
 template <typename T, int NV>
 __global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const Policy p, const float* weights,
-                                                           Stat* stats, RowState* state, float scale, T* d,
-                                                           int64_t d_stride) {
+                                                                 Stat* stats, RowState* state, float scale, T* d,
+                                                                 int64_t d_stride) {
   constexpr int THREADS = 1024, VEC = Logit<T>::kVec, STRIDE = THREADS * VEC, K = 4;
   static_assert(NV % K == 0, "whole groups");
   __shared__ Stat red[THREADS / 64];
@@ -579,7 +579,7 @@ __global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const P
   }
   const T* row = (const T*)r.z + i * r.stride;
   const float f_t = t < r.v ? (float)row[t] : __builtin_nanf("");
-  // chunks past the row's end re-read its last whole one and are left out below
+  // held chunks past the row's end re-read its last whole one and are left out below
   const int e0 = (int)threadIdx.x * VEC, whole = r.v / VEC * VEC;
   Chunk q[NV / K][K];
 #pragma unroll
@@ -602,7 +602,9 @@ __global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const P
         }
     }
   }
-  const bool has_tail = (whole - e0) % STRIDE == 0;  // this thread's next chunk is the row's incomplete one
+  st = thread_stats<T, THREADS>(row, NV * STRIDE, r.v, r.c, st);
+  // the incomplete last chunk of a row that ends among the held ones
+  const bool has_tail = whole < NV * STRIDE && (whole - e0) % STRIDE == 0 && whole >= e0;
   if (has_tail)
     for (int e = whole; e < r.v; ++e) {
       const float f = (float)row[e], m = fmaxf(st.m, f);
@@ -615,7 +617,7 @@ __global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const P
   }
   const float w = weight_of(p, i, weights);
   const float g = (w != 0.0f ? policy_g(p, policy_row(p, i, logprob_of(r, f_t - st.m, st.s)), w) : 0.0f) * scale;
-  const float k1 = -g * (1.0f / st.s), c = r.c, m = st.m;
+  const float inv_s = 1.0f / st.s, k1 = -g * inv_s, c = r.c, m = st.m;
   auto value = [&](float f) { return k1 * pow2((f - m) * c); };
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -632,8 +634,8 @@ __global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const P
   }
   if (has_tail)
     for (int e = whole; e < r.v; ++e) out[e] = (T)value((float)row[e]);
-  // the target's element again, by the thread that wrote it
-  if (t < r.v && (int)(t / VEC) % THREADS == (int)threadIdx.x) out[t] = (T)(g + value(f_t));
+  if (t < NV * STRIDE && t < r.v && (int)(t / VEC) % THREADS == (int)threadIdx.x) out[t] = (T)(g + value(f_t));
+  if (NV * STRIDE < r.v) write_gradient<T, THREADS>(row, out, NV * STRIDE, r.v, t, f_t, g, m, inv_s, c);
 }
 
 // and the rows' terms, 256 rows a workgroup; the last workgroup to finish adds the workgroups' sums,
@@ -773,6 +775,11 @@ Cut make_cut(int64_t n, int64_t v, int dtype) {
 // Log-probabilities take a launch less with a workgroup a whole row: 5.5 us against 8.2 for 64 KB a
 // row, 9.8 against 8.1 for one row of 300 KB, 12.7 against 16.2 for 200 such rows.
 constexpr int64_t kWholeRowBytes = 128 << 10, kWholeRows = 64;
+
+// policy_held_kernel holds 8 chunks a thread of rows above kHeldShort bytes, 20 above kHeldLong.  1,024 rows
+// against policy_row_kernel: 66 KB 41.6 us for 38.6, 100 KB 59.9 for 66.4; 8 against 20 chunks: 140 KB 69.7 and
+// 69.1 (75.6 not held), 260 KB 131 and 120 (136), 608 KB (fp32) 284 and 257 (312).
+constexpr int64_t kHeldShort = 80 << 10, kHeldLong = 128 << 10;
 
 Cut whole_rows(int64_t v, int dtype) { return {v * value_bytes(dtype) > 32768 ? 1024 : 256, 1, (int)v}; }
 
@@ -939,13 +946,13 @@ int eg_policy_loss(const eg_logits* logits, const eg_policy* policy, float* logp
       using T = decltype(zero);
       const dim3 grid = row_grid(cut, r.n);
       const float scale = grad_scale / logits->temperature;
-#ifndef NOHELD
-      const int64_t chunks = (r.v * (int64_t)sizeof(T) + 16383) / 16384;
-      if (chunks > 8 && chunks <= 20)
-        policy_held_kernel<T, 20><<<grid, 1024, 0, st>>>(r, p, weights, stats, kept, scale, (T*)d_logits, d_stride);
-      else
-#endif
-      if (cut.threads == 1024)
+      const int64_t bytes = r.v * (int64_t)sizeof(T);
+      auto held = [&](auto kernel) { kernel<<<grid, 1024, 0, st>>>(r, p, weights, stats, kept, scale, (T*)d_logits, d_stride); };
+      if (bytes > kHeldLong)
+        held(policy_held_kernel<T, 20>);
+      else if (bytes > kHeldShort)
+        held(policy_held_kernel<T, 8>);
+      else if (cut.threads == 1024)
         policy_row_kernel<T, 1024><<<grid, 1024, 0, st>>>(r, p, weights, stats, kept, scale, (T*)d_logits, d_stride);
       else
         policy_row_kernel<T, 256><<<grid, 256, 0, st>>>(r, p, weights, stats, kept, scale, (T*)d_logits, d_stride);

@@ -22,7 +22,8 @@ pytestmark = pytest.mark.gpu
 EPS = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 TINY = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -24}
 ALL = [torch.float32, torch.bfloat16, torch.float16]
-SIZES = [(1, 1), (1, 7), (3, 8), (5, 1003), (4, 4096), (600, 129), (2, 50_257), (3, 151_936), (530, 40_001)]
+SIZES = [(1, 1), (1, 7), (3, 8), (5, 1003), (4, 4096), (600, 129), (2, 50_257), (3, 151_936), (530, 40_001),
+         (515, 50_257), (513, 163_841)]
 
 
 def make(n, v, dtype, seed, pad=0, offset=0, ignored=0.3, int32=False):
