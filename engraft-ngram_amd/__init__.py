@@ -7,7 +7,8 @@ scatter + Adam + requantisation on the touched overlay rows).  Host code is
 Python on PyTorch-ROCm; every stage runs in hand-written gfx950 HIP kernels
 behind the C ABI of ``include/engraft_ngram.h`` (``libengraft_ngram.so``);
 ``OverlayEmb``'s differentiable gather is a C++ autograd function over two of
-those entry points (``_eg_autograd.so``, host code built beside the library).
+those entry points (``_eg_autograd.so``, host code built beside the library,
+with the losses' and the weight updates' calls from torch).
 
 Modules mirror the reference's:
   table       -- ``engraft.table``            (DeviceTable = PleTable duck type)
@@ -21,6 +22,10 @@ Modules mirror the reference's:
   damage      -- ``engraft.damage``           vectorized ngram_rows / scan_hits
   overlay_sum -- ``engraft.replica.overlay_sum`` the overlay merge
   ple         -- ``engraft.replica.layers``   ple_forward / PleWeights, ``engraft.lens`` PleReplica
+
+Beside the path, without a counterpart in the reference:
+  losses      -- log-probabilities, policy and preference losses of next-token logits, with their gradient
+  muon        -- orthogonalised updates of the PLE block's projection weights
 """
 from . import _lib  # noqa: F401
 

@@ -18,6 +18,13 @@
 // zero.  A target beyond the vocabulary gives NaN (lp and gradient), never a
 // read out of range.
 //
+// Bound by HBM, 2,047 x 151,936 bf16 of which 30 % of the rows are left out: the statistics
+// read 435 MB in 80 us (5.4 TB/s; a large copy moves 6.5), the gradient pass reads them
+// again and writes 622 MB in 172 us (6.1 TB/s, the rows read last first, so that some are still
+// in the Infinity Cache: first to last 205 us).  The policy loss, whose g needs its own row
+// alone, does both in one workgroup a row and reads the logits once: 204 us for 1,057 MB.
+// A thread keeps four 16-byte loads in flight (up to 20 where the row is held); 8 to 18 made no difference.
+//
 // Sums are fp32 per thread and workgroup (a thread adds at most a few hundred terms),
 // sums over rows and sequences fp64; no floating atomics, so a call gives the same
 // bits every time.

@@ -4,6 +4,7 @@
 // step of 16 matrices) of interpreter time, more than the kernels of a small one.
 // Host code only, in the autograd module; the entry points are the library's own,
 // handed over as addresses.
+#include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -147,6 +148,7 @@ const float* values(const Tensor& t) { return (const float*)t.data_ptr(); }
 
 Tensor token_logprobs(const Tensor& logits, const Tensor& targets, double temperature, int64_t stream) {
   const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(logits.is_cuda() ? std::optional<c10::Device>(logits.device()) : std::nullopt);
   const Logits l = make_logits(logits, targets, temperature);
   Tensor lp = empty_floats(l.c.n, logits);
   const Scratch s = make_scratch(l, 0, false, logits);
@@ -161,6 +163,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, MaybeTensor> policy(const Ten
                                           double temperature, int64_t reduction, bool grad,
                                           const MaybeTensor& out, double grad_scale, int64_t stream) {
   const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(logits.is_cuda() ? std::optional<c10::Device>(logits.device()) : std::nullopt);
   const Logits l = make_logits(logits, targets, temperature);
   const int64_t n = l.c.n;
   const auto dev = logits.device();
@@ -194,6 +197,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, MaybeTensor> preference(const
                                               const Tensor& ref_lp, double beta, double smoothing, double temperature,
                                               bool grad, const MaybeTensor& out, double grad_scale, int64_t stream) {
   const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(logits.is_cuda() ? std::optional<c10::Device>(logits.device()) : std::nullopt);
   const Logits l = make_logits(logits, targets, temperature);
   const int64_t n = l.c.n;
   const auto dev = logits.device();
@@ -217,6 +221,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, MaybeTensor> preference(const
 Tensor logits_grad(const Tensor& logits, const Tensor& targets, double temperature, const Tensor& state,
                    const Tensor& upstream, int64_t stream) {
   const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(logits.is_cuda() ? std::optional<c10::Device>(logits.device()) : std::nullopt);
   const Tensor d = gradient(logits, true, std::nullopt);
   const Logits l = make_logits(logits, targets, temperature);
   const Tensor up = upstream.to(torch::kFloat32);
@@ -246,6 +251,7 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
           const std::vector<float>& coefficients, int64_t steps, int64_t planes, bool nesterov, double momentum,
           double eps, double keep, double lr, bool update, int64_t stream) {
   const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(!params.empty() && params[0].is_cuda() ? std::optional<c10::Device>(params[0].device()) : std::nullopt);
   if (params.size() != grads.size() || (update && params.size() != momenta.size()))
     refuse(params.size(), " params, ", grads.size(), " grads and ", momenta.size(), " momenta");
   // matrices of one shape, types and strides share their launches
@@ -287,7 +293,8 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
     std::tie(o.rows, o.cols, o.param_dtype, o.grad_dtype, strides[0][0], strides[0][1], strides[1][0], strides[1][1],
              strides[2][0], strides[2][1]) = key;
     o.count = (int32_t)group.params.size();
-    o.planes = planes != 0 ? (int32_t)planes : o.param_dtype == EG_DTYPE_F32 ? 2 : 1;
+    // one plane's update is 2^-9 of itself off: less than a bf16 weight's rounding, more than an f16 one's
+    o.planes = planes != 0 ? (int32_t)planes : o.param_dtype == EG_DTYPE_BF16 ? 1 : 2;
     o.params = group.params.data();
     o.grads = group.grads.data();
     o.momenta = update ? group.momenta.data() : nullptr;

@@ -15,9 +15,10 @@ on the fp16 matrix cores), then a step:
 * ``MuonState``     -- the same with the momenta kept;
 * ``orthogonalize`` -- X alone.
 
-Products: fp32 weights take fp32 accuracy (operands as two fp16 planes, 22 bits,
-three products), bf16 and f16 weights one product of 11-bit operands, whose
-error stays below the weight's own rounding; ``products`` overrides."""
+Products: f32 and f16 weights take fp32 accuracy (operands as two fp16 planes, 22
+bits, three products), bf16 weights one product of 11-bit operands, whose update is
+off by about 2^-9 of itself, below the weight's own rounding; ``products``
+("fp16x3", "fp16") overrides."""
 from __future__ import annotations
 
 import torch

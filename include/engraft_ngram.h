@@ -39,6 +39,10 @@
  *   eg_split_bf16x6, eg_gemm_bf16x6, eg_split_f16, eg_gemm_f16x3
  *                    ple_forward's projections and their backward
  *                                                    engraft/replica/layers.py:594-606
+ *
+ * Without a counterpart there (what a training step needs beside the path):
+ *   eg_token_logprobs, eg_policy_loss, eg_preference_loss, eg_logits_grad
+ *   eg_muon_step
  */
 #ifndef ENGRAFT_NGRAM_H
 #define ENGRAFT_NGRAM_H

@@ -12,6 +12,17 @@ from tests.conftest import ROOT
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(scope="module", autouse=True)
+def memory_returned():
+    """What torch's allocator keeps of these tests' tensors goes back: other tests read its statistics."""
+    yield
+    import gc
+
+    import torch
+    gc.collect()
+    torch.cuda.empty_cache()
+
+
 def test_example_trains(cuda):
     spec = importlib.util.spec_from_file_location("answer_descent", ROOT / "examples" / "answer_descent.py")
     example = importlib.util.module_from_spec(spec)

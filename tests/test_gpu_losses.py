@@ -19,6 +19,17 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(scope="module", autouse=True)
+def memory_returned():
+    """What torch's allocator keeps of these tests' tensors goes back: other tests read its statistics."""
+    yield
+    import gc
+
+    import torch
+    gc.collect()
+    torch.cuda.empty_cache()
+
 EPS = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 TINY = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -24}
 ALL = [torch.float32, torch.bfloat16, torch.float16]

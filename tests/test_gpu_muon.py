@@ -18,6 +18,17 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(scope="module", autouse=True)
+def memory_returned():
+    """What torch's allocator keeps of these tests' tensors goes back: other tests read its statistics."""
+    yield
+    import gc
+
+    import torch
+    gc.collect()
+    torch.cuda.empty_cache()
+
 ROUNDING = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}  # half a unit in the last place
 QUINTIC = (3.4445, -4.7750, 2.0315)
 SHAPES = [(1, 1), (1, 40), (40, 1), (2, 3), (31, 33), (64, 64), (65, 130), (130, 65), (128, 640), (257, 200),
@@ -244,3 +255,17 @@ def test_block_sees_the_step(cuda):
     assert torch.equal(after, ple.ple_forward(emb, hidden, fresh, hist, hp)[0]) and not torch.equal(after, before)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         before.square().sum().backward()
+
+
+def test_products_by_type(cuda):
+    """Without `products`: f32 and f16 weights take three products, bf16 weights one; an f16 weight's update
+    is then off by its own rounding alone."""
+    from engraft_ngram_amd import muon
+    for dtype, products in ((torch.float32, "fp16x3"), (torch.float16, "fp16x3"), (torch.bfloat16, "fp16")):
+        x = random((200, 300), dtype, 6)
+        assert torch.equal(muon.orthogonalize(x), muon.orthogonalize(x, products=products))
+    w, g = random((90, 90), torch.float16, 7, 0.02), random((90, 90), torch.float32, 8)
+    new = w.clone()
+    muon.muon_step([new], [g], [torch.zeros_like(g)], lr=0.2)
+    want = w.double() - 0.2 * plain(1.95 * g)
+    assert ((new.double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -24 + 0.2 * 64 * 2.0 ** -23).all()
