@@ -332,3 +332,42 @@ def test_in_a_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(res.loss, want.loss) and torch.equal(d, dw) and torch.equal(res.logprobs, want.logprobs)
+
+
+@pytest.mark.parametrize("n,v", [(12, 700), (40, 151_936), (600, 3001)])
+def test_preference_in_place(cuda, n, v):
+    """The gradient over the logits: the bits of the gradient beside them, in parts and whole rows."""
+    from engraft_ngram_amd import losses
+    z, t = make(n, v, torch.bfloat16, n)
+    seg = torch.arange(n, device="cuda") * 4 // n
+    ref = torch.zeros(4, device="cuda")
+    res, d = losses.preference_loss_grad(z, t, seg, ref)
+    version = z._version
+    res2, d2 = losses.preference_loss_grad(z, t, seg, ref, out=z)
+    assert d2 is z and torch.equal(d2, d) and torch.equal(res2.loss, res.loss) and z._version > version
+
+
+def test_offsets_past_32_bits(cuda):
+    """More than 2^31 logits: the last rows as on their own, in every kernel that many rows take."""
+    from engraft_ngram_amd import losses
+    n, v, tail = 14_200, 151_936, 40
+    assert (n - tail) * v > 2 ** 31
+    z = torch.zeros((n, v), dtype=torch.bfloat16, device="cuda")
+    t = torch.full((n,), -100, device="cuda")
+    z[-tail:], t[-tail:] = make(tail, v, torch.bfloat16, 3)
+    a = torch.randn(n, device="cuda")
+    lp = losses.token_logprobs(z, t)
+    want = losses.token_logprobs(z[-tail:].contiguous(), t[-tail:])
+    assert_within(lp[-tail:], want.double(), 2.0 ** -20)
+    assert (lp[:-tail] == 0).all()
+    d = torch.full_like(z, 7.0)
+    res, _ = losses.policy_loss_grad(z, t, a, reduction="sum", out=d)
+    few, d_few = losses.policy_loss_grad(z[-tail:].contiguous(), t[-tail:], a[-tail:], reduction="sum")
+    # the two take their rows' sums in other orders: fp32's rounding of p, then bf16's
+    assert_within(d[-tail:], d_few.double(), 2.0 ** -7 * d_few.double().abs() + 2.0 ** -60)
+    assert (d[:-tail] == 0).all()
+    d.fill_(7.0)
+    seg = torch.zeros(n, dtype=torch.int64, device="cuda")
+    seg[-tail // 2:] = 1
+    losses.preference_loss_grad(z, t, seg, torch.zeros(2, device="cuda"), out=d)
+    assert (d[:-tail] == 0).all() and (d[-tail:][t[-tail:] >= 0].abs().sum(1) > 0).all()
