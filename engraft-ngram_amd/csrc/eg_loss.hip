@@ -11,7 +11,8 @@
 // maximum and sum of each thread joined in a fixed order), a kernel of one
 // workgroup turns them into the rows' lp, the loss and every row's g
 // (logprobs_finish, policy_finish, preference_finish), and a second pass reads the
-// logits and writes d (logits_grad_kernel).  The differences z - M are taken
+// logits and writes d (logits_grad_kernel; policy_few_kernel and preference_few_kernel
+// do the last two in one launch).  The differences z - M are taken
 // before the multiplication by c, so a row of the type's lowest value gives a
 // uniform softmax and -inf gives exact zeros.  A row whose target is negative is left
 // out: its logits are not read (NaN there is harmless), its lp is 0 and its gradient
@@ -277,11 +278,6 @@ __device__ inline int64_t segment_of(const Segments& s, int64_t i) {
   return s.ids32 ? (int64_t)((const int32_t*)s.ids)[i] : ((const int64_t*)s.ids)[i];
 }
 
-// What the gradient pass needs of a row: g (dL / d lp), M and 1 / S.
-struct RowState {
-  float g, m, inv_s;
-};
-
 // Elements [e0, e1) of a row that is left out.
 template <typename T, int THREADS>
 __device__ inline void write_zeros(T* out, int e0, int e1) {
@@ -292,38 +288,49 @@ __device__ inline void write_zeros(T* out, int e0, int e1) {
   for (; e < e1; ++e) out[e] = (T)0.0f;
 }
 
+// What the gradient pass needs of a row: g (dL / d lp), M and 1 / S.
+struct RowState {
+  float g, m, inv_s;
+};
+
 // Elements [e0, e1) of g ([j == t] - 2^(c (z_j - m)) inv_s); f_t is z_t, read before anything
-// is written (out may be the row itself).
-template <typename T, int THREADS>
-__device__ inline void write_gradient(const T* row, T* out, int e0, int e1, int64_t t, float f_t, float g, float m,
-                                      float inv_s, float c) {
-  constexpr int VEC = Logit<T>::kVec, K = 4;
-  const float k = -g * inv_s;
-  auto value = [&](float f) { return k * pow2((f - m) * c); };
+// is written (out may be the row itself).  The row's state is asked for once the first loads are on
+// their way (by every thread: it may synchronise).
+template <typename T, int THREADS, typename State>
+__device__ inline void write_gradient(const T* row, T* out, int e0, int e1, int64_t t, float f_t, float c, State&& state) {
+  constexpr int VEC = Logit<T>::kVec, K = 4, NEXT = THREADS * VEC;
   int e = e0 + (int)threadIdx.x * VEC;
-  for (; e + (K - 1) * THREADS * VEC + VEC <= e1; e += K * THREADS * VEC) {
-    Chunk q[K];
+  Chunk q[K];
+  auto load = [&] {
 #pragma unroll
-    for (int j = 0; j < K; ++j) q[j] = *(const Chunk*)(row + e + j * THREADS * VEC);
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-      float f[VEC];
-      Logit<T>::unpack(q[j], f);
-#pragma unroll
-      for (int x = 0; x < VEC; ++x) f[x] = value(f[x]);
-      stream_out(out + e + j * THREADS * VEC, Logit<T>::pack(f));
-    }
-  }
-  for (; e + VEC <= e1; e += THREADS * VEC) {
+    for (int j = 0; j < K; ++j)
+      if (e + j * NEXT + VEC <= e1) q[j] = *(const Chunk*)(row + e + j * NEXT);
+  };
+  load();
+  const RowState st = state();
+  const float m = st.m, k = -st.g * st.inv_s;
+  auto value = [&](float f) { return k * pow2((f - m) * c); };
+  auto store = [&](int at, const Chunk& chunk) {
     float f[VEC];
-    Logit<T>::unpack(*(const Chunk*)(row + e), f);
+    Logit<T>::unpack(chunk, f);
 #pragma unroll
     for (int x = 0; x < VEC; ++x) f[x] = value(f[x]);
-    stream_out(out + e, Logit<T>::pack(f));
+    stream_out(out + at, Logit<T>::pack(f));
+  };
+  for (; e + (K - 1) * NEXT + VEC <= e1; load()) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) store(e + j * NEXT, q[j]);
+    e += K * NEXT;
   }
-  for (; e < e1; ++e) out[e] = (T)value((float)row[e]);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j)
+    if (e + j * NEXT + VEC <= e1) store(e + j * NEXT, q[j]);
+  // the row's incomplete chunk, by the thread whose turn it is
+  const int whole = e0 + (e1 - e0) / VEC * VEC;
+  if ((whole - e0) / VEC % THREADS == (int)threadIdx.x)
+    for (int x = whole; x < e1; ++x) out[x] = (T)value((float)row[x]);
   // the target's element again, by the thread that wrote it
-  if (t >= e0 && t < e1 && (int)((t - e0) / VEC) % THREADS == (int)threadIdx.x) out[t] = (T)(g + value(f_t));
+  if (t >= e0 && t < e1 && (int)((t - e0) / VEC) % THREADS == (int)threadIdx.x) out[t] = (T)(st.g + value(f_t));
 }
 
 // Grid (parts, rows): a part of a row's gradient; scale holds 1 / temperature.  g is the state's, or
@@ -345,19 +352,22 @@ __global__ __launch_bounds__(THREADS) void logits_grad_kernel(const Rows r, int 
   }
   const T* row = (const T*)r.z + i * r.stride;
   const float f_t = t >= e0 && t < e1 ? (float)row[t] : 0.0f;
-  RowState st = state[i];
-  if (d_seq != nullptr) {
-    const int64_t s = segment_of(seg, i);
-    st.g = s >= 0 && s < seg.n ? d_seq[s] : 0.0f;
-  }
-  const float g = st.g * (upstream != nullptr ? scale * *upstream : scale);
   if (row == out) __syncthreads();  // everyone has read f_t
-  write_gradient<T, THREADS>(row, out, e0, e1, t, f_t, g, st.m, st.inv_s, r.c);
+  write_gradient<T, THREADS>(row, out, e0, e1, t, f_t, r.c, [&] {
+    RowState st = state[i];
+    if (d_seq != nullptr) {
+      const int64_t s = segment_of(seg, i);
+      st.g = s >= 0 && s < seg.n ? d_seq[s] : 0.0f;
+    }
+    st.g *= upstream != nullptr ? scale * *upstream : scale;
+    return st;
+  });
 }
 
 // ---- one workgroup over all rows ------------------------------------------------------------
 
 constexpr int kFinish = 1024;
+constexpr int64_t kFewRows = 256, kFewSegments = 2048;  // of the few-row kernels: a row a thread, segments in LDS
 
 template <int THREADS>
 __device__ inline double block_sum64(double x, double* red) {
@@ -434,8 +444,9 @@ __device__ inline float policy_g(const Policy& p, const PolicyRow& q, float w) {
   return w * g;
 }
 
-// One workgroup of kFinish threads: the weight of a row with a target, weights[segment] by
-// segment, otherwise weights[0].  Counts are kept in the same place.
+// One workgroup: the weight of a row with a target, weights[segment] by segment, otherwise
+// weights[0].  Counts are kept in the same place.
+template <int THREADS>
 __device__ inline void policy_weights(const Rows& r, const Policy& p, float* weights) {
   __shared__ int total;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -443,14 +454,14 @@ __device__ inline void policy_weights(const Rows& r, const Policy& p, float* wei
   const bool by_segment = p.reduction == EG_REDUCE_SEQUENCE;
   if (tid == 0) total = 0;
   if (by_segment)
-    for (int64_t s = tid; s < p.seg.n; s += kFinish) counts[s] = 0;
+    for (int64_t s = tid; s < p.seg.n; s += THREADS) counts[s] = 0;
   __syncthreads();
   int some = 0;
   if (p.reduction == EG_REDUCE_TOKEN)
 #pragma unroll 4
-    for (int64_t i = tid; i < r.n; i += kFinish) some += target_of(r, i) >= 0;
+    for (int64_t i = tid; i < r.n; i += THREADS) some += target_of(r, i) >= 0;
   if (by_segment)
-    for (int64_t i = tid; i < r.n; i += kFinish) {
+    for (int64_t i = tid; i < r.n; i += THREADS) {
       const bool in = target_of(r, i) >= 0;
       const int64_t s = segment_of(p.seg, i);
       // one addition for the rows of a wavefront that share a segment
@@ -464,7 +475,7 @@ __device__ inline void policy_weights(const Rows& r, const Policy& p, float* wei
     }
   __syncthreads();
   if (by_segment)
-    for (int64_t s = tid; s < p.seg.n; s += kFinish) some += __hip_atomic_load(counts + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) > 0;
+    for (int64_t s = tid; s < p.seg.n; s += THREADS) some += __hip_atomic_load(counts + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) > 0;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) some += __shfl_xor(some, o);
   if (lane == 0) atomicAdd(&total, some);
@@ -473,7 +484,7 @@ __device__ inline void policy_weights(const Rows& r, const Policy& p, float* wei
   if (!by_segment) {
     if (tid == 0) weights[0] = (float)all;
   } else {
-    for (int64_t s = tid; s < p.seg.n; s += kFinish) {
+    for (int64_t s = tid; s < p.seg.n; s += THREADS) {
       const int c = __hip_atomic_load(counts + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       weights[s] = (float)(all / (double)max(c, 1));
     }
@@ -508,35 +519,74 @@ __device__ inline void policy_rows(const Rows& r, const Policy& p, int64_t i0, i
         sum[0] += (double)w * ((double)(q.free <= q.held ? -q.free : -q.held) + (p.ref_lp != nullptr ? (double)p.kl_coef * kl : 0.0));
         sum[1] += (double)w * kl;
         sum[2] += q.free > q.held ? (double)w : 0.0;
-        if (!DONE) st.g = policy_g(p, q, w);
+        if (!DONE && state != nullptr) st.g = policy_g(p, q, w);
       }
     }
     lp_out[i] = (float)lp;
-    if (!DONE) state[i] = st;
+    if (!DONE && state != nullptr) state[i] = st;
   }
 }
 
-// One workgroup over all rows: weights, lp, state; sums[3] = loss, KL, clipped share.
+// One workgroup over all rows: weights, lp, state (where kept); sums[3] = loss, KL, clipped share.
+template <typename T, int THREADS>
+__device__ inline void policy_all(const Rows& r, const Policy& p, int parts, const Stat* stats, float* weights,
+                                  float* lp_out, RowState* state, float* sums) {
+  __shared__ double red[THREADS / 64];
+  policy_weights<THREADS>(r, p, weights);
+  __syncthreads();
+  double sum[3] = {0.0, 0.0, 0.0};
+  policy_rows<T, THREADS, false>(r, p, 0, r.n, parts, stats, weights, lp_out, state, sum);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const double x = block_sum64<THREADS>(sum[k], red);
+    if (threadIdx.x == 0) sums[k] = (float)x;
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kFinish) void policy_finish(const Rows r, const Policy p, int parts, const Stat* stats,
                                                          float* weights, float* lp_out, RowState* state, float* sums) {
-  __shared__ double red[kFinish / 64];
-  policy_weights(r, p, weights);
-  __syncthreads();
-  double sum[3] = {0.0, 0.0, 0.0};
-  policy_rows<T, kFinish, false>(r, p, 0, r.n, parts, stats, weights, lp_out, state, sum);
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    const double x = block_sum64<kFinish>(sum[k], red);
-    if (threadIdx.x == 0) sums[k] = (float)x;
+  policy_all<T, kFinish>(r, p, parts, stats, weights, lp_out, state, sums);
+}
+
+// Few rows in parts: every workgroup of the gradient finds its row's weight and g for itself, while
+// its logits are on their way, and one more does what policy_finish does: two launches for three
+// (bf16 rows of 151936 logits: 4 rows 11.2 us for 13.7, 90 rows 22.1 for 25.3, 250 rows 40.6 for 45.7).  Grid (parts, rows + 1); the gradient is not in the logits' place.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void policy_few_kernel(const Rows r, const Policy p, int parts, int part_len,
+                                                             const Stat* stats, float* lp_out, float* sums, float scale,
+                                                             T* d, int64_t d_stride) {
+  __shared__ float weights[kFewSegments];
+  const int64_t i = (int64_t)blockIdx.y - 1;
+  if (i < 0) {
+    if (blockIdx.x == 0) policy_all<T, THREADS>(r, p, parts, stats, weights, lp_out, nullptr, sums);
+    return;
   }
+  int e0, e1;
+  part_range(r.v, parts, part_len, (int)blockIdx.x, e0, e1);
+  const int64_t t = target_of(r, i);
+  T* out = d + i * d_stride;
+  if (t < 0) {
+    write_zeros<T, THREADS>(out, e0, e1);
+    return;
+  }
+  const T* row = (const T*)r.z + i * r.stride;
+  const float f_t = t < r.v ? (float)row[t] : __builtin_nanf("");
+  write_gradient<T, THREADS>(row, out, e0, e1, t, f_t, r.c, [&] {
+    const Stat st = row_stat(stats, i, parts, r.c);
+    const PolicyRow terms = policy_row(p, i, logprob_of(r, f_t - st.m, st.s));
+    policy_weights<THREADS>(r, p, weights);
+    __syncthreads();
+    const float w = weight_of(p, i, weights);
+    return RowState{(w != 0.0f ? policy_g(p, terms, w) : 0.0f) * scale, st.m, 1.0f / st.s};
+  });
 }
 
 // Many rows: the weights first,
 __global__ __launch_bounds__(kFinish) void policy_weights_kernel(const Rows r, const Policy p, float* weights,
                                                                  int* finished) {
   if (threadIdx.x == 0) *finished = 0;
-  policy_weights(r, p, weights);
+  policy_weights<kFinish>(r, p, weights);
 }
 
 // then a workgroup a row, its statistics and its gradient: the second reading of the row (300 KB
@@ -564,7 +614,7 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const Rows r, const
   }
   const float w = weight_of(p, i, weights);
   const float g = w != 0.0f ? policy_g(p, policy_row(p, i, logprob_of(r, f_t - st.m, st.s)), w) : 0.0f;
-  write_gradient<T, THREADS>(row, out, 0, r.v, t, f_t, g * scale, st.m, 1.0f / st.s, r.c);
+  write_gradient<T, THREADS>(row, out, 0, r.v, t, f_t, r.c, [&] { return RowState{g * scale, st.m, 1.0f / st.s}; });
 }
 
 // or, of longer rows, with the first NV chunks a thread held in registers from the one to the other
@@ -642,7 +692,7 @@ __global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const P
   if (has_tail)
     for (int e = whole; e < r.v; ++e) out[e] = (T)value((float)row[e]);
   if (t < NV * STRIDE && t < r.v && (int)(t / VEC) % THREADS == (int)threadIdx.x) out[t] = (T)(g + value(f_t));
-  if (NV * STRIDE < r.v) write_gradient<T, THREADS>(row, out, NV * STRIDE, r.v, t, f_t, g, m, inv_s, c);
+  if (NV * STRIDE < r.v) write_gradient<T, THREADS>(row, out, NV * STRIDE, r.v, t, f_t, c, [&] { return RowState{g, m, inv_s}; });
 }
 
 // and the rows' terms, 256 rows a workgroup; the last workgroup to finish adds the workgroups' sums,
@@ -685,25 +735,53 @@ struct Preference {
   float beta, smoothing;
 };
 
-// One workgroup: lp, the sequences' sums, margins, loss and state.  starts [2 pairs + 1],
-// d_seq and seq_sum [2 pairs] and lp64 [n] are scratch.
-template <typename T>
-__global__ __launch_bounds__(kFinish) void preference_finish(const Rows r, const Preference p, int parts,
-                                                             const Stat* stats, int64_t* starts, float* d_seq,
-                                                             double* seq_sum, double* lp64, float* lp_out, float* seq_out,
-                                                             float* margins, RowState* state, float* loss_out,
-                                                             bool has_lp, bool has_grad) {
-  __shared__ double red[kFinish / 64];
+__device__ inline int64_t held_segment(const Preference& p, int64_t i) {
+  const int64_t s = segment_of(p.seg, i);
+  return s < 0 ? (int64_t)-1 : s > p.seg.n ? p.seg.n : s;
+}
+
+// A wavefront: the sum of rows [start, end) of lp.
+__device__ inline double sequence_sum(const double* lp, int64_t start, int64_t end) {
+  double sum = 0.0;
+  for (int64_t i = start + (threadIdx.x & 63); i < end; i += 64) sum += lp[i];
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+  return sum;
+}
+
+struct Pair {
+  double h, loss;
+  float g;  // dL / d the chosen answer's sum; the rejected one's is -g
+};
+
+__device__ inline Pair pair_of(const Preference& p, int64_t q, double chosen, double rejected, bool unordered) {
+  // segments out of order have no sums: NaN
+  const double h = unordered ? __builtin_nan("") : (double)p.beta * ((chosen - (double)p.ref_lp[2 * q]) -
+                                                                    (rejected - (double)p.ref_lp[2 * q + 1]));
+  const double e = exp(-fabs(h)), tail = log1p(e);  // -log sigma(h) = tail + max(-h, 0)
+  const double small = e / (1.0 + e), large = 1.0 / (1.0 + e);
+  const double up = h >= 0.0 ? large : small, down = h >= 0.0 ? small : large;  // sigma(h), sigma(-h)
+  const double eps = (double)p.smoothing;
+  return {h, (tail + (1.0 - eps) * fmax(-h, 0.0) + eps * fmax(h, 0.0)) + (h != h ? h : 0.0),
+          (float)((double)p.beta * (eps * up - (1.0 - eps) * down) / (double)(p.seg.n / 2))};
+}
+
+// One workgroup: lp, the sequences' sums, margins, loss and state (where kept).  starts [2 pairs + 1],
+// d_seq and seq_sum [2 pairs] and lp64 [n] (given with has_lp) are scratch.
+template <typename T, int THREADS>
+__device__ inline void preference_all(const Rows& r, const Preference& p, int parts, const Stat* stats, int64_t* starts,
+                                      float* d_seq, double* seq_sum, double* lp64, float* lp_out, float* seq_out,
+                                      float* margins, RowState* state, float* loss_out, bool has_lp, bool has_grad) {
+  __shared__ double red[THREADS / 64];
   __shared__ int unordered;
   const int tid = threadIdx.x;
   const int64_t count = p.seg.n, pairs = count / 2;
   if (tid == 0) unordered = 0;
   __syncthreads();
-  auto held = [&](int64_t s) { return s < 0 ? (int64_t)-1 : s > count ? count : s; };
-  for (int64_t i = tid; i < r.n; i += kFinish) {
+  for (int64_t i = tid; i < r.n; i += THREADS) {
     const int64_t t = target_of(r, i);
     // starts[s]: the first row of segment s or a later one
-    const int64_t s = held(segment_of(p.seg, i)), before = i > 0 ? held(segment_of(p.seg, i - 1)) : -1;
+    const int64_t s = held_segment(p, i), before = i > 0 ? held_segment(p, i - 1) : -1;
     for (int64_t q = before + 1; q <= s; ++q) starts[q] = i;
     if (before > s) unordered = 1;
     if (i == r.n - 1)
@@ -717,16 +795,13 @@ __global__ __launch_bounds__(kFinish) void preference_finish(const Rows r, const
     }
     lp64[i] = lp;
     lp_out[i] = (float)lp;
-    state[i] = st;
+    if (state != nullptr) state[i] = st;
   }
   if (r.n == 0)
-    for (int64_t q = tid; q <= count; q += kFinish) starts[q] = 0;
+    for (int64_t q = tid; q <= count; q += THREADS) starts[q] = 0;
   __syncthreads();
-  for (int64_t s = tid >> 6; s < count; s += kFinish / 64) {
-    double sum = 0.0;
-    for (int64_t i = starts[s] + (tid & 63); i < starts[s + 1]; i += 64) sum += lp64[i];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+  for (int64_t s = tid >> 6; s < count; s += THREADS / 64) {
+    const double sum = sequence_sum(lp64, starts[s], starts[s + 1]);
     if ((tid & 63) == 0) {
       seq_sum[s] = sum;
       seq_out[s] = (float)sum;
@@ -734,28 +809,97 @@ __global__ __launch_bounds__(kFinish) void preference_finish(const Rows r, const
   }
   __syncthreads();
   double loss = 0.0;
-  for (int64_t q = tid; q < pairs; q += kFinish) {
-    // segments out of order have no sums: NaN
-    const double h = unordered ? __builtin_nan("") : (double)p.beta * ((seq_sum[2 * q] - (double)p.ref_lp[2 * q]) -
-                                                                    (seq_sum[2 * q + 1] - (double)p.ref_lp[2 * q + 1]));
-    const double e = exp(-fabs(h)), tail = log1p(e);  // -log sigma(h) = tail + max(-h, 0)
-    const double small = e / (1.0 + e), large = 1.0 / (1.0 + e);
-    const double up = h >= 0.0 ? large : small, down = h >= 0.0 ? small : large;  // sigma(h), sigma(-h)
-    const double eps = (double)p.smoothing;
-    loss += (tail + (1.0 - eps) * fmax(-h, 0.0) + eps * fmax(h, 0.0)) + (h != h ? h : 0.0);
-    const float g = (float)((double)p.beta * (eps * up - (1.0 - eps) * down) / (double)pairs);
-    d_seq[2 * q] = g;
-    d_seq[2 * q + 1] = -g;
-    margins[q] = (float)h;
+  for (int64_t q = tid; q < pairs; q += THREADS) {
+    const Pair x = pair_of(p, q, seq_sum[2 * q], seq_sum[2 * q + 1], unordered);
+    loss += x.loss;
+    d_seq[2 * q] = x.g;
+    d_seq[2 * q + 1] = -x.g;
+    margins[q] = (float)x.h;
   }
-  loss = block_sum64<kFinish>(loss, red);
+  loss = block_sum64<THREADS>(loss, red);
   if (tid == 0) loss_out[0] = (float)(loss / (double)max(pairs, (int64_t)1));
-  if (has_grad) return;  // the gradient kernel takes d_seq
+  if (has_grad) return;  // the gradient kernel finds g itself
   __syncthreads();
-  for (int64_t i = tid; i < r.n; i += kFinish) {
+  for (int64_t i = tid; i < r.n; i += THREADS) {
     const int64_t s = segment_of(p.seg, i);
     if (s >= 0 && s < count && target_of(r, i) >= 0) state[i].g = d_seq[s];
   }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kFinish) void preference_finish(const Rows r, const Preference p, int parts,
+                                                             const Stat* stats, int64_t* starts, float* d_seq,
+                                                             double* seq_sum, double* lp64, float* lp_out, float* seq_out,
+                                                             float* margins, RowState* state, float* loss_out,
+                                                             bool has_lp, bool has_grad) {
+  preference_all<T, kFinish>(r, p, parts, stats, starts, d_seq, seq_sum, lp64, lp_out, seq_out, margins, state, loss_out,
+                             has_lp, has_grad);
+}
+
+// Few rows in parts (at most kFewRows): as policy_few_kernel; a workgroup sums its row's pair itself
+// (4 rows 11.8 us for 14.6, 90 rows 21.2 for 24.6, 250 rows 40.9 for 45.5).  Held to 64 registers, two
+// workgroups of 1024 to a CU, it spills 16 in the pair's arithmetic; with the 83 it asks for, one to a
+// CU, 37 rows of f32 take 23.4 us for 19.1 and the three launches 21.3.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS, 8) void preference_few_kernel(const Rows r, const Preference p, int parts,
+                                                                 int part_len, const Stat* stats, int64_t* starts,
+                                                                 float* d_seq, double* seq_sum, double* lp64,
+                                                                 float* lp_out, float* seq_out, float* margins,
+                                                                 float* loss_out, float scale, T* d, int64_t d_stride) {
+  static_assert(THREADS >= kFewRows, "a row a thread");
+  __shared__ double lps[kFewRows], sums[2];
+  __shared__ int64_t bounds[3];
+  __shared__ int unordered;
+  const int64_t i = (int64_t)blockIdx.y - 1;
+  if (i < 0) {
+    if (blockIdx.x == 0)
+      preference_all<T, THREADS>(r, p, parts, stats, starts, d_seq, seq_sum, lp64, lp_out, seq_out, margins, nullptr,
+                                 loss_out, false, true);
+    return;
+  }
+  int e0, e1;
+  part_range(r.v, parts, part_len, (int)blockIdx.x, e0, e1);
+  const int64_t t = target_of(r, i);
+  T* out = d + i * d_stride;
+  if (t < 0) {
+    write_zeros<T, THREADS>(out, e0, e1);
+    return;
+  }
+  const T* row = (const T*)r.z + i * r.stride;
+  const float f_t = t < r.v ? (float)row[t] : __builtin_nanf("");
+  write_gradient<T, THREADS>(row, out, e0, e1, t, f_t, r.c, [&] {
+    const Stat st = row_stat(stats, i, parts, r.c);
+    const int64_t mine = segment_of(p.seg, i), first = mine & ~(int64_t)1;
+    if (threadIdx.x == 0) unordered = 0;
+    __syncthreads();
+    const int64_t j = threadIdx.x;
+    if (j < r.n) {
+      const int64_t s = held_segment(p, j), before = j > 0 ? held_segment(p, j - 1) : -1;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        if (before < first + q && first + q <= s) bounds[q] = j;
+        if (j == r.n - 1 && s < first + q) bounds[q] = r.n;
+      }
+      if (before > s) unordered = 1;
+      const int64_t tj = target_of(r, j);
+      double lp = 0.0;
+      if (tj >= 0 && s >= first && s <= first + 1) {
+        const Stat sj = row_stat(stats, j, parts, r.c);
+        lp = logprob_of(r, z_below_m<T>(r, j, tj, sj.m), sj.s);
+      }
+      lps[j] = lp;
+    }
+    __syncthreads();
+    const bool in = mine >= 0 && mine < p.seg.n;
+    if (in && threadIdx.x < 128) {
+      const int w = threadIdx.x >> 6;
+      const double sum = sequence_sum(lps, bounds[w], bounds[w + 1]);
+      if ((threadIdx.x & 63) == 0) sums[w] = sum;
+    }
+    __syncthreads();
+    const float g = in ? pair_of(p, first / 2, sums[0], sums[1], unordered).g : 0.0f;
+    return RowState{(mine & 1 ? -g : g) * scale, st.m, 1.0f / st.s};
+  });
 }
 
 // ---- host side --------------------------------------------------------------------------------
@@ -821,6 +965,12 @@ int64_t stats_bytes(int64_t n, const Cut& cut) { return (n * cut.parts * (int64_
 dim3 row_grid(const Cut& cut, int64_t n) {
   const int64_t y = std::min<int64_t>(n, 32768);
   return dim3((unsigned)cut.parts, (unsigned)y, (unsigned)((n + y - 1) / y));
+}
+
+// Whether the gradient's workgroups find what they need of the loss themselves: rows in parts, and the
+// gradient not in the logits' place (other rows' logits are read meanwhile).
+bool few_rows(const Rows& r, const Cut& cut, const void* d) {
+  return d != nullptr && d != r.z && r.n >= 1 && r.n <= kFewRows && cut.parts > 1;
 }
 
 template <typename F>
@@ -969,6 +1119,19 @@ int eg_policy_loss(const eg_logits* logits, const eg_policy* policy, float* logp
   } else if (int rc = launch_stats(r, logits->dtype, cut, stats, st); rc != EG_OK) {
     return rc;
   }
+  if (few_rows(r, cut, d_logits) && p.seg.n <= kFewSegments)
+    return by_dtype(logits->dtype, [&](auto zero) {
+      using T = decltype(zero);
+      const dim3 grid((unsigned)cut.parts, (unsigned)r.n + 1);
+      const float scale = grad_scale / logits->temperature;
+      if (cut.threads == 1024)
+        policy_few_kernel<T, 1024><<<grid, 1024, 0, st>>>(r, p, cut.parts, cut.part_len, stats, logprobs, sums, scale,
+                                                          (T*)d_logits, d_stride);
+      else
+        policy_few_kernel<T, 256><<<grid, 256, 0, st>>>(r, p, cut.parts, cut.part_len, stats, logprobs, sums, scale,
+                                                        (T*)d_logits, d_stride);
+      return launch_status("policy_few_kernel");
+    });
   const int rc = by_dtype(logits->dtype, [&](auto zero) {
     using T = decltype(zero);
     const dim3 grid((unsigned)((r.n + 255) / 256));
@@ -1019,6 +1182,21 @@ int eg_preference_loss(const eg_logits* logits, const eg_preference* preference,
   if (int rc = launch_stats(r, logits->dtype, cut, stats, (hipStream_t)stream, {nullptr, whole ? lp64 : nullptr});
       rc != EG_OK)
     return rc;
+  if (few_rows(r, cut, d_logits))
+    return by_dtype(logits->dtype, [&](auto zero) {
+      using T = decltype(zero);
+      const dim3 grid((unsigned)cut.parts, (unsigned)r.n + 1);
+      const float scale = grad_scale / logits->temperature;
+      if (cut.threads == 1024)
+        preference_few_kernel<T, 1024><<<grid, 1024, 0, (hipStream_t)stream>>>(
+            r, p, cut.parts, cut.part_len, stats, starts, d_seq, seq_sum, lp64, logprobs, sequence_logprobs, margins, loss,
+            scale, (T*)d_logits, d_stride);
+      else
+        preference_few_kernel<T, 256><<<grid, 256, 0, (hipStream_t)stream>>>(
+            r, p, cut.parts, cut.part_len, stats, starts, d_seq, seq_sum, lp64, logprobs, sequence_logprobs, margins, loss,
+            scale, (T*)d_logits, d_stride);
+      return launch_status("preference_few_kernel");
+    });
   int rc = by_dtype(logits->dtype, [&](auto zero) {
     using T = decltype(zero);
     preference_finish<T><<<1, kFinish, 0, (hipStream_t)stream>>>(r, p, cut.parts, stats, starts, d_seq, seq_sum,

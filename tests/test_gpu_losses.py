@@ -371,3 +371,35 @@ def test_offsets_past_32_bits(cuda):
     seg[-tail // 2:] = 1
     losses.preference_loss_grad(z, t, seg, torch.zeros(2, device="cuda"), out=d)
     assert (d[:-tail] == 0).all() and (d[-tail:][t[-tail:] >= 0].abs().sum(1) > 0).all()
+
+
+@pytest.mark.parametrize("n", [1, 2, 37, 256, 257])
+@pytest.mark.parametrize("dtype", ALL)
+def test_few_rows_against_in_place(cuda, n, dtype):
+    """Few long rows find what they need of the loss in the gradient's launch, unless the gradient replaces
+    the logits: the same bits either way, and autograd's."""
+    from engraft_ngram_amd import losses
+    v = 20_011
+    z, t = make(n, v, dtype, n)
+    gen = torch.Generator().manual_seed(n)
+    a, old, ref = (torch.randn(n, generator=gen).cuda() for _ in range(3))
+    seg = torch.arange(n, device="cuda") * 10 // n - 1  # -1 to 8, the last of no pair
+    unordered = seg.flip(0) if n > 2 else seg
+
+    def policy(z, count, **kw):
+        return losses.policy_loss_grad(z, t, a, old, ref_logprobs=ref, segment_ids=unordered, n_segments=count,
+                                       kl_coef=0.1, reduction="sequence", **kw)
+
+    def preference(z, ids, **kw):
+        return losses.preference_loss_grad(z, t, ids, torch.zeros(8, device="cuda"), **kw)
+
+    for f, arg in ((policy, 9), (policy, 3000), (preference, seg), (preference, unordered)):
+        res, d = f(z, arg)
+        same = z.clone()
+        res2, d2 = f(same, arg, out=same)
+        assert torch.equal(d.isnan(), d2.isnan()) and torch.equal(d.nan_to_num(), d2.nan_to_num())
+        for x, y in zip(vars(res).values(), vars(res2).values()):
+            assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(), y.nan_to_num())
+        if n > 2 and arg is unordered:
+            rows = (unordered >= 0) & (unordered < 8) & (t >= 0)
+            assert res.loss.isnan() and d[rows].isnan().all() and not d[~rows].any()
