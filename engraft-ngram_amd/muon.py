@@ -15,10 +15,11 @@ on the fp16 matrix cores), then a step:
 * ``MuonState``     -- the same with the momenta kept;
 * ``orthogonalize`` -- X alone.
 
-Products: f32 and f16 weights take fp32 accuracy (operands as two fp16 planes, 22
-bits, three products), bf16 weights one product of 11-bit operands, whose update is
-off by about 2^-9 of itself, below the weight's own rounding; ``products``
-("fp16x3", "fp16") overrides."""
+Products: a step takes fp32 accuracy whatever the weights' type (operands as two fp16
+planes, 22 bits, three products: ``products="fp16x3"``).  ``products="fp16"`` is one
+product of 11-bit operands, in half the time or less: X is then off by 1.1e-3 of itself,
+which moves some bf16 weights by one unit in the last place.  ``orthogonalize`` takes it
+by itself for a bf16 matrix, whose X is rounded to 8 bits in the end."""
 from __future__ import annotations
 
 import torch
@@ -53,7 +54,8 @@ def muon_step(params, grads, momenta, *, lr: float, weight_decay: float = 0.0, m
     ``[count, rows, cols]``, each matrix an update of its own), in place, with
     ``momenta`` (f32, the same shapes), in place, from ``grads``.  Any strides, one device;
     matrices of one shape, type and strides share their launches.  ``coefficients``:
-    one (a, b, c) for every Newton-Schulz step, or one each."""
+    one (a, b, c) for every Newton-Schulz step, or one each.  ``products``: "fp16x3" (None: the
+    same) or "fp16"."""
     _run(list(params), list(grads), list(momenta), steps, coefficients, products, nesterov, momentum, eps,
          1.0 - lr * weight_decay, lr, True)
 
@@ -61,7 +63,8 @@ def muon_step(params, grads, momenta, *, lr: float, weight_decay: float = 0.0, m
 def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC, eps: float = 1e-7,
                   out: torch.Tensor | None = None, products: str | None = None) -> torch.Tensor:
     """``x`` (f32, bf16 or f16 ``[rows, cols]`` or ``[count, rows, cols]``) with every matrix's
-    singular values driven to about 1, in ``x``'s type.  ``out``: where it is written (``x`` for in place)."""
+    singular values driven to about 1, in ``x``'s type.  ``out``: where it is written (``x`` for in place).
+    ``products`` None: "fp16" for bf16, "fp16x3" otherwise."""
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     _run([out], [x], [], steps, coefficients, products, False, 0.0, eps, 0.0, 0.0, False)
