@@ -303,6 +303,7 @@ SIGNATURES = {
                                      c_void_p, c_void_p, c_int64, ctypes.c_float, c_void_p, c_int64, c_void_p]),
     "eg_logits_grad": (c_int32, [POINTER(EgLogits), c_void_p, c_void_p, ctypes.c_float, c_void_p, c_int64, c_void_p]),
     "eg_muon_workspace_size": (c_int64, [c_int64, c_int64, c_int32, c_int32]),
+    "eg_muon_check": (c_int32, [POINTER(EgMuon)]),
     "eg_muon_step": (c_int32, [POINTER(EgMuon), c_void_p, c_int64, c_void_p]),
 }
 
@@ -363,7 +364,7 @@ def autograd_ext():
                for f in ("eg_gather_slots", "eg_scatter_grad_apply", "eg_last_error")))
     mod.init_ops({f: ctypes.cast(getattr(lib, f), c_void_p).value
                   for f in ("eg_loss_workspace_size", "eg_token_logprobs", "eg_policy_loss", "eg_preference_loss",
-                            "eg_logits_grad", "eg_muon_workspace_size", "eg_muon_step", "eg_last_error")}, EgError)
+                            "eg_logits_grad", "eg_muon_workspace_size", "eg_muon_check", "eg_muon_step", "eg_last_error")}, EgError)
     _EXT = mod
     return mod
 

@@ -1132,6 +1132,8 @@ int64_t eg_muon_workspace_size(int64_t rows, int64_t cols, int32_t count, int32_
   return make_layout(rows, cols, std::min(count, (int32_t)kMaxBatch), planes).total;
 }
 
+int eg_muon_check(const eg_muon* muon) { return check_muon(muon); }
+
 int eg_muon_step(const eg_muon* muon, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_muon(muon); rc != EG_OK) return rc;
   if (muon->count == 0) return EG_OK;

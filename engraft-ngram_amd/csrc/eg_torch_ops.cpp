@@ -31,6 +31,7 @@ struct Entry {
   decltype(&eg_preference_loss) preference = nullptr;
   decltype(&eg_logits_grad) logits_grad = nullptr;
   decltype(&eg_muon_workspace_size) muon_workspace = nullptr;
+  decltype(&eg_muon_check) muon_check = nullptr;
   decltype(&eg_muon_step) muon = nullptr;
   decltype(&eg_last_error) last_error = nullptr;
 };
@@ -245,7 +246,8 @@ void check_writable(const Tensor& t, const char* name) {
       refuse(name, " is written and must not be expanded, got strides ", t.strides());
 }
 
-// A momentum step of params (update), or the orthogonalised grads written to params (no momenta).
+// A momentum step of params (update), or the orthogonalised grads written to params (no momenta): of
+// all of them, or of none where one is refused or the workspace is not to be had.
 // planes 0: two, but for a bf16 X alone, which is rounded to 8 bits when it is written: one.
 void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& momenta,
           const std::vector<float>& coefficients, int64_t steps, int64_t planes, bool nesterov, double momentum,
@@ -257,6 +259,8 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
   // matrices of one shape, types and strides share their launches
   using Key = std::tuple<int64_t, int64_t, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t>;
   struct Group {
+    std::vector<size_t> members;
+    eg_muon call;
     std::vector<void*> params;
     std::vector<const void*> grads;
     std::vector<float*> momenta;
@@ -280,6 +284,7 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
     const Tensor* m = update ? &momenta[i] : nullptr;
     Group& to = groups[Key{w.size(r), w.size(c), dtype_code(w), dtype_code(d), w.stride(r), w.stride(c), d.stride(r),
                            d.stride(c), m ? m->stride(r) : 0, m ? m->stride(c) : 0}];
+    to.members.push_back(i);
     const int64_t count = w.dim() == 3 ? w.size(0) : 1;
     for (int64_t k = 0; k < count; ++k) {
       to.params.push_back((char*)w.data_ptr() + (count > 1 ? k * w.stride(0) * (int64_t)w.element_size() : 0));
@@ -287,8 +292,10 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
       if (m) to.momenta.push_back((float*)m->data_ptr() + (count > 1 ? k * m->stride(0) : 0));
     }
   }
+  // everything that can be refused comes before the first launch
+  int64_t need = 0;
   for (auto& [key, group] : groups) {
-    eg_muon o = {};
+    eg_muon& o = group.call = {};
     int64_t* const strides[3] = {o.param_stride, o.grad_stride, o.momentum_stride};
     std::tie(o.rows, o.cols, o.param_dtype, o.grad_dtype, strides[0][0], strides[0][1], strides[1][0], strides[1][1],
              strides[2][0], strides[2][1]) = key;
@@ -306,14 +313,21 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
     o.eps = (float)eps;
     o.keep = update ? (float)keep : 0.0f;
     o.rate = update ? (float)(lr * std::sqrt(std::max(1.0, (double)o.rows / (double)o.cols))) : -1.0f;
-    const int64_t need = g.muon_workspace(o.rows, o.cols, o.count, o.planes);
-    if (need < 0) refuse("matrices of ", o.rows, " x ", o.cols, ": 1 to 2^20 rows and columns");
-    // from torch's allocator on the current stream, which owns it until the call's work is done
-    const Tensor ws = torch::empty({need}, params[0].options().dtype(torch::kUInt8));
-    check(g.muon(&o, ws.data_ptr(), need, (void*)stream));
+    check(g.muon_check(&o));
+    need = std::max(need, g.muon_workspace(o.rows, o.cols, o.count, o.planes));
   }
-  for (const auto& t : params) written(t);
-  for (const auto& t : momenta) written(t);
+  if (groups.empty()) return;
+  // from torch's allocator on the current stream, which owns it until the work is done; the groups
+  // take turns with it
+  const Tensor ws = torch::empty({need}, params[0].options().dtype(torch::kUInt8));
+  for (auto& [key, group] : groups) {
+    const int rc = g.muon(&group.call, ws.data_ptr(), need, (void*)stream);
+    for (const size_t i : group.members) {  // some launches may be on their way whatever came of the rest
+      written(params[i]);
+      if (update) written(momenta[i]);
+    }
+    check(rc);
+  }
 }
 
 void init_ops(const std::map<std::string, int64_t>& at, pybind11::object error) {
@@ -324,6 +338,7 @@ void init_ops(const std::map<std::string, int64_t>& at, pybind11::object error) 
   set(g.preference, "eg_preference_loss");
   set(g.logits_grad, "eg_logits_grad");
   set(g.muon_workspace, "eg_muon_workspace_size");
+  set(g.muon_check, "eg_muon_check");
   set(g.muon, "eg_muon_step");
   set(g.last_error, "eg_last_error");
   g_error = error.release();

@@ -819,6 +819,9 @@ typedef struct eg_muon {
 /* Bytes of eg_muon_step's workspace (256-byte aligned); -1 for a bad argument. */
 int64_t eg_muon_workspace_size(int64_t rows, int64_t cols, int32_t count, int32_t planes);
 
+/* What eg_muon_step refuses of `muon`, without a launch: for a caller with several to do whole or not at all. */
+int eg_muon_check(const eg_muon* muon);
+
 int eg_muon_step(const eg_muon* muon, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -38,3 +38,50 @@ def test_every_weight(cuda, shape, dtype):
     if dtype == torch.float16:
         tol = tol + 2.0 ** -25  # below the smallest normal number
     assert ((new.double() - want).abs() <= tol).all()
+
+
+# ---- steps that are refused ---------------------------------------------------------------------
+
+def test_a_step_is_whole_or_not_at_all(cuda):
+    """Matrices of a shape that is refused beside others: no weight, momentum or version of any is touched;
+    and a step counts as a version of each weight and momentum."""
+    from engraft_ngram_amd import muon
+    w, m = random((8, 8), torch.float32, 1), random((8, 8), torch.float32, 2)
+    far = torch.zeros(((1 << 20) + 1, 1), device=cuda)
+    before = w.clone(), m.clone(), w._version, m._version, far._version
+    state = muon.MuonState([w, far], [m, torch.zeros_like(far)])
+    for weights in ([0, 1], [1, 0]):
+        params, momenta = [(w, far)[i] for i in weights], [(m, state.momenta[1])[i] for i in weights]
+        with pytest.raises(ValueError, match="2\\^20"):
+            muon.muon_step(params, [torch.ones_like(p) for p in params], momenta, lr=0.1)
+    with pytest.raises(ValueError, match="2\\^20"):
+        state.step([torch.ones_like(w), torch.ones_like(far)], lr=0.1)
+    assert torch.equal(w, before[0]) and torch.equal(m, before[1]) and state.step_count == 0
+    assert (w._version, m._version, far._version) == before[2:]
+    # a rate that overflows for the tall shape alone
+    tall = torch.zeros((4000, 1), device=cuda)
+    with pytest.raises(ValueError, match="not finite"):
+        muon.muon_step([w, tall], [w.clone(), tall.clone()], [m, tall.clone()], lr=1e37)
+    assert torch.equal(w, before[0]) and torch.equal(m, before[1])
+    muon.muon_step([w, tall], [w.clone(), tall.clone()], [m, torch.zeros_like(tall)], lr=0.1)
+    assert w._version > before[2] and m._version > before[3]
+
+
+def test_memory_for_the_step_is_had_before_it(cuda):
+    """A workspace that torch's allocator refuses for the last shape leaves the first one's weights alone."""
+    from engraft_ngram_amd import muon
+    w, m = random((8, 8), torch.float32, 1), random((8, 8), torch.float32, 2)
+    big = torch.zeros((4096, 4096), device=cuda)
+    before = w.clone(), m.clone(), w._version
+    grads, momenta = [w.clone(), big.clone()], [m, big.clone()]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    held = torch.cuda.memory_reserved(0)
+    torch.cuda.set_per_process_memory_fraction((held + (64 << 20)) / total)
+    try:
+        with pytest.raises(RuntimeError, match="out of memory"):
+            muon.muon_step([w, big], grads, momenta, lr=0.1)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert torch.equal(w, before[0]) and torch.equal(m, before[1]) and w._version == before[2]

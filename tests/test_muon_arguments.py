@@ -71,3 +71,15 @@ def test_host_tensors_are_refused():
         muon.orthogonalize(w)
     with pytest.raises(ValueError, match="on the GPU"):
         muon.MuonState([w])
+
+
+def test_check_says_what_a_step_would():
+    """eg_muon_check refuses what eg_muon_step refuses, and launches nothing."""
+    from engraft_ngram_amd import _lib
+    lib = _lib.load()
+    for bad in (dict(rows=0), dict(cols=(1 << 20) + 1), dict(planes=3), dict(rate=float("inf"))):
+        o = _muon(**bad)
+        said = [(f(ctypes.byref(o), *rest), lib.eg_last_error()) for f, rest in
+                ((lib.eg_muon_check, ()), (lib.eg_muon_step, (256, 1 << 40, None)))]
+        assert said[0] == said[1] and said[0][0] == _lib.EG_ERR_ARG
+    assert lib.eg_muon_check(ctypes.byref(_muon(count=0))) == _lib.EG_OK
