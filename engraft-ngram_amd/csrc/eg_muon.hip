@@ -30,6 +30,7 @@
 // four consecutive rows of a column, which is how X^T's runs are laid out, and X's
 // go through LDS.  Rows and columns are padded with zeros to multiples of 64.
 #include "eg_common.h"
+#include "eg_overlap.h"
 
 #include <math.h>
 
@@ -1120,6 +1121,24 @@ int check_muon(const eg_muon* o) {
   return EG_OK;
 }
 
+// What a launch writes lies apart from itself and from what its other workgroups read or write.
+int check_apart(const eg_muon* o) {
+  std::vector<Operand> all;
+  all.reserve(3 * (size_t)o->count);
+  const int64_t param = o->param_dtype == EG_DTYPE_F32 ? 4 : 2, grad = o->grad_dtype == EG_DTYPE_F32 ? 4 : 2;
+  for (int i = 0; i < o->count; ++i) {
+    all.push_back({Operand::kParam, (size_t)i, {o->params[i], o->rows, o->cols, o->param_stride[0], o->param_stride[1], param}});
+    all.push_back({Operand::kGrad, (size_t)i, {o->grads[i], o->rows, o->cols, o->grad_stride[0], o->grad_stride[1], grad}});
+    if (o->momenta != nullptr)
+      all.push_back({Operand::kMomentum, (size_t)i,
+                     {o->momenta[i], o->rows, o->cols, o->momentum_stride[0], o->momentum_stride[1], 4}});
+  }
+  const Operand *x, *y;
+  if (!find_overlap(all, x, y)) return EG_OK;
+  EG_CHECK_ARG(x != y, "%s of matrix %zu overlap themselves", name_of(x->kind), x->matrix);
+  EG_CHECK_ARG(false, "%s of matrix %zu overlap %s of matrix %zu", name_of(x->kind), x->matrix, name_of(y->kind), y->matrix);
+}
+
 }  // namespace
 }  // namespace eg
 
@@ -1132,7 +1151,10 @@ int64_t eg_muon_workspace_size(int64_t rows, int64_t cols, int32_t count, int32_
   return make_layout(rows, cols, std::min(count, (int32_t)kMaxBatch), planes).total;
 }
 
-int eg_muon_check(const eg_muon* muon) { return check_muon(muon); }
+int eg_muon_check(const eg_muon* muon) {
+  if (int rc = check_muon(muon); rc != EG_OK) return rc;
+  return check_apart(muon);
+}
 
 int eg_muon_step(const eg_muon* muon, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_muon(muon); rc != EG_OK) return rc;
@@ -1142,6 +1164,7 @@ int eg_muon_step(const eg_muon* muon, void* workspace, int64_t workspace_bytes, 
     return set_error(EG_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                      (long long)need);
   EG_CHECK_ARG((uintptr_t)workspace % 256 == 0, "workspace must be 256-byte aligned");
+  if (int rc = check_apart(muon); rc != EG_OK) return rc;
   for (int first = 0; first < muon->count; first += kMaxBatch) {
     const int count = std::min(muon->count - first, kMaxBatch);
     const Layout l = make_layout(muon->rows, muon->cols, count, muon->planes);

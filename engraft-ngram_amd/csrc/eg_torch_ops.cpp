@@ -17,6 +17,7 @@
 #include <tuple>
 #include <vector>
 
+#include "eg_overlap.h"
 #include "engraft_ngram.h"
 
 namespace {
@@ -266,6 +267,8 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
     std::vector<float*> momenta;
   };
   std::map<Key, Group> groups;
+  std::vector<eg::Operand> operands;  // of all groups: one may not write what another's launches still read
+  size_t matrices = 0;
   for (size_t i = 0; i < params.size(); ++i) {
     const Tensor &w = params[i], &d = grads[i];
     if (update) check_matrix(w, "params", nullptr);
@@ -287,12 +290,18 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
     to.members.push_back(i);
     const int64_t count = w.dim() == 3 ? w.size(0) : 1;
     for (int64_t k = 0; k < count; ++k) {
-      to.params.push_back((char*)w.data_ptr() + (count > 1 ? k * w.stride(0) * (int64_t)w.element_size() : 0));
-      to.grads.push_back((const char*)d.data_ptr() + (count > 1 ? k * d.stride(0) * (int64_t)d.element_size() : 0));
-      if (m) to.momenta.push_back((float*)m->data_ptr() + (count > 1 ? k * m->stride(0) : 0));
+      auto matrix = [&](const Tensor& t, eg::Operand::Kind kind) {
+        char* at = (char*)t.data_ptr() + (count > 1 ? k * t.stride(0) * (int64_t)t.element_size() : 0);
+        operands.push_back({kind, matrices, {at, t.size(r), t.size(c), t.stride(r), t.stride(c), (int64_t)t.element_size()}});
+        return at;
+      };
+      to.params.push_back(matrix(w, eg::Operand::kParam));
+      to.grads.push_back(matrix(d, eg::Operand::kGrad));
+      if (m) to.momenta.push_back((float*)matrix(*m, eg::Operand::kMomentum));
+      ++matrices;
     }
   }
-  // everything that can be refused comes before the first launch
+  // everything that can be refused comes before the first launch; the groups are checked by themselves first
   int64_t need = 0;
   for (auto& [key, group] : groups) {
     eg_muon& o = group.call = {};
@@ -317,6 +326,11 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
     need = std::max(need, g.muon_workspace(o.rows, o.cols, o.count, o.planes));
   }
   if (groups.empty()) return;
+  if (groups.size() > 1) {
+    const eg::Operand *x, *y;
+    if (eg::find_overlap(operands, x, y))
+      refuse(eg::name_of(x->kind), " of matrix ", x->matrix, " overlap ", eg::name_of(y->kind), " of matrix ", y->matrix);
+  }
   // from torch's allocator on the current stream, which owns it until the work is done; the groups
   // take turns with it
   const Tensor ws = torch::empty({need}, params[0].options().dtype(torch::kUInt8));

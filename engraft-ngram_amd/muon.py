@@ -53,10 +53,11 @@ def muon_step(params, grads, momenta, *, lr: float, weight_decay: float = 0.0, m
     """One step of ``params`` (a list of f32, bf16 or f16 ``[rows, cols]`` or
     ``[count, rows, cols]``, each matrix an update of its own), in place, with
     ``momenta`` (f32, the same shapes), in place, from ``grads``.  Any strides, one device;
-    matrices of one shape, type and strides share their launches.  A step is whole or not at all:
-    where a matrix is refused, or there is no memory for the workspace, nothing is stepped.  ``coefficients``:
-    one (a, b, c) for every Newton-Schulz step, or one each.  ``products``: "fp16x3" (None: the
-    same) or "fp16"."""
+    matrices of one shape, type and strides share their launches.  Weights and momenta must not
+    overlap themselves, each other (a weight given twice is refused) or the gradients, but a weight may
+    be over its own gradient.  A step is whole or not at all: where a matrix is refused, or there is no
+    memory for the workspace, nothing is stepped.  ``coefficients``: one (a, b, c) for every
+    Newton-Schulz step, or one each.  ``products``: "fp16x3" (None: the same) or "fp16"."""
     _run(list(params), list(grads), list(momenta), steps, coefficients, products, nesterov, momentum, eps,
          1.0 - lr * weight_decay, lr, True)
 

@@ -801,7 +801,9 @@ int eg_logits_grad(const eg_logits* logits, const float* state, const float* ups
  *   params[i] = keep params[i] - rate X         (keep 0: params[i] is not read)
  * on the fp16 matrix cores with fp32 sums: planes 2 (22-bit operands, three
  * products) or 1 (11-bit operands).  The coefficients must keep the bound of the
- * singular values, 1 at first, between 1/16 and 16. */
+ * singular values, 1 at first, between 1/16 and 16.  params and
+ * momenta must not overlap themselves, each other or the grads (refused; matrices whose columns lie apart, of
+ * different strides, are not looked through), except a matrix's own gradient and param. */
 typedef struct eg_muon {
   int64_t rows, cols;
   int32_t count;

@@ -85,3 +85,44 @@ def test_memory_for_the_step_is_had_before_it(cuda):
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert torch.equal(w, before[0]) and torch.equal(m, before[1]) and w._version == before[2]
+
+
+def test_overlapping_outputs_are_refused(cuda):
+    """A weight given twice, matrices that share elements, a momentum over a gradient or a weight; what only
+    lies side by side, and x's own place, are taken."""
+    from engraft_ngram_amd import muon
+    w, g = random((60, 80), torch.float32, 1), random((60, 80), torch.float32, 2)
+
+    def zeros(n=1):
+        return [torch.zeros((60, 80), device=cuda) for _ in range(n)]
+
+    flat = torch.zeros(20_000, device=cuda)
+    rows = flat.as_strided((60, 80), (1, 1))
+    m = zeros()[0]
+    square = random((2, 64, 64), torch.float32, 3)
+    for params, grads, momenta in (
+            ([w, w], [g, g], zeros(2)), ([w, w[:, :40]], [g, g[:, :40]], [m, torch.zeros((60, 40), device=cuda)]),
+            ([w, w.T], [g, g.T], [m, torch.zeros((80, 60), device=cuda)]), ([rows], [g], [m]), ([w], [g], [w]),
+            ([w], [m], [m]), ([w, w + 1.0], [g, g], [m, m]), ([w], [g], [rows]),
+            ([flat[:4800].view(60, 80), flat[4799:9599].view(60, 80)], [g, g], zeros(2)),
+            ([w, w + 1.0], [g, w], zeros(2))):
+        kept = [t.clone() for t in (*params, *momenta)]
+        with pytest.raises(ValueError, match="overlap"):
+            muon.muon_step(params, grads, momenta, lr=0.1)
+        assert all(torch.equal(a, b) for a, b in zip(kept, (*params, *momenta)))
+    over = square.view(-1)[64:64 + 4096].view(64, 64)  # of x alone: x is read whole before anything is written
+    want = muon.orthogonalize(square[0])
+    assert torch.equal(muon.orthogonalize(square[0], out=over), want)
+    # columns of one buffer, halves of a batch, x's own place and its transpose's
+    both = torch.cat([w, w + 1.0], 1)
+    apart = [w.clone(), w + 1.0]
+    muon.muon_step([both[:, :80], both[:, 80:]], [g, g], zeros(2), lr=0.1)
+    muon.muon_step(apart, [g, g], zeros(2), lr=0.1)
+    assert torch.equal(both, torch.cat(apart, 1))
+    want = muon.orthogonalize(square)
+    turned = square.clone()
+    muon.orthogonalize(square, out=square)
+    assert torch.equal(square, want)
+    want = muon.orthogonalize(turned[0])
+    muon.orthogonalize(turned[0], out=turned[0].T)
+    assert torch.equal(turned[0].T, want)

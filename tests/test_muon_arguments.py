@@ -83,3 +83,42 @@ def test_check_says_what_a_step_would():
                 ((lib.eg_muon_check, ()), (lib.eg_muon_step, (256, 1 << 40, None)))]
         assert said[0] == said[1] and said[0][0] == _lib.EG_ERR_ARG
     assert lib.eg_muon_check(ctypes.byref(_muon(count=0))) == _lib.EG_OK
+
+
+@pytest.mark.parametrize("what,param,grad,momentum", [
+    ("params of matrix 0 overlap themselves", [(0, 3, 5), (4096, 4, 1)], 1 << 20, 1 << 21),
+    ("params of matrix 0 overlap params of matrix 1", [(0, 4, 1), (12, 4, 1)], 1 << 20, 1 << 21),
+    ("params of matrix 0 overlap params of matrix 1", [(0, 4, 1), (0, 4, 1)], 1 << 20, 1 << 21),
+    ("grads of matrix 0 overlap params of matrix 1", [(0, 4, 1), ((1 << 18) + 1, 4, 1)], 1 << 18, 1 << 21),
+    ("momenta", [(0, 4, 1), (1 << 18, 4, 1)], 1 << 20, 1 << 20),
+])
+def test_overlaps_are_refused(what, param, grad, momentum):
+    """Matrices of 6 x 4 f32 at element offsets and strides; gradients and momenta lie one after the other."""
+    from engraft_ngram_amd import _lib
+    lib = _lib.load()
+    base = 1 << 30
+    for (a, row, col), (b, _, _) in [param]:
+        o = _muon(rows=6, cols=4, count=2)
+        lists = [(ctypes.c_void_p * 2)(base + 4 * x, base + 4 * y) for x, y in
+                 ((a, b), (grad, grad + 24), (momentum, momentum + 24))]
+        o.params, o.grads, o.momenta = (ctypes.cast(x, ctypes.c_void_p) for x in lists)
+        o.param_stride[:] = [row, col]
+        o.grad_stride[:] = o.momentum_stride[:] = [4, 1]
+        assert lib.eg_muon_check(ctypes.byref(o)) == _lib.EG_ERR_ARG
+        assert what in lib.eg_last_error().decode(), lib.eg_last_error()
+        assert lib.eg_muon_step(ctypes.byref(o), 256, 1 << 40, None) == _lib.EG_ERR_ARG
+
+
+def test_what_lies_apart_is_taken():
+    """Columns of one buffer, rows between rows, a gradient in its own weight's place."""
+    from engraft_ngram_amd import _lib
+    lib = _lib.load()
+    base = 1 << 30
+    for params, grads, stride in (((0, 4), (1 << 20, 1 << 20), (8, 1)), ((0, 8), (1 << 20, 1 << 20), (16, 1)),
+                                  ((0, 24), (0, 24), (4, 1)), ((0, 6), (0, 6), (1, 12)), ((0, 1), (1 << 20, 1 << 20), (8, 2))):
+        o = _muon(rows=6, cols=4, count=2)
+        lists = [(ctypes.c_void_p * 2)(*(base + 4 * x for x in at)) for at in (params, grads, (1 << 24, (1 << 24) + 24))]
+        o.params, o.grads, o.momenta = (ctypes.cast(x, ctypes.c_void_p) for x in lists)
+        o.param_stride[:] = o.grad_stride[:] = list(stride)
+        o.momentum_stride[:] = [4, 1]
+        assert lib.eg_muon_check(ctypes.byref(o)) == _lib.EG_OK, (params, lib.eg_last_error())
