@@ -30,6 +30,7 @@
 // sums over rows and sequences fp64; no floating atomics, so a call gives the same
 // bits every time.
 #include "eg_common.h"
+#include "eg_overlap.h"
 
 #include <algorithm>
 
@@ -1018,6 +1019,18 @@ int check_grad(const eg_logits* l, const void* d, int64_t d_stride) {
   EG_CHECK_ARG((uintptr_t)d % value_bytes(l->dtype) == 0, "d_logits is not aligned to its type");
   EG_CHECK_ARG(d != l->data || d_stride == l->row_stride || l->n <= 1,
                "d_logits in place of the logits must have their row stride");
+  const int64_t size = value_bytes(l->dtype);
+  EG_CHECK_ARG(d == l->data || !overlap({d, l->n, l->v, d_stride, 1, size}, {l->data, l->n, l->v, l->row_stride, 1, size}),
+               "d_logits overlap the logits: they may be in their place or apart from them");
+  return EG_OK;
+}
+
+// An argument that is read while the gradient is written.
+int check_apart(const eg_logits* l, const void* d, int64_t d_stride, const void* x, int64_t count, int64_t size,
+                const char* name) {
+  EG_CHECK_ARG(d == nullptr || x == nullptr ||
+                   !overlap({d, l->n, l->v, d_stride, 1, value_bytes(l->dtype)}, {x, 1, count, count, 1, size}),
+               "d_logits overlap %s", name);
   return EG_OK;
 }
 
@@ -1082,8 +1095,15 @@ int eg_policy_loss(const eg_logits* logits, const eg_policy* policy, float* logp
       return rc;
     EG_CHECK_ARG(r.n == 0 || policy->segment_ids != nullptr, "segment_ids is NULL");
   }
-  if (d_logits != nullptr)
+  if (d_logits != nullptr) {
     if (int rc = check_grad(logits, d_logits, d_stride); rc != EG_OK) return rc;
+    const int64_t target = logits->targets_i32 != 0 ? 4 : 8, id = policy->segment_ids_i32 != 0 ? 4 : 8;
+    const struct { const void* x; int64_t size; const char* name; } read[] = {
+        {logits->targets, target, "targets"}, {p.advantages, 4, "advantages"}, {p.old_lp, 4, "old_logprobs"},
+        {p.ref_lp, 4, "ref_logprobs"}, {p.seg.ids, id, "segment_ids"}};
+    for (const auto& a : read)
+      if (int rc = check_apart(logits, d_logits, d_stride, a.x, r.n, a.size, a.name); rc != EG_OK) return rc;
+  }
   const Cut cut = make_cut(r.n, r.v, logits->dtype);
   const int64_t first = stats_bytes(r.n, cut);
   EG_CHECK_WORKSPACE(first + (p.seg.n + 1) * 24 + r.n * 8 + 64);
@@ -1161,8 +1181,15 @@ int eg_preference_loss(const eg_logits* logits, const eg_preference* preference,
                "logprobs, state or segment_ids is NULL");
   EG_CHECK_ARG(preference->label_smoothing >= 0.0f && preference->label_smoothing <= 1.0f,
                "label_smoothing=%g must be in [0, 1]", (double)preference->label_smoothing);
-  if (d_logits != nullptr)
+  if (d_logits != nullptr) {
     if (int rc = check_grad(logits, d_logits, d_stride); rc != EG_OK) return rc;
+    const int64_t target = logits->targets_i32 != 0 ? 4 : 8, id = preference->segment_ids_i32 != 0 ? 4 : 8;
+    const struct { const void* x; int64_t count, size; const char* name; } read[] = {
+        {logits->targets, r.n, target, "targets"}, {preference->segment_ids, r.n, id, "segment_ids"},
+        {preference->ref_logprobs, 2 * preference->n_pairs, 4, "ref_logprobs"}};
+    for (const auto& a : read)
+      if (int rc = check_apart(logits, d_logits, d_stride, a.x, a.count, a.size, a.name); rc != EG_OK) return rc;
+  }
   Preference p;
   if (int rc = check_segments(preference->segment_ids, preference->segment_ids_i32, 2 * preference->n_pairs, &p.seg);
       rc != EG_OK)
@@ -1215,6 +1242,10 @@ int eg_logits_grad(const eg_logits* logits, const float* state, const float* ups
   if (int rc = check_logits(logits, &r); rc != EG_OK) return rc;
   EG_CHECK_ARG(r.n == 0 || state != nullptr, "state is NULL");
   if (int rc = check_grad(logits, d_logits, d_stride); rc != EG_OK) return rc;
+  if (int rc = check_apart(logits, d_logits, d_stride, logits->targets, r.n, logits->targets_i32 != 0 ? 4 : 8, "targets");
+      rc != EG_OK)
+    return rc;
+  if (int rc = check_apart(logits, d_logits, d_stride, state, 3 * r.n, 4, "state"); rc != EG_OK) return rc;
   return launch_grad(r, logits->dtype, make_cut(r.n, r.v, logits->dtype), (const RowState*)state, upstream,
                      grad_scale / logits->temperature, d_logits, d_stride, (hipStream_t)stream);
 }

@@ -153,7 +153,8 @@ def policy_loss_grad(logits: torch.Tensor, targets: torch.Tensor, advantages: to
                      grad_scale: float = 1.0, out: torch.Tensor | None = None) -> tuple[PolicyLoss, torch.Tensor]:
     """:func:`policy_loss` and the gradient of ``grad_scale`` times it, as
     ``(PolicyLoss, d_logits)`` without autograd.  ``out``: where the gradient is
-    written (the logits themselves for in place)."""
+    written (the logits themselves for in place; over part of them, or over
+    another argument, is refused)."""
     _, loss, kl, clipped, lp, d = _policy(logits, targets, advantages, old_logprobs, ref_logprobs, segment_ids, n_segments,
                                           clip, kl_coef, temperature, reduction, True, out, grad_scale)
     return PolicyLoss(loss, kl, clipped, lp), d
@@ -184,7 +185,8 @@ def preference_loss_grad(logits: torch.Tensor, targets: torch.Tensor, segment_id
                          out: torch.Tensor | None = None) -> tuple[PreferenceLoss, torch.Tensor]:
     """:func:`preference_loss` and the gradient of ``grad_scale`` times it, as
     ``(PreferenceLoss, d_logits)`` without autograd.  ``out``: where the gradient is
-    written (the logits themselves for in place)."""
+    written (the logits themselves for in place; over part of them, or over
+    another argument, is refused)."""
     _, loss, margins, seqs, lp, d = _preference(logits, targets, segment_ids, ref_logprobs, beta, label_smoothing,
                                                 temperature, True, out, grad_scale)
     return PreferenceLoss(loss, margins, seqs, lp), d

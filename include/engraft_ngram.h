@@ -770,7 +770,8 @@ int eg_token_logprobs(const eg_logits* logits, float* logprobs, void* workspace,
 /* sums f32 [3]: the loss, the weighted KL term (without kl_coef) and the weighted
  * share of clipped rows; logprobs f32 [n].  state f32 [n, 3]: without d_logits, what
  * eg_logits_grad takes.  With d_logits (the logits' type, rows d_stride apart; may be
- * the logits themselves) the gradient of grad_scale times the loss (state is scratch then).  A
+ * the logits themselves) the gradient of grad_scale times the loss (state is scratch then);
+ * d_logits that overlap the logits otherwise, or another argument, are refused.  A
  * gradient of 512 rows or more takes its logits from HBM once. */
 int eg_policy_loss(const eg_logits* logits, const eg_policy* policy, float* logprobs, float* sums, float* state,
                    void* d_logits, int64_t d_stride, float grad_scale, void* workspace, int64_t workspace_bytes,

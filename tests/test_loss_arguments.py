@@ -102,3 +102,35 @@ def test_python_arguments_are_checked_on_the_gpu(cuda):
             ("label_smoothing", lambda: losses.preference_loss(z, t, t, a[:2], label_smoothing=2.0))):
         with pytest.raises(ValueError, match=match):
             call()
+
+
+def test_overlapping_gradients_are_refused():
+    """d_logits in the logits' place, apart, or between their rows; over some of them or another argument never.  Elements of
+    bf16; 4 rows of 100 at 0, 250 apart."""
+    from engraft_ngram_amd import _lib
+    lib = _lib.load()
+    base, far = 1 << 30, 1 << 40
+    l = _logits(data=base, row_stride=250, targets=far)
+    p = _lib.EgPolicy(far + 1000, far + 2000, far + 3000, far + 4000, 3, 0, 2, 0.2, 0.2, 0.1)
+    q = _lib.EgPreference(far + 1000, far + 2000, 3, 0, 0.1, 0.0)
+
+    def calls(at, stride):
+        at = base + 2 * at
+        yield lib.eg_policy_loss, (ctypes.byref(l), ctypes.byref(p), far, far, far, at, stride, 1.0, 256, 0, None)
+        yield lib.eg_preference_loss, (ctypes.byref(l), ctypes.byref(q), far, far, far, far, far, at, stride, 1.0, 256, 0, None)
+
+    for at, stride in ((250, 250), (1, 250), (99, 250), (-99, 250), (849, 100), (-300, 100), (0, 249), (-50, 130)):
+        for fn, args in calls(at, stride):
+            rc, msg = _refusal(fn, *args)
+            assert rc == _lib.EG_ERR_ARG and ("overlap the logits" in msg or "row stride" in msg), (at, stride, msg)
+        rc, msg = _refusal(lib.eg_logits_grad, ctypes.byref(l), far, None, 1.0, base + 2 * at, stride, None)
+        assert rc == _lib.EG_ERR_ARG
+    for at, stride in ((0, 250), (100, 250), (-100, 250), (150, 250), (850, 100), (-400, 100)):
+        for fn, args in calls(at, stride):  # as far as the workspace, which is too small
+            rc, msg = _refusal(fn, *args)
+            assert rc == _lib.EG_ERR_WORKSPACE, (at, stride, msg)
+    start = (far - base) // 2
+    for at, names in ((start + 10, "targets"), (start + 502, "advantages segment_ids"), (start + 1005, "old_logprobs ref_logprobs")):
+        for fn, args in calls(at, 100):
+            rc, msg = _refusal(fn, *args)
+            assert rc == _lib.EG_ERR_ARG and any(f"overlap {x}" in msg for x in names.split()), (at, msg)
