@@ -441,7 +441,7 @@ __device__ inline PolicyRow policy_row(const Policy& p, int64_t i, double lp) {
 // dL / d lp of a row of weight w; few enough operations for every thread of a workgroup to do.
 __device__ inline float policy_g(const Policy& p, const PolicyRow& q, float w) {
   float g = q.free > q.held ? 0.0f : -q.free;  // NaN stays
-  if (p.ref_lp != nullptr) g -= p.kl_coef * q.up;
+  if (p.kl_coef != 0.0f) g -= p.kl_coef * q.up;  // a term of no weight may be infinite
   return w * g;
 }
 
@@ -516,8 +516,8 @@ __device__ inline void policy_rows(const Rows& r, const Policy& p, int64_t i0, i
       st = {0.0f, rs.m, 1.0f / rs.s};
       if (w != 0.0f) {
         const PolicyRow q = policy_row(p, i, lp);
-        const double kl = (double)q.up - (double)q.diff;
-        sum[0] += (double)w * ((double)(q.free <= q.held ? -q.free : -q.held) + (p.ref_lp != nullptr ? (double)p.kl_coef * kl : 0.0));
+        const double kl = q.up == INFINITY ? INFINITY : (double)q.up - (double)q.diff;  // d may be infinite too
+        sum[0] += (double)w * ((double)(q.free <= q.held ? -q.free : -q.held) + (p.kl_coef != 0.0f ? (double)p.kl_coef * kl : 0.0));
         sum[1] += (double)w * kl;
         sum[2] += q.free > q.held ? (double)w : 0.0;
         if (!DONE && state != nullptr) st.g = policy_g(p, q, w);

@@ -39,3 +39,45 @@ def test_overlapping_gradients_are_refused(cuda):
         want = call()[1]
         assert torch.equal(call(out=buf[:n, v:])[1], want)
         assert torch.equal(call(out=buf[:n, v:v + v])[1], want) and torch.equal(z, kept[:n, :v])
+
+
+# few rows in parts, few and some and many rows in one part each, held rows
+SHAPES = [(5, 20_011), (37, 701), (300, 701), (600, 701), (520, 50_257)]
+
+
+def masked_targets(n, v, dtype, seed):
+    """make()'s rows, the target of the first rows with one at -inf."""
+    z, t = make(n, v, dtype, seed, ignored=0.2 if n > 10 else 0.0)
+    rows = torch.nonzero(t >= 0)[:3, 0]
+    z[rows, t[rows]] = -math.inf
+    return z, t, rows
+
+
+@pytest.mark.parametrize("reduction", ["sum", "token", "sequence"])
+@pytest.mark.parametrize("n,v", SHAPES)
+def test_a_reference_without_a_kl_term(cuda, n, v, reduction):
+    """kl_coef 0 with a reference (to report KL): loss and gradient are those without it, also where the policy gives a
+    target no probability (KL is infinite there) or 1e-40 of the reference's."""
+    from engraft_ngram_amd import losses
+    z, t, rows = masked_targets(n, v, torch.float32, 1)
+    far = torch.nonzero(t >= 0)[3, 0]
+    z[far, t[far]] = -100.0
+    a = torch.randn(n, generator=torch.Generator().manual_seed(2)).cuda()
+    old, ref = torch.full((n,), -3.0, device=cuda), torch.full((n,), -2.5, device=cuda)
+    seg = torch.arange(n, device=cuda) * 3 // n
+    kw = dict(segment_ids=seg, n_segments=3, reduction=reduction)
+    want, d_want = losses.policy_loss_grad(z, t, a, old, **kw)
+    res, d = losses.policy_loss_grad(z, t, a, old, ref_logprobs=ref, **kw)
+    assert want.loss.isfinite() and d_want.isfinite().all()
+    assert torch.equal(res.loss, want.loss) and torch.equal(d, d_want)
+    assert float(res.kl) == math.inf
+    leaf = z.clone().requires_grad_()
+    auto = losses.policy_loss(leaf, t, a, old, ref_logprobs=ref, **kw)
+    auto.loss.backward()
+    assert torch.equal(auto.loss.detach(), want.loss) and torch.equal(leaf.grad, d_want) and float(auto.kl) == math.inf
+    # with a KL term the loss is as infinite as the term; rows without an infinite one keep their gradient
+    res, d = losses.policy_loss_grad(z, t, a, old, ref_logprobs=ref, kl_coef=0.1, **kw)
+    assert float(res.loss) == math.inf and float(res.kl) == math.inf
+    rest = torch.ones(n, dtype=torch.bool, device=cuda)
+    rest[rows] = rest[far] = False
+    assert d[rest].isfinite().all()
