@@ -763,7 +763,9 @@ __device__ inline Pair pair_of(const Preference& p, int64_t q, double chosen, do
   const double small = e / (1.0 + e), large = 1.0 / (1.0 + e);
   const double up = h >= 0.0 ? large : small, down = h >= 0.0 ? small : large;  // sigma(h), sigma(-h)
   const double eps = (double)p.smoothing;
-  return {h, (tail + (1.0 - eps) * fmax(-h, 0.0) + eps * fmax(h, 0.0)) + (h != h ? h : 0.0),
+  // an answer the policy cannot give (lp -inf) makes h infinite: a term of no weight stays out
+  const double lost = eps < 1.0 ? (1.0 - eps) * fmax(-h, 0.0) : 0.0, won = eps > 0.0 ? eps * fmax(h, 0.0) : 0.0;
+  return {h, (tail + lost + won) + (h != h ? h : 0.0),
           (float)((double)p.beta * (eps * up - (1.0 - eps) * down) / (double)(p.seg.n / 2))};
 }
 

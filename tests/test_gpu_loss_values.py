@@ -81,3 +81,32 @@ def test_a_reference_without_a_kl_term(cuda, n, v, reduction):
     rest = torch.ones(n, dtype=torch.bool, device=cuda)
     rest[rows] = rest[far] = False
     assert d[rest].isfinite().all()
+
+
+@pytest.mark.parametrize("n,v", SHAPES)
+def test_infinite_margins(cuda, n, v):
+    """A masked token in the rejected answer: the pair is won beyond doubt, -log sigma(inf) = 0; in the chosen one: lost, an
+    infinite loss.  With smoothing 1 the two change places; between, both are infinite.  The other pair stays as it is."""
+    from engraft_ngram_amd import losses
+    for which, eps, want in ((1, 0.0, 0.0), (0, 0.0, math.inf), (0, 1.0, 0.0), (1, 1.0, math.inf), (1, 0.1, math.inf),
+                             (0, 0.1, math.inf)):
+        z, t = make(n, v, torch.float32, 3, ignored=0.0)
+        seg = torch.arange(n, device=cuda) * 4 // n
+        ref = torch.zeros(4, device=cuda)
+        row = int(torch.nonzero(seg == which)[0, 0])
+        z[row, t[row]] = -math.inf
+        lp = plain(z, t, 1.0)[0]
+        h = 0.1 * (lp[seg == 2].sum() - lp[seg == 3].sum())
+        other = -((1 - eps) * torch.nn.functional.logsigmoid(h) + eps * torch.nn.functional.logsigmoid(-h))
+        res, d = losses.preference_loss_grad(z, t, seg, ref, label_smoothing=eps)
+        assert float(res.margins[0]) == (math.inf if which == 1 else -math.inf)
+        if want == 0.0:
+            assert_within(res.loss, other / 2, 0.05 * n * lp_error(40.0) + 2.0 ** -23 * other)
+            assert (d[seg < 2] == 0).all()
+        else:
+            assert float(res.loss) == want
+        assert d.isfinite().all() and (d[seg >= 2] != 0).any()
+        leaf = z.clone().requires_grad_()
+        auto = losses.preference_loss(leaf, t, seg, ref, label_smoothing=eps)
+        auto.loss.backward()
+        assert torch.equal(auto.loss.detach(), res.loss) and torch.equal(leaf.grad, d)
