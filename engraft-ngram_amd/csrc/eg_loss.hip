@@ -230,6 +230,11 @@ __device__ inline double logprob_of(const Rows& r, float z_below_m, float s) {
   return (double)z_below_m * r.inv_temp - log_of(s);
 }
 
+// With the logarithm in 64 bits too: for what a row's own thread adds to a loss.
+__device__ inline double exact_logprob_of(const Rows& r, float z_below_m, float s) {
+  return (double)z_below_m * r.inv_temp - log((double)s);
+}
+
 // z_t - M, NaN for a target beyond the vocabulary.
 template <typename T>
 __device__ inline float z_below_m(const Rows& r, int64_t i, int64_t t, float m) {
@@ -419,43 +424,56 @@ struct Policy {
   float clip_low, clip_high, kl_coef;
 };
 
-struct PolicyRow {
-  float ratio, free, held;  // r, r A, clamp(r) A
-  float diff, up;           // d, e^d - 1
+// r A and clamp(r) A.
+template <typename Real>
+struct Surrogate {
+  Real free, held;
 };
 
-// Differences of log-probabilities in 64 bits, their exponentials in fp32.
-__device__ inline PolicyRow policy_row(const Policy& p, int64_t i, double lp) {
-  PolicyRow q;
-  const float a = p.advantages[i];
-  q.ratio = p.old_lp != nullptr ? expf((float)(lp - (double)p.old_lp[i])) : (lp == lp ? 1.0f : (float)lp);
-  const float lo = 1.0f - p.clip_low, hi = 1.0f + p.clip_high;
-  const float held_ratio = q.ratio < lo ? lo : q.ratio > hi ? hi : q.ratio;  // NaN stays
-  q.free = q.ratio * a;
-  q.held = held_ratio * a;
-  q.diff = p.ref_lp != nullptr ? (float)((double)p.ref_lp[i] - lp) : 0.0f;
-  q.up = p.ref_lp != nullptr ? expm1f(q.diff) : 0.0f;
-  return q;
+template <typename Real>
+__device__ inline Surrogate<Real> surrogate(const Policy& p, Real ratio, Real advantage) {
+  const Real lo = (Real)1 - (Real)p.clip_low, hi = (Real)1 + (Real)p.clip_high;
+  const Real held = ratio < lo ? lo : ratio > hi ? hi : ratio;  // NaN stays
+  return {ratio * advantage, held * advantage};
 }
 
-// dL / d lp of a row of weight w; few enough operations for every thread of a workgroup to do.
-__device__ inline float policy_g(const Policy& p, const PolicyRow& q, float w) {
+// dL / d lp of row i, of weight w: differences of log-probabilities in 64 bits, their exponentials in fp32
+// (a gradient's terms do not cancel), few enough operations for every thread of a workgroup to do.
+__device__ inline float policy_g(const Policy& p, int64_t i, double lp, float w) {
+  const float ratio = p.old_lp != nullptr ? expf((float)(lp - (double)p.old_lp[i])) : (lp == lp ? 1.0f : (float)lp);
+  const Surrogate<float> q = surrogate(p, ratio, p.advantages[i]);
   float g = q.free > q.held ? 0.0f : -q.free;  // NaN stays
-  if (p.kl_coef != 0.0f) g -= p.kl_coef * q.up;  // a term of no weight may be infinite
+  // a term of no weight may be infinite
+  if (p.ref_lp != nullptr && p.kl_coef != 0.0f) g -= p.kl_coef * expm1f((float)((double)p.ref_lp[i] - lp));
   return w * g;
 }
 
+// What row i, of weight w, adds to the loss, the KL term and the clipped share, all in 64 bits.
+__device__ inline void add_policy_terms(const Policy& p, int64_t i, double lp, double w, double (&sum)[3]) {
+  const double ratio = p.old_lp != nullptr ? exp(lp - (double)p.old_lp[i]) : (lp == lp ? 1.0 : lp);
+  const Surrogate<double> q = surrogate(p, ratio, (double)p.advantages[i]);
+  double loss = q.free > q.held ? -q.held : -q.free;  // NaN stays
+  if (p.ref_lp != nullptr) {
+    const double diff = (double)p.ref_lp[i] - lp, up = expm1(diff);
+    const double kl = up == (double)INFINITY ? up : up - diff;  // diff may be infinite too
+    if (p.kl_coef != 0.0f) loss += (double)p.kl_coef * kl;
+    sum[1] += w * kl;
+  }
+  sum[0] += w * loss;
+  if (q.free > q.held) sum[2] += w;
+}
+
 // One workgroup: the weight of a row with a target, weights[segment] by segment, otherwise
-// weights[0].  Counts are kept in the same place.
+// weights[0].  Counts are kept in the same place, the first half of a weight's.
 template <int THREADS>
-__device__ inline void policy_weights(const Rows& r, const Policy& p, float* weights) {
+__device__ inline void policy_weights(const Rows& r, const Policy& p, double* weights) {
   __shared__ int total;
   const int tid = threadIdx.x, lane = tid & 63;
   int* counts = (int*)weights;
   const bool by_segment = p.reduction == EG_REDUCE_SEQUENCE;
   if (tid == 0) total = 0;
   if (by_segment)
-    for (int64_t s = tid; s < p.seg.n; s += THREADS) counts[s] = 0;
+    for (int64_t s = tid; s < p.seg.n; s += THREADS) counts[2 * s] = 0;
   __syncthreads();
   int some = 0;
   if (p.reduction == EG_REDUCE_TOKEN)
@@ -470,39 +488,39 @@ __device__ inline void policy_weights(const Rows& r, const Policy& p, float* wei
       while (left != 0) {
         const int64_t one = __shfl(s, __ffsll((unsigned long long)left) - 1);
         const uint64_t same = __ballot(s == one) & left;
-        if (lane == __ffsll((unsigned long long)same) - 1) atomicAdd(counts + one, __popcll(same));
+        if (lane == __ffsll((unsigned long long)same) - 1) atomicAdd(counts + 2 * one, __popcll(same));
         left &= ~same;
       }
     }
   __syncthreads();
   if (by_segment)
-    for (int64_t s = tid; s < p.seg.n; s += THREADS) some += __hip_atomic_load(counts + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) > 0;
+    for (int64_t s = tid; s < p.seg.n; s += THREADS) some += __hip_atomic_load(counts + 2 * s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) > 0;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) some += __shfl_xor(some, o);
   if (lane == 0) atomicAdd(&total, some);
   __syncthreads();
   const double all = p.reduction == EG_REDUCE_SUM ? 1.0 : 1.0 / (double)max(total, 1);
   if (!by_segment) {
-    if (tid == 0) weights[0] = (float)all;
+    if (tid == 0) weights[0] = all;
   } else {
     for (int64_t s = tid; s < p.seg.n; s += THREADS) {
-      const int c = __hip_atomic_load(counts + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      weights[s] = (float)(all / (double)max(c, 1));
+      const int c = __hip_atomic_load(counts + 2 * s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      weights[s] = all / (double)max(c, 1);
     }
   }
 }
 
-__device__ inline float weight_of(const Policy& p, int64_t i, const float* weights) {
+__device__ inline double weight_of(const Policy& p, int64_t i, const double* weights) {
   if (p.reduction != EG_REDUCE_SEQUENCE) return weights[0];
   const int64_t s = segment_of(p.seg, i);
-  return s >= 0 && s < p.seg.n ? weights[s] : 0.0f;
+  return s >= 0 && s < p.seg.n ? weights[s] : 0.0;
 }
 
 // The rows from tid on, THREADS apart within [i0, i1): lp, state and the thread's sums.  DONE: the
 // gradient is written (perhaps over the logits), z_t - M is in the place of the state's g.
 template <typename T, int THREADS, bool DONE>
 __device__ inline void policy_rows(const Rows& r, const Policy& p, int64_t i0, int64_t i1, int parts,
-                                   const Stat* stats, const float* weights, float* lp_out, RowState* state,
+                                   const Stat* stats, const double* weights, float* lp_out, RowState* state,
                                    double (&sum)[3]) {
   for (int64_t i = i0 + threadIdx.x; i < i1; i += THREADS) {
     const int64_t t = target_of(r, i);
@@ -511,16 +529,13 @@ __device__ inline void policy_rows(const Rows& r, const Policy& p, int64_t i0, i
     if (t >= 0) {
       const Stat rs = row_stat(stats, i, parts, r.c);
       const float below = DONE ? state[i].g : z_below_m<T>(r, i, t, rs.m);
-      lp = logprob_of(r, below, rs.s);
-      const float w = weight_of(p, i, weights);
+      lp = exact_logprob_of(r, below, rs.s);
+      const double w = weight_of(p, i, weights);
       st = {0.0f, rs.m, 1.0f / rs.s};
-      if (w != 0.0f) {
-        const PolicyRow q = policy_row(p, i, lp);
-        const double kl = q.up == INFINITY ? INFINITY : (double)q.up - (double)q.diff;  // d may be infinite too
-        sum[0] += (double)w * ((double)(q.free <= q.held ? -q.free : -q.held) + (p.kl_coef != 0.0f ? (double)p.kl_coef * kl : 0.0));
-        sum[1] += (double)w * kl;
-        sum[2] += q.free > q.held ? (double)w : 0.0;
-        if (!DONE && state != nullptr) st.g = policy_g(p, q, w);
+      if (w != 0.0) {
+        add_policy_terms(p, i, lp, w, sum);
+        // with the bits of the kernels that find g by themselves
+        if (!DONE && state != nullptr) st.g = policy_g(p, i, logprob_of(r, below, rs.s), (float)w);
       }
     }
     lp_out[i] = (float)lp;
@@ -530,7 +545,7 @@ __device__ inline void policy_rows(const Rows& r, const Policy& p, int64_t i0, i
 
 // One workgroup over all rows: weights, lp, state (where kept); sums[3] = loss, KL, clipped share.
 template <typename T, int THREADS>
-__device__ inline void policy_all(const Rows& r, const Policy& p, int parts, const Stat* stats, float* weights,
+__device__ inline void policy_all(const Rows& r, const Policy& p, int parts, const Stat* stats, double* weights,
                                   float* lp_out, RowState* state, float* sums) {
   __shared__ double red[THREADS / 64];
   policy_weights<THREADS>(r, p, weights);
@@ -546,18 +561,19 @@ __device__ inline void policy_all(const Rows& r, const Policy& p, int parts, con
 
 template <typename T>
 __global__ __launch_bounds__(kFinish) void policy_finish(const Rows r, const Policy p, int parts, const Stat* stats,
-                                                         float* weights, float* lp_out, RowState* state, float* sums) {
+                                                         double* weights, float* lp_out, RowState* state, float* sums) {
   policy_all<T, kFinish>(r, p, parts, stats, weights, lp_out, state, sums);
 }
 
 // Few rows in parts: every workgroup of the gradient finds its row's weight and g for itself, while
 // its logits are on their way, and one more does what policy_finish does: two launches for three
-// (bf16 rows of 151936 logits: 4 rows 11.2 us for 13.7, 90 rows 22.1 for 25.3, 250 rows 40.6 for 45.7).  Grid (parts, rows + 1); the gradient is not in the logits' place.
+// (bf16 rows of 151936 logits: 4 rows 11.2 us for 13.7, 90 rows 22.1 for 25.3, 250 rows 40.6 for 45.7).  Grid (parts, rows + 1); the gradient is not in the logits' place.  Held to 64
+// registers of the 113 that the 64-bit terms ask for: 37 rows of f32 18 to 20 us, as with fp32 terms.
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void policy_few_kernel(const Rows r, const Policy p, int parts, int part_len,
+__global__ __launch_bounds__(THREADS, 8) void policy_few_kernel(const Rows r, const Policy p, int parts, int part_len,
                                                              const Stat* stats, float* lp_out, float* sums, float scale,
                                                              T* d, int64_t d_stride) {
-  __shared__ float weights[kFewSegments];
+  __shared__ double weights[kFewSegments];
   const int64_t i = (int64_t)blockIdx.y - 1;
   if (i < 0) {
     if (blockIdx.x == 0) policy_all<T, THREADS>(r, p, parts, stats, weights, lp_out, nullptr, sums);
@@ -575,16 +591,17 @@ __global__ __launch_bounds__(THREADS) void policy_few_kernel(const Rows r, const
   const float f_t = t < r.v ? (float)row[t] : __builtin_nanf("");
   write_gradient<T, THREADS>(row, out, e0, e1, t, f_t, r.c, [&] {
     const Stat st = row_stat(stats, i, parts, r.c);
-    const PolicyRow terms = policy_row(p, i, logprob_of(r, f_t - st.m, st.s));
+    const double lp = logprob_of(r, f_t - st.m, st.s);
+    const float g1 = policy_g(p, i, lp, 1.0f);
     policy_weights<THREADS>(r, p, weights);
     __syncthreads();
-    const float w = weight_of(p, i, weights);
-    return RowState{(w != 0.0f ? policy_g(p, terms, w) : 0.0f) * scale, st.m, 1.0f / st.s};
+    const float w = (float)weight_of(p, i, weights);
+    return RowState{(w != 0.0f ? w * g1 : 0.0f) * scale, st.m, 1.0f / st.s};
   });
 }
 
 // Many rows: the weights first,
-__global__ __launch_bounds__(kFinish) void policy_weights_kernel(const Rows r, const Policy p, float* weights,
+__global__ __launch_bounds__(kFinish) void policy_weights_kernel(const Rows r, const Policy p, double* weights,
                                                                  int* finished) {
   if (threadIdx.x == 0) *finished = 0;
   policy_weights<kFinish>(r, p, weights);
@@ -593,7 +610,7 @@ __global__ __launch_bounds__(kFinish) void policy_weights_kernel(const Rows r, c
 // then a workgroup a row, its statistics and its gradient: the second reading of the row (300 KB
 // of a 150,000-word vocabulary in bf16) comes from the caches,
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void policy_row_kernel(const Rows r, const Policy p, const float* weights,
+__global__ __launch_bounds__(THREADS) void policy_row_kernel(const Rows r, const Policy p, const double* weights,
                                                              Stat* stats, RowState* state, float scale, T* d,
                                                              int64_t d_stride) {
   __shared__ Stat red[THREADS / 64];
@@ -613,15 +630,15 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const Rows r, const
     stats[i] = st;
     state[i].g = f_t - st.m;
   }
-  const float w = weight_of(p, i, weights);
-  const float g = w != 0.0f ? policy_g(p, policy_row(p, i, logprob_of(r, f_t - st.m, st.s)), w) : 0.0f;
+  const float w = (float)weight_of(p, i, weights);
+  const float g = w != 0.0f ? policy_g(p, i, logprob_of(r, f_t - st.m, st.s), w) : 0.0f;
   write_gradient<T, THREADS>(row, out, 0, r.v, t, f_t, r.c, [&] { return RowState{g * scale, st.m, 1.0f / st.s}; });
 }
 
 // or, of longer rows, with the first NV chunks a thread held in registers from the one to the other
 // (16 KB a chunk of 1,024 threads: NV 20 is a whole CU's and holds all of 151,936 bf16),
 template <typename T, int NV>
-__global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const Policy p, const float* weights,
+__global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const Policy p, const double* weights,
                                                                  Stat* stats, RowState* state, float scale, T* d,
                                                                  int64_t d_stride) {
   constexpr int THREADS = 1024, VEC = Logit<T>::kVec, STRIDE = THREADS * VEC, K = 4;
@@ -673,8 +690,8 @@ __global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const P
     stats[i] = st;
     state[i].g = f_t - st.m;
   }
-  const float w = weight_of(p, i, weights);
-  const float g = (w != 0.0f ? policy_g(p, policy_row(p, i, logprob_of(r, f_t - st.m, st.s)), w) : 0.0f) * scale;
+  const float w = (float)weight_of(p, i, weights);
+  const float g = (w != 0.0f ? policy_g(p, i, logprob_of(r, f_t - st.m, st.s), w) : 0.0f) * scale;
   const float inv_s = 1.0f / st.s, k1 = -g * inv_s, c = r.c, m = st.m;
   auto value = [&](float f) { return k1 * pow2((f - m) * c); };
 #pragma unroll
@@ -700,7 +717,7 @@ __global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const P
 // in order.
 template <typename T, bool DONE>
 __global__ __launch_bounds__(256) void policy_terms_kernel(const Rows r, const Policy p, const Stat* stats,
-                                                           const float* weights, float* lp_out, RowState* state,
+                                                           const double* weights, float* lp_out, RowState* state,
                                                            double* partial, int* finished, float* sums) {
   __shared__ double red[4];
   __shared__ int last;
@@ -1111,7 +1128,7 @@ int eg_policy_loss(const eg_logits* logits, const eg_policy* policy, float* logp
   EG_CHECK_WORKSPACE(first + (p.seg.n + 1) * 24 + r.n * 8 + 64);
   Stat* stats = (Stat*)workspace;
   double* partial = (double*)((char*)workspace + first);  // 3 of every 256 rows
-  float* weights = (float*)(partial + r.n);
+  double* weights = partial + r.n;
   int* finished = (int*)(weights + p.seg.n + 1);
   const hipStream_t st = (hipStream_t)stream;
   RowState* kept = (RowState*)state;

@@ -110,3 +110,42 @@ def test_infinite_margins(cuda, n, v):
         auto = losses.preference_loss(leaf, t, seg, ref, label_smoothing=eps)
         auto.loss.backward()
         assert torch.equal(auto.loss.detach(), res.loss) and torch.equal(leaf.grad, d)
+
+
+def exact_rows(n, v, seed):
+    """Logits of 0 and -inf: a row's sum is a whole number and its target's log-probability -log of it."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    some = torch.randint(2, v + 1, (n,), generator=g, device="cuda")
+    z = torch.zeros((n, v), device="cuda").masked_fill_(torch.arange(v, device="cuda") >= some[:, None], -math.inf)
+    return z, torch.zeros(n, dtype=torch.int64, device="cuda"), -some.double().log()
+
+
+@pytest.mark.parametrize("reduction", ["sum", "token", "sequence"])
+@pytest.mark.parametrize("n,v", [(6, 20_011), (64, 1003), (700, 1003)])
+def test_losses_that_nearly_cancel(cuda, n, v, reduction):
+    """Rows whose log-probabilities are exact: the loss and the KL term are off by the 64-bit terms' rounding (below 2^-44 of
+    the terms' sizes, expm1 and log included) and fp32's of the result, however little the sums come to."""
+    from engraft_ngram_amd import losses
+    z, t, lp = exact_rows(n, v, 5)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    seg = torch.arange(n, device=cuda) * 3 // n
+    shift = torch.randn(n, generator=g, device=cuda).double() * 0.05
+    old = (lp - shift).float()
+    ref = (lp + torch.randn(n, generator=g, device=cuda).double() * 1e-3).float()
+    ratio, diff = (lp - old.double()).exp(), ref.double() - lp
+    w = torch.ones(n, dtype=torch.float64, device=cuda)
+    if reduction == "token":
+        w = w / n
+    if reduction == "sequence":
+        w = w / (3 * torch.bincount(seg, minlength=3)[seg])
+    a = torch.randn(n, generator=g, device=cuda)
+    kl = torch.expm1(diff) - diff
+    a[-1] = 0.0  # the last row takes up the others' sum, but for its fp32 rounding
+    a[-1] = (-(w * ratio * a.double()).sum() / (w[-1] * ratio[-1])).float()
+    terms = w * ratio * a.double()
+    kw = dict(ref_logprobs=ref, segment_ids=seg, n_segments=3, reduction=reduction, clip=(1.0, 1e6))
+    for make_loss in (lambda: losses.policy_loss_grad(z, t, a, old, **kw)[0], lambda: losses.policy_loss(z, t, a, old, **kw)):
+        res = make_loss()
+        assert_within(res.loss, -terms.sum(), 2.0 ** -24 * terms.sum().abs() + 2.0 ** -44 * terms.abs().sum())
+        assert_within(res.kl, (w * kl).sum(), 2.0 ** -24 * (w * kl).sum() + 2.0 ** -44 * (w * diff.abs()).sum())
+        assert_within(res.logprobs, lp, 2.0 ** -23 * lp.abs())
