@@ -40,6 +40,87 @@ def test_every_weight(cuda, shape, dtype):
     assert ((new.double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("wt", [torch.float16, torch.float32])
+def test_two_planes_step(cuda, wt):
+    """Three products in a step of f16 weights as of f32 ones: two steps, to 64 2^-23 of X besides the weights' rounding."""
+    from engraft_ngram_amd import muon
+    lr, shape = 0.05, (96, 200)
+    w, m = random(shape, wt, 1, 0.1), torch.zeros(shape, device=cuda)
+    want_w, want_m, tol = w.double(), m.double(), 0.0
+    for step in range(2):
+        g = random(shape, torch.float32, 20 + step, 1e-3)
+        muon.muon_step([w], [g], [m], lr=lr, momentum=0.9)
+        want_m = 0.9 * want_m + g.double()
+        x = plain(g.double() + 0.9 * want_m)
+        want_w = want_w - lr * x
+        tol = tol + lr * 64 * 2.0 ** -23 * x.norm() + 2 * ROUNDING[wt] * want_w.norm()
+        assert (w.double() - want_w).norm() <= tol
+
+
+# ---- the products of 128 x 128 tiles ------------------------------------------------------------
+
+def tiles(shape, count=1):
+    """128 x 128 tiles of (a symmetric product, the step's product)."""
+    m, n = sorted(-(-x // 64) * 64 for x in shape)
+    m, n = -(-m // 128), -(-n // 128)
+    return count * m * (m + 1) // 2, count * m * n
+
+
+def limits():
+    """(few, many): the tile counts between which products take 128 x 128 tiles of four wavefronts."""
+    text = (ROOT / "engraft-ngram_amd" / "csrc" / "eg_muon.hip").read_text()
+    found = re.search(r"kFewTiles = (\d+), kManyTiles = (\d+);", text)
+    return int(found[1]), int(found[2])
+
+
+@pytest.mark.parametrize("products", ["fp16x3", "fp16"])
+@pytest.mark.parametrize("shape", [(2113, 2177), (2177, 2113), (2000, 3000), (3000, 2000)])
+def test_large_tiles(cuda, shape, products):
+    """Products of more than kFewTiles tiles, partial last tiles among them, wide and tall: X, and a step of
+    weights inside a padded buffer, nothing of which is written outside."""
+    from engraft_ngram_amd import muon
+    few, many = limits()
+    assert few < tiles(shape)[0] and tiles(shape)[1] < many
+    u = 2.0 ** -23 if products == "fp16x3" else 2.0 ** -12
+    for dtype in (torch.float32, torch.bfloat16):
+        x = random(shape, dtype, 7)
+        want = plain(x)
+        got = muon.orthogonalize(x, products=products)
+        assert off(got, want) <= 64 * u + ROUNDING[dtype], (dtype, off(got, want))
+        assert torch.equal(got, muon.orthogonalize(x, products=products))
+        buf = torch.full((shape[0] + 2, shape[1] + 7), 7.0, dtype=dtype, device=cuda)
+        w = buf[1:-1, 3:-4]
+        w.copy_(random(shape, dtype, 8, 0.02))
+        before = w.double()
+        muon.muon_step([w], [x], [torch.zeros(shape, device=cuda)], lr=0.1, momentum=0.0, products=products)
+        rate = 0.1 * math.sqrt(max(1.0, shape[0] / shape[1]))
+        new = before - rate * want
+        assert (w.double() - new).norm() <= rate * 64 * u * want.norm() + ROUNDING[dtype] * new.norm()
+        w.fill_(7.0)
+        assert (buf == 7.0).all()
+
+
+@pytest.mark.parametrize("products", ["fp16x3", "fp16"])
+@pytest.mark.parametrize("shape", [(800, 1030), (1030, 800)])
+def test_many_tiles(cuda, shape, products):
+    """A batch whose step's product has at least kManyTiles tiles (one wavefront a tile with one plane): the first,
+    a middle and the last matrix against the formula, every one against its own call in smaller tiles."""
+    from engraft_ngram_amd import muon
+    few, many = limits()
+    count = 24
+    assert few < tiles(shape, count)[0] and many <= tiles(shape, count)[1] and tiles(shape)[1] <= few
+    u = 2.0 ** -23 if products == "fp16x3" else 2.0 ** -12
+    x = random((count, *shape), torch.bfloat16, 9)
+    got = torch.full(x.shape, 7.0, device=cuda)
+    muon.orthogonalize(x, out=got, products=products)
+    for i in range(count):
+        if i in (0, 11, count - 1):
+            assert off(got[i], plain(x[i])) <= 64 * u, off(got[i], plain(x[i]))
+        one = torch.empty(shape, device=cuda)
+        muon.orthogonalize(x[i], out=one, products=products)
+        assert off(got[i], one.double()) <= 128 * u
+
+
 # ---- steps that are refused ---------------------------------------------------------------------
 
 def test_a_step_is_whole_or_not_at_all(cuda):
