@@ -149,3 +149,56 @@ def test_losses_that_nearly_cancel(cuda, n, v, reduction):
         assert_within(res.loss, -terms.sum(), 2.0 ** -24 * terms.sum().abs() + 2.0 ** -44 * terms.abs().sum())
         assert_within(res.kl, (w * kl).sum(), 2.0 ** -24 * (w * kl).sum() + 2.0 ** -44 * (w * diff.abs()).sum())
         assert_within(res.logprobs, lp, 2.0 ** -23 * lp.abs())
+
+
+@pytest.mark.parametrize("n", [1, 37, 256, 257])
+@pytest.mark.parametrize("dtype", ALL)
+def test_few_rows_against_autograd(cuda, n, dtype):
+    """Few long rows: loss and gradient of the one call and of autograd have the same bits."""
+    from engraft_ngram_amd import losses
+    z, t = make(n, 20_011, dtype, n)
+    gen = torch.Generator().manual_seed(n)
+    a, old, ref = (torch.randn(n, generator=gen).cuda() for _ in range(3))
+    seg = torch.arange(n, device=cuda) * 10 // n - 1  # -1 to 8, the last of no pair
+    sums = torch.zeros(8, device=cuda)
+    policy = dict(ref_logprobs=ref, segment_ids=seg.flip(0), n_segments=9, kl_coef=0.1, reduction="sequence")
+    for grad, loss in ((lambda x: losses.policy_loss_grad(x, t, a, old, **policy), lambda x: losses.policy_loss(x, t, a, old, **policy)),
+                       (lambda x: losses.preference_loss_grad(x, t, seg, sums), lambda x: losses.preference_loss(x, t, seg, sums))):
+        res, d = grad(z)
+        leaf = z.detach().requires_grad_()
+        auto = loss(leaf)
+        auto.loss.backward()
+        assert torch.equal(leaf.grad, d) and not d.isnan().any()
+        for x, y in zip(vars(res).values(), vars(auto).values()):
+            assert torch.equal(x, y.detach())
+
+
+@pytest.mark.parametrize("n,v,dtype", [(14_200, 151_936, torch.bfloat16), (43_000, 50_257, torch.float16),
+                                       (540_000, 4001, torch.float16)])
+def test_many_rows_past_32_bits(cuda, n, v, dtype):
+    """More than 2^31 logits, in whole rows of every plan (held 20 and 8 chunks, not held): log-probabilities and the
+    gradients of both losses of the last rows are those of the rows on their own."""
+    from engraft_ngram_amd import losses
+    tail = 40
+    assert (n - tail) * v > 2 ** 31
+    z = torch.zeros((n, v), dtype=dtype, device=cuda)
+    t = torch.full((n,), -100, device=cuda)
+    z[-tail:], t[-tail:] = make(tail, v, dtype, 3)
+    a, seg = torch.randn(n, device=cuda), torch.zeros(n, dtype=torch.int64, device=cuda)
+    seg[-tail // 2:] = 1
+    few = z[-tail:].contiguous(), t[-tail:]
+    assert_within(losses.token_logprobs(z, t)[-tail:], losses.token_logprobs(*few).double(), 2.0 ** -20)
+    d = torch.empty_like(z)
+    unit = {torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10}[dtype]
+    policy = dict(reduction="sum", grad_scale=1024.0)
+    sums = torch.zeros(2, device=cuda)
+    for all_rows, own in (
+            (lambda: losses.policy_loss_grad(z, t, a, out=d, **policy), lambda: losses.policy_loss_grad(*few, a[-tail:], **policy)),
+            (lambda: losses.preference_loss_grad(z, t, seg, sums, grad_scale=1024.0, out=d),
+             lambda: losses.preference_loss_grad(*few, seg[-tail:], sums, grad_scale=1024.0))):
+        d.fill_(7.0)
+        all_rows()
+        want = own()[1].double()
+        # the rows' sums are taken in other orders: fp32's rounding of p, then the type's
+        assert_within(d[-tail:], want, unit * want.abs() + 2.0 ** -23)
+        assert not d[:-tail].any() and (want[few[1] >= 0].abs().amax(1) > 0).all()
