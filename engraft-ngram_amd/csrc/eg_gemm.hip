@@ -58,6 +58,7 @@
 // remapped so that each XCD takes a contiguous run of tiles, grouped 8 row
 // tiles deep, whose A and B panels its own L2 shares.
 #include "eg_common.h"
+#include "eg_lds.h"
 
 #include <algorithm>
 #include <mutex>
@@ -1786,20 +1787,7 @@ int launch_gemm(const Shape& sh, void (*kernel)(const Args), const char* name, A
   const int64_t blocks = pp.dp + (pp.sk_groups > 0 ? (int64_t)pp.sk_groups : (tiles - pp.dp) * pp.pieces);
   EG_CHECK_ARG(blocks < (1LL << 31), "too many workgroups");
   hipStream_t st = (hipStream_t)stream;
-  // the dynamic LDS attribute, once per device and kernel
-  static std::mutex mu;
-  static std::vector<std::pair<const void*, int>> done;
-  int dev = 0;
-  EG_CHECK_HIP(hipGetDevice(&dev));
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    const std::pair<const void*, int> key((const void*)kernel, dev);
-    if (std::find(done.begin(), done.end(), key) == done.end()) {
-      EG_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)sh.lds));
-      done.push_back(key);
-    }
-  }
+  EG_CHECK_HIP(allow_lds((const void*)kernel, (int)sh.lds));
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(sh.threads), sh.lds, st, g);
   rc = launch_status(name);
   if (rc != 0 || pp.dp == tiles) return rc;

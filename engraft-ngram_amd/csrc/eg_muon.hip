@@ -30,6 +30,7 @@
 // four consecutive rows of a column, which is how X^T's runs are laid out, and X's
 // go through LDS.  Rows and columns are padded with zeros to multiples of 64.
 #include "eg_common.h"
+#include "eg_lds.h"
 #include "eg_overlap.h"
 
 #include <math.h>
@@ -876,11 +877,7 @@ int launch_product_as(const ProductArgs& args, const Matrices& mats, int count, 
   a.tiles_q = tq;
   const int tiles = EPI == kGram || EPI == kPoly ? tq * (tq + 1) / 2 : tp * tq;
   auto kernel = muon_product_kernel<PLANES, T, NW, DEPTH, EPI>;
-  if (bytes > 65536) {
-    static const hipError_t set =
-        hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    EG_CHECK_HIP(set);
-  }
+  if (bytes > 65536) EG_CHECK_HIP(allow_lds((const void*)kernel, bytes));
   kernel<<<dim3((unsigned)tiles, (unsigned)count), NW * 64, bytes, stream>>>(a, mats);
   return launch_status("muon_product_kernel");
 }
@@ -987,9 +984,7 @@ int run_small(const eg_muon* o, const Matrices& mats, int count, const Layout& l
   }
   const int bytes = (int)small_bytes(l);
   auto kernel = muon_small_kernel<PLANES>;
-  static const hipError_t set =
-      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kSmallBytes);
-  EG_CHECK_HIP(set);
+  EG_CHECK_HIP(allow_lds((const void*)kernel, kSmallBytes));
   kernel<<<dim3((unsigned)count), kSmallWaves * 64, bytes, stream>>>(a, mats);
   return launch_status("muon_small_kernel");
 }
