@@ -95,7 +95,7 @@ struct UpdateArgs {
   int grad_dtype, has_momentum, nesterov;
   float mu;
   int tiles_c, tiles;  // 64 x 64 tiles along a row, and in all
-  float* partials;     // [matrix][tile]: sums of u^2
+  double* partials;    // [matrix][tile]: sums of u^2, in 64 bits: a square of 1e20 or 1e-23 has no place in fp32
 };
 
 // u of an element, from the gradient and the momentum after its update.
@@ -115,9 +115,10 @@ __device__ inline TilePart tile_part(const UpdateArgs& a, unsigned tile) {
 // Grid (tiles, matrices): a 64 x 64 tile's momentum, and its part of |u|^2.  Bound by HBM: the
 // gradient and the momentum read, the momentum written.
 template <typename G>
-__device__ inline float momentum_tile(const UpdateArgs& a, const G* grad, float* mom) {
+__device__ inline double momentum_tile(const UpdateArgs& a, const G* grad, float* mom) {
   const TilePart p = tile_part(a, blockIdx.x);
-  float g[4][4], m[4][4], sum = 0.0f;
+  float g[4][4], m[4][4];
+  double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t r = min(p.r0 + 16 * i, a.rows - 1);
@@ -132,7 +133,7 @@ __device__ inline float momentum_tile(const UpdateArgs& a, const G* grad, float*
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       now[k] = a.has_momentum ? a.mu * m[i][k] + g[i][k] : 0.0f;
-      const float u = update_of(a, g[i][k], now[k]);
+      const double u = (double)update_of(a, g[i][k], now[k]);
       sum += u * u;
     }
     if (!a.has_momentum) continue;
@@ -152,9 +153,9 @@ __device__ inline float momentum_tile(const UpdateArgs& a, const G* grad, float*
 }
 
 __global__ __launch_bounds__(256) void muon_momentum_kernel(const UpdateArgs a, const Matrices mats) {
-  __shared__ float red[4];
+  __shared__ double red[4];
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float sum = 0.0f;
+  double sum = 0.0;
   by_type(a.grad_dtype, [&](auto zero) {
     using G = decltype(zero);
     sum = momentum_tile(a, (const G*)mats.grad[b], mats.momentum[b]);
@@ -173,6 +174,12 @@ struct PlanesArgs {
   int64_t batch_row, batch_col;  // bytes from one matrix to the next
   int64_t k16_row, k16_col;      // fragments along a row of u, of u^T
 };
+
+// scale / (|u| + eps) from |u|^2, finite also where both are tiny (zeros stay zeros).
+__device__ inline float scale_of(double square, float scale, float eps) {
+  const double s = (double)scale / (sqrt(square) + (double)eps);
+  return s > 3.4e38 ? 3.4e38f : (float)s;  // NaN stays
+}
 
 // v's planes.  v is one fp32 value to the compiler: rounded to fp16 as part of the
 // multiplication that made it (v_fma_mixlo_f16) in one place and by itself in the
@@ -211,18 +218,9 @@ __global__ __launch_bounds__(256) void muon_planes_kernel(const PlanesArgs p, co
   const unsigned at_tile = gridDim.x - 1 - blockIdx.x;
   const int64_t tr = at_tile / a.tiles_c, tc = at_tile % a.tiles_c;
   double sum = 0.0;
-  // four partial sums a load, eight loads in flight
-  struct __attribute__((packed, aligned(4))) Four {
-    float x[4];
-  };
-  const float* part = a.partials + (int64_t)b * a.tiles;
-  const int fours = a.tiles / 4;
+  const double* part = a.partials + (int64_t)b * a.tiles;
 #pragma unroll 8
-  for (int i = threadIdx.x; i < fours; i += 256) {
-    const Four v = *(const Four*)(part + 4 * i);
-    sum += (double)(v.x[0] + v.x[1]) + (double)(v.x[2] + v.x[3]);
-  }
-  if (threadIdx.x < a.tiles % 4) sum += (double)part[4 * fours + threadIdx.x];
+  for (int i = threadIdx.x; i < a.tiles; i += 256) sum += part[i];
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane == 0) red[wave] = sum;
@@ -246,8 +244,7 @@ __global__ __launch_bounds__(256) void muon_planes_kernel(const PlanesArgs p, co
             at.r0 + 16 * i < a.rows && at.c + k < a.cols ? update_of(a, g[i][k], m[i][k]) : 0.0f;
   });
   __syncthreads();
-  const float norm = sqrtf((float)(red[0] + red[1] + red[2] + red[3]));
-  const float s = p.scale / (norm + p.eps);
+  const float s = scale_of(red[0] + red[1] + red[2] + red[3], p.scale, p.eps);
   char* by_row = p.by_row + (int64_t)b * p.batch_row;
   char* by_col = p.by_col + (int64_t)b * p.batch_col;
 #pragma unroll
@@ -680,11 +677,12 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
   char* xt = x + m * n * 2 * PLANES;            // X^T by rows
   char* gram = xt + m * n * 2 * PLANES;
   char* poly = gram + m * m * 2 * PLANES;
-  float* red = (float*)gram;
+  double* red = (double*)gram;
 
   // momentum; a thread has 8 rows of a column in each of its units
   const int chunks = a.pc / 64, units = a.pr / 8 * chunks;
-  float u[UNITS][8], sum = 0.0f;
+  float u[UNITS][8];
+  double sum = 0.0;
   by_type(a.grad_dtype, [&](auto zero) {
     using G = decltype(zero);
     const G* grad = (const G*)mats.grad[b];
@@ -726,7 +724,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         u[i][r] = r0 + r < a.rows && c < a.cols ? u[i][r] : 0.0f;
-        sum += u[i][r] * u[i][r];
+        sum += (double)u[i][r] * (double)u[i][r];
       }
     }
   });
@@ -734,10 +732,10 @@ __global__ __launch_bounds__(kSmallWaves * 64) void muon_small_kernel(const Smal
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane == 0) red[wave] = sum;
   __syncthreads();
-  float total = 0.0f;
+  double total = 0.0;
 #pragma unroll
   for (int w = 0; w < kSmallWaves; ++w) total += red[w];
-  const float s = a.scale / (sqrtf(total) + a.eps);
+  const float s = scale_of(total, a.scale, a.eps);
   char* by_row = tall ? xt : x;
   char* by_col = tall ? x : xt;
 #pragma unroll
@@ -864,7 +862,7 @@ Layout make_layout(int64_t rows, int64_t cols, int64_t count, int planes) {
   l.x = l.m * l.n * 2 * planes;
   l.a = l.m * l.m * 2 * planes;
   l.tiles = (l.m / 64) * (l.n / 64);
-  l.partials = (count * l.tiles * 4 + 255) / 256 * 256;
+  l.partials = (count * l.tiles * 8 + 255) / 256 * 256;
   l.total = l.partials + count * (3 * l.x + 2 * l.a);
   return l;
 }
@@ -999,7 +997,7 @@ int run_muon(const eg_muon* o, int first, int count, const Layout& l, char* ws, 
   }
   const UpdateArgs update = {o->rows, o->cols, {o->grad_stride[0], o->grad_stride[1]},
                              {o->momentum_stride[0], o->momentum_stride[1]}, o->grad_dtype, o->momenta != nullptr,
-                             o->nesterov, o->momentum, (int)(pad64(o->cols) / 64), (int)l.tiles, (float*)ws};
+                             o->nesterov, o->momentum, (int)(pad64(o->cols) / 64), (int)l.tiles, (double*)ws};
   if (small_bytes(l) <= kSmallBytes && o->steps <= kSmallSteps && near(o, o->param_stride) && near(o, o->grad_stride) &&
       near(o, o->momentum_stride))
     return run_small<PLANES>(o, mats, count, l, stream);

@@ -121,6 +121,18 @@ def test_many_tiles(cuda, shape, products):
         assert off(got[i], one.double()) <= 128 * u
 
 
+@pytest.mark.parametrize("shape", [(70, 90), (200, 300)])
+@pytest.mark.parametrize("size", [1e-32, 1e-25, 1e-21, 1e21, 1e30, 1e37])
+def test_norms_whose_squares_leave_fp32(cuda, shape, size):
+    """|u|^2 below fp32's smallest number or above its largest: the same direction."""
+    from engraft_ngram_amd import muon
+    x = random(shape, torch.float32, 11, size)
+    got = muon.orthogonalize(x, eps=1e-34)
+    assert off(got, plain(x, eps=1e-34)) <= 64 * 2.0 ** -23
+    zeros = torch.zeros(shape, device=cuda)
+    assert (muon.orthogonalize(zeros, eps=1e-34) == 0).all()
+
+
 # ---- steps that are refused ---------------------------------------------------------------------
 
 def test_a_step_is_whole_or_not_at_all(cuda):
