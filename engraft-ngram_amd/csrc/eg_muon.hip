@@ -167,8 +167,26 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(const UpdateArgs a, 
   if (threadIdx.x == 0) a.partials[(int64_t)b * a.tiles + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
+// Grid (matrices): |u|^2 of matrices of many tiles, where every workgroup of the planes kernel would
+// read them all.
+__global__ __launch_bounds__(1024) void muon_norm_kernel(const double* partials, int tiles, double* squares) {
+  __shared__ double red[16];
+  const double* part = partials + (int64_t)blockIdx.x * tiles;
+  double sum = 0.0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < tiles; i += 1024) sum += part[i];
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 16; ++w) sum += red[w];
+  squares[blockIdx.x] = sum;
+}
+
 struct PlanesArgs {
   UpdateArgs u;
+  const double* squares;  // [matrix]: |u|^2; NULL: the partial sums' sum
   float eps, scale;     // x = u / (|u| + eps), kept times scale
   char *by_row, *by_col;  // fragments of u and of u^T
   int64_t batch_row, batch_col;  // bytes from one matrix to the next
@@ -206,8 +224,7 @@ __device__ inline void store_run(char* at, int lane, const float (&v)[8]) {
 
 // Grid (padded tiles, matrices): a 64 x 64 tile of x as fragments of both orders.  Bound by HBM: u's
 // parts read again, both orders written; 26 M elements of bf16 gradient and fp32 momentum to one plane
-// 51 us (262 MB, 5.1 TB/s; 68 with the partial sums loaded one by one), the momentum kernel before it
-// 48 us (262 MB, 5.5 TB/s).
+// 51 us (262 MB, 5.1 TB/s), the momentum kernel before it 48 us (262 MB, 5.5 TB/s).
 template <int PLANES>
 __global__ __launch_bounds__(256) void muon_planes_kernel(const PlanesArgs p, const Matrices mats) {
   __shared__ float tile[64][65];
@@ -217,13 +234,15 @@ __global__ __launch_bounds__(256) void muon_planes_kernel(const PlanesArgs p, co
   // the tiles the momentum kernel did last first: they are still cached
   const unsigned at_tile = gridDim.x - 1 - blockIdx.x;
   const int64_t tr = at_tile / a.tiles_c, tc = at_tile % a.tiles_c;
-  double sum = 0.0;
-  const double* part = a.partials + (int64_t)b * a.tiles;
+  if (p.squares == nullptr) {
+    double sum = 0.0;
+    const double* part = a.partials + (int64_t)b * a.tiles;
 #pragma unroll 8
-  for (int i = threadIdx.x; i < a.tiles; i += 256) sum += part[i];
+    for (int i = threadIdx.x; i < a.tiles; i += 256) sum += part[i];
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
-  if (lane == 0) red[wave] = sum;
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) red[wave] = sum;
+  }
   by_type(a.grad_dtype, [&](auto zero) {
     using G = decltype(zero);
     const G* grad = (const G*)mats.grad[b];
@@ -244,7 +263,7 @@ __global__ __launch_bounds__(256) void muon_planes_kernel(const PlanesArgs p, co
             at.r0 + 16 * i < a.rows && at.c + k < a.cols ? update_of(a, g[i][k], m[i][k]) : 0.0f;
   });
   __syncthreads();
-  const float s = scale_of(red[0] + red[1] + red[2] + red[3], p.scale, p.eps);
+  const float s = scale_of(p.squares != nullptr ? p.squares[b] : red[0] + red[1] + red[2] + red[3], p.scale, p.eps);
   char* by_row = p.by_row + (int64_t)b * p.batch_row;
   char* by_col = p.by_col + (int64_t)b * p.batch_col;
 #pragma unroll
@@ -851,7 +870,7 @@ struct Layout {
   int64_t m, n;          // padded, m <= n
   int64_t x, a;          // bytes of X (or X^T), of A (or B)
   int64_t tiles;         // 64 x 64 tiles of the padded matrix
-  int64_t partials;      // bytes of all matrices' partial sums
+  int64_t partials;      // bytes of all matrices' partial sums, and of their sums
   int64_t total;
 };
 
@@ -862,7 +881,7 @@ Layout make_layout(int64_t rows, int64_t cols, int64_t count, int planes) {
   l.x = l.m * l.n * 2 * planes;
   l.a = l.m * l.m * 2 * planes;
   l.tiles = (l.m / 64) * (l.n / 64);
-  l.partials = (count * l.tiles * 8 + 255) / 256 * 256;
+  l.partials = (count * (l.tiles + 1) * 8 + 255) / 256 * 256;
   l.total = l.partials + count * (3 * l.x + 2 * l.a);
   return l;
 }
@@ -946,6 +965,11 @@ bool near(const eg_muon* o, const int64_t* stride) {
   return span(o->rows, stride[0]) + span(o->cols, stride[1]) < (double)(1 << 29);
 }
 
+// Matrices of more 64 x 64 tiles have a launch for their norm: read by every workgroup, the partial sums are
+// 8 bytes times the square of the tiles.  A step of one iteration, with the launch and without it: 4096 x 4096
+// (4,096 tiles) 433 and 429 us, 10240 x 2560 395 and 404, 16384 x 4096 1,411 and 1,522, 16384 x 16384 20,960 and 22,780.
+constexpr int64_t kOwnSumTiles = 4096;
+
 // Bytes of LDS that X, X^T, A and B take.
 int64_t small_bytes(const Layout& l) { return 2 * (l.x + l.a); }
 
@@ -1022,6 +1046,13 @@ int run_muon(const eg_muon* o, int first, int count, const Layout& l, char* ws, 
   pa.k16_col = pad64(o->rows) / 16;
   muon_momentum_kernel<<<dim3((unsigned)l.tiles, (unsigned)count), 256, 0, stream>>>(pa.u, mats);
   if (int rc = launch_status("muon_momentum_kernel"); rc != EG_OK) return rc;
+  pa.squares = nullptr;
+  if (l.tiles > kOwnSumTiles) {
+    double* squares = (double*)ws + count * l.tiles;
+    muon_norm_kernel<<<dim3((unsigned)count), 1024, 0, stream>>>((const double*)ws, (int)l.tiles, squares);
+    if (int rc = launch_status("muon_norm_kernel"); rc != EG_OK) return rc;
+    pa.squares = squares;
+  }
   muon_planes_kernel<PLANES><<<dim3((unsigned)l.tiles, (unsigned)count), 256, 0, stream>>>(pa, mats);
   if (int rc = launch_status("muon_planes_kernel"); rc != EG_OK) return rc;
 

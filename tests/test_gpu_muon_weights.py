@@ -121,6 +121,17 @@ def test_many_tiles(cuda, shape, products):
         assert off(got[i], one.double()) <= 128 * u
 
 
+def test_norm_of_many_parts(cuda):
+    """A matrix of some thousand 64 x 64 tiles: its norm is the sum of as many parts, taken by the workgroups that use it
+    or, above kOwnSumTiles, in a launch of its own."""
+    from engraft_ngram_amd import muon
+    own = int(re.search(r"kOwnSumTiles = (\d+);", (ROOT / "engraft-ngram_amd" / "csrc" / "eg_muon.hip").read_text())[1])
+    assert 66_000 // 64 < own < 300_001 // 64
+    for shape in ((40, 300_001), (300_001, 40), (64, 66_000)):
+        x = random(shape, torch.float32, 10)
+        assert off(muon.orthogonalize(x, steps=1), plain(x, steps=1)) <= 64 * 2.0 ** -23
+
+
 @pytest.mark.parametrize("shape", [(70, 90), (200, 300)])
 @pytest.mark.parametrize("size", [1e-32, 1e-25, 1e-21, 1e21, 1e30, 1e37])
 def test_norms_whose_squares_leave_fp32(cuda, shape, size):
