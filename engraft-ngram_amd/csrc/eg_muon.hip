@@ -46,7 +46,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kRun = 1024;       // bytes of a fragment: 32 rows x 16 k of fp16
-constexpr int kMaxBatch = 64;    // matrices a launch
+constexpr int kMaxBatch = 64;    // matrices a launch, at most
 
 // Byte offset of fragment (row block, k / 16, plane) in an operand of k16 fragments a row block.
 template <int PLANES>
@@ -886,6 +886,17 @@ Layout make_layout(int64_t rows, int64_t cols, int64_t count, int planes) {
   return l;
 }
 
+// Workspace that a launch's matrices may take together; one alone takes what it needs.  Nothing is lost by it: 40 fp32
+// matrices of 2560 x 2560 998 us each, 16 a launch (2.1 GB), 996 all in one (5.2 GB); 16 of 4096 x 4096 3,667 and 3,700.
+constexpr int64_t kMaxWorkspace = int64_t{2} << 30;
+
+// Matrices a launch.
+int launch_count(int64_t rows, int64_t cols, int64_t count, int planes) {
+  count = std::min<int64_t>(count, kMaxBatch);
+  while (count > 1 && make_layout(rows, cols, count, planes).total > kMaxWorkspace) --count;
+  return (int)count;
+}
+
 template <int PLANES, int T, int NW, int DEPTH, Epilogue EPI>
 int launch_product_as(const ProductArgs& args, const Matrices& mats, int count, hipStream_t stream) {
   ProductArgs a = args;
@@ -1172,7 +1183,7 @@ extern "C" {
 
 int64_t eg_muon_workspace_size(int64_t rows, int64_t cols, int32_t count, int32_t planes) {
   if (rows < 1 || cols < 1 || count < 0 || rows > (1 << 20) || cols > (1 << 20) || planes < 1 || planes > 2) return -1;
-  return make_layout(rows, cols, std::min(count, (int32_t)kMaxBatch), planes).total;
+  return make_layout(rows, cols, launch_count(rows, cols, count, planes), planes).total;
 }
 
 int eg_muon_check(const eg_muon* muon) {
@@ -1189,8 +1200,9 @@ int eg_muon_step(const eg_muon* muon, void* workspace, int64_t workspace_bytes, 
                      (long long)need);
   EG_CHECK_ARG((uintptr_t)workspace % 256 == 0, "workspace must be 256-byte aligned");
   if (int rc = check_apart(muon); rc != EG_OK) return rc;
-  for (int first = 0; first < muon->count; first += kMaxBatch) {
-    const int count = std::min(muon->count - first, kMaxBatch);
+  const int most = launch_count(muon->rows, muon->cols, muon->count, muon->planes);
+  for (int first = 0; first < muon->count; first += most) {
+    const int count = std::min(muon->count - first, most);
     const Layout l = make_layout(muon->rows, muon->cols, count, muon->planes);
     const int rc = muon->planes == 2 ? run_muon<2>(muon, first, count, l, (char*)workspace, (hipStream_t)stream)
                                      : run_muon<1>(muon, first, count, l, (char*)workspace, (hipStream_t)stream);

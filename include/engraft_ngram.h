@@ -819,7 +819,8 @@ typedef struct eg_muon {
   float momentum, eps, keep, rate;
 } eg_muon;
 
-/* Bytes of eg_muon_step's workspace (256-byte aligned); -1 for a bad argument. */
+/* Bytes of eg_muon_step's workspace (256-byte aligned), at most 2 GiB or what one matrix takes; -1 for a bad
+ * argument. */
 int64_t eg_muon_workspace_size(int64_t rows, int64_t cols, int32_t count, int32_t planes);
 
 /* What eg_muon_step refuses of `muon`, without a launch: for a caller with several to do whole or not at all. */

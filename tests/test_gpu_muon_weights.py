@@ -191,6 +191,21 @@ def test_memory_for_the_step_is_had_before_it(cuda):
     assert torch.equal(w, before[0]) and torch.equal(m, before[1]) and w._version == before[2]
 
 
+def test_workspace_is_bounded(cuda):
+    """Large matrices share a launch only as far as their workspace stays within a bound; each as on its own."""
+    from engraft_ngram_amd import _lib, muon
+    lib = _lib.load()
+    one = lib.eg_muon_workspace_size(4096, 4096, 1, 2)
+    assert lib.eg_muon_workspace_size(4096, 4096, 64, 2) <= max(one, 2 << 30) < 64 * one
+    x = random((3, 8192, 8192), torch.bfloat16, 12)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = muon.orthogonalize(x, steps=1, products="fp16x3")
+    assert torch.cuda.max_memory_allocated() - before <= got.numel() * 2 + (2 << 30)
+    for i in range(3):
+        assert torch.equal(got[i], muon.orthogonalize(x[i], steps=1, products="fp16x3"))
+
+
 def test_overlapping_outputs_are_refused(cuda):
     """A weight given twice, matrices that share elements, a momentum over a gradient or a weight; what only
     lies side by side, and x's own place, are taken."""

@@ -122,3 +122,15 @@ def test_what_lies_apart_is_taken():
         o.param_stride[:] = o.grad_stride[:] = list(stride)
         o.momentum_stride[:] = [4, 1]
         assert lib.eg_muon_check(ctypes.byref(o)) == _lib.EG_OK, (params, lib.eg_last_error())
+
+
+def test_workspace_does_not_grow_with_every_matrix():
+    """Many large matrices share at most 2 GiB; one alone takes what it needs, whatever that is."""
+    from engraft_ngram_amd import _lib
+    size = _lib.load().eg_muon_workspace_size
+    for planes in (1, 2):
+        for rows, cols in ((2560, 2560), (4096, 4096), (10_240, 2560), (20_000, 20_000)):
+            one = size(rows, cols, 1, planes)
+            assert one <= size(rows, cols, 64, planes) <= max(one, 2 << 30)
+            assert size(rows, cols, 1000, planes) == size(rows, cols, 64, planes)
+    assert size(64, 256, 64, 2) > 60 * (size(64, 256, 2, 2) - size(64, 256, 1, 2))
