@@ -218,21 +218,17 @@ __device__ inline void part_range(int v, int parts, int part_len, int p, int& e0
   e1 = p + 1 == parts ? v : e0 + part_len;
 }
 
-// ln S to about 2^-23 absolute: fp32's, corrected once by S e^-y - 1.
-__device__ inline double log_of(float s) {
-  const float y = logf(s);
-  return (double)y + (double)fmaf(s, expf(-y), -1.0f);
-}
-
 // In 64 bits: a loss is a sum of terms that nearly cancel, and an fp32 lp's rounding (half a
 // unit in the last place, 2^-21 at -10) would be most of its error.
 __device__ inline double logprob_of(const Rows& r, float z_below_m, float s) {
-  return (double)z_below_m * r.inv_temp - log_of(s);
+  return (double)z_below_m * r.inv_temp - log((double)s);
 }
 
-// With the logarithm in 64 bits too: for what a row's own thread adds to a loss.
-__device__ inline double exact_logprob_of(const Rows& r, float z_below_m, float s) {
-  return (double)z_below_m * r.inv_temp - log((double)s);
+// The same where every thread of a workgroup finds it, for the row's g: ln S to about 2^-23 absolute,
+// fp32's, corrected once by S e^-y - 1.
+__device__ inline double quick_logprob_of(const Rows& r, float z_below_m, float s) {
+  const float y = logf(s);
+  return (double)z_below_m * r.inv_temp - ((double)y + (double)fmaf(s, expf(-y), -1.0f));
 }
 
 // z_t - M, NaN for a target beyond the vocabulary.
@@ -529,13 +525,13 @@ __device__ inline void policy_rows(const Rows& r, const Policy& p, int64_t i0, i
     if (t >= 0) {
       const Stat rs = row_stat(stats, i, parts, r.c);
       const float below = DONE ? state[i].g : z_below_m<T>(r, i, t, rs.m);
-      lp = exact_logprob_of(r, below, rs.s);
+      lp = logprob_of(r, below, rs.s);
       const double w = weight_of(p, i, weights);
       st = {0.0f, rs.m, 1.0f / rs.s};
       if (w != 0.0) {
         add_policy_terms(p, i, lp, w, sum);
         // with the bits of the kernels that find g by themselves
-        if (!DONE && state != nullptr) st.g = policy_g(p, i, logprob_of(r, below, rs.s), (float)w);
+        if (!DONE && state != nullptr) st.g = policy_g(p, i, quick_logprob_of(r, below, rs.s), (float)w);
       }
     }
     lp_out[i] = (float)lp;
@@ -591,7 +587,7 @@ __global__ __launch_bounds__(THREADS, 8) void policy_few_kernel(const Rows r, co
   const float f_t = t < r.v ? (float)row[t] : __builtin_nanf("");
   write_gradient<T, THREADS>(row, out, e0, e1, t, f_t, r.c, [&] {
     const Stat st = row_stat(stats, i, parts, r.c);
-    const double lp = logprob_of(r, f_t - st.m, st.s);
+    const double lp = quick_logprob_of(r, f_t - st.m, st.s);
     const float g1 = policy_g(p, i, lp, 1.0f);
     policy_weights<THREADS>(r, p, weights);
     __syncthreads();
@@ -631,7 +627,7 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const Rows r, const
     state[i].g = f_t - st.m;
   }
   const float w = (float)weight_of(p, i, weights);
-  const float g = w != 0.0f ? policy_g(p, i, logprob_of(r, f_t - st.m, st.s), w) : 0.0f;
+  const float g = w != 0.0f ? policy_g(p, i, quick_logprob_of(r, f_t - st.m, st.s), w) : 0.0f;
   write_gradient<T, THREADS>(row, out, 0, r.v, t, f_t, r.c, [&] { return RowState{g * scale, st.m, 1.0f / st.s}; });
 }
 
@@ -691,7 +687,7 @@ __global__ __launch_bounds__(1024) void policy_held_kernel(const Rows r, const P
     state[i].g = f_t - st.m;
   }
   const float w = (float)weight_of(p, i, weights);
-  const float g = (w != 0.0f ? policy_g(p, i, logprob_of(r, f_t - st.m, st.s), w) : 0.0f) * scale;
+  const float g = (w != 0.0f ? policy_g(p, i, quick_logprob_of(r, f_t - st.m, st.s), w) : 0.0f) * scale;
   const float inv_s = 1.0f / st.s, k1 = -g * inv_s, c = r.c, m = st.m;
   auto value = [&](float f) { return k1 * pow2((f - m) * c); };
 #pragma unroll

@@ -151,6 +151,40 @@ def test_losses_that_nearly_cancel(cuda, n, v, reduction):
         assert_within(res.logprobs, lp, 2.0 ** -23 * lp.abs())
 
 
+@pytest.mark.parametrize("n,v", [(6, 20_011), (64, 1003), (300, 1003), (700, 1003)])
+def test_margins_that_nearly_cancel(cuda, n, v):
+    """Rows whose log-probabilities are exact, references within 1e-4 of the sums: margins and loss are off by the 64-bit
+    sums' rounding and fp32's of the result."""
+    from engraft_ngram_amd import losses
+    z, t, lp = exact_rows(n, v, 7)
+    seg = torch.arange(n, device=cuda) * 4 // n
+    seqs = torch.stack([lp[seg == s].sum() for s in range(4)])
+    ref = (seqs + torch.randn(4, generator=torch.Generator().manual_seed(1)).cuda().double() * 1e-4).float()
+    gain = seqs - ref.double()
+    h = 0.125 * (gain[0::2] - gain[1::2])
+    want = -torch.nn.functional.logsigmoid(h).mean()
+    for make_loss in (lambda: losses.preference_loss_grad(z, t, seg, ref, beta=0.125)[0],
+                      lambda: losses.preference_loss(z, t, seg, ref, beta=0.125)):
+        res = make_loss()
+        assert_within(res.margins, h, 2.0 ** -24 * h.abs() + 2.0 ** -44 * seqs.abs().max())
+        assert_within(res.loss, want, 2.0 ** -24 * want + 2.0 ** -44 * seqs.abs().max())
+    assert_within(losses.token_logprobs(z, t), lp, 2.0 ** -23 * lp.abs())
+
+
+@pytest.mark.parametrize("n,v,dtype", [(5, 151_936, torch.bfloat16), (600, 701, torch.float32), (520, 50_257, torch.float16),
+                                       (520, 151_936, torch.bfloat16)])
+def test_one_value_of_a_logprob(cuda, n, v, dtype):
+    """Where rows are cut alike, the three calls give a row's log-probability the same bits: a policy's scores are the
+    log-probabilities its loss then starts from."""
+    from engraft_ngram_amd import losses
+    z, t = make(n, v, dtype, 13)
+    a, seg, ref = torch.ones(n, device=cuda), torch.arange(n, device=cuda) * 2 // n, torch.zeros(2, device=cuda)
+    lp = losses.token_logprobs(z, t)
+    for res in (losses.policy_loss_grad(z, t, a)[0], losses.policy_loss(z, t, a), losses.preference_loss_grad(z, t, seg, ref)[0],
+                losses.preference_loss(z, t, seg, ref)):
+        assert torch.equal(res.logprobs, lp)
+
+
 @pytest.mark.parametrize("n", [1, 37, 256, 257])
 @pytest.mark.parametrize("dtype", ALL)
 def test_few_rows_against_autograd(cuda, n, dtype):
