@@ -168,12 +168,23 @@ __device__ inline void add_chunks(const Chunk (&q)[K], float c, Stat& st) {
 #pragma unroll
     for (int i = 0; i < VEC; i += 2) m = max3(m, f[k][i], f[k][i + 1]);
   }
+  // a chunk's terms by themselves first, in pairs: added to the row's largest one by one, each would lose
+  // what is below that one's last place
   float s = st.s * pow2((st.m - m) * c);
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int k = 0; k < K; ++k) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) s += pow2((f[k][i] - m) * c);
-  st = {m, s};
+    for (int i = 0; i < VEC; ++i) f[k][i] = pow2((f[k][i] - m) * c);
+#pragma unroll
+    for (int o = VEC / 2; o >= 1; o /= 2)
+#pragma unroll
+      for (int i = 0; i < o; ++i) f[k][i] += f[k][i + o];
+  }
+#pragma unroll
+  for (int o = K / 2; o >= 1; o /= 2)
+#pragma unroll
+    for (int k = 0; k < o; ++k) f[k][0] += f[k + o][0];
+  st = {m, s + f[0][0]};
 }
 
 // A thread's statistics of elements [e0, e1) of a row, e0 a multiple of the chunk.

@@ -185,6 +185,24 @@ def test_one_value_of_a_logprob(cuda, n, v, dtype):
         assert torch.equal(res.logprobs, lp)
 
 
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n", [3, 70, 600])
+def test_many_small_terms_beside_one(cuda, n, dtype):
+    """A target at 0 among 151,935 logits of -17: each of their terms, 4.1e-8, is lost when it is added to the target's 1 alone.
+    The sum (1.0063) is rounded where a thread adds a group of chunks (at most 10) and where threads and wavefronts
+    are joined (at most 25 times in a row, 19 more over parts): 54 roundings of 2^-24."""
+    from engraft_ngram_amd import losses
+    v = 151_936
+    z = torch.full((n, v), -17.0, dtype=dtype, device=cuda)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(n)).cuda()
+    z[torch.arange(n, device=cuda), t] = 0.0
+    want = -math.log1p((v - 1) * math.exp(-17.0))
+    lp = losses.token_logprobs(z, t)
+    assert float((lp.double() - want).abs().max()) <= 54 * 2.0 ** -24
+    res, _ = losses.policy_loss_grad(z, t, torch.ones(n, device=cuda), out=z)
+    assert float((res.logprobs.double() - want).abs().max()) <= 54 * 2.0 ** -24
+
+
 @pytest.mark.parametrize("n", [1, 37, 256, 257])
 @pytest.mark.parametrize("dtype", ALL)
 def test_few_rows_against_autograd(cuda, n, dtype):
