@@ -780,7 +780,6 @@ struct Pair {
 };
 
 __device__ inline Pair pair_of(const Preference& p, int64_t q, double chosen, double rejected, bool unordered) {
-  // segments out of order have no sums: NaN
   const double h = unordered ? __builtin_nan("") : (double)p.beta * ((chosen - (double)p.ref_lp[2 * q]) -
                                                                     (rejected - (double)p.ref_lp[2 * q + 1]));
   const double e = exp(-fabs(h)), tail = log1p(e);  // -log sigma(h) = tail + max(-h, 0)
@@ -828,7 +827,8 @@ __device__ inline void preference_all(const Rows& r, const Preference& p, int pa
     for (int64_t q = tid; q <= count; q += THREADS) starts[q] = 0;
   __syncthreads();
   for (int64_t s = tid >> 6; s < count; s += THREADS / 64) {
-    const double sum = sequence_sum(lp64, starts[s], starts[s + 1]);
+    // segments out of order have no sums (several rows may have written a start): NaN
+    const double sum = unordered ? __builtin_nan("") : sequence_sum(lp64, starts[s], starts[s + 1]);
     if ((tid & 63) == 0) {
       seq_sum[s] = sum;
       seq_out[s] = (float)sum;

@@ -173,7 +173,7 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, segment_ids: to
 
         mean_p(-(1 - label_smoothing) log sigma(h_p) - label_smoothing log sigma(-h_p))
 
-    Segments out of order give NaN.  The logits must not change before the
+    Segments out of order give NaN (sums, margins, loss, gradient).  The logits must not change before the
     backward."""
     return PreferenceLoss(*_PreferenceLoss.apply(logits, targets, segment_ids, ref_logprobs, beta, label_smoothing,
                                                  temperature))

@@ -748,8 +748,8 @@ typedef struct eg_policy {
 /* The preference loss of paired log ratios: with s_k the sum of segment k's
  * log-probabilities and h_p = beta ((s_2p - ref_2p) - (s_2p+1 - ref_2p+1)),
  *   mean_p(-(1 - label_smoothing) log sigma(h_p) - label_smoothing log sigma(-h_p)).
- * segment_ids [n] int64 (or int32), not decreasing (otherwise margins, loss and
- * gradient are NaN); rows outside [0, 2 n_pairs) belong to no sequence.
+ * segment_ids [n] int64 (or int32), not decreasing (otherwise the sums, margins, loss
+ * and gradient are NaN); rows outside [0, 2 n_pairs) belong to no sequence.
  * ref_logprobs [2 n_pairs]. */
 typedef struct eg_preference {
   const void* segment_ids;

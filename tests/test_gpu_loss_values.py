@@ -203,6 +203,19 @@ def test_many_small_terms_beside_one(cuda, n, dtype):
     assert float((res.logprobs.double() - want).abs().max()) <= 54 * 2.0 ** -24
 
 
+@pytest.mark.parametrize("n,v", [(256, 20_011), (257, 20_011), (600, 701)])
+def test_unordered_segments_have_no_sums(cuda, n, v):
+    """Segments out of order: the sequences' sums are NaN like the margins, the same in every call; log-probabilities stay."""
+    from engraft_ngram_amd import losses
+    z, t = make(n, v, torch.bfloat16, n)
+    lp = losses.preference_loss(z, t, torch.zeros_like(t), torch.zeros(2, device=cuda)).logprobs
+    for seg in ((torch.arange(n, device=cuda) * 10 // n).flip(0), torch.arange(n, device=cuda) % 7):
+        ref = torch.zeros(10, device=cuda)
+        for res in (losses.preference_loss_grad(z, t, seg, ref)[0], losses.preference_loss(z, t, seg, ref)):
+            assert res.sequence_logprobs.isnan().all() and res.margins.isnan().all() and res.loss.isnan()
+            assert torch.equal(res.logprobs, lp)
+
+
 @pytest.mark.parametrize("n", [1, 37, 256, 257])
 @pytest.mark.parametrize("dtype", ALL)
 def test_few_rows_against_autograd(cuda, n, dtype):
