@@ -53,34 +53,34 @@ inline bool overlaps_itself(const Extent& x) {
 // otherwise (columns apart, of different steps) taken to be apart.
 inline bool overlap(const Extent& a, const Extent& b) {
   if (a.empty() || b.empty() || a.end() <= b.at || b.end() <= a.at) return false;
-  if (a.rows_whole() && b.rows_whole()) {
-    // b's row of a's row, from the first on that ends behind it: at most one look a row of a
-    const Extent &few = a.count[0] <= b.count[0] ? a : b, &many = a.count[0] <= b.count[0] ? b : a;
-    for (int64_t i = 0; i < few.count[0]; ++i) {
-      const int64_t lo = few.at + i * few.step[0], hi = lo + few.row_bytes();
-      const int64_t past = lo - many.at - many.row_bytes();  // rows that start at or before this end before lo
-      const int64_t j = past < 0 || many.step[0] == 0 ? (past < 0 ? 0 : 1) : past / many.step[0] + 1;
-      if (j < many.count[0] && many.at + j * many.step[0] < hi) return true;
+  if (a.step[0] == b.step[0] && a.step[1] == b.step[1]) {
+    // an element of a at (i, j) and one of b at (k, l): x = (k - i) step[0] + (l - j) step[1] + b.at - a.at
+    const int64_t d = b.at - a.at, s0 = a.step[0], s1 = a.step[1];
+    auto floor_div = [](int64_t n, int64_t m) { return n / m - (n % m < 0 ? 1 : 0); };
+    int64_t first = 1 - a.count[0], last = b.count[0] - 1;
+    if (s0 > 0) {
+      first = std::max(first, floor_div(-b.item - (b.count[1] - 1) * s1 - d, s0));
+      last = std::min(last, floor_div(a.item + (a.count[1] - 1) * s1 - d, s0));
+    }
+    for (int64_t t = first; t <= last; ++t) {
+      const int64_t rest = d + t * s0;
+      const int64_t u0 = s1 > 0 ? floor_div(-rest, s1) : 0;
+      for (int64_t u = u0; u <= u0 + 1; ++u) {
+        if (u < 1 - a.count[1] || u > b.count[1] - 1) continue;
+        const int64_t x = rest + u * s1;
+        if (x > -b.item && x < a.item) return true;
+      }
     }
     return false;
   }
-  if (a.step[0] != b.step[0] || a.step[1] != b.step[1]) return false;
-  // an element of a at (i, j) and one of b at (k, l): x = (k - i) step[0] + (l - j) step[1] + b.at - a.at
-  const int64_t d = b.at - a.at, s0 = a.step[0], s1 = a.step[1];
-  auto floor_div = [](int64_t n, int64_t m) { return n / m - (n % m < 0 ? 1 : 0); };
-  int64_t first = 1 - a.count[0], last = b.count[0] - 1;
-  if (s0 > 0) {
-    first = std::max(first, floor_div(-b.item - (b.count[1] - 1) * s1 - d, s0));
-    last = std::min(last, floor_div(a.item + (a.count[1] - 1) * s1 - d, s0));
-  }
-  for (int64_t t = first; t <= last; ++t) {
-    const int64_t rest = d + t * s0;
-    const int64_t u0 = s1 > 0 ? floor_div(-rest, s1) : 0;
-    for (int64_t u = u0; u <= u0 + 1; ++u) {
-      if (u < 1 - a.count[1] || u > b.count[1] - 1) continue;
-      const int64_t x = rest + u * s1;
-      if (x > -b.item && x < a.item) return true;
-    }
+  if (!a.rows_whole() || !b.rows_whole()) return false;
+  // b's row of a's row, from the first on that ends behind it: at most one look a row of a
+  const Extent &few = a.count[0] <= b.count[0] ? a : b, &many = a.count[0] <= b.count[0] ? b : a;
+  for (int64_t i = 0; i < few.count[0]; ++i) {
+    const int64_t lo = few.at + i * few.step[0], hi = lo + few.row_bytes();
+    const int64_t past = lo - many.at - many.row_bytes();  // rows that start at or before this end before lo
+    const int64_t j = past < 0 || many.step[0] == 0 ? (past < 0 ? 0 : 1) : past / many.step[0] + 1;
+    if (j < many.count[0] && many.at + j * many.step[0] < hi) return true;
   }
   return false;
 }
