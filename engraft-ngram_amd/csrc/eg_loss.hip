@@ -8,27 +8,31 @@
 //   d_j = g ([j == t] - 2^(c (z_j - M)) / S) / temperature,   g = dL / d lp:
 //
 // a pass over the logits gives M and S of every row (row_stats_kernel, the running
-// maximum and sum of each thread joined in a fixed order), a kernel of one
-// workgroup turns them into the rows' lp, the loss and every row's g
-// (logprobs_finish, policy_finish, preference_finish), and a second pass reads the
-// logits and writes d (logits_grad_kernel; policy_few_kernel and preference_few_kernel
-// do the last two in one launch).  The differences z - M are taken
+// maximum and sum of each thread joined in a fixed order), then the rows' lp, the loss and
+// every row's g are found (logprobs_finish, a thread a row; policy_finish and preference_finish,
+// one workgroup over all rows), and a second pass reads the logits and writes d
+// (logits_grad_kernel; policy_few_kernel and preference_few_kernel do the last two in one
+// launch).  The differences z - M are taken
 // before the multiplication by c, so a row of the type's lowest value gives a
 // uniform softmax and -inf gives exact zeros.  A row whose target is negative is left
 // out: its logits are not read (NaN there is harmless), its lp is 0 and its gradient
 // zero.  A target beyond the vocabulary gives NaN (lp and gradient), never a
-// read out of range.
+// read out of range.  A term whose coefficient is zero (kl_coef, label_smoothing) adds nothing,
+// however large it is.
 //
 // Bound by HBM, 2,047 x 151,936 bf16 of which 30 % of the rows are left out: the statistics
-// read 435 MB in 80 us (5.4 TB/s; a large copy moves 6.5), the gradient pass reads them
-// again and writes 622 MB in 172 us (6.1 TB/s, the rows read last first, so that some are still
+// read 435 MB in 79 us (5.5 TB/s; a large copy moves 6.5), the gradient pass reads them
+// again and writes 622 MB in 173 us (6.1 TB/s, the rows read last first, so that some are still
 // in the Infinity Cache: first to last 205 us).  The policy loss, whose g needs its own row
-// alone, does both in one workgroup a row and reads the logits once: 204 us for 1,057 MB.
+// alone, does both in one workgroup a row and reads the logits once: 202 us for 1,057 MB.
 // A thread keeps four 16-byte loads in flight (up to 20 where the row is held); 8 to 18 made no difference.
 //
-// Sums are fp32 per thread and workgroup (a thread adds at most a few hundred terms),
-// sums over rows and sequences fp64; no floating atomics, so a call gives the same
-// bits every time.
+// A row's sum is fp32: a thread adds the terms of a chunk's group (16 or 32) in pairs, then the groups one by
+// one (v / 32,768 of them for 16-bit logits in a workgroup of 1,024: 5 at 151,936).  Over 151,936 bf16 logits a
+// log-probability is 7e-8 off (deviation; torch's fp32 form 6e-8) with a mean of -9e-8 at temperature 1, which is the
+// rounding of c: its second half as one more multiplication a logit took the mean to -5e-9 and the
+// policy loss from 207 to 213 us.  What one thread adds of a row (lp, ratio, KL, weights) and sums over rows
+// and sequences are fp64; no floating atomics, so a call gives the same bits every time.
 #include "eg_common.h"
 #include "eg_overlap.h"
 
@@ -951,7 +955,9 @@ Cut make_cut(int64_t n, int64_t v, int dtype) {
 }
 
 // Log-probabilities take a launch less with a workgroup a whole row: 5.5 us against 8.2 for 64 KB a
-// row, 9.8 against 8.1 for one row of 300 KB, 12.7 against 16.2 for 200 such rows.
+// row, 9.8 against 8.1 for one row of 300 KB, 12.7 against 16.2 for 200 such rows, 8.0 against 8.5 for 64 of
+// 200 KB.  Of longer rows 64 are few: 12.3 us for 63 in parts at 9.8 (300 KB), 15.9 at 12.4 (608 KB); by the
+// slopes the sides meet at about 120 and 100 rows.
 constexpr int64_t kWholeRowBytes = 128 << 10, kWholeRows = 64;
 
 // policy_held_kernel holds 8 chunks a thread of rows above kHeldShort bytes, 20 above kHeldLong.  1,024 rows

@@ -224,7 +224,7 @@ __device__ inline void store_run(char* at, int lane, const float (&v)[8]) {
 
 // Grid (padded tiles, matrices): a 64 x 64 tile of x as fragments of both orders.  Bound by HBM: u's
 // parts read again, both orders written; 26 M elements of bf16 gradient and fp32 momentum to one plane
-// 51 us (262 MB, 5.1 TB/s), the momentum kernel before it 48 us (262 MB, 5.5 TB/s).
+// 44 us (262 MB, 5.9 TB/s), to two 62 (367 MB), the momentum kernel before it 50 us (262 MB, 5.3 TB/s).
 template <int PLANES>
 __global__ __launch_bounds__(256) void muon_planes_kernel(const PlanesArgs p, const Matrices mats) {
   __shared__ float tile[64][65];
@@ -338,7 +338,7 @@ struct ProductShape {
 // 2560 (two planes, 0.95 PFLOP/s of products) 41 are the loop, whose MFMAs alone take 36 at the 1.7 GHz
 // the card keeps under them.  The same tiles through LDS (direct-to-LDS loads, a ring of 2 to 5 stages,
 // fragments read half a step ahead) took 58 to 63 us: LDS reads and writes take as long as the
-// MFMAs.  10240 x 2560, one plane: X X^T 70 us (1.0 PFLOP/s; through LDS 98).
+// MFMAs.  10240 x 2560: X X^T 174 us with two planes (1.2 PFLOP/s of products), 69 with one (1.0; through LDS 98).
 template <int PLANES, int T, int NW, int DEPTH, Epilogue EPI>
 __global__ __launch_bounds__(NW * 64, NW < 4 ? 1 : NW / 4) void muon_product_kernel(const ProductArgs a, const Matrices mats) {
   using Shape = ProductShape<T, NW>;
@@ -677,8 +677,8 @@ __device__ inline void store_planes(char* to, const BlockPlanes<PLANES>& o, int 
 }
 
 // Grid (matrices): the whole step of one matrix, in one launch where the products take 17: 16 bf16 matrices
-// of 64 x 256 28.7 us (160), 9 us of launch, loads and stores and 3.4 us a step, most of it the vector
-// work on blocks between the products.  X, X^T, A and B stay in LDS as fragments; every
+// of 64 x 256 42.3 us with two planes, 28.9 with one (160 in 17 launches; 9 us of launch, loads and stores and
+// 3.4 us a step, most of it the vector work on blocks between the products).  X, X^T, A and B stay in LDS as fragments; every
 // block of a product is one wavefront's, X's and X^T's blocks both computed (B X and X^T B) rather
 // than turned.  The two have to be the same values to the last bit, hence TURNED: a
 // difference between X and X^T is not damped as X's own errors are, it grows by a step's a.
