@@ -8,7 +8,7 @@ Python on PyTorch-ROCm; every stage runs in hand-written gfx950 HIP kernels
 behind the C ABI of ``include/engraft_ngram.h`` (``libengraft_ngram.so``);
 ``OverlayEmb``'s differentiable gather is a C++ autograd function over two of
 those entry points (``_eg_autograd.so``, host code built beside the library,
-with the losses' and the weight updates' calls from torch).
+with the losses', the weight updates', the 8-bit products' and the norms' calls from torch).
 
 Modules mirror the reference's:
   table       -- ``engraft.table``            (DeviceTable = PleTable duck type)
@@ -26,6 +26,9 @@ Modules mirror the reference's:
 Beside the path, without a counterpart in the reference:
   losses      -- log-probabilities, policy and preference losses of next-token logits, with their gradient
   muon        -- orthogonalised updates of the PLE block's projection weights
+  fp8         -- products of weights in 8 bits with a scale for each block of 128, and the gradient of their input
+  norm        -- the residual's addition and the RMS norm of the sum, in 16 or 32 bits or in 8 with scales, with gradients
+  clip        -- the norm of all gradients of a step, and their clipping
 """
 from . import _lib  # noqa: F401
 

@@ -202,6 +202,65 @@ class EgMuon(ctypes.Structure):
     ]
 
 
+class EgFp8Matrix(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p),
+        ("scales", c_void_p),
+        ("rows", c_int64),
+        ("k", c_int64),
+        ("stride", c_int64),
+        ("scale_stride", c_int64),
+        ("block_rows", c_int32),
+    ]
+
+
+class EgNorm(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("residual", c_void_p),
+        ("weight", c_void_p),
+        ("x_dtype", c_int32),
+        ("r_dtype", c_int32),
+        ("w_dtype", c_int32),
+        ("eps", ctypes.c_float),
+        ("rows", c_int64),
+        ("d", c_int64),
+        ("x_stride", c_int64),
+        ("r_stride", c_int64),
+    ]
+
+
+class EgNormGrad(ctypes.Structure):
+    _fields_ = [
+        ("d_y", c_void_p),
+        ("h", c_void_p),
+        ("d_residual", c_void_p),
+        ("weight", c_void_p),
+        ("rstd", c_void_p),
+        ("dy_dtype", c_int32),
+        ("h_dtype", c_int32),
+        ("w_dtype", c_int32),
+        ("rows", c_int64),
+        ("d", c_int64),
+        ("dy_stride", c_int64),
+        ("h_stride", c_int64),
+        ("dr_stride", c_int64),
+    ]
+
+
+class EgClipTensor(ctypes.Structure):
+    _fields_ = [
+        ("g", c_void_p),
+        ("out", c_void_p),
+        ("rows", c_int64),
+        ("cols", c_int64),
+        ("g_stride", c_int64),
+        ("out_stride", c_int64),
+        ("g_dtype", c_int32),
+        ("out_dtype", c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES = {
     "eg_last_error": (c_char_p, []),
@@ -305,6 +364,22 @@ SIGNATURES = {
     "eg_muon_workspace_size": (c_int64, [c_int64, c_int64, c_int32, c_int32]),
     "eg_muon_check": (c_int32, [POINTER(EgMuon)]),
     "eg_muon_step": (c_int32, [POINTER(EgMuon), c_void_p, c_int64, c_void_p]),
+    "eg_fp8_quantize": (c_int32, [c_void_p, c_int32, c_int64, POINTER(EgFp8Matrix), c_void_p]),
+    "eg_fp8_quantize_weight": (c_int32, [c_void_p, c_int32, c_int64, c_int64, POINTER(EgFp8Matrix), POINTER(EgFp8Matrix),
+                                         c_void_p]),
+    "eg_fp8_dequantize": (c_int32, [POINTER(EgFp8Matrix), c_void_p, c_int32, c_int64, c_void_p]),
+    "eg_fp8_product": (c_int32, [POINTER(EgFp8Matrix), POINTER(EgFp8Matrix), POINTER(EgFp8Matrix), c_void_p, c_int64,
+                                 c_void_p, c_int64, c_int32, c_void_p]),
+    "eg_fp8_linear_workspace_size": (c_int64, [c_int64, c_int64]),
+    "eg_fp8_linear": (c_int32, [c_void_p, c_int32, c_int64, c_int64, POINTER(EgFp8Matrix), POINTER(EgFp8Matrix), c_void_p,
+                                c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
+    "eg_add_rms_norm": (c_int32, [POINTER(EgNorm), c_void_p, c_int64, c_void_p, c_int32, c_int64, POINTER(EgFp8Matrix),
+                                  c_void_p, c_void_p]),
+    "eg_add_rms_norm_grad_workspace_size": (c_int64, [c_int64, c_int64]),
+    "eg_add_rms_norm_grad": (c_int32, [POINTER(EgNormGrad), c_void_p, c_int32, c_int64, c_void_p, c_int32, c_int64,
+                                       c_void_p, c_int32, c_void_p, c_int64, c_void_p]),
+    "eg_clip_workspace_size": (c_int64, [POINTER(EgClipTensor), c_int64]),
+    "eg_clip_grads": (c_int32, [POINTER(EgClipTensor), c_int64, ctypes.c_float, c_void_p, c_void_p, c_int64, c_void_p]),
 }
 
 _LIB = None
@@ -364,7 +439,11 @@ def autograd_ext():
                for f in ("eg_gather_slots", "eg_scatter_grad_apply", "eg_last_error")))
     mod.init_ops({f: ctypes.cast(getattr(lib, f), c_void_p).value
                   for f in ("eg_loss_workspace_size", "eg_token_logprobs", "eg_policy_loss", "eg_preference_loss",
-                            "eg_logits_grad", "eg_muon_workspace_size", "eg_muon_check", "eg_muon_step", "eg_last_error")}, EgError)
+                            "eg_logits_grad", "eg_muon_workspace_size", "eg_muon_check", "eg_muon_step", "eg_fp8_quantize",
+                            "eg_fp8_quantize_weight", "eg_fp8_dequantize", "eg_fp8_product", "eg_fp8_linear",
+                            "eg_fp8_linear_workspace_size", "eg_add_rms_norm", "eg_add_rms_norm_grad",
+                            "eg_add_rms_norm_grad_workspace_size", "eg_clip_grads", "eg_clip_workspace_size",
+                            "eg_last_error")}, EgError)
     _EXT = mod
     return mod
 
@@ -404,6 +483,17 @@ def stream_ptr(device=None) -> int:
     else:
         idx = torch.device(device).index
     return int(raw(torch.cuda.current_device() if idx is None else idx))
+
+
+DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}  # eg_dtype
+
+
+def dtype_code(dtype, name: str = "out_dtype") -> int:
+    """``eg_dtype`` of a torch dtype; another raises ValueError."""
+    code = DTYPES.get(str(dtype))
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {dtype!r}")
+    return code
 
 
 def ptr(t) -> int | None:

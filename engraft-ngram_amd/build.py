@@ -62,7 +62,7 @@ def build(verbose: bool = False) -> Path:
     tmp = LIB_PATH.with_suffix(".so.tmp")
     ext_tmp = EXT_PATH.with_suffix(".so.tmp")
     cmd = [
-        hipcc(), "-O3", "-std=c++17", f"--offload-arch={ARCH}", "-fPIC", "-shared",
+        hipcc(), "-O3", "-std=c++17", f"--offload-arch={ARCH}", "-fPIC", "-shared", "-parallel-jobs=8",
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-Wno-unused-command-line-argument",
         "-I", str(ROOT / "include"), "-I", str(PKG / "csrc"),

@@ -1,0 +1,278 @@
+// The norm of all gradients of a step, and their clipping:
+//
+//   N = sqrt(sum over all tensors of g^2),   out = g max_norm / N where N > max_norm, g otherwise
+//
+// Bound by its bytes.  Two kinds of launch: every workgroup adds the squares of its tiles (8,192 values
+// of one tensor each) in 64 bits, which neither overflow nor lose small tensors beside large
+// ones, and writes its sum; then every workgroup adds all of these sums (a few KB from L2, in one order) and
+// writes its tiles' values, from the last one on: what was read last is in the caches.  The
+// tensors are kernel arguments, 48 a launch, so that nothing is copied to the device.
+#include <algorithm>
+#include <vector>
+
+#include "eg_fp8.h"
+#include "eg_overlap.h"
+
+namespace eg {
+namespace {
+
+constexpr int kTensors = 48;      // a launch
+constexpr int kTile = 8192;       // values
+constexpr int kThreads = 256;
+constexpr int kMostGroups = 1024; // workgroups a launch
+
+struct ClipTensor {
+  const void* g;
+  void* out;
+  int64_t cols, g_stride, out_stride;
+  int64_t values;
+  int32_t g_dtype, out_dtype;
+  int64_t first_tile;             // of the launch's
+};
+
+struct ClipArgs {
+  ClipTensor t[kTensors];
+  int count;
+  int64_t tiles;
+  double* sums;                   // this launch's, one a workgroup
+};
+
+// The tensor of a tile.
+__device__ inline int tensor_of(const ClipArgs& a, int64_t tile) {
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.t[mid].first_tile <= tile) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ inline double wave_sum64(double x) {
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) x += __shfl_xor(x, i);
+  return x;
+}
+
+// f(a zero of the type)
+template <typename F>
+__device__ inline void device_type(int32_t dtype, const F& f) {
+  if (dtype == EG_DTYPE_F32) f((float)0);
+  else if (dtype == EG_DTYPE_BF16) f((__bf16)0);
+  else f((_Float16)0);
+}
+
+// Whole rows are one row; otherwise a value's place is found by its row.
+__device__ inline int64_t place(int64_t i, int64_t cols, int64_t stride) { return cols == stride ? i : i / cols * stride + i % cols; }
+
+// Values i .. i + 7 of a tensor (zeros past its end).
+template <typename T>
+__device__ inline void read8(const ClipTensor& t, int64_t i, float (&v)[8]) {
+  const T* const g = (const T*)t.g;
+  const int64_t left = t.values - i;
+  if (t.cols == t.g_stride) {
+    load8(g + i, left > 8 ? 8 : (int)left, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k < left ? (float)g[place(i + k, t.cols, t.g_stride)] : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ inline void write8(const ClipTensor& t, int64_t i, const float (&v)[8]) {
+  T* const o = (T*)t.out;
+  const int64_t left = t.values - i;
+  if (t.cols == t.out_stride) {
+    store8(o + i, left > 8 ? 8 : (int)left, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < left) o[place(i + k, t.cols, t.out_stride)] = (T)v[k];
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void squares_kernel(const ClipArgs a) {
+  __shared__ double part[kThreads / 64];
+  double s = 0.0;
+  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+    const ClipTensor& t = a.t[tensor_of(a, tile)];
+    const int64_t i0 = (tile - t.first_tile) * kTile + threadIdx.x * 8;
+    device_type(t.g_dtype, [&](auto z) {
+#pragma unroll
+      for (int j = 0; j < kTile / (kThreads * 8); ++j) {
+        float v[8];
+        read8<decltype(z)>(t, i0 + j * kThreads * 8, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += (double)v[k] * (double)v[k];
+      }
+    });
+  }
+  s = wave_sum64(s);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int i = 0; i < kThreads / 64; ++i) s += part[i];
+    a.sums[blockIdx.x] = s;
+  }
+}
+
+// The root of the sum of `count` sums, in every thread.
+__device__ inline double root_of_sums(const double* sums, int64_t count, double* part) {
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += kThreads) s += sums[i];
+  s = wave_sum64(s);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = 0.0;
+  for (int i = 0; i < kThreads / 64; ++i) s += part[i];
+  return sqrt(s);
+}
+
+__global__ __launch_bounds__(kThreads) void scale_kernel(const ClipArgs a, const double* sums, int64_t count, float max_norm, float* norm) {
+  __shared__ double part[kThreads / 64];
+  const double root = root_of_sums(sums, count, part);
+  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)root;
+  const bool clips = root > (double)max_norm && root <= 1.7976931348623157e308;
+  const double factor = clips ? (double)max_norm / root : 1.0;  // as a float it could leave the normal numbers
+  for (int64_t k = blockIdx.x; k < a.tiles; k += gridDim.x) {
+    const int64_t tile = a.tiles - 1 - k;
+    const ClipTensor& t = a.t[tensor_of(a, tile)];
+    if (!clips && t.out == t.g) continue;  // as they are
+    const int64_t i0 = (tile - t.first_tile) * kTile + threadIdx.x * 8;
+    device_type(t.g_dtype, [&](auto z) {
+      device_type(t.out_dtype, [&](auto y) {
+#pragma unroll
+        for (int j = 0; j < kTile / (kThreads * 8); ++j) {
+          const int64_t i = i0 + j * kThreads * 8;
+          float v[8];
+          read8<decltype(z)>(t, i, v);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = clips ? (float)((double)v[q] * factor) : v[q];
+          write8<decltype(y)>(t, i, v);
+        }
+      });
+    });
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void norm_of_sums_kernel(const double* sums, int64_t count, float* norm) {
+  __shared__ double part[kThreads / 64];
+  const double root = root_of_sums(sums, count, part);
+  if (threadIdx.x == 0) *norm = (float)root;
+}
+
+// Launches of at most kTensors tensors: [first, last) of those that hold values.
+struct Launch {
+  ClipArgs args;
+  int groups;
+};
+
+int64_t tiles_of(const eg_clip_tensor& t) { return (t.rows * t.cols + kTile - 1) / kTile; }
+
+int groups_of(int64_t tiles) { return (int)std::min<int64_t>(tiles, kMostGroups); }
+
+int check_tensors(const eg_clip_tensor* tensors, int64_t count) {
+  EG_CHECK_ARG(count >= 0 && (tensors != nullptr || count == 0), "clip: count=%lld", (long long)count);
+  bool outs = false, none = false;
+  for (int64_t i = 0; i < count; ++i) {
+    const eg_clip_tensor& t = tensors[i];
+    EG_CHECK_ARG(t.rows >= 0 && t.cols >= 0 && t.rows < (1ll << 40) && t.cols < (1ll << 40) &&
+                     (t.cols == 0 || t.rows <= (1ll << 44) / t.cols),
+                 "clip: tensor %lld is %lld x %lld", (long long)i, (long long)t.rows, (long long)t.cols);
+    if (t.rows == 0 || t.cols == 0) continue;
+    if (const int rc = check_values(t.g, t.g_dtype, t.rows, t.cols, t.g_stride, "clip: a gradient"); rc != EG_OK) return rc;
+    (t.out != nullptr ? outs : none) = true;
+    if (t.out != nullptr)
+      if (const int rc = check_values(t.out, t.out_dtype, t.rows, t.cols, t.out_stride, "clip: an output"); rc != EG_OK) return rc;
+  }
+  EG_CHECK_ARG(!(outs && none), "clip: some tensors have an output and some none");
+  return EG_OK;
+}
+
+}  // namespace
+}  // namespace eg
+
+using namespace eg;
+
+extern "C" {
+
+int64_t eg_clip_workspace_size(const eg_clip_tensor* tensors, int64_t count) {
+  if (count < 0 || (tensors == nullptr && count > 0)) return -1;
+  int64_t sums = 0, tiles = 0;
+  int held = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (tensors[i].rows <= 0 || tensors[i].cols <= 0) continue;
+    tiles += tiles_of(tensors[i]);
+    if (++held == kTensors) {
+      sums += groups_of(tiles);
+      tiles = held = 0;
+    }
+  }
+  return (sums + groups_of(tiles)) * 8;
+}
+
+int eg_clip_grads(const eg_clip_tensor* tensors, int64_t count, float max_norm, float* norm, void* workspace,
+                  int64_t workspace_bytes, void* stream) try {
+  if (const int rc = check_tensors(tensors, count); rc != EG_OK) return rc;
+  EG_CHECK_ARG(norm != nullptr, "clip: NULL norm");
+  EG_CHECK_ARG(max_norm >= 0.0f, "clip: max_norm=%g", (double)max_norm);
+  const int64_t need = eg_clip_workspace_size(tensors, count);
+  if (workspace_bytes < need)
+    return set_error(EG_ERR_WORKSPACE, "clip needs %lld bytes of workspace, got %lld", (long long)need, (long long)workspace_bytes);
+  EG_CHECK_ARG(need == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "clip: the workspace must be 16-byte aligned");
+  // a tensor's output is a param here and its gradient a grad: it may be in its own gradient's place, of the
+  // same type and stride, and must not overlap anything else
+  std::vector<Operand> operands;
+  bool scales = false;
+  for (int64_t i = 0; i < count; ++i) {
+    const eg_clip_tensor& t = tensors[i];
+    if (t.rows == 0 || t.cols == 0) continue;
+    operands.push_back({Operand::kGrad, (size_t)i, {t.g, t.rows, t.cols, t.g_stride, 1, item_size(t.g_dtype)}});
+    if (t.out == nullptr) continue;
+    scales = true;
+    const Extent out(t.out, t.rows, t.cols, t.out_stride, 1, item_size(t.out_dtype));
+    const bool in_place = t.out == t.g && t.out_dtype == t.g_dtype && (t.out_stride == t.g_stride || t.rows == 1);
+    EG_CHECK_ARG(in_place || !overlap(out, operands.back().extent), "clip: output %lld overlaps its gradient and is not in its place", (long long)i);
+    operands.push_back({Operand::kParam, (size_t)i, out});
+  }
+  if (scales) {
+    const Operand *x, *y;
+    if (find_overlap(operands, x, y)) {
+      auto name = [](const Operand* o) { return o->kind == Operand::kParam ? "output" : "gradient"; };
+      return set_error(EG_ERR_ARG, "clip: %s %lld overlaps %s %lld", name(x), (long long)x->matrix, name(y), (long long)y->matrix);
+    }
+  }
+  std::vector<Launch> launches;
+  double* at = (double*)workspace;
+  for (int64_t i = 0; i < count; ++i) {
+    const eg_clip_tensor& t = tensors[i];
+    if (t.rows == 0 || t.cols == 0) continue;
+    if (launches.empty() || launches.back().args.count == kTensors) launches.push_back({});
+    ClipArgs& a = launches.back().args;
+    const bool g_whole = t.rows == 1 || t.g_stride == t.cols, out_whole = t.rows == 1 || t.out_stride == t.cols;
+    a.t[a.count++] = {t.g, t.out, t.cols, g_whole ? t.cols : t.g_stride, out_whole ? t.cols : t.out_stride, t.rows * t.cols,
+                      t.g_dtype, t.out_dtype, a.tiles};
+    a.tiles += tiles_of(t);
+  }
+  int64_t sums = 0;
+  for (Launch& l : launches) {
+    l.groups = groups_of(l.args.tiles);
+    l.args.sums = at + sums;
+    sums += l.groups;
+    squares_kernel<<<l.groups, kThreads, 0, (hipStream_t)stream>>>(l.args);
+    if (const int rc = launch_status("squares_kernel"); rc != EG_OK) return rc;
+  }
+  if (!scales) {
+    norm_of_sums_kernel<<<1, kThreads, 0, (hipStream_t)stream>>>(at, sums, norm);
+    return launch_status("norm_of_sums_kernel");
+  }
+  for (size_t i = launches.size(); i-- > 0;) {
+    scale_kernel<<<launches[i].groups, kThreads, 0, (hipStream_t)stream>>>(launches[i].args, at, sums, max_norm, i == 0 ? norm : nullptr);
+    if (const int rc = launch_status("scale_kernel"); rc != EG_OK) return rc;
+  }
+  return EG_OK;
+} catch (...) {
+  return set_error(EG_ERR_HIP, "clip: no host memory for %lld tensors", (long long)count);
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-// The losses' and the orthogonalised step's calls from torch tensors: argument
+// The losses', the weight updates', the 8-bit products' and the norms' calls from torch tensors: argument
 // checks, output and workspace allocation and the library call in one C++ function
 // each.  From Python through ctypes the same calls take 10 us (a loss) to 100 us (a
 // step of 16 matrices) of interpreter time, more than the kernels of a small one.
@@ -34,6 +34,17 @@ struct Entry {
   decltype(&eg_muon_workspace_size) muon_workspace = nullptr;
   decltype(&eg_muon_check) muon_check = nullptr;
   decltype(&eg_muon_step) muon = nullptr;
+  decltype(&eg_fp8_quantize) fp8_quantize = nullptr;
+  decltype(&eg_fp8_quantize_weight) fp8_quantize_weight = nullptr;
+  decltype(&eg_fp8_dequantize) fp8_dequantize = nullptr;
+  decltype(&eg_fp8_product) fp8_product = nullptr;
+  decltype(&eg_fp8_linear) fp8_linear = nullptr;
+  decltype(&eg_fp8_linear_workspace_size) fp8_linear_workspace = nullptr;
+  decltype(&eg_add_rms_norm) norm = nullptr;
+  decltype(&eg_add_rms_norm_grad) norm_grad = nullptr;
+  decltype(&eg_add_rms_norm_grad_workspace_size) norm_grad_workspace = nullptr;
+  decltype(&eg_clip_grads) clip = nullptr;
+  decltype(&eg_clip_workspace_size) clip_workspace = nullptr;
   decltype(&eg_last_error) last_error = nullptr;
 };
 Entry g;
@@ -344,6 +355,310 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
   }
 }
 
+// ---- products of 8-bit blocks --------------------------------------------------------------------
+
+std::optional<c10::Device> gpu_of(const Tensor& t) {
+  return t.is_cuda() ? std::optional<c10::Device>(t.device()) : std::nullopt;
+}
+
+torch::ScalarType type_of(int64_t code, const char* name) {
+  switch (code) {
+    case EG_DTYPE_F32: return torch::kFloat32;
+    case EG_DTYPE_BF16: return torch::kBFloat16;
+    case EG_DTYPE_F16: return torch::kFloat16;
+    default: refuse(name, " must be f32, bf16 or f16");
+  }
+}
+
+// Rows of unit stride that lie apart: the tensor itself, or a copy (of a transpose, of expanded rows).
+Tensor rows_2d(const Tensor& t, const char* name) {
+  if (t.dim() != 2 || dtype_code(t) < 0 || !t.is_cuda())
+    refuse(name, " must be f32, bf16 or f16 [rows, cols] on the GPU, got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+  const bool fits = (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+  return fits ? t : t.contiguous();
+}
+
+eg_fp8_matrix blocks_of(const Tensor& q, const Tensor& scales, int64_t k, int32_t block_rows, const char* name, const torch::Device& dev) {
+  if (q.dim() != 2 || q.scalar_type() != torch::kFloat8_e4m3fn || q.device() != dev || !q.is_cuda())
+    refuse(name, ": q must be float8_e4m3fn [rows, k in whole blocks] on ", dev, ", got ", q.scalar_type(), " ", q.sizes(), " on ", q.device());
+  const int64_t rows = q.size(0), blocks = (k + 127) / 128;
+  if (k < 1 || q.size(1) < blocks * 128 || (q.size(1) > 1 && q.stride(1) != 1))
+    refuse(name, ": rows of q must hold the ", blocks, " blocks of k=", k, " at unit stride, got ", q.sizes(), " with strides ", q.strides());
+  if (scales.dim() != 2 || scales.scalar_type() != torch::kFloat8_e8m0fnu || scales.device() != dev ||
+      scales.size(0) != (rows + block_rows - 1) / block_rows || scales.size(1) < (blocks + 3) / 4 * 4 ||
+      (scales.size(1) > 1 && scales.stride(1) != 1))
+    refuse(name, ": scales must be float8_e8m0fnu [", (rows + block_rows - 1) / block_rows, ", ", (blocks + 3) / 4 * 4, "] on ", dev,
+           " at unit stride, got ", scales.scalar_type(), " ", scales.sizes(), " on ", scales.device());
+  return {rows > 0 ? q.data_ptr() : nullptr, rows > 0 ? (uint8_t*)scales.data_ptr() : nullptr, rows, k, row_stride(q),
+          row_stride(scales), block_rows};
+}
+
+std::pair<Tensor, Tensor> empty_blocks(int64_t rows, int64_t k, int64_t block_rows, const Tensor& like) {
+  const int64_t blocks = (k + 127) / 128;
+  return {torch::empty({rows, blocks * 128}, like.options().dtype(torch::kFloat8_e4m3fn)),
+          torch::empty({(rows + block_rows - 1) / block_rows, (blocks + 3) / 4 * 4}, like.options().dtype(torch::kFloat8_e8m0fnu))};
+}
+
+// (q, scales)
+std::tuple<Tensor, Tensor> fp8_quantize(const Tensor& x_, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(gpu_of(x_));
+  const Tensor x = rows_2d(x_, "x");
+  if (x.size(1) < 1) refuse("x must have at least one column");
+  const auto [q, scales] = empty_blocks(x.size(0), x.size(1), 1, x);
+  const eg_fp8_matrix out = blocks_of(q, scales, x.size(1), 1, "x", x.device());
+  check(g.fp8_quantize(rows_of(x, x.size(0)), dtype_code(x), row_stride(x), &out, (void*)stream));
+  return {q, scales};
+}
+
+// (q, scales, the transpose's q and scales)
+std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> fp8_quantize_weight(const Tensor& w, bool transpose, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(gpu_of(w));
+  if (w.dim() != 2 || dtype_code(w) < 0 || !w.is_cuda() || w.size(0) < 1 || w.size(1) < 1)
+    refuse("a weight must be f32, bf16 or f16 [n, k] on the GPU, got ", w.scalar_type(), " ", w.sizes(), " on ", w.device());
+  const auto [q, scales] = empty_blocks(w.size(0), w.size(1), 128, w);
+  const eg_fp8_matrix out = blocks_of(q, scales, w.size(1), 128, "weight", w.device());
+  if (!transpose) {
+    check(g.fp8_quantize_weight(w.data_ptr(), dtype_code(w), w.stride(0), w.stride(1), &out, nullptr, (void*)stream));
+    return {q, scales, std::nullopt, std::nullopt};
+  }
+  const auto [qt, scales_t] = empty_blocks(w.size(1), w.size(0), 128, w);
+  const eg_fp8_matrix out_t = blocks_of(qt, scales_t, w.size(0), 128, "weight", w.device());
+  check(g.fp8_quantize_weight(w.data_ptr(), dtype_code(w), w.stride(0), w.stride(1), &out, &out_t, (void*)stream));
+  return {q, scales, qt, scales_t};
+}
+
+Tensor fp8_dequantize(const Tensor& q, const Tensor& scales, int64_t k, int64_t block_rows, int64_t dtype, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(gpu_of(q));
+  const eg_fp8_matrix m = blocks_of(q, scales, k, (int32_t)block_rows, "blocks", q.device());
+  const Tensor out = torch::empty({m.rows, k}, q.options().dtype(type_of(dtype, "dtype")));
+  check(g.fp8_dequantize(&m, rows_of(out, m.rows), (int32_t)dtype, k, (void*)stream));
+  return out;
+}
+
+struct Outputs {
+  std::vector<Tensor> y;
+  eg_fp8_matrix b[2];
+  void* at[2] = {nullptr, nullptr};
+  int64_t ld[2] = {0, 0};
+  bool two;
+};
+
+// The weight's rows in one group, or in two from row `split` on, and an output for each.
+Outputs outputs(int64_t m, const eg_fp8_matrix& w, int64_t split, int64_t dtype, const Tensor& like) {
+  Outputs o;
+  o.two = split > 0;
+  if (o.two && (split % 128 != 0 || split >= w.rows)) refuse("split must be a multiple of 128 below the weight's ", w.rows, " rows, got ", split);
+  o.b[0] = o.b[1] = w;
+  if (o.two) {
+    o.b[0].rows = split;
+    o.b[1].rows = w.rows - split;
+    o.b[1].q = (char*)w.q + split * w.stride;
+    o.b[1].scales = w.scales + split / 128 * w.scale_stride;
+  }
+  for (int i = 0; i < (o.two ? 2 : 1); ++i) {
+    o.y.push_back(torch::empty({m, o.b[i].rows}, like.options().dtype(type_of(dtype, "out_dtype"))));
+    o.at[i] = o.y[i].numel() > 0 ? o.y[i].data_ptr() : nullptr;
+    o.ld[i] = o.b[i].rows;
+  }
+  return o;
+}
+
+std::vector<Tensor> fp8_linear(const Tensor& x_, const Tensor& q, const Tensor& scales, int64_t k, int64_t split, int64_t dtype, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(gpu_of(x_));
+  const Tensor x = rows_2d(x_, "x");
+  const eg_fp8_matrix w = blocks_of(q, scales, k, 128, "weight", x.device());
+  if (x.size(1) != k) refuse("x must be [m, ", k, "], got ", x.sizes());
+  Outputs o = outputs(x.size(0), w, split, dtype, x);
+  const int64_t need = g.fp8_linear_workspace(x.size(0), k);
+  if (need < 0) refuse("a product of ", x.sizes(), " values");
+  const Tensor ws = need > 0 ? torch::empty({need}, x.options().dtype(torch::kUInt8)) : Tensor();
+  check(g.fp8_linear(rows_of(x, x.size(0)), dtype_code(x), x.size(0), row_stride(x), &o.b[0], o.two ? &o.b[1] : nullptr, o.at[0], o.ld[0],
+                     o.at[1], o.ld[1], (int32_t)dtype, need > 0 ? ws.data_ptr() : nullptr, need, (void*)stream));
+  return o.y;
+}
+
+std::vector<Tensor> fp8_product(const Tensor& xq, const Tensor& x_scales, const Tensor& q, const Tensor& scales, int64_t k, int64_t split,
+                                int64_t dtype, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(gpu_of(xq));
+  const eg_fp8_matrix a = blocks_of(xq, x_scales, k, 1, "x", xq.device()), w = blocks_of(q, scales, k, 128, "weight", xq.device());
+  Outputs o = outputs(a.rows, w, split, dtype, xq);
+  check(g.fp8_product(&a, &o.b[0], o.two ? &o.b[1] : nullptr, o.at[0], o.ld[0], o.at[1], o.ld[1], (int32_t)dtype, (void*)stream));
+  return o.y;
+}
+
+// ---- norms ---------------------------------------------------------------------------------------
+
+void check_vector(const MaybeTensor& w, int64_t d, const char* name, const torch::Device& dev) {
+  if (w && (w->dim() != 1 || w->size(0) != d || dtype_code(*w) < 0 || w->device() != dev))
+    refuse(name, " must be f32, bf16 or f16 [", d, "] on ", dev, ", got ", w->scalar_type(), " ", w->sizes(), " on ", w->device());
+}
+
+// (y or its q, y's scales, h, rstd); dtype -1: blocks
+std::tuple<Tensor, MaybeTensor, Tensor, MaybeTensor> norm(const Tensor& x_, const MaybeTensor& residual, const MaybeTensor& weight, double eps,
+                                                          int64_t dtype, bool stats, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(gpu_of(x_));
+  const Tensor x = rows_2d(x_, "x");
+  const int64_t rows = x.size(0), d = x.size(1);
+  if (d < 1) refuse("x must have at least one column");
+  Tensor r;
+  if (residual) {
+    r = rows_2d(*residual, "residual");
+    if (r.sizes() != x.sizes() || r.device() != x.device()) refuse("residual must be ", x.sizes(), " on ", x.device(), ", got ", r.sizes(), " on ", r.device());
+    if (r.scalar_type() != x.scalar_type() && r.scalar_type() != torch::kFloat32)
+      refuse("residual must be of x's type or f32, got ", r.scalar_type(), " beside ", x.scalar_type());
+  }
+  check_vector(weight, d, "weight", x.device());
+  const Tensor w = weight ? weight->contiguous() : Tensor();
+  const Tensor h = residual ? torch::empty({rows, d}, r.options()) : x;
+  const Tensor rstd = stats ? empty_floats(rows, x) : Tensor();
+  eg_norm o = {};
+  o.x = rows_of(x, rows);
+  o.x_dtype = dtype_code(x);
+  o.x_stride = row_stride(x);
+  if (residual) {
+    o.residual = rows_of(r, rows);
+    o.r_dtype = dtype_code(r);
+    o.r_stride = row_stride(r);
+  }
+  if (weight) {
+    o.weight = w.data_ptr();
+    o.w_dtype = dtype_code(w);
+  }
+  o.eps = (float)eps;
+  o.rows = rows;
+  o.d = d;
+  float* const stat = stats && rows > 0 ? (float*)rstd.data_ptr() : nullptr;
+  void* const sum = residual ? rows_of(h, rows) : nullptr;
+  if (dtype < 0) {
+    const auto [q, scales] = empty_blocks(rows, d, 1, x);
+    const eg_fp8_matrix y = blocks_of(q, scales, d, 1, "y", x.device());
+    check(g.norm(&o, sum, d, nullptr, 0, 0, &y, stat, (void*)stream));
+    return {q, scales, h, stats ? MaybeTensor(rstd) : std::nullopt};
+  }
+  const Tensor y = torch::empty({rows, d}, x.options().dtype(type_of(dtype, "out_dtype")));
+  check(g.norm(&o, sum, d, rows_of(y, rows), (int32_t)dtype, d, nullptr, stat, (void*)stream));
+  return {y, std::nullopt, h, stats ? MaybeTensor(rstd) : std::nullopt};
+}
+
+// (d_x of `dtype`, the same of `dtype2` (-1: none), the weight's of its type)
+std::tuple<Tensor, MaybeTensor, MaybeTensor> norm_grad(const Tensor& d_y_, const Tensor& h_, const Tensor& rstd_, const MaybeTensor& weight,
+                                                       const MaybeTensor& d_res, int64_t dtype, int64_t dtype2, bool weight_grad, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  const c10::OptionalDeviceGuard on(gpu_of(h_));
+  const Tensor h = rows_2d(h_, "h"), d_y = rows_2d(d_y_, "d_y");
+  const int64_t rows = h.size(0), d = h.size(1);
+  if (d < 1) refuse("h must have at least one column");
+  if (d_y.sizes() != h.sizes() || d_y.device() != h.device()) refuse("d_y must be ", h.sizes(), " on ", h.device(), ", got ", d_y.sizes(), " on ", d_y.device());
+  if (rstd_.dim() != 1 || rstd_.size(0) != rows || rstd_.scalar_type() != torch::kFloat32 || rstd_.device() != h.device())
+    refuse("rstd must be f32 [", rows, "] on ", h.device(), ", got ", rstd_.scalar_type(), " ", rstd_.sizes(), " on ", rstd_.device());
+  const Tensor rstd = rstd_.contiguous();
+  check_vector(weight, d, "weight", h.device());
+  if (weight_grad && !weight) refuse("the weight's gradient without a weight");
+  const Tensor w = weight ? weight->contiguous() : Tensor();
+  Tensor dr;
+  if (d_res) {
+    dr = rows_2d(*d_res, "d_residual");
+    if (dr.sizes() != h.sizes() || dr.device() != h.device() || dr.scalar_type() != h.scalar_type())
+      refuse("d_residual must be ", h.scalar_type(), " ", h.sizes(), " on ", h.device(), ", got ", dr.scalar_type(), " ", dr.sizes(), " on ", dr.device());
+  }
+  eg_norm_grad o = {};
+  o.d_y = rows_of(d_y, rows);
+  o.dy_dtype = dtype_code(d_y);
+  o.dy_stride = row_stride(d_y);
+  o.h = rows_of(h, rows);
+  o.h_dtype = dtype_code(h);
+  o.h_stride = row_stride(h);
+  if (d_res) {
+    o.d_residual = rows_of(dr, rows);
+    o.dr_stride = row_stride(dr);
+  }
+  if (weight) {
+    o.weight = w.data_ptr();
+    o.w_dtype = dtype_code(w);
+  }
+  o.rstd = rows > 0 ? (const float*)rstd.data_ptr() : nullptr;
+  o.rows = rows;
+  o.d = d;
+  const Tensor d_x = torch::empty({rows, d}, h.options().dtype(type_of(dtype, "the gradient's type")));
+  const Tensor d_x2 = dtype2 >= 0 ? torch::empty({rows, d}, h.options().dtype(type_of(dtype2, "the gradient's type"))) : Tensor();
+  const Tensor d_w = weight_grad ? torch::empty({d}, w.options()) : Tensor();
+  const int64_t need = weight_grad ? g.norm_grad_workspace(rows, d) : 0;
+  const Tensor ws = need > 0 ? torch::empty({need}, h.options().dtype(torch::kUInt8)) : Tensor();
+  check(g.norm_grad(&o, rows_of(d_x, rows), (int32_t)dtype, d, rows_of(d_x2, rows), (int32_t)dtype2, d, weight_grad ? d_w.data_ptr() : nullptr,
+                    weight_grad ? dtype_code(d_w) : 0, need > 0 ? ws.data_ptr() : nullptr, std::max<int64_t>(need, 0), (void*)stream));
+  return {d_x, dtype2 >= 0 ? MaybeTensor(d_x2) : std::nullopt, weight_grad ? MaybeTensor(d_w) : std::nullopt};
+}
+
+// ---- the norm of all gradients --------------------------------------------------------------------
+
+struct Rows {
+  int64_t rows, cols, stride;
+};
+
+// A tensor's values as rows of unit stride, in the order of its dimensions; in any order that leaves no
+// gaps where `any_order`.
+Rows rows_of_any(const Tensor& t, bool any_order, const char* name) {
+  if (t.is_contiguous() || (any_order && t.is_non_overlapping_and_dense())) return {1, t.numel(), t.numel()};
+  std::vector<std::pair<int64_t, int64_t>> dims;  // size and stride, those that continue one another as one
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) == 1) continue;
+    if (!dims.empty() && dims.back().second == t.size(i) * t.stride(i))
+      dims.back() = {dims.back().first * t.size(i), t.stride(i)};
+    else
+      dims.push_back({t.size(i), t.stride(i)});
+  }
+  if (dims.size() == 2 && dims[1].second == 1 && dims[0].second >= dims[1].first) return {dims[0].first, dims[1].first, dims[0].second};
+  refuse(name, " must be without gaps, or rows of unit stride, got ", t.sizes(), " with strides ", t.strides());
+}
+
+// The norm; with `outs` (or in place) the clipped gradients too.
+Tensor clip(const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& outs, double max_norm, int64_t stream) {
+  const at::AutoDispatchBelowADInplaceOrView no_autograd;
+  if (grads.empty()) refuse("no gradients");
+  if (outs && outs->size() != grads.size()) refuse(grads.size(), " gradients and ", outs->size(), " outputs");
+  const c10::OptionalDeviceGuard on(gpu_of(grads[0]));
+  std::vector<eg_clip_tensor> tensors;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& t = grads[i];
+    if (dtype_code(t) < 0 || !t.is_cuda() || t.device() != grads[0].device())
+      refuse("gradients must be f32, bf16 or f16 on one GPU, got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+    eg_clip_tensor c = {};
+    c.g_dtype = dtype_code(t);
+    const Tensor* o = outs ? &(*outs)[i] : nullptr;
+    if (o != nullptr && (dtype_code(*o) < 0 || o->device() != t.device() || o->sizes() != t.sizes()))
+      refuse("an output must be f32, bf16 or f16 ", t.sizes(), " on ", t.device(), ", got ", o->scalar_type(), " ", o->sizes(), " on ", o->device());
+    const bool alike = o == nullptr || o->strides() == t.strides();
+    Rows a = rows_of_any(t, alike, "a gradient"), b = o ? rows_of_any(*o, alike, "an output") : a;
+    if (a.rows == 1 && b.rows > 1) a = {b.rows, b.cols, b.cols};
+    if (b.rows == 1 && a.rows > 1) b = {a.rows, a.cols, a.cols};
+    if (a.cols != b.cols) refuse("an output's rows of ", b.cols, " values for a gradient's of ", a.cols);
+    c.rows = a.rows;
+    c.cols = a.cols;
+    c.g_stride = a.stride;
+    c.out_stride = b.stride;
+    if (t.numel() > 0) {
+      c.g = t.data_ptr();
+      c.out = o ? o->data_ptr() : nullptr;
+    }
+    if (o) c.out_dtype = dtype_code(*o);
+    tensors.push_back(c);
+  }
+  const Tensor result = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
+  const int64_t need = g.clip_workspace(tensors.data(), (int64_t)tensors.size());
+  const Tensor ws = torch::empty({std::max<int64_t>(need, 16)}, grads[0].options().dtype(torch::kUInt8));
+  check(g.clip(tensors.data(), (int64_t)tensors.size(), (float)max_norm, (float*)result.data_ptr(), ws.data_ptr(), std::max<int64_t>(need, 0),
+               (void*)stream));
+  if (outs)
+    for (const Tensor& o : *outs) written(o);
+  return result;
+}
+
 void init_ops(const std::map<std::string, int64_t>& at, pybind11::object error) {
   auto set = [&](auto& fn, const char* name) { fn = reinterpret_cast<std::decay_t<decltype(fn)>>(at.at(name)); };
   set(g.loss_workspace, "eg_loss_workspace_size");
@@ -354,6 +669,17 @@ void init_ops(const std::map<std::string, int64_t>& at, pybind11::object error) 
   set(g.muon_workspace, "eg_muon_workspace_size");
   set(g.muon_check, "eg_muon_check");
   set(g.muon, "eg_muon_step");
+  set(g.fp8_quantize, "eg_fp8_quantize");
+  set(g.fp8_quantize_weight, "eg_fp8_quantize_weight");
+  set(g.fp8_dequantize, "eg_fp8_dequantize");
+  set(g.fp8_product, "eg_fp8_product");
+  set(g.fp8_linear, "eg_fp8_linear");
+  set(g.fp8_linear_workspace, "eg_fp8_linear_workspace_size");
+  set(g.norm, "eg_add_rms_norm");
+  set(g.norm_grad, "eg_add_rms_norm_grad");
+  set(g.norm_grad_workspace, "eg_add_rms_norm_grad_workspace_size");
+  set(g.clip, "eg_clip_grads");
+  set(g.clip_workspace, "eg_clip_workspace_size");
   set(g.last_error, "eg_last_error");
   g_error = error.release();
 }
@@ -367,4 +693,12 @@ void bind_ops(pybind11::module_& m) {
   m.def("preference", &preference);
   m.def("logits_grad", &logits_grad);
   m.def("muon", &muon);
+  m.def("fp8_quantize", &fp8_quantize);
+  m.def("fp8_quantize_weight", &fp8_quantize_weight);
+  m.def("fp8_dequantize", &fp8_dequantize);
+  m.def("fp8_linear", &fp8_linear);
+  m.def("fp8_product", &fp8_product);
+  m.def("norm", &norm);
+  m.def("norm_grad", &norm_grad);
+  m.def("clip", &clip);
 }

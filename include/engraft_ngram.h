@@ -828,6 +828,122 @@ int eg_muon_check(const eg_muon* muon);
 
 int eg_muon_step(const eg_muon* muon, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Products of 8-bit floating point ------------------------------------------------
+ *
+ * The block's projections kept in 8 bits, served and trained through.  No counterpart in
+ * the reference, whose projections are fp32 (engraft/replica/layers.py:594-606). */
+
+/* A matrix [rows, k] in blocks: e4m3 values q, and for each 128 values along a row (the
+ * last block may be short) and block_rows rows (1 or 128) a scale 2^e as the byte e + 127
+ * (e8m0).  Element (r, c) is q[r * stride + c] * 2^(scales[(r / block_rows) * scale_stride + c / 128] - 127).
+ * Strides in bytes: `stride` a multiple of 16, at least k rounded up to 128; scale_stride a
+ * multiple of 4, at least the blocks rounded up to 4.  q 16-byte and scales 4-byte aligned.
+ * The bytes of q from k to the end of the last block are zeros. */
+typedef struct eg_fp8_matrix {
+  void* q;
+  uint8_t* scales;
+  int64_t rows, k;
+  int64_t stride, scale_stride;
+  int32_t block_rows;
+} eg_fp8_matrix;
+
+/* The blocks (block_rows 1) of x [out->rows, out->k] of `dtype`, rows row_stride elements apart:
+ * e is the least with max|x| <= 448 * 2^e over the block's finite values (not below -127; 0 for a block of
+ * zeros), q the nearest e4m3 of x * 2^-e, ties to even; NaN and infinities become NaN. */
+int eg_fp8_quantize(const void* x, int32_t dtype, int64_t row_stride, const eg_fp8_matrix* out, void* stream);
+
+/* The same of a weight [out->rows, out->k], a scale for each 128 x 128 block (block_rows 128), element
+ * (r, c) at x[r * row_stride + c * col_stride]; with out_t (NULL: not wanted) [k, rows] the transpose, the
+ * same values under the same scales. */
+int eg_fp8_quantize_weight(const void* x, int32_t dtype, int64_t row_stride, int64_t col_stride,
+                           const eg_fp8_matrix* out, const eg_fp8_matrix* out_t, void* stream);
+
+/* The values that `m` stands for, as `dtype`, rows row_stride apart (exact in bf16 and f32 where they
+ * are in its normal range). */
+int eg_fp8_dequantize(const eg_fp8_matrix* m, void* out, int32_t dtype, int64_t row_stride, void* stream);
+
+/* C [m, n] = A B^T and, with b2, C2 [m, n2] = A B2^T: a in blocks of rows (block_rows 1), b and b2
+ * weights (block_rows 128) of the same k; C of `dtype`, rows ldc apart.  f32 outputs come from exact products and
+ * fp32 sums; bf16 and f16 ones of more than 32 rows from the fp8 matrix cores, whose sums of eight products drop
+ * what lies 2^-13 below the largest of them (about 1.5e-5 of an output, a hundredth of bf16's rounding). */
+int eg_fp8_product(const eg_fp8_matrix* a, const eg_fp8_matrix* b, const eg_fp8_matrix* b2, void* c, int64_t ldc,
+                   void* c2, int64_t ldc2, int32_t dtype, void* stream);
+
+/* The same from A's values x [m, b->k] of x_dtype, rows x_stride apart, whose blocks are taken on the way
+ * (eg_fp8_quantize's).  Workspace of eg_fp8_linear_workspace_size bytes, 16-byte aligned (0 up to 32 rows). */
+int64_t eg_fp8_linear_workspace_size(int64_t m, int64_t k);
+int eg_fp8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t x_stride, const eg_fp8_matrix* b,
+                  const eg_fp8_matrix* b2, void* c, int64_t ldc, void* c2, int64_t ldc2, int32_t dtype,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- The residual's addition and the RMS norm of the sum ------------------------------
+ *
+ * What stands between the block's output and the projections behind it (the reference's
+ * rms norm without the addition: engraft/replica/layers.py). */
+
+/* x [rows, d], residual the same (of x's type or f32) or NULL, weight [d] or NULL (1), rows stride
+ * elements apart. */
+typedef struct eg_norm {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  int32_t x_dtype, r_dtype, w_dtype;
+  float eps;
+  int64_t rows, d;
+  int64_t x_stride, r_stride;
+} eg_norm;
+
+/* h = x + residual, rounded to the residual's type (without a residual h is x and not written);
+ * y = h w / sqrt(mean(h^2) + eps) in 32 bits, written as y (y_dtype) or in blocks as y8 (eg_fp8_quantize's):
+ * one of the two.  rstd f32 [rows] (NULL: not wanted): 1 / sqrt(...), for the gradient.  h may be in
+ * the place of x or of the residual; any other overlap is refused.  d up to 40,960. */
+int eg_add_rms_norm(const eg_norm* norm, void* h, int64_t h_stride, void* y, int32_t y_dtype, int64_t y_stride,
+                    const eg_fp8_matrix* y8, float* rstd, void* stream);
+
+/* d_y [rows, d] the gradient of y, h and rstd of the forward, d_residual (h's type; NULL: none) the gradient
+ * of h from elsewhere, weight as in the forward. */
+typedef struct eg_norm_grad {
+  const void* d_y;
+  const void* h;
+  const void* d_residual;
+  const void* weight;
+  const float* rstd;
+  int32_t dy_dtype, h_dtype, w_dtype;
+  int64_t rows, d;
+  int64_t dy_stride, h_stride, dr_stride;
+} eg_norm_grad;
+
+/* The gradient of h (of x and of the residual alike) as d_x and, in a second type, as d_x2 (NULL: not
+ * wanted), and the weight's, d_weight [d] (NULL: not wanted; then no workspace either).  Sums in 32 bits, in
+ * a fixed order.  Outputs must not overlap the inputs.  d up to 20,480.  Workspace 16-byte aligned. */
+int64_t eg_add_rms_norm_grad_workspace_size(int64_t rows, int64_t d);
+int eg_add_rms_norm_grad(const eg_norm_grad* grad, void* d_x, int32_t dx_dtype, int64_t dx_stride, void* d_x2,
+                         int32_t dx2_dtype, int64_t dx2_stride, void* d_weight, int32_t dw_dtype, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* ---- The norm of all gradients, and their clipping --------------------------------------
+ *
+ * What stands between a step's gradients and its weight updates; no counterpart in the reference. */
+
+/* A gradient [rows, cols], rows g_stride elements apart, and where its clipped values go (NULL: the norm
+ * alone is wanted; the gradient itself for in place). */
+typedef struct eg_clip_tensor {
+  const void* g;
+  void* out;
+  int64_t rows, cols;
+  int64_t g_stride, out_stride;
+  int32_t g_dtype, out_dtype;
+} eg_clip_tensor;
+
+/* norm f32 [1] = sqrt of the sum of all squares of `count` tensors (a HOST array), added in 64 bits in a fixed
+ * order; with an `out`, out = g * max_norm / norm where norm > max_norm, and g otherwise (a norm that is not
+ * finite leaves the values as they are).  Either all tensors have an `out` or none.  What is written
+ * must not overlap another tensor, nor its own gradient but in place (refused).  Workspace of
+ * eg_clip_workspace_size bytes, 16-byte aligned. */
+int64_t eg_clip_workspace_size(const eg_clip_tensor* tensors, int64_t count);
+int eg_clip_grads(const eg_clip_tensor* tensors, int64_t count, float max_norm, float* norm, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
