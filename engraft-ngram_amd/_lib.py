@@ -221,7 +221,6 @@ class EgNorm(ctypes.Structure):
         ("weight", c_void_p),
         ("x_dtype", c_int32),
         ("r_dtype", c_int32),
-        ("w_dtype", c_int32),
         ("eps", ctypes.c_float),
         ("rows", c_int64),
         ("d", c_int64),
@@ -239,7 +238,6 @@ class EgNormGrad(ctypes.Structure):
         ("rstd", c_void_p),
         ("dy_dtype", c_int32),
         ("h_dtype", c_int32),
-        ("w_dtype", c_int32),
         ("rows", c_int64),
         ("d", c_int64),
         ("dy_stride", c_int64),
@@ -369,15 +367,16 @@ SIGNATURES = {
                                          c_void_p]),
     "eg_fp8_dequantize": (c_int32, [POINTER(EgFp8Matrix), c_void_p, c_int32, c_int64, c_void_p]),
     "eg_fp8_product": (c_int32, [POINTER(EgFp8Matrix), POINTER(EgFp8Matrix), POINTER(EgFp8Matrix), c_void_p, c_int64,
-                                 c_void_p, c_int64, c_int32, c_void_p]),
-    "eg_fp8_linear_workspace_size": (c_int64, [c_int64, c_int64]),
+                                 c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
+    "eg_fp8_product_workspace_size": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
+    "eg_fp8_linear_workspace_size": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
     "eg_fp8_linear": (c_int32, [c_void_p, c_int32, c_int64, c_int64, POINTER(EgFp8Matrix), POINTER(EgFp8Matrix), c_void_p,
                                 c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
     "eg_add_rms_norm": (c_int32, [POINTER(EgNorm), c_void_p, c_int64, c_void_p, c_int32, c_int64, POINTER(EgFp8Matrix),
                                   c_void_p, c_void_p]),
     "eg_add_rms_norm_grad_workspace_size": (c_int64, [c_int64, c_int64]),
     "eg_add_rms_norm_grad": (c_int32, [POINTER(EgNormGrad), c_void_p, c_int32, c_int64, c_void_p, c_int32, c_int64,
-                                       c_void_p, c_int32, c_void_p, c_int64, c_void_p]),
+                                       c_void_p, c_void_p, c_int64, c_void_p]),
     "eg_clip_workspace_size": (c_int64, [POINTER(EgClipTensor), c_int64]),
     "eg_clip_grads": (c_int32, [POINTER(EgClipTensor), c_int64, ctypes.c_float, c_void_p, c_void_p, c_int64, c_void_p]),
 }
@@ -441,7 +440,7 @@ def autograd_ext():
                   for f in ("eg_loss_workspace_size", "eg_token_logprobs", "eg_policy_loss", "eg_preference_loss",
                             "eg_logits_grad", "eg_muon_workspace_size", "eg_muon_check", "eg_muon_step", "eg_fp8_quantize",
                             "eg_fp8_quantize_weight", "eg_fp8_dequantize", "eg_fp8_product", "eg_fp8_linear",
-                            "eg_fp8_linear_workspace_size", "eg_add_rms_norm", "eg_add_rms_norm_grad",
+                            "eg_fp8_linear_workspace_size", "eg_fp8_product_workspace_size", "eg_add_rms_norm", "eg_add_rms_norm_grad",
                             "eg_add_rms_norm_grad_workspace_size", "eg_clip_grads", "eg_clip_workspace_size",
                             "eg_last_error")}, EgError)
     _EXT = mod

@@ -90,20 +90,36 @@ __device__ inline void write8(const ClipTensor& t, int64_t i, const float (&v)[8
   }
 }
 
+constexpr int kReads = kTile / (kThreads * 8);  // eight values each, a thread and tile
+
+// A tile's values: all loads are on their way before the first is waited for.
+template <typename T>
+__device__ inline void read_tile(const ClipTensor& t, int64_t tile, float (&v)[kReads][8]) {
+  const int64_t i0 = (tile - t.first_tile) * kTile + threadIdx.x * 8;
+  if (t.cols == t.g_stride && (tile - t.first_tile + 1) * kTile <= t.values) {
+    Raw8<T> r[kReads];
+#pragma unroll
+    for (int j = 0; j < kReads; ++j) r[j] = load_raw<false>((const T*)t.g + i0 + j * kThreads * 8, 0, 8);
+#pragma unroll
+    for (int j = 0; j < kReads; ++j) values_of<false, T>(r[j], 0, 8, v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kReads; ++j) read8<T>(t, i0 + j * kThreads * 8, v[j]);
+  }
+}
+
 __global__ __launch_bounds__(kThreads) void squares_kernel(const ClipArgs a) {
   __shared__ double part[kThreads / 64];
   double s = 0.0;
   for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const ClipTensor& t = a.t[tensor_of(a, tile)];
-    const int64_t i0 = (tile - t.first_tile) * kTile + threadIdx.x * 8;
     device_type(t.g_dtype, [&](auto z) {
+      float v[kReads][8];
+      read_tile<decltype(z)>(t, tile, v);
 #pragma unroll
-      for (int j = 0; j < kTile / (kThreads * 8); ++j) {
-        float v[8];
-        read8<decltype(z)>(t, i0 + j * kThreads * 8, v);
+      for (int j = 0; j < kReads; ++j)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s += (double)v[k] * (double)v[k];
-      }
+        for (int k = 0; k < 8; ++k) s += (double)v[j][k] * (double)v[j][k];
     });
   }
   s = wave_sum64(s);
@@ -139,18 +155,17 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(const ClipArgs a, const
     const ClipTensor& t = a.t[tensor_of(a, tile)];
     if (!clips && t.out == t.g) continue;  // as they are
     const int64_t i0 = (tile - t.first_tile) * kTile + threadIdx.x * 8;
-    device_type(t.g_dtype, [&](auto z) {
-      device_type(t.out_dtype, [&](auto y) {
+    float v[kReads][8];
+    device_type(t.g_dtype, [&](auto z) { read_tile<decltype(z)>(t, tile, v); });
+    if (clips) {
 #pragma unroll
-        for (int j = 0; j < kTile / (kThreads * 8); ++j) {
-          const int64_t i = i0 + j * kThreads * 8;
-          float v[8];
-          read8<decltype(z)>(t, i, v);
+      for (int j = 0; j < kReads; ++j)
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] = clips ? (float)((double)v[q] * factor) : v[q];
-          write8<decltype(y)>(t, i, v);
-        }
-      });
+        for (int q = 0; q < 8; ++q) v[j][q] = (float)((double)v[j][q] * factor);
+    }
+    device_type(t.out_dtype, [&](auto y) {
+#pragma unroll
+      for (int j = 0; j < kReads; ++j) write8<decltype(y)>(t, i0 + j * kThreads * 8, v[j]);
     });
   }
 }

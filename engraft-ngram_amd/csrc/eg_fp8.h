@@ -41,6 +41,62 @@ __device__ inline void load8(const T* __restrict__ p, int valid, float (&v)[8]) 
   }
 }
 
+// A lane's eight values of a row of d, from column `at` on, in two steps, so that many loads are on their way before the first
+// is waited for: their bytes, by a load without a branch (a lane past the row's end reads its first or last
+// eight; `tiny`: rows of less than eight, one by one), and their values, zeros in the place of what does not
+// exist.  RAGGED: d is no multiple of eight, and the lane at the end reads the row's last eight and moves them.
+template <typename T>
+struct Raw8 {
+  i32x4 w[sizeof(T) / 2];
+};
+
+template <bool RAGGED, typename T>
+__device__ inline Raw8<T> load_raw(const T* __restrict__ row, int at, int d) {
+  typedef i32x4 unaligned __attribute__((aligned(2)));
+  Raw8<T> r;
+  if (RAGGED && d < 8) {
+    T x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = row[min(at + i, d - 1)];
+    __builtin_memcpy(&r, x, sizeof(r));
+    return r;
+  }
+  const T* const p = row + (RAGGED ? min(at, d - 8) : at < d ? at : 0);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = ((const unaligned*)p)[i];
+  return r;
+}
+
+template <bool RAGGED, typename T>
+__device__ inline void values_of(Raw8<T> r, int at, int d, float (&v)[8]) {
+  const int left = d - at;
+  if (RAGGED && d >= 8) {
+    const int by = left < 8 ? (8 - left) & 7 : 0;  // (all are zeros below where none is left)
+    if constexpr (sizeof(T) == 2) {
+      r.w[0] = __builtin_bit_cast(i32x4, __builtin_bit_cast(unsigned __int128, r.w[0]) >> (16 * by));
+    } else {
+#pragma unroll
+      for (int step = 4; step > 0; step >>= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int from = i + step < 8 ? r.w[((i + step) & 7) >> 2][(i + step) & 3] : 0;
+          r.w[i >> 2][i & 3] = by & step ? from : r.w[i >> 2][i & 3];
+        }
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[0][i] = left > 0 ? r.w[0][i] : 0;
+    const t8 x = __builtin_bit_cast(t8, r.w[0]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = RAGGED && d < 8 && i >= left ? 0.0f : (float)x[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = left > (RAGGED && d < 8 ? i : 0) ? __int_as_float(r.w[i >> 2][i & 3]) : 0.0f;
+  }
+}
+
 template <typename T>
 __device__ inline void store8(T* __restrict__ p, int valid, const float (&v)[8]) {
   if (valid >= 8) {
@@ -109,8 +165,18 @@ __device__ inline void store_blocks(const float (&v)[8], uint8_t* __restrict__ q
                                     int g, int blocks, int lane) {
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = finite_max(top, v[i]);
-  const int byte = scale_byte(row_max(top));
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+    top = a > top ? a : top;
+  }
+  top = row_max(top);
+  if (__builtin_expect(top >= 0x7f800000u, 0)) {  // (the same in a block's 16 lanes)
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = finite_max(top, v[i]);
+    top = row_max(top);
+  }
+  const int byte = scale_byte(top);
   const int block = 4 * g + (lane >> 4);
   if (block < blocks) *(u32x2*)(q_row + (int64_t)g * 512 + lane * 8) = quantize8(v, scale_inverse(byte));
   uint32_t packed = 0;

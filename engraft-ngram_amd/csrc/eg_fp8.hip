@@ -15,12 +15,14 @@
 // what their registers held.  Here its results are used again by the next step of a loop, which holds them outside.
 #include "eg_fp8.h"
 
+#include <algorithm>
+
 #include "eg_lds.h"
 
 namespace eg {
 namespace {
 
-constexpr int kXcds = 8;
+constexpr int kXcds = 8, kCUs = 256;
 constexpr int kGroupM = 8;  // row tiles a group: see grouped()
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -156,11 +158,20 @@ struct ProductArgs {
   int64_t m, n[2];
   int blocks;  // of 128 along k
   int tiles_m, tiles_n0, tiles_n;
+  // pieces along k of `per` blocks each, which write their sums piece_stride outputs apart
+  int pieces, per;
+  int64_t piece_stride;
   // the few-row kernel's unquantised A
   const void* x;
   int64_t ldx;
   int k;
 };
+
+__device__ inline i32x8 join(const i32x4 (&x)[2]) {
+  return i32x8{x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+}
+
+constexpr int kFewBlocks = 5;  // blocks of k that a wavefront of the few-row kernel has in flight
 
 // Eight e4m3 bytes times 2^e (`scale`: its float) as bf16, exactly.
 __device__ inline bf16x8 widen8(int lo, int hi, float scale) {
@@ -174,18 +185,24 @@ __device__ inline bf16x8 widen8(int lo, int hi, float scale) {
 // The float that the widening conversions take for a scale's byte: they read its exponent alone.
 __device__ inline float byte_as_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// Few rows: reading B bounds the product.  A workgroup 16 columns, its wavefronts every KW-th block of k,
-// their sums added in order through LDS.  A lane's weights are 32 consecutive bytes of a column's row: the
+// Few rows: reading B bounds the product.  A wavefront 16 columns and every kw-th block of k, at most U of them
+// in flight at once (all of its own up to U kw blocks); a workgroup kw wavefronts of each of cw column groups, whose sums
+// are added in order through LDS.  A lane's weights are 32 consecutive bytes of a column's row: the
 // 16 rows of 128 bytes that a load takes are whole lines, and go straight to registers.  B is the MFMA's first
 // operand, so that a lane ends up with four consecutive columns of a row.  FUSED: A's blocks are taken
-// here, into LDS, while the first weights are on their way (a few rows: every workgroup does it).
+// here, into LDS (rows 16 bytes more than their blocks apart: 16 rows' chunks lie in different banks), while the
+// first weights are on their way; every workgroup does it.
 template <int G, bool FUSED, typename X, typename Out>
-__global__ __launch_bounds__(1024) void few_rows_kernel(const ProductArgs p) {
-  constexpr int U = 4;  // blocks of k in flight a wavefront
+__global__ __launch_bounds__(1024) void few_rows_kernel(const ProductArgs p, int kw) {
+  constexpr int U = kFewBlocks;
+  constexpr bool EXACT = sizeof(Out) == 4;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = blockDim.x >> 6;
-  const int grp = (int)blockIdx.x < p.tiles_n0 ? 0 : 1;
-  const int64_t n0 = (int64_t)((int)blockIdx.x - (grp ? p.tiles_n0 : 0)) * 16, n = p.n[grp];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cw = (int)(blockDim.x >> 6) / kw;
+  const int wk = wave % kw, wc = wave / kw;
+  const int tiles = p.tiles_n0 + (int)((p.n[1] + 15) >> 4);
+  const int tile = min((int)blockIdx.x * cw + wc, tiles - 1);  // the last workgroup's spare wavefronts repeat the last tile
+  const int grp = tile < p.tiles_n0 ? 0 : 1;
+  const int64_t n0 = (int64_t)(tile - (grp ? p.tiles_n0 : 0)) * 16, n = p.n[grp];
   const int64_t col = n0 + (lane & 15) < n ? n0 + (lane & 15) : n - 1;
   const uint8_t* const w = p.b[grp] + col * p.ldb[grp] + (lane >> 4) * 32;
   const uint8_t* const w_scales = p.b_scales[grp] + (n0 >> 7) * p.ldb_scales[grp];
@@ -202,76 +219,97 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(const ProductArgs p) {
       ws[u] = w_scales[kb];
     }
   };
-  load_weights(wave);
+  load_weights(wk);
 
-  const int kp = blocks * 128, sp = (blocks + 3) & ~3;
+  const int row_bytes = blocks * 128 + 16, scale_bytes = (blocks + 3) & ~3;
+  uint8_t* const scales = lds + p.m * row_bytes;
   if constexpr (FUSED) {
-    const int groups = sp >> 2;
-    for (int64_t unit = wave; unit < p.m * groups; unit += kw) {
-      const int row = (int)(unit / groups), g = (int)(unit - (int64_t)row * groups), at = g * 512 + lane * 8;
+    const int groups = scale_bytes >> 2, waves = kw * cw;
+    for (int unit = wave; unit < (int)p.m * groups; unit += waves) {
+      const int row = unit / groups, g = unit - row * groups, at = g * 512 + lane * 8;
       float v[8];
       load8((const X*)p.x + row * p.ldx + at, p.k - at, v);
-      store_blocks(v, lds + row * kp, lds + p.m * kp + row * sp, g, blocks, lane);
+      store_blocks(v, lds + row * row_bytes, scales + row * scale_bytes, g, blocks, lane);
     }
     __syncthreads();
   }
 
+  // A's rows past the last one are the last one's: not stored
+  int64_t row[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) row[g] = min((int64_t)(16 * g + (lane & 15)), p.m - 1);
+  i32x4 xf[2][G][2];  // of a block and the next one
+  uint32_t xs[2][G];
+  auto load_rows = [&](int to, int kb) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint8_t* const q = FUSED ? lds + row[g] * row_bytes + kb * 128 + (lane >> 4) * 32
+                                     : p.a + row[g] * p.lda + (int64_t)kb * 128 + (lane >> 4) * 32;
+      xf[to][g][0] = *(const i32x4*)q;
+      xf[to][g][1] = *(const i32x4*)(q + 16);
+      xs[to][g] = FUSED ? scales[row[g] * scale_bytes + kb] : p.a_scales[row[g] * p.lda_scales + kb];
+    }
+  };
+
   f32x4 acc[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) acc[g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int kb0 = wave; kb0 < blocks; kb0 += U * kw) {
-    if (kb0 != wave) load_weights(kb0);
+  for (int kb0 = wk; kb0 < blocks; kb0 += U * kw) {
+    if (kb0 != wk) load_weights(kb0);
+    load_rows(0, kb0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int kb = kb0 + u * kw;
       if (kb < blocks) {
-        const float s = byte_as_scale(ws[u]);
-        bf16x8 wv[4];
+        if (u + 1 < U) load_rows((u + 1) & 1, kb + kw < blocks ? kb + kw : kb);
+        if constexpr (EXACT) {
+          const float s = byte_as_scale(ws[u]);
+          bf16x8 wv[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) wv[i] = widen8(wf[u][i >> 1][2 * (i & 1)], wf[u][i >> 1][2 * (i & 1) + 1], s);
+          for (int i = 0; i < 4; ++i) wv[i] = widen8(wf[u][i >> 1][2 * (i & 1)], wf[u][i >> 1][2 * (i & 1) + 1], s);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const int64_t row = 16 * g + (lane & 15);
-          i32x4 xf[2] = {};
-          uint32_t xs = 127;
-          if (row < p.m) {
-            if constexpr (FUSED) {
-              const uint8_t* q = lds + row * kp + kb * 128 + (lane >> 4) * 32;
-              xf[0] = *(const i32x4*)q;
-              xf[1] = *(const i32x4*)(q + 16);
-              xs = lds[p.m * kp + row * sp + kb];
-            } else {
-              const uint8_t* q = p.a + row * p.lda + (int64_t)kb * 128 + (lane >> 4) * 32;
-              xf[0] = *(const i32x4*)q;
-              xf[1] = *(const i32x4*)(q + 16);
-              xs = p.a_scales[row * p.lda_scales + kb];
-            }
+          for (int g = 0; g < G; ++g) {
+            const i32x4* const x = xf[u & 1][g];
+            const float t = byte_as_scale(xs[u & 1][g]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[i], widen8(x[i >> 1][2 * (i & 1)], x[i >> 1][2 * (i & 1) + 1], t),
+                                                               acc[g], 0, 0, 0);
           }
-          const float t = byte_as_scale(xs);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                wv[i], widen8(xf[i >> 1][2 * (i & 1)], xf[i >> 1][2 * (i & 1) + 1], t), acc[g], 0, 0, 0);
+          for (int g = 0; g < G; ++g)
+            acc[g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(wf[u]), join(xf[u & 1][g]), acc[g], 0, 0, 0, (int)ws[u], 0,
+                                                                      (int)xs[u & 1][g]);
         }
       }
     }
   }
+  // the products are used outside of branches first
+#pragma unroll
+  for (int g = 0; g < G; ++g) asm volatile("" : "+v"(acc[g]));
   // the wavefronts' sums, in order; a lane: row lane % 16, columns 4 (lane / 16) .. + 3
   if constexpr (FUSED) __syncthreads();
   f32x4* const sums = (f32x4*)lds;
 #pragma unroll
   for (int g = 0; g < G; ++g) sums[(wave * G + g) * 64 + lane] = acc[g];
   __syncthreads();
-  for (int g = wave; g < G; g += kw) {
-    f32x4 t = sums[g * 64 + lane];
-    for (int i = 1; i < kw; ++i) t += sums[(i * G + g) * 64 + lane];
-    const int64_t row = 16 * g + (lane & 15);
+  if ((int)blockIdx.x * cw + wc >= tiles) return;
+  for (int g = wk; g < G; g += kw) {
+    f32x4 t = sums[(wc * kw * G + g) * 64 + lane];
+    for (int i = 1; i < kw; ++i) t += sums[((wc * kw + i) * G + g) * 64 + lane];
+    const int64_t r = 16 * g + (lane & 15);
     const int64_t c0 = n0 + 4 * (lane >> 4);
-    if (row < p.m) {
-      Out* const c = (Out*)p.c[grp] + row * p.ldc[grp] + c0;
+    if (r < p.m) {
+      Out* const c = (Out*)p.c[grp] + r * p.ldc[grp] + c0;
+      if (c0 + 4 <= n) {
+        typedef Out o4 __attribute__((ext_vector_type(4), aligned(sizeof(Out))));
+        *(o4*)c = o4{(Out)t[0], (Out)t[1], (Out)t[2], (Out)t[3]};
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c0 + i < n) c[i] = (Out)t[i];
+        for (int i = 0; i < 4; ++i)
+          if (c0 + i < n) c[i] = (Out)t[i];
+      }
     }
   }
 }
@@ -295,27 +333,53 @@ __device__ inline int xcd_order(int b, int nb) {
   return x * per + (x < extra ? x : extra) + i;
 }
 
+// Eight 16-bit outputs of a row from four registers of each of two groups: lanes below 32 hold columns 0..3
+// of group a (and the lanes above them 4..7), and so of group b, 8 columns on.  The halves change places,
+// so that a lane below 32 has a's eight columns and the one above it b's.
+template <typename Out>
+__device__ inline i32x4 pack_groups(const f32x16& v, int g) {
+  typedef Out o4 __attribute__((ext_vector_type(4)));
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  const u2 a = __builtin_bit_cast(u2, o4{(Out)v[4 * g], (Out)v[4 * g + 1], (Out)v[4 * g + 2], (Out)v[4 * g + 3]});
+  const u2 b = __builtin_bit_cast(u2, o4{(Out)v[4 * g + 4], (Out)v[4 * g + 5], (Out)v[4 * g + 6], (Out)v[4 * g + 7]});
+  const u2 x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+  const u2 y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+  return i32x4{(int)x[0], (int)y[0], (int)x[1], (int)y[1]};
+}
+
 // A tile of BM x BN outputs, WM x WN wavefronts of 32 TI x 32 TJ.  A stage holds a block of k: A's BM
 // rows and B's BN rows of 128 bytes, then a dword of each row's scales (the four blocks around this
 // one).  The 16-byte chunk c of row r sits in slot c ^ ((r >> 1) & 7): the 16 lanes that a fragment
 // read serves at a time (one chunk of 16 consecutive rows) then touch 16 different 16-byte
-// banks.  A direct-to-LDS load fills 8 rows (1 KB).
-template <int BM, int BN, int WM, int WN, int STAGES, bool EXACT, typename Out>
-__global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs p) {
+// banks.  A direct-to-LDS load fills 8 rows (1 KB).  Two stages.
+//
+// B's fragment is the MFMA's first operand, so that a lane's registers are consecutive columns of one row of C.
+//
+// PIPED (tiles of which two fit a CU): a block's two halves (64 k) are two sets of fragments; a set is read between
+// the MFMAs of the other one.  In the middle of block kb, once every wavefront has read all of it (the barrier),
+// the loads of block kb + 2 go out into its place, one at a time between the MFMAs of its second half.
+// Otherwise (8 wavefronts, whose second set would not fit the registers) the loads of block kb + 1 go out
+// at the start of block kb, and the two wavefronts of a SIMD fill each other's waits.
+template <int BM, int BN, int WM, int WN, bool PIPED, bool EXACT, typename Out>
+__global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void product_kernel(const ProductArgs p) {
+  constexpr bool BY_ROW = sizeof(Out) == 2;
   constexpr int NW = WM * WN, TI = BM / WM / 32, TJ = BN / WN / 32;
   constexpr int LPW = (BM + BN) / 8 / NW;   // loads a wavefront and stage
-  constexpr int SPW = (BM + BN) / NW;       // rows whose scales a wavefront fetches
+  constexpr int SPW = (BM + BN) / NW;       // rows whose scales a wavefront fetches, 64 a load
+  constexpr int SL = (SPW + 63) / 64;
   constexpr int SCALES = (BM + BN) * 128;   // where a stage's scales are
   constexpr int STAGE = (BM + BN) * 132;
-  static_assert((BM / 8) % NW == 0 && (BN / 8) % NW == 0 && SPW <= 64 && BM % SPW == 0, "a wavefront's loads stay in one operand");
+  static_assert((BM / 8) % NW == 0 && (BN / 8) % NW == 0, "a wavefront's j-th load stays in one operand");
+  static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && (BM + BN) % NW == 0, "whole fragments");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
-  grouped(xcd_order(blockIdx.x, p.tiles_m * p.tiles_n), p.tiles_m, p.tiles_n, tm, tn);
+  const int tiles = p.tiles_m * p.tiles_n, piece = (int)blockIdx.x / tiles;
+  grouped(xcd_order((int)blockIdx.x - piece * tiles, tiles), p.tiles_m, p.tiles_n, tm, tn);
   const int grp = tn < p.tiles_n0 ? 0 : 1;
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)(grp ? tn - p.tiles_n0 : tn) * BN;
   const int64_t n = p.n[grp];
-  const int blocks = p.blocks;
+  const int first = piece * p.per, blocks = min(p.per, p.blocks - first);  // this piece's
 
   // load j of a stage: 8 rows from row 8 (wave + NW j) of A's, then B's.  Rows past m or n read the last one:
   // their products only reach outputs that are not stored.
@@ -330,27 +394,29 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   }
   const uint8_t* const a0 = p.a + m0 * p.lda;
   const uint8_t* const b0 = p.b[grp] + n0 * p.ldb[grp];
-  // this lane's row of scales
-  const uint8_t* scale_row;
-  {
-    const int e = wave * SPW + (lane < SPW ? lane : 0);
-    if (wave * SPW < BM) {
-      const int64_t r = m0 + e < p.m ? m0 + e : p.m - 1;
-      scale_row = p.a_scales + r * p.lda_scales;
-    } else {
-      const int64_t r = n0 + e - BM < n ? n0 + e - BM : n - 1;
-      scale_row = p.b_scales[grp] + (r >> 7) * p.ldb_scales[grp];
-    }
-  }
-  auto issue = [&](int kb, int slot) {
-    uint8_t* const st = lds + slot * STAGE;
+  // this lane's rows of scales
+  const uint8_t* scale_row[SL];
 #pragma unroll
-    for (int j = 0; j < LPW; ++j) {
-      const uint8_t* base = (NW * j < BM / 8 ? a0 : b0) + (int64_t)kb * 128;
-      __builtin_amdgcn_global_load_lds((const void*)(base + off[j]), (lds_void*)(st + (wave + NW * j) * 1024), 16, 0, 0);
-    }
-    if (lane < SPW)
-      __builtin_amdgcn_global_load_lds((const void*)(scale_row + (kb & ~3)), (lds_void*)(st + SCALES + wave * SPW * 4), 4, 0, 0);
+  for (int i = 0; i < SL; ++i) {
+    const int e = wave * SPW + i * 64 + (i * 64 + lane < SPW ? lane : 0);
+    const int64_t ra = m0 + e < p.m ? m0 + e : p.m - 1, rb = n0 + e - BM < n ? n0 + e - BM : n - 1;
+    scale_row[i] = e < BM ? p.a_scales + ra * p.lda_scales : p.b_scales[grp] + (rb >> 7) * p.ldb_scales[grp];
+  }
+  auto load = [&](int kb, int j) {
+    const uint8_t* base = (NW * j < BM / 8 ? a0 : b0) + (int64_t)(first + kb) * 128;
+    __builtin_amdgcn_global_load_lds((const void*)(base + off[j]), (lds_void*)(lds + (kb & 1) * STAGE + (wave + NW * j) * 1024), 16, 0, 0);
+  };
+  auto load_scales = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < SL; ++i)
+      if (i * 64 + lane < SPW)
+        __builtin_amdgcn_global_load_lds((const void*)(scale_row[i] + ((first + kb) & ~3)),
+                                         (lds_void*)(lds + (kb & 1) * STAGE + SCALES + (wave * SPW + i * 64) * 4), 4, 0, 0);
+  };
+  auto load_all = [&](int kb) {  // LPW + SL loads
+    load_scales(kb);
+#pragma unroll
+    for (int j = 0; j < LPW; ++j) load(kb, j);
   };
 
   const int wm = wave / WN, wn = wave % WN;
@@ -362,118 +428,331 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
+  // a half's fragments, A's rows then B's: a lane holds 32 bytes (chunks 4 h + 2 (lane / 32) and the next) of row
+  // lane % 32 of its 32
+  constexpr int Q = TI + TJ, SETS = PIPED ? 2 : 1;
+  i32x8 f[SETS][Q];
+  uint32_t sc[Q], next_sc[Q];
+  const int x = (lane >> 1) & 7;
+  uint32_t at[2];  // of a lane's first chunk in its row, by half; the other one is 16 away
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
-    if (s < blocks) issue(s, s);
-  int slot = 0;
-  for (int kb = 0; kb < blocks; ++kb) {
-    // this wavefront's part of block kb is in LDS and its reads of block kb - 1 are in registers; after the barrier,
-    // every wavefront's are
-    if (kb + STAGES - 1 <= blocks)
-      wait_vm<(STAGES - 2) * (LPW + 1)>();
-    else
-      wait_vm<0>();
-    wait_lgkm0();
-    __builtin_amdgcn_s_barrier();
-    if (kb + STAGES - 1 < blocks) issue(kb + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
-    const uint8_t* const st = lds + slot * STAGE;
-    const int shift = (kb & 3) * 8;
-    uint32_t sa[TI], sb[TJ];
+  for (int h = 0; h < 2; ++h) at[h] = (lane & 31) * 128 + (((h * 4 + (lane >> 5) * 2) ^ x) << 4);
+  auto row_of = [&](int q) { return q < TI ? (wm * TI + q) * 32 : BM + (wn * TJ + q - TI) * 32; };
+  auto read = [&](int kb, int h, int q) {
+    const uint8_t* const st = lds + (kb & 1) * STAGE + row_of(q) * 128;
+    const i32x4 lo = *(const i32x4*)(st + at[h]), hi = *(const i32x4*)(st + (at[h] ^ 16));
+    f[SETS == 2 ? h : 0][q] = i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  auto scale_at = [&](int kb, int q) {
+    return *(const uint32_t*)(lds + (kb & 1) * STAGE + SCALES + (row_of(q) + (lane & 31)) * 4) >> (((first + kb) & 3) * 8);
+  };
+  constexpr int QUARTERS = EXACT ? 4 : 1, PRODUCTS = TI * TJ, STEPS = QUARTERS * PRODUCTS;
+  // a half's products, with `between(t)` after the t-th of STEPS
+  auto half = [&](int h, auto between) {
+    const int set = SETS == 2 ? h : 0;
 #pragma unroll
-    for (int i = 0; i < TI; ++i) sa[i] = *(const uint32_t*)(st + SCALES + ((wm * TI + i) * 32 + (lane & 31)) * 4) >> shift;
+    for (int s = 0; s < QUARTERS; ++s) {
+      bf16x8 w[Q];
+      if constexpr (EXACT) {
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) sb[j] = *(const uint32_t*)(st + SCALES + (BM + (wn * TJ + j) * 32 + (lane & 31)) * 4) >> shift;
+        for (int q = 0; q < Q; ++q) w[q] = widen8(f[set][q][2 * s], f[set][q][2 * s + 1], byte_as_scale(sc[q] & 255u));
+      }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      i32x8 fa[TI], fb[TJ];
-      auto fragment = [&](int row) {
-        const int c = h * 4 + (lane >> 5) * 2, x = (row >> 1) & 7;
-        const i32x4 lo = *(const i32x4*)(st + row * 128 + (c ^ x) * 16);
-        const i32x4 hi = *(const i32x4*)(st + row * 128 + ((c + 1) ^ x) * 16);
-        return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      };
-#pragma unroll
-      for (int i = 0; i < TI; ++i) fa[i] = fragment((wm * TI + i) * 32 + (lane & 31));
-#pragma unroll
-      for (int j = 0; j < TJ; ++j) fb[j] = fragment(BM + (wn * TJ + j) * 32 + (lane & 31));
-      if constexpr (!EXACT) {
-#pragma unroll
-        for (int i = 0; i < TI; ++i)
-#pragma unroll
-          for (int j = 0; j < TJ; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[i], fb[j], acc[i][j], 0, 0, 0, (int)sa[i], 0, (int)sb[j]);
-      } else {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          bf16x8 wa[TI], wb[TJ];
-#pragma unroll
-          for (int i = 0; i < TI; ++i) wa[i] = widen8(fa[i][2 * s], fa[i][2 * s + 1], byte_as_scale(sa[i] & 255u));
-#pragma unroll
-          for (int j = 0; j < TJ; ++j) wb[j] = widen8(fb[j][2 * s], fb[j][2 * s + 1], byte_as_scale(sb[j] & 255u));
-#pragma unroll
-          for (int i = 0; i < TI; ++i)
-#pragma unroll
-            for (int j = 0; j < TJ; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wa[i], wb[j], acc[i][j], 0, 0, 0);
-        }
+      for (int t = 0; t < PRODUCTS; ++t) {
+        const int i = t / TJ, j = t % TJ, one = BY_ROW ? TI + j : i, two = BY_ROW ? i : TI + j;
+        if constexpr (EXACT)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[one], w[two], acc[i][j], 0, 0, 0);
+        else
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f[set][one], f[set][two], acc[i][j], 0, 0, 0, (int)sc[one], 0,
+                                                                      (int)sc[two]);
+        between(s * PRODUCTS + t);
       }
     }
-    slot = slot + 1 == STAGES ? 0 : slot + 1;
+  };
+
+  load_all(0);
+  if constexpr (PIPED) {
+    if (blocks > 1) {
+      load_all(1);
+      wait_vm<LPW + SL>();
+    } else {
+      wait_vm<0>();
+    }
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      read(0, 0, q);
+      sc[q] = scale_at(0, q);
+    }
+    // a fragment's reads after each of the first products
+    constexpr int PER = (Q + STEPS - 1) / STEPS;
+    auto reads_at = [&](int t, auto one) {
+#pragma unroll
+      for (int q = t * PER; q < t * PER + PER; ++q)
+        if (q < Q) one(q);
+    };
+    for (int kb = 0; kb + 1 < blocks; ++kb) {
+      half(0, [&](int t) {
+        __builtin_amdgcn_sched_barrier(0);
+        reads_at(t, [&](int q) { read(kb, 1, q); });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      // this wavefront's part of block kb + 1 is in LDS and its reads of block kb are in registers; after the
+      // barrier, every wavefront's are
+      wait_vm<0>();
+      wait_lgkm0();
+      __builtin_amdgcn_s_barrier();
+      const bool more = kb + 2 < blocks;
+      half(1, [&](int t) {
+        __builtin_amdgcn_sched_barrier(0);
+        reads_at(t, [&](int q) {
+          read(kb + 1, 0, q);
+          next_sc[q] = scale_at(kb + 1, q);
+        });
+        if (more) {
+          if (t == 0) load_scales(kb + 2);
+          if (t < LPW) load(kb + 2, t);
+          if (t == STEPS - 1)
+#pragma unroll
+            for (int j = STEPS; j < LPW; ++j) load(kb + 2, j);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+#pragma unroll
+      for (int q = 0; q < Q; ++q) sc[q] = next_sc[q];
+    }
+    half(0, [&](int t) { reads_at(t, [&](int q) { read(blocks - 1, 1, q); }); });
+    half(1, [](int) {});
+  } else {
+    for (int kb = 0; kb < blocks; ++kb) {
+      // this wavefront's part of block kb is in LDS and its reads of block kb - 1 are in registers; after the
+      // barrier, every wavefront's are
+      wait_vm<0>();
+      wait_lgkm0();
+      __builtin_amdgcn_s_barrier();
+      if (kb + 1 < blocks) load_all(kb + 1);
+#pragma unroll
+      for (int q = 0; q < Q; ++q) sc[q] = scale_at(kb, q);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) read(kb, h, q);
+        half(h, [](int) {});
+      }
+    }
   }
-  // D: lane l holds column l % 32 and rows 8 (r / 4) + 4 (l / 32) + r % 4 of its 32 x 32
-  Out* const c = (Out*)p.c[grp];
-  const int64_t ldc = p.ldc[grp];
+  // the last products are used outside the branches below
 #pragma unroll
   for (int i = 0; i < TI; ++i)
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) {
-      const int64_t col = n0 + (wn * TJ + j) * 32 + (lane & 31);
+    for (int j = 0; j < TJ; ++j) asm volatile("" : "+v"(acc[i][j]));
+
+  Out* const c = (Out*)p.c[grp] + piece * p.piece_stride;
+  const int64_t ldc = p.ldc[grp];
+  if constexpr (BY_ROW) {
+    // D: lane l holds row l % 32 of C's 32 x 32 and columns 8 (r / 4) + 4 (l / 32) + r % 4
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t row = m0 + (wm * TI + i) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        if (row < p.m && col < n) c[row * ldc + col] = (Out)acc[i][j][r];
-      }
+    for (int i = 0; i < TI; ++i) {
+      const int64_t row = m0 + (wm * TI + i) * 32 + (lane & 31);
+      if (row >= p.m) continue;
+      Out* const c_row = c + row * ldc;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+          typedef Out o8 __attribute__((ext_vector_type(8), aligned(2)));
+          const o8 v = __builtin_bit_cast(o8, pack_groups<Out>(acc[i][j], g));
+          const int64_t col = n0 + (wn * TJ + j) * 32 + 8 * g + 8 * (lane >> 5);
+          if (col + 8 <= n) {
+            *(o8*)(c_row + col) = v;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (col + e < n) c_row[col + e] = v[e];
+          }
+        }
     }
+  } else {
+    // D: lane l holds column l % 32 and rows 8 (r / 4) + 4 (l / 32) + r % 4: whole lines of a row
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        const int64_t col = n0 + (wn * TJ + j) * 32 + (lane & 31);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int64_t row = m0 + (wm * TI + i) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+          if (row < p.m && col < n) c[row * ldc + col] = (Out)acc[i][j][r];
+        }
+      }
+  }
+}
+
+// The pieces' sums, in order: eight outputs of a group's [m, n] (dense in the pieces) a thread.
+template <typename Out>
+__global__ __launch_bounds__(256) void piece_sum_kernel(const float* __restrict__ sums, int pieces, int64_t piece_stride, int64_t m,
+                                                        int64_t n, Out* __restrict__ c, int64_t ldc) {
+  const int64_t per = (n + 7) >> 3, i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per, col = (i - row * per) * 8;
+  if (row >= m) return;
+  const int valid = (int)min(n - col, (int64_t)8);
+  float v[8];
+  load8(sums + row * n + col, valid, v);
+  for (int q = 1; q < pieces; ++q) {
+    float x[8];
+    load8(sums + q * piece_stride + row * n + col, valid, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += x[e];
+  }
+  store8(c + row * ldc + col, valid, v);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
 
-constexpr int kFewRows = 32;     // rows of the few-row kernel
-constexpr int kFusedRows = 4;    // rows whose blocks it takes itself
-constexpr int64_t kFusedBytes = 48 << 10;
+constexpr int kFewRows = 32;  // of the few-row kernel; 33 rows of 2560 x 10240 take 8.0 us in 64 x 64 tiles, and 15.7 in four groups of 16
+constexpr int64_t kFusedBytes = 64 << 10;
 
-template <int BM, int BN, int WM, int WN, int STAGES, bool EXACT, typename Out>
+template <int BM, int BN, int WM, int WN, bool PIPED, bool EXACT, typename Out>
 int launch_tiles(ProductArgs p, hipStream_t st) {
   p.tiles_m = (int)((p.m + BM - 1) / BM);
   p.tiles_n0 = (int)((p.n[0] + BN - 1) / BN);
   p.tiles_n = p.tiles_n0 + (int)((p.n[1] + BN - 1) / BN);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   if (tiles > INT32_MAX) return set_error(EG_ERR_UNSUPPORTED, "fp8 product: %lld tiles", (long long)tiles);
-  const auto kernel = product_kernel<BM, BN, WM, WN, STAGES, EXACT, Out>;
-  constexpr int bytes = STAGES * (BM + BN) * 132;
+  const auto kernel = product_kernel<BM, BN, WM, WN, PIPED, EXACT, Out>;
+  constexpr int bytes = 2 * (BM + BN) * 132;
   EG_CHECK_HIP(allow_lds((const void*)kernel, bytes));
-  kernel<<<(unsigned)tiles, WM * WN * 64, bytes, st>>>(p);
+  kernel<<<(unsigned)(tiles * p.pieces), WM * WN * 64, bytes, st>>>(p);
   return launch_status("product_kernel");
 }
 
+// What a tile costs, in the time that the fp8 (or, EXACT, the bf16) matrix cores take for a product at 256 x 256:
+// `each` an output where all CUs are full (measured at 8192^3), `resident` tiles a CU at once.
+struct Tile {
+  int bm, bn, resident;
+  float each, each_exact;
+};
+constexpr Tile kTiles[] = {
+    {256, 256, 1, 1.00f, 1.00f},  // fp8 437 us, bf16 816 us of 8192^3
+    {256, 320, 1, 0.92f, 0.93f},  // 507 (205 tiles of 5/4, five rounds for four), 954
+    {256, 192, 1, 1.05f, 1.00f},  // 503, 908
+    {128, 128, 2, 1.17f, 1.09f},  // 514, 887
+    {128, 160, 1, 1.50f, 1.14f},  // 678, 935
+    {64, 128, 3, 1.48f, 1.26f},   // 658, 1024
+    {64, 64, 4, 1.94f, 1.49f},    // 858, 1209
+};
+
+// The tile for m x (n0, n1) outputs: the least time of the CU that gets the most tiles.  A block of a tile of four
+// wavefronts that has its CU to itself takes 14,000 outputs' time (12,000 EXACT) and 0.95 (0.8) an output: its loads' latency.
+template <bool EXACT>
+int choose_tile(int64_t m, int64_t n0, int64_t n1) {
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+    const Tile& t = kTiles[i];
+    const double area = (double)t.bm * t.bn, each = (EXACT ? t.each_exact : t.each) * area;
+    const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n0 + t.bn - 1) / t.bn + (n1 + t.bn - 1) / t.bn);
+    const int64_t a_cu = (tiles + kCUs - 1) / kCUs;
+    const double alone = t.bm == 256 ? 0.0 : EXACT ? 12000 + 0.8 * area : 14000 + 0.95 * area;
+    auto cost = [&](int64_t count) { return count == 0 ? 0.0 : std::max(alone, count * each); };
+    const double time = (a_cu / t.resident) * cost(t.resident) + cost(a_cu % t.resident);
+    if (i == 0 || time < least) {
+      best = i;
+      least = time;
+    }
+  }
+  return best;
+}
+
+// Pieces along k of a long product whose 64 x 64 tiles are few: as many as make three workgroups a CU, of at least 10 blocks
+// each; their fp32 sums are added in order by a launch of its own.  bf16 outputs of 256 x 10240 x 2560 (160 tiles): 21 us
+// in four pieces, 43 in one; 500 rows (320 tiles) 32 and 43; 256 x 2560 x 2560 13 in two, 9 in one.
+int pieces_of(int64_t m, int64_t n0, int64_t n1, int blocks) {
+  if (m <= kFewRows) return 1;
+  const int64_t tiles = ((m + 63) / 64) * ((n0 + 63) / 64 + (n1 + 63) / 64);
+  if (tiles == 0) return 1;
+  const int pieces = blocks < 24 ? 1 : (int)std::min<int64_t>(3 * kCUs / tiles, blocks / 10);
+  return std::max(1, pieces);
+}
+
+// Bytes of the pieces' sums.
+int64_t piece_bytes(int64_t m, int64_t n0, int64_t n1, int64_t k) {
+  const int pieces = pieces_of(m, n0, n1, (int)((k + 127) / 128));
+  return pieces > 1 ? (int64_t)pieces * m * (n0 + n1) * 4 : 0;
+}
+
 template <bool EXACT, typename Out>
-int launch_product(const ProductArgs& p, hipStream_t st) {
-  auto tiles = [&](int bm, int bn) { return ((p.m + bm - 1) / bm) * ((p.n[0] + bn - 1) / bn + (p.n[1] + bn - 1) / bn); };
-  if (tiles(256, 256) >= 128) return launch_tiles<256, 256, 2, 4, 2, EXACT, Out>(p, st);
-  if (tiles(128, 128) >= 256) return launch_tiles<128, 128, 2, 2, 2, EXACT, Out>(p, st);
-  return launch_tiles<64, 64, 2, 2, 4, EXACT, Out>(p, st);
+int launch_product(ProductArgs p, float* sums, hipStream_t st) {
+  p.pieces = pieces_of(p.m, p.n[0], p.n[1], p.blocks);
+  p.per = (p.blocks + p.pieces - 1) / p.pieces;
+  if (p.pieces > 1) {
+    p.pieces = (p.blocks + p.per - 1) / p.per;  // none is empty
+    ProductArgs to = p;
+    to.piece_stride = p.m * (p.n[0] + p.n[1]);
+    to.c[0] = sums;
+    to.c[1] = sums + p.m * p.n[0];
+    to.ldc[0] = p.n[0];
+    to.ldc[1] = p.n[1];
+    if (const int rc = launch_tiles<64, 64, 2, 2, true, EXACT, float>(to, st); rc != EG_OK) return rc;
+    for (int i = 0; i < 2; ++i) {
+      if (p.n[i] == 0) continue;
+      const int64_t groups = (p.m * ((p.n[i] + 7) / 8) + 255) / 256;
+      piece_sum_kernel<Out><<<(unsigned)groups, 256, 0, st>>>((const float*)to.c[i], p.pieces, to.piece_stride, p.m, p.n[i], (Out*)p.c[i], p.ldc[i]);
+      if (const int rc = launch_status("piece_sum_kernel"); rc != EG_OK) return rc;
+    }
+    return EG_OK;
+  }
+  switch (choose_tile<EXACT>(p.m, p.n[0], p.n[1])) {
+    case 0: return launch_tiles<256, 256, 2, 4, false, EXACT, Out>(p, st);
+    case 1: return launch_tiles<256, 320, 4, 2, false, EXACT, Out>(p, st);
+    case 2: return launch_tiles<256, 192, 4, 2, false, EXACT, Out>(p, st);
+    case 3: return launch_tiles<128, 128, 2, 2, true, EXACT, Out>(p, st);
+    case 4: return launch_tiles<128, 160, 4, 1, true, EXACT, Out>(p, st);
+    case 5: return launch_tiles<64, 128, 2, 2, true, EXACT, Out>(p, st);
+    default: return launch_tiles<64, 64, 2, 2, true, EXACT, Out>(p, st);
+  }
+}
+
+// How the few-row kernel is launched: kw wavefronts share a column group's blocks of k, so many that each has all of its
+// blocks in flight at once; cw column groups a workgroup.  FUSED: at least four wavefronts, and as many
+// column groups as leave 128 workgroups, for the rows' blocks that each of them takes.
+struct FewPlan {
+  int kw, cw;
+};
+FewPlan few_plan(int64_t m, int blocks, int64_t tiles, bool takes_blocks) {
+  FewPlan f = {1, 1};
+  while (f.kw < 16 && (blocks + f.kw - 1) / f.kw > kFewBlocks) f.kw *= 2;
+  if (takes_blocks) {
+    f.kw = std::max(f.kw, 4);
+    while (m > 2 && f.kw * f.cw < 16 && tiles / (2 * f.cw) >= 128) f.cw *= 2;
+  }
+  return f;
+}
+
+// LDS of the rows' blocks, where the few-row kernel takes them itself.
+int64_t fused_bytes(int64_t m, int64_t k) {
+  const int64_t blocks = (k + 127) / 128;
+  return m * (blocks * 128 + 16 + ((blocks + 3) & ~(int64_t)3));
+}
+
+// Whether it does: they fit, and a thread takes at most 64 values of them.  At 2560 x 10240, 24 rows (60 values a
+// thread): 15.9 us, and 13.5 after a launch of 2.5 for the blocks; at 2560 x 2560, 4 rows (40): 6.6 and 4.4 + 2.5,
+// 8 rows (80): 9.1 and 4.5 + 2.5.
+bool fused(int64_t m, int64_t k, int64_t n0, int64_t n1) {
+  if (m > kFewRows || fused_bytes(m, k) > kFusedBytes) return false;
+  const int blocks = (int)((k + 127) / 128);
+  const FewPlan f = few_plan(m, blocks, (n0 + 15) / 16 + (n1 + 15) / 16, true);
+  return m * blocks * 128 <= 64 * 64 * f.kw * f.cw;
 }
 
 template <int G, bool FUSED, typename X>
 int launch_few(ProductArgs p, int32_t dtype, hipStream_t st) {
   p.tiles_n0 = (int)((p.n[0] + 15) / 16);
   const int64_t tiles = p.tiles_n0 + (p.n[1] + 15) / 16;
-  // wavefronts a workgroup: about four blocks of k each, so that all their loads are in flight at once
-  const int kw = p.blocks <= 4 ? 1 : p.blocks <= 8 ? 2 : p.blocks <= 24 ? 4 : p.blocks <= 48 ? 8 : 16;
-  const int64_t a_bytes = FUSED ? p.m * (p.blocks * 128 + ((p.blocks + 3) & ~3)) : 0;
-  const int64_t bytes = a_bytes > kw * G * 1024 ? a_bytes : kw * G * 1024;
+  const FewPlan f = few_plan(p.m, p.blocks, tiles, FUSED);
+  const int64_t a_bytes = FUSED ? fused_bytes(p.m, p.k) : 0, sums = (int64_t)f.kw * f.cw * G * 1024;
   return with_type(dtype, [&](auto out) {
-    few_rows_kernel<G, FUSED, X, decltype(out)><<<(unsigned)tiles, kw * 64, bytes, st>>>(p);
+    few_rows_kernel<G, FUSED, X, decltype(out)>
+        <<<(unsigned)((tiles + f.cw - 1) / f.cw), f.kw * f.cw * 64, a_bytes > sums ? a_bytes : sums, st>>>(p, f.kw);
     return launch_status("few_rows_kernel");
   });
 }
@@ -520,20 +799,32 @@ int check_product(const eg_fp8_matrix* b, const eg_fp8_matrix* b2, void* c, int6
   return EG_OK;
 }
 
-int run_product(const ProductArgs& p, int32_t dtype, hipStream_t st) {
+int run_product(const ProductArgs& p, int32_t dtype, float* sums, hipStream_t st) {
   if (p.m == 0 || p.n[0] == 0) return EG_OK;
   if (p.m <= 16) return launch_few<1, false, float>(p, dtype, st);
   if (p.m <= kFewRows) return launch_few<2, false, float>(p, dtype, st);
   switch (dtype) {
-    case EG_DTYPE_F32: return launch_product<true, float>(p, st);
-    case EG_DTYPE_BF16: return launch_product<false, __bf16>(p, st);
-    default: return launch_product<false, _Float16>(p, st);
+    case EG_DTYPE_F32: return launch_product<true, float>(p, sums, st);
+    case EG_DTYPE_BF16: return launch_product<false, __bf16>(p, sums, st);
+    default: return launch_product<false, _Float16>(p, sums, st);
   }
 }
 
-bool fused(int64_t m, int64_t k) {
+int check_workspace(const void* workspace, int64_t bytes, int64_t need, const char* what) {
+  if (bytes < need)
+    return set_error(EG_ERR_WORKSPACE, "%s needs %lld bytes of workspace, got %lld", what, (long long)need, (long long)bytes);
+  EG_CHECK_ARG(need == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "%s: the workspace must be 16-byte aligned", what);
+  return EG_OK;
+}
+
+// Bytes of A's blocks, a multiple of 16.
+int64_t block_bytes(int64_t m, int64_t k) {
   const int64_t blocks = (k + 127) / 128;
-  return m <= kFusedRows && m * (blocks * 128 + blocks + 3) <= kFusedBytes;
+  return (m * (blocks * 128 + (blocks + 3) / 4 * 4) + 15) / 16 * 16;
+}
+
+bool known_size(int64_t m, int64_t n, int64_t n2, int64_t k) {
+  return m >= 0 && m < (1ll << 31) && n >= 0 && n < (1ll << 31) && n2 >= 0 && n2 < (1ll << 31) && k >= 1 && k <= (1 << 22);
 }
 
 }  // namespace
@@ -616,23 +907,26 @@ int eg_fp8_dequantize(const eg_fp8_matrix* m, void* out, int32_t dtype, int64_t 
   });
 }
 
+int64_t eg_fp8_product_workspace_size(int64_t m, int64_t n, int64_t n2, int64_t k) {
+  return known_size(m, n, n2, k) ? piece_bytes(m, n, n2, k) : -1;
+}
+
 int eg_fp8_product(const eg_fp8_matrix* a, const eg_fp8_matrix* b, const eg_fp8_matrix* b2, void* c, int64_t ldc, void* c2,
-                   int64_t ldc2, int32_t dtype, void* stream) {
+                   int64_t ldc2, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (const int rc = check_fp8(a, 1, "a"); rc != EG_OK) return rc;
   ProductArgs p;
   if (const int rc = check_product(b, b2, c, ldc, c2, ldc2, dtype, a->rows, a->k, &p); rc != EG_OK) return rc;
+  if (const int rc = check_workspace(workspace, workspace_bytes, piece_bytes(p.m, p.n[0], p.n[1], p.k), "fp8_product"); rc != EG_OK) return rc;
   p.a = (const uint8_t*)a->q;
   p.a_scales = a->scales;
   p.lda = a->stride;
   p.lda_scales = a->scale_stride;
-  return run_product(p, dtype, (hipStream_t)stream);
+  return run_product(p, dtype, (float*)workspace, (hipStream_t)stream);
 }
 
-int64_t eg_fp8_linear_workspace_size(int64_t m, int64_t k) {
-  if (m < 0 || m >= (1ll << 31) || k < 1 || k > (1 << 22)) return -1;
-  if (fused(m, k)) return 0;
-  const int64_t blocks = (k + 127) / 128;
-  return m * (blocks * 128 + (blocks + 3) / 4 * 4);
+int64_t eg_fp8_linear_workspace_size(int64_t m, int64_t n, int64_t n2, int64_t k) {
+  if (!known_size(m, n, n2, k)) return -1;
+  return fused(m, k, n, n2) ? 0 : block_bytes(m, k) + piece_bytes(m, n, n2, k);
 }
 
 int eg_fp8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t x_stride, const eg_fp8_matrix* b, const eg_fp8_matrix* b2,
@@ -644,21 +938,24 @@ int eg_fp8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t x_stride, c
   if (const int rc = check_product(b, b2, c, ldc, c2, ldc2, dtype, m, b->k, &p); rc != EG_OK) return rc;
   if (const int rc = check_values(x, x_dtype, m, b->k, x_stride, "fp8_linear"); rc != EG_OK) return rc;
   if (m == 0 || p.n[0] == 0) return EG_OK;
-  if (fused(m, b->k)) {
+  const int64_t k = b->k, need = eg_fp8_linear_workspace_size(m, b->rows, b2 ? b2->rows : 0, k);
+  if (const int rc = check_workspace(workspace, workspace_bytes, need, "fp8_linear"); rc != EG_OK) return rc;
+  if (fused(m, k, p.n[0], p.n[1])) {
     p.x = x;
     p.ldx = x_stride;
     return with_type(x_dtype, [&](auto t) {
-      return launch_few<1, true, decltype(t)>(p, dtype, (hipStream_t)stream);
+      using X = decltype(t);
+      return m <= 16 ? launch_few<1, true, X>(p, dtype, (hipStream_t)stream) : launch_few<2, true, X>(p, dtype, (hipStream_t)stream);
     });
   }
-  const int64_t need = eg_fp8_linear_workspace_size(m, b->k);
-  if (workspace_bytes < need)
-    return set_error(EG_ERR_WORKSPACE, "fp8_linear needs %lld bytes of workspace, got %lld", (long long)need, (long long)workspace_bytes);
-  EG_CHECK_ARG(workspace != nullptr && (uintptr_t)workspace % 16 == 0, "fp8_linear: the workspace must be 16-byte aligned");
   const int64_t kp = (int64_t)p.blocks * 128;
-  const eg_fp8_matrix a = {workspace, (uint8_t*)workspace + m * kp, m, b->k, kp, (p.blocks + 3) / 4 * 4, 1};
+  const eg_fp8_matrix a = {workspace, (uint8_t*)workspace + m * kp, m, k, kp, (p.blocks + 3) / 4 * 4, 1};
   if (const int rc = eg_fp8_quantize(x, x_dtype, x_stride, &a, stream); rc != EG_OK) return rc;
-  return eg_fp8_product(&a, b, b2, c, ldc, c2, ldc2, dtype, stream);
+  p.a = (const uint8_t*)a.q;
+  p.a_scales = a.scales;
+  p.lda = a.stride;
+  p.lda_scales = a.scale_stride;
+  return run_product(p, dtype, (float*)((uint8_t*)workspace + block_bytes(m, k)), (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -5,9 +5,12 @@
 //   d_h = d_residual + r (w d_y) - h r^3 / d sum(w d_y h),   d_w = sum over rows of d_y h r
 //
 // Bound by its bytes: every row is read once, held in registers between its sum and its output, and
-// written once.  A row is W wavefronts' (1 to 16), of which each holds CH pieces of 512 values, eight
+// written once.  A row is w wavefronts' (1 to 16), of which each holds CH pieces of 512 values, eight
 // consecutive ones a lane: a piece is four blocks of the 8-bit output, whose largest values are found
-// within 16 lanes.  Weights are read once by a wavefront, which takes rows gridDim apart.
+// within 16 lanes.  One piece a wavefront up to d = 8192 (d = 2560: five wavefronts a row): a wavefront a row
+// of 2560 held five, and its registers left four wavefronts a SIMD, or spilled; 61 us for 8,188 rows of bf16.
+#include <algorithm>
+
 #include "eg_fp8.h"
 #include "eg_overlap.h"
 
@@ -18,16 +21,6 @@ struct Value {
   const void* p;
   int32_t dtype;
 };
-
-// Eight values whose type is known at run time (one branch for the wavefront).
-__device__ inline void load8_any(const Value& v, int64_t at, int valid, float (&x)[8]) {
-  if (v.dtype == EG_DTYPE_F32)
-    load8((const float*)v.p + at, valid, x);
-  else if (v.dtype == EG_DTYPE_BF16)
-    load8((const __bf16*)v.p + at, valid, x);
-  else
-    load8((const _Float16*)v.p + at, valid, x);
-}
 
 __device__ inline void store8_any(void* p, int32_t dtype, int64_t at, int valid, const float (&x)[8]) {
   if (dtype == EG_DTYPE_F32)
@@ -62,7 +55,8 @@ __device__ inline float row_sum(float x, int w, int row_of_block, int wave_of_ro
 }
 
 struct NormArgs {
-  Value x, residual, weight;  // weight.p NULL: 1
+  Value x, residual;
+  const float* weight;        // NULL: 1
   int64_t x_stride, r_stride;
   int64_t rows;
   int d, w;                   // w: wavefronts a row
@@ -84,21 +78,18 @@ __device__ inline float rounded(float x) {
 }
 
 // R void: no residual (h is x, and not written).
-template <typename X, typename R, int CH>
+template <typename X, typename R, int CH, bool RAGGED>
 __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
   __shared__ float part[2][16];
   constexpr bool ADD = !std::is_same<R, void>::value;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slot = wave / a.w, w = wave - slot * a.w, rows_here = (blockDim.x >> 6) / a.w;
+  const bool weighted = a.weight != nullptr;
   int at[CH], left[CH];
-  float g[CH][8];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     at[c] = (c * a.w + w) * 512 + lane * 8;
     left[c] = a.d - at[c];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) g[c][i] = 1.0f;
-    if (a.weight.p != nullptr) load8_any(a.weight, at[c], left[c], g[c]);
   }
   const int blocks = (a.d + 127) >> 7;
   int parity = 0;
@@ -106,16 +97,32 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
     const bool live = first + slot < a.rows;
     const int64_t row = live ? first + slot : a.rows - 1;
     float v[CH][8];
+    const X* const x = (const X*)a.x.p + row * a.x_stride;
+    Raw8<X> raw_x[CH];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) load8((const X*)a.x.p + row * a.x_stride + at[c], left[c], v[c]);
+    for (int c = 0; c < CH; ++c) raw_x[c] = load_raw<RAGGED>(x, at[c], a.d);
     if constexpr (ADD) {
-      float r[CH][8];
+      const R* const res = (const R*)a.residual.p + row * a.r_stride;
+      Raw8<R> raw_r[CH];
 #pragma unroll
-      for (int c = 0; c < CH; ++c) load8((const R*)a.residual.p + row * a.r_stride + at[c], left[c], r[c]);
+      for (int c = 0; c < CH; ++c) raw_r[c] = load_raw<RAGGED>(res, at[c], a.d);
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
+      for (int c = 0; c < CH; ++c) {
+        float r[8];
+        values_of<RAGGED, X>(raw_x[c], at[c], a.d, v[c]);
+        values_of<RAGGED, R>(raw_r[c], at[c], a.d, r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] = rounded<R>(v[c][i] + r[c][i]);
+        for (int i = 0; i < 8; ++i) v[c][i] = rounded<R>(v[c][i] + r[i]);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) values_of<RAGGED, X>(raw_x[c], at[c], a.d, v[c]);
+    }
+    // the weights' loads (from L2) take the registers that the row's bytes had, and the time of its sum
+    Raw8<float> raw_g[CH];
+    if (weighted) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) raw_g[c] = load_raw<RAGGED>(a.weight, at[c], a.d);
     }
     float s = 0.0f;
 #pragma unroll
@@ -132,7 +139,13 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
       if constexpr (ADD) store8((R*)a.h + row * a.h_stride + at[c], left[c], v[c]);
       float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = v[c][i] * rstd * g[c][i];
+      for (int i = 0; i < 8; ++i) y[i] = v[c][i] * rstd;
+      if (weighted) {
+        float g[8];
+        values_of<RAGGED, float>(raw_g[c], at[c], a.d, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= g[i];
+      }
       if (a.y_dtype >= 0) {
         store8_any(a.y, a.y_dtype, row * a.y_stride + at[c], left[c], y);
       } else {
@@ -145,7 +158,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
 }
 
 struct GradArgs {
-  Value d_y, h, d_res, weight;  // d_res.p, weight.p NULL: none
+  Value d_y, h, d_res;          // d_res.p NULL: none
+  const float* weight;          // NULL: 1
   int64_t dy_stride, h_stride, dr_stride;
   const float* rstd;
   int64_t rows;
@@ -160,24 +174,21 @@ struct GradArgs {
 };
 
 // D: d_y's type; T: h's (and d_res's).
-template <typename D, typename T, int CH>
-__global__ __launch_bounds__(CH <= 2 ? 1024 : 512) void norm_grad_kernel(const GradArgs a) {
+template <typename D, typename T, int CH, bool RAGGED>
+__global__ __launch_bounds__(1024) void norm_grad_kernel(const GradArgs a) {
   __shared__ float part[2][16];
   extern __shared__ float sums[];  // [d]: a workgroup's share of the weight's gradient, with several rows in flight
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slot = wave / a.w, w = wave - slot * a.w, rows_here = (blockDim.x >> 6) / a.w;
+  const bool weighted = a.weight != nullptr;
   int at[CH], left[CH];
-  float g[CH][8], d_w[CH][8];
+  float d_w[CH][8];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     at[c] = (c * a.w + w) * 512 + lane * 8;
     left[c] = a.d - at[c];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      g[c][i] = 1.0f;
-      d_w[c][i] = 0.0f;
-    }
-    if (a.weight.p != nullptr) load8_any(a.weight, at[c], left[c], g[c]);
+    for (int i = 0; i < 8; ++i) d_w[c][i] = 0.0f;
   }
   const float inv_d = 1.0f / (float)a.d;
   int parity = 0;
@@ -185,22 +196,44 @@ __global__ __launch_bounds__(CH <= 2 ? 1024 : 512) void norm_grad_kernel(const G
     const bool live = first + slot < a.rows;
     const int64_t row = live ? first + slot : a.rows - 1;
     float p[CH][8], u[CH][8];
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      load8((const D*)a.d_y.p + row * a.dy_stride + at[c], left[c], p[c]);
-      load8((const T*)a.h.p + row * a.h_stride + at[c], left[c], u[c]);
-    }
+    const D* const d_y = (const D*)a.d_y.p + row * a.dy_stride;
+    const T* const h = (const T*)a.h.p + row * a.h_stride;
+    const T* const d_res = (const T*)a.d_res.p + row * a.dr_stride;
     const float rstd = a.rstd[row];
+    Raw8<D> raw_p[CH];
+    Raw8<T> raw_u[CH], raw_r[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) raw_p[c] = load_raw<RAGGED>(d_y, at[c], a.d);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) raw_u[c] = load_raw<RAGGED>(h, at[c], a.d);
+    Raw8<float> raw_g[CH];
+    if (weighted) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) raw_g[c] = load_raw<RAGGED>(a.weight, at[c], a.d);
+    }
+    if (a.d_res.p != nullptr) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) raw_r[c] = load_raw<RAGGED>(d_res, at[c], a.d);
+    }
     float s = 0.0f;
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c) {
+      values_of<RAGGED, D>(raw_p[c], at[c], a.d, p[c]);
+      values_of<RAGGED, T>(raw_u[c], at[c], a.d, u[c]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         u[c][i] *= rstd;
         d_w[c][i] = live ? d_w[c][i] + p[c][i] * u[c][i] : d_w[c][i];
-        p[c][i] *= g[c][i];
-        s += p[c][i] * u[c][i];
       }
+      if (weighted) {
+        float g[8];
+        values_of<RAGGED, float>(raw_g[c], at[c], a.d, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[c][i] *= g[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += p[c][i] * u[c][i];
+    }
     s = row_sum(s, a.w, slot, w, part[parity]) * inv_d;
     parity ^= 1;
     if (!live) continue;
@@ -209,7 +242,7 @@ __global__ __launch_bounds__(CH <= 2 ? 1024 : 512) void norm_grad_kernel(const G
       float o[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = 0.0f;
-      if (a.d_res.p != nullptr) load8((const T*)a.d_res.p + row * a.dr_stride + at[c], left[c], o);
+      if (a.d_res.p != nullptr) values_of<RAGGED, T>(raw_r[c], at[c], a.d, o);
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] += rstd * (p[c][i] - u[c][i] * s);
       store8_any(a.d_x, a.dx_dtype, row * a.dx_stride + at[c], left[c], o);
@@ -237,61 +270,51 @@ __global__ __launch_bounds__(CH <= 2 ? 1024 : 512) void norm_grad_kernel(const G
   }
 }
 
-// d_w: the workgroups' partial sums, in order: 64 columns a workgroup, four rows at a time.
-__global__ __launch_bounds__(256) void weight_grad_kernel(const float* __restrict__ partial, int count, int d, void* d_w, int32_t dtype) {
-  __shared__ float s[4][64];
+// d_w: the workgroups' partial sums, in order: 64 columns a workgroup, whose wavefronts take every 16th of them.
+__global__ __launch_bounds__(1024) void weight_grad_kernel(const float* __restrict__ partial, int count, int d, float* __restrict__ d_w) {
+  __shared__ float s[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = blockIdx.x * 64 + lane;
   float x = 0.0f;
   if (c < d) {
 #pragma unroll 8
-    for (int i = wave; i < count; i += 4) x += partial[(int64_t)i * d + c];
+    for (int i = wave; i < count; i += 16) x += partial[(int64_t)i * d + c];
   }
   s[wave][lane] = x;
   __syncthreads();
   if (wave == 0 && c < d) {
-    x = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
-    if (dtype == EG_DTYPE_F32)
-      ((float*)d_w)[c] = x;
-    else if (dtype == EG_DTYPE_BF16)
-      ((__bf16*)d_w)[c] = (__bf16)x;
-    else
-      ((_Float16*)d_w)[c] = (_Float16)x;
+    x = s[0][lane];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) x += s[i][lane];
+    d_w[c] = x;
   }
 }
 
-// Wavefronts a row, and pieces a wavefront holds (at most `most`): one wavefront a row where there are rows
-// enough to fill the card (`rows` >= 4 a CU), more where rows are few or long.
+constexpr int64_t kMaxWidth = 40 * 512;
+
+// Wavefronts a row, and pieces a wavefront holds.
 struct Split {
   int w, ch;
 };
-Split split_of(int64_t rows, int64_t d, int most) {
-  const int pieces = (int)((d + 511) / 512);
-  int w = 1;
-  while (w < 16 && ((pieces + w - 1) / w > most || (rows * w < 1024 && w < pieces))) w *= 2;
-  return {w, (pieces + w - 1) / w};
+Split split_of(int64_t d) {
+  const int pieces = (int)((d + 511) / 512), ch = (pieces + 15) / 16;
+  return {(pieces + ch - 1) / ch, ch};
 }
 
-constexpr int kHeld = 5, kGradHeld = 5;
-constexpr int64_t kMaxWidth = 16 * kHeld * 512, kMaxGradWidth = 8 * kGradHeld * 512;
-
-// f(the kernel's pieces a wavefront as a constant): 1, 2 or 5, so that 2,560 values are whole
+// f(the kernel's pieces a wavefront as a constant)
 template <typename F>
 int with_pieces(int ch, const F& f) {
-  if (ch <= 1) return f(std::integral_constant<int, 1>{});
-  if (ch <= 2) return f(std::integral_constant<int, 2>{});
-  return f(std::integral_constant<int, 5>{});
+  if (ch == 1) return f(std::integral_constant<int, 1>{});
+  if (ch == 2) return f(std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, 3>{});
 }
 
-int grad_split(int64_t rows, int64_t d, Split* s, int* threads, int64_t* groups) {
-  *s = split_of(rows, d, kGradHeld);
-  if (s->w == 16 && s->ch > 2) *s = {8, (int)((d + 511) / 512 + 7) / 8};
-  *threads = s->w * 64 > 256 ? s->w * 64 : 256;
-  const int64_t per = *threads / 64 / s->w;
-  // two workgroups a CU of four wavefronts, one of more: every workgroup adds a row of partial sums
-  const int64_t most = *threads > 256 ? 256 : 512;
-  *groups = (rows + per - 1) / per < most ? (rows + per - 1) / per : most;
-  return EG_OK;
+// Rows that a workgroup has in flight, and workgroups: all rows' of the forward; of the gradient two of up to 16 wavefronts a CU,
+// since every one adds a row of partial sums of the weight's.
+int rows_at_once(int w, int wavefronts) { return w > wavefronts ? 1 : wavefronts / w; }
+int64_t grad_groups(int64_t rows, int w) {
+  const int at_once = rows_at_once(w, 16);
+  return std::min<int64_t>((rows + at_once - 1) / at_once, 512);
 }
 
 int check_apart(const void* a, int64_t rows, int64_t cols, int64_t stride, int item, const void* b, int64_t b_rows, int64_t b_cols,
@@ -320,8 +343,7 @@ int eg_add_rms_norm(const eg_norm* o, void* h, int64_t h_stride, void* y, int32_
     EG_CHECK_ARG(o->r_dtype == o->x_dtype || o->r_dtype == EG_DTYPE_F32, "add_rms_norm: a residual of x's type or f32 expected");
     if (const int rc = check_values(h, o->r_dtype, o->rows, o->d, h_stride, "add_rms_norm: h"); rc != EG_OK) return rc;
   }
-  EG_CHECK_ARG(o->weight == nullptr || known_dtype(o->w_dtype), "add_rms_norm: weight dtype=%d", o->w_dtype);
-  EG_CHECK_ARG(o->weight == nullptr || (uintptr_t)o->weight % item_size(o->w_dtype) == 0, "add_rms_norm: misaligned weight");
+  EG_CHECK_ARG((uintptr_t)o->weight % 4 == 0, "add_rms_norm: misaligned weight");
   EG_CHECK_ARG((y != nullptr) != (y8 != nullptr) || o->rows == 0, "add_rms_norm: y or y8 expected");
   const int xs = item_size(o->x_dtype);
   int64_t out_cols = o->d, out_stride = y_stride;
@@ -350,17 +372,19 @@ int eg_add_rms_norm(const eg_norm* o, void* h, int64_t h_stride, void* y, int32_
     if (!(h == o->x && h_stride == o->x_stride && o->x_dtype == o->r_dtype))
       if (const int rc = check_apart(h, o->rows, o->d, h_stride, rs, o->x, o->rows, o->d, o->x_stride, xs, "add_rms_norm: h overlaps x"); rc != EG_OK) return rc;
   }
-  const Split s = split_of(o->rows, o->d, kHeld);
-  const int threads = s.w * 64 > 256 ? s.w * 64 : 256;
-  const int64_t per = threads / 64 / s.w, need = (o->rows + per - 1) / per, most = 8 * 256 * 256 / threads;
-  const NormArgs a = {{o->x, o->x_dtype}, {o->residual, o->r_dtype}, {o->weight, o->w_dtype}, o->x_stride, o->r_stride, o->rows,
+  const Split s = split_of(o->d);
+  const int at_once = rows_at_once(s.w, 4), threads = at_once * s.w * 64;
+  const int64_t groups = std::min<int64_t>((o->rows + at_once - 1) / at_once, 1 << 20);
+  const NormArgs a = {{o->x, o->x_dtype}, {o->residual, o->r_dtype}, o->weight, o->x_stride, o->r_stride, o->rows,
                       (int)o->d, s.w, o->eps, h, h_stride, y8 ? y8->q : y, y8 ? -1 : y_dtype, y8 ? y8->stride : y_stride,
                       y8 ? y8->scales : nullptr, y8 ? y8->scale_stride : 0, rstd};
   auto launch = [&](auto x, auto r) {
     using X = decltype(x);
     using R = typename decltype(r)::type;
     return with_pieces(s.ch, [&](auto ch) {
-      norm_kernel<X, R, decltype(ch)::value><<<(unsigned)(need < most ? need : most), threads, 0, (hipStream_t)stream>>>(a);
+      constexpr int CH = decltype(ch)::value;
+      const auto kernel = o->d % 8 != 0 ? norm_kernel<X, R, CH, true> : norm_kernel<X, R, CH, false>;
+      kernel<<<(unsigned)groups, threads, 0, (hipStream_t)stream>>>(a);
       return launch_status("norm_kernel");
     });
   };
@@ -372,31 +396,26 @@ int eg_add_rms_norm(const eg_norm* o, void* h, int64_t h_stride, void* y, int32_
 }
 
 int64_t eg_add_rms_norm_grad_workspace_size(int64_t rows, int64_t d) {
-  if (rows < 0 || d < 1 || d > kMaxGradWidth) return -1;
-  Split s;
-  int threads;
-  int64_t groups;
-  grad_split(rows, d, &s, &threads, &groups);
-  return groups * d * 4;
+  if (rows < 0 || d < 1 || d > kMaxWidth) return -1;
+  return grad_groups(rows, split_of(d).w) * d * 4;
 }
 
 int eg_add_rms_norm_grad(const eg_norm_grad* o, void* d_x, int32_t dx_dtype, int64_t dx_stride, void* d_x2, int32_t dx2_dtype,
-                         int64_t dx2_stride, void* d_weight, int32_t dw_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+                         int64_t dx2_stride, float* d_weight, void* workspace, int64_t workspace_bytes, void* stream) {
   EG_CHECK_ARG(o != nullptr, "add_rms_norm_grad: NULL");
   EG_CHECK_ARG(o->rows >= 0 && o->d >= 1, "add_rms_norm_grad: %lld rows of %lld", (long long)o->rows, (long long)o->d);
-  if (o->d > kMaxGradWidth)
-    return set_error(EG_ERR_UNSUPPORTED, "add_rms_norm_grad: rows of %lld values, at most %lld", (long long)o->d, (long long)kMaxGradWidth);
+  if (o->d > kMaxWidth)
+    return set_error(EG_ERR_UNSUPPORTED, "add_rms_norm_grad: rows of %lld values, at most %lld", (long long)o->d, (long long)kMaxWidth);
   if (const int rc = check_values(o->d_y, o->dy_dtype, o->rows, o->d, o->dy_stride, "add_rms_norm_grad: d_y"); rc != EG_OK) return rc;
   if (const int rc = check_values(o->h, o->h_dtype, o->rows, o->d, o->h_stride, "add_rms_norm_grad: h"); rc != EG_OK) return rc;
   if (o->d_residual != nullptr)
     if (const int rc = check_values(o->d_residual, o->h_dtype, o->rows, o->d, o->dr_stride, "add_rms_norm_grad: d_residual"); rc != EG_OK) return rc;
-  EG_CHECK_ARG(o->weight == nullptr || (known_dtype(o->w_dtype) && (uintptr_t)o->weight % item_size(o->w_dtype) == 0),
-               "add_rms_norm_grad: weight");
+  EG_CHECK_ARG((uintptr_t)o->weight % 4 == 0, "add_rms_norm_grad: misaligned weight");
   EG_CHECK_ARG(o->rstd != nullptr || o->rows == 0, "add_rms_norm_grad: NULL rstd");
   if (const int rc = check_values(d_x, dx_dtype, o->rows, o->d, dx_stride, "add_rms_norm_grad: d_x"); rc != EG_OK) return rc;
   if (d_x2 != nullptr)
     if (const int rc = check_values(d_x2, dx2_dtype, o->rows, o->d, dx2_stride, "add_rms_norm_grad: d_x2"); rc != EG_OK) return rc;
-  EG_CHECK_ARG(d_weight == nullptr || (known_dtype(dw_dtype) && (uintptr_t)d_weight % item_size(dw_dtype) == 0), "add_rms_norm_grad: d_weight");
+  EG_CHECK_ARG((uintptr_t)d_weight % 4 == 0, "add_rms_norm_grad: misaligned d_weight");
   const struct {
     const void* p;
     int64_t stride;
@@ -410,26 +429,27 @@ int eg_add_rms_norm_grad(const eg_norm_grad* o, void* d_x, int32_t dx_dtype, int
     if (d_x2 != nullptr)
       if (const int rc = check_apart(d_x2, o->rows, o->d, dx2_stride, item_size(dx2_dtype), in.p, o->rows, o->d, in.stride, in.item, in.name); rc != EG_OK) return rc;
   }
-  Split s;
-  int threads;
-  int64_t groups;
-  grad_split(o->rows, o->d, &s, &threads, &groups);
+  const Split s = split_of(o->d);
+  const int rows_here = rows_at_once(s.w, 16), threads = rows_here * s.w * 64;
+  const int64_t groups = grad_groups(o->rows, s.w);
   if (d_weight != nullptr) {
     if (workspace_bytes < groups * o->d * 4)
       return set_error(EG_ERR_WORKSPACE, "add_rms_norm_grad needs %lld bytes of workspace, got %lld", (long long)(groups * o->d * 4),
                        (long long)workspace_bytes);
     EG_CHECK_ARG(groups == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "add_rms_norm_grad: the workspace must be 16-byte aligned");
   }
-  const GradArgs a = {{o->d_y, o->dy_dtype}, {o->h, o->h_dtype}, {o->d_residual, o->h_dtype}, {o->weight, o->w_dtype}, o->dy_stride,
+  const GradArgs a = {{o->d_y, o->dy_dtype}, {o->h, o->h_dtype}, {o->d_residual, o->h_dtype}, o->weight, o->dy_stride,
                       o->h_stride, o->dr_stride, o->rstd, o->rows, (int)o->d, s.w, d_x, dx_dtype, dx_stride, d_x2, dx2_dtype, dx2_stride,
                       d_weight ? (float*)workspace : nullptr};
-  const int rows_here = threads / 64 / s.w;
   if (o->rows > 0) {
     const int rc = with_type(o->dy_dtype, [&](auto dy) {
       return with_type(o->h_dtype, [&](auto t) {
         return with_pieces(s.ch, [&](auto ch) {
-          norm_grad_kernel<decltype(dy), decltype(t), decltype(ch)::value>
-              <<<(unsigned)groups, threads, d_weight && rows_here > 1 ? o->d * 4 : 0, (hipStream_t)stream>>>(a);
+          using D = decltype(dy);
+          using T = decltype(t);
+          constexpr int CH = decltype(ch)::value;
+          const auto kernel = o->d % 8 != 0 ? norm_grad_kernel<D, T, CH, true> : norm_grad_kernel<D, T, CH, false>;
+          kernel<<<(unsigned)groups, threads, d_weight && rows_here > 1 ? o->d * 4 : 0, (hipStream_t)stream>>>(a);
           return launch_status("norm_grad_kernel");
         });
       });
@@ -437,7 +457,7 @@ int eg_add_rms_norm_grad(const eg_norm_grad* o, void* d_x, int32_t dx_dtype, int
     if (rc != EG_OK) return rc;
   }
   if (d_weight != nullptr) {
-    weight_grad_kernel<<<(unsigned)((o->d + 63) / 64), 256, 0, (hipStream_t)stream>>>((const float*)workspace, (int)groups, (int)o->d, d_weight, dw_dtype);
+    weight_grad_kernel<<<(unsigned)((o->d + 63) / 64), 1024, 0, (hipStream_t)stream>>>((const float*)workspace, (int)groups, (int)o->d, d_weight);
     return launch_status("weight_grad_kernel");
   }
   return EG_OK;

@@ -38,6 +38,7 @@ struct Entry {
   decltype(&eg_fp8_quantize_weight) fp8_quantize_weight = nullptr;
   decltype(&eg_fp8_dequantize) fp8_dequantize = nullptr;
   decltype(&eg_fp8_product) fp8_product = nullptr;
+  decltype(&eg_fp8_product_workspace_size) fp8_product_workspace = nullptr;
   decltype(&eg_fp8_linear) fp8_linear = nullptr;
   decltype(&eg_fp8_linear_workspace_size) fp8_linear_workspace = nullptr;
   decltype(&eg_add_rms_norm) norm = nullptr;
@@ -473,7 +474,7 @@ std::vector<Tensor> fp8_linear(const Tensor& x_, const Tensor& q, const Tensor& 
   const eg_fp8_matrix w = blocks_of(q, scales, k, 128, "weight", x.device());
   if (x.size(1) != k) refuse("x must be [m, ", k, "], got ", x.sizes());
   Outputs o = outputs(x.size(0), w, split, dtype, x);
-  const int64_t need = g.fp8_linear_workspace(x.size(0), k);
+  const int64_t need = g.fp8_linear_workspace(x.size(0), o.b[0].rows, o.two ? o.b[1].rows : 0, k);
   if (need < 0) refuse("a product of ", x.sizes(), " values");
   const Tensor ws = need > 0 ? torch::empty({need}, x.options().dtype(torch::kUInt8)) : Tensor();
   check(g.fp8_linear(rows_of(x, x.size(0)), dtype_code(x), x.size(0), row_stride(x), &o.b[0], o.two ? &o.b[1] : nullptr, o.at[0], o.ld[0],
@@ -487,7 +488,11 @@ std::vector<Tensor> fp8_product(const Tensor& xq, const Tensor& x_scales, const 
   const c10::OptionalDeviceGuard on(gpu_of(xq));
   const eg_fp8_matrix a = blocks_of(xq, x_scales, k, 1, "x", xq.device()), w = blocks_of(q, scales, k, 128, "weight", xq.device());
   Outputs o = outputs(a.rows, w, split, dtype, xq);
-  check(g.fp8_product(&a, &o.b[0], o.two ? &o.b[1] : nullptr, o.at[0], o.ld[0], o.at[1], o.ld[1], (int32_t)dtype, (void*)stream));
+  const int64_t need = g.fp8_product_workspace(a.rows, o.b[0].rows, o.two ? o.b[1].rows : 0, k);
+  if (need < 0) refuse("a product of ", a.rows, " rows of ", k, " values");
+  const Tensor ws = need > 0 ? torch::empty({need}, xq.options().dtype(torch::kUInt8)) : Tensor();
+  check(g.fp8_product(&a, &o.b[0], o.two ? &o.b[1] : nullptr, o.at[0], o.ld[0], o.at[1], o.ld[1], (int32_t)dtype,
+                      need > 0 ? ws.data_ptr() : nullptr, need, (void*)stream));
   return o.y;
 }
 
@@ -514,7 +519,7 @@ std::tuple<Tensor, MaybeTensor, Tensor, MaybeTensor> norm(const Tensor& x_, cons
       refuse("residual must be of x's type or f32, got ", r.scalar_type(), " beside ", x.scalar_type());
   }
   check_vector(weight, d, "weight", x.device());
-  const Tensor w = weight ? weight->contiguous() : Tensor();
+  const Tensor w = weight ? weight->to(torch::kFloat32).contiguous() : Tensor();
   const Tensor h = residual ? torch::empty({rows, d}, r.options()) : x;
   const Tensor rstd = stats ? empty_floats(rows, x) : Tensor();
   eg_norm o = {};
@@ -526,10 +531,7 @@ std::tuple<Tensor, MaybeTensor, Tensor, MaybeTensor> norm(const Tensor& x_, cons
     o.r_dtype = dtype_code(r);
     o.r_stride = row_stride(r);
   }
-  if (weight) {
-    o.weight = w.data_ptr();
-    o.w_dtype = dtype_code(w);
-  }
+  if (weight) o.weight = values(w);
   o.eps = (float)eps;
   o.rows = rows;
   o.d = d;
@@ -560,7 +562,7 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> norm_grad(const Tensor& d_y_, const
   const Tensor rstd = rstd_.contiguous();
   check_vector(weight, d, "weight", h.device());
   if (weight_grad && !weight) refuse("the weight's gradient without a weight");
-  const Tensor w = weight ? weight->contiguous() : Tensor();
+  const Tensor w = weight ? weight->to(torch::kFloat32).contiguous() : Tensor();
   Tensor dr;
   if (d_res) {
     dr = rows_2d(*d_res, "d_residual");
@@ -578,10 +580,7 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> norm_grad(const Tensor& d_y_, const
     o.d_residual = rows_of(dr, rows);
     o.dr_stride = row_stride(dr);
   }
-  if (weight) {
-    o.weight = w.data_ptr();
-    o.w_dtype = dtype_code(w);
-  }
+  if (weight) o.weight = values(w);
   o.rstd = rows > 0 ? (const float*)rstd.data_ptr() : nullptr;
   o.rows = rows;
   o.d = d;
@@ -590,9 +589,9 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> norm_grad(const Tensor& d_y_, const
   const Tensor d_w = weight_grad ? torch::empty({d}, w.options()) : Tensor();
   const int64_t need = weight_grad ? g.norm_grad_workspace(rows, d) : 0;
   const Tensor ws = need > 0 ? torch::empty({need}, h.options().dtype(torch::kUInt8)) : Tensor();
-  check(g.norm_grad(&o, rows_of(d_x, rows), (int32_t)dtype, d, rows_of(d_x2, rows), (int32_t)dtype2, d, weight_grad ? d_w.data_ptr() : nullptr,
-                    weight_grad ? dtype_code(d_w) : 0, need > 0 ? ws.data_ptr() : nullptr, std::max<int64_t>(need, 0), (void*)stream));
-  return {d_x, dtype2 >= 0 ? MaybeTensor(d_x2) : std::nullopt, weight_grad ? MaybeTensor(d_w) : std::nullopt};
+  check(g.norm_grad(&o, rows_of(d_x, rows), (int32_t)dtype, d, rows_of(d_x2, rows), (int32_t)dtype2, d, weight_grad ? (float*)d_w.data_ptr() : nullptr,
+                    need > 0 ? ws.data_ptr() : nullptr, std::max<int64_t>(need, 0), (void*)stream));
+  return {d_x, dtype2 >= 0 ? MaybeTensor(d_x2) : std::nullopt, weight_grad ? MaybeTensor(d_w.to(weight->scalar_type())) : std::nullopt};
 }
 
 // ---- the norm of all gradients --------------------------------------------------------------------
@@ -673,6 +672,7 @@ void init_ops(const std::map<std::string, int64_t>& at, pybind11::object error) 
   set(g.fp8_quantize_weight, "eg_fp8_quantize_weight");
   set(g.fp8_dequantize, "eg_fp8_dequantize");
   set(g.fp8_product, "eg_fp8_product");
+  set(g.fp8_product_workspace, "eg_fp8_product_workspace_size");
   set(g.fp8_linear, "eg_fp8_linear");
   set(g.fp8_linear_workspace, "eg_fp8_linear_workspace_size");
   set(g.norm, "eg_add_rms_norm");

@@ -16,8 +16,7 @@ infinities become NaN.  The weight is frozen: its gradient is not to be had (the
 
 ``product`` takes the blocks of ``x`` (f32, bf16 or f16) itself; its gradient takes those of the
 output's gradient, along the other axis.  f32 outputs come from exact products and fp32 sums;
-16-bit ones of more than 32 rows from the fp8 matrix cores, about 1.5e-5 of an output off (bf16
-rounds by 2e-3).  The reference's projections are fp32 (``engraft/replica/layers.py:594-606``)."""
+16-bit ones from the fp8 matrix cores, about 1.5e-5 of an output off (bf16 rounds by 2e-3).  The reference's projections are fp32 (``engraft/replica/layers.py:594-606``)."""
 from __future__ import annotations
 
 import torch

@@ -10,7 +10,7 @@ output (or any layer's) and the projections behind it.
 * ``normed_product``             -- ``fp8.product`` of the normed rows, the norm writing them in 8
                                     bits, differentiable.
 
-``x`` is f32, bf16 or f16 ``[..., d]``, d up to 40,960 (20,480 for gradients); the residual of x's type or f32;
+``x`` is f32, bf16 or f16 ``[..., d]``, d up to 20,480; the residual of x's type or f32;
 the weight f32, bf16 or f16 ``[d]`` or None (1).  Norms and sums are 32 bits.  The reference's rms norm is a torch expression
 (``engraft/lens.py:282-287``), its additions are apart."""
 from __future__ import annotations

@@ -864,14 +864,16 @@ int eg_fp8_dequantize(const eg_fp8_matrix* m, void* out, int32_t dtype, int64_t 
 
 /* C [m, n] = A B^T and, with b2, C2 [m, n2] = A B2^T: a in blocks of rows (block_rows 1), b and b2
  * weights (block_rows 128) of the same k; C of `dtype`, rows ldc apart.  f32 outputs come from exact products and
- * fp32 sums; bf16 and f16 ones of more than 32 rows from the fp8 matrix cores, whose sums of eight products drop
- * what lies 2^-13 below the largest of them (about 1.5e-5 of an output, a hundredth of bf16's rounding). */
+ * fp32 sums; bf16 and f16 ones from the fp8 matrix cores, whose sums of eight products drop what lies 2^-13 below
+ * the largest of them (about 1.5e-5 of an output, 1 / 100 of bf16's rounding).  The order of a sum depends on m and
+ * the outputs' sizes (deterministic for one of each).  Workspace 16-byte aligned. */
+int64_t eg_fp8_product_workspace_size(int64_t m, int64_t n, int64_t n2, int64_t k);
 int eg_fp8_product(const eg_fp8_matrix* a, const eg_fp8_matrix* b, const eg_fp8_matrix* b2, void* c, int64_t ldc,
-                   void* c2, int64_t ldc2, int32_t dtype, void* stream);
+                   void* c2, int64_t ldc2, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* The same from A's values x [m, b->k] of x_dtype, rows x_stride apart, whose blocks are taken on the way
- * (eg_fp8_quantize's).  Workspace of eg_fp8_linear_workspace_size bytes, 16-byte aligned (0 up to 32 rows). */
-int64_t eg_fp8_linear_workspace_size(int64_t m, int64_t k);
+/* The same from A's values x [m, b->k] of x_dtype, rows x_stride apart, whose blocks (eg_fp8_quantize's) are taken
+ * on the way. */
+int64_t eg_fp8_linear_workspace_size(int64_t m, int64_t n, int64_t n2, int64_t k);
 int eg_fp8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t x_stride, const eg_fp8_matrix* b,
                   const eg_fp8_matrix* b2, void* c, int64_t ldc, void* c2, int64_t ldc2, int32_t dtype,
                   void* workspace, int64_t workspace_bytes, void* stream);
@@ -881,13 +883,13 @@ int eg_fp8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t x_stride, c
  * What stands between the block's output and the projections behind it (the reference's
  * rms norm without the addition: engraft/replica/layers.py). */
 
-/* x [rows, d], residual the same (of x's type or f32) or NULL, weight [d] or NULL (1), rows stride
+/* x [rows, d], residual the same (of x's type or f32) or NULL, weight f32 [d] or NULL (1), rows stride
  * elements apart. */
 typedef struct eg_norm {
   const void* x;
   const void* residual;
-  const void* weight;
-  int32_t x_dtype, r_dtype, w_dtype;
+  const float* weight;
+  int32_t x_dtype, r_dtype;
   float eps;
   int64_t rows, d;
   int64_t x_stride, r_stride;
@@ -896,7 +898,7 @@ typedef struct eg_norm {
 /* h = x + residual, rounded to the residual's type (without a residual h is x and not written);
  * y = h w / sqrt(mean(h^2) + eps) in 32 bits, written as y (y_dtype) or in blocks as y8 (eg_fp8_quantize's):
  * one of the two.  rstd f32 [rows] (NULL: not wanted): 1 / sqrt(...), for the gradient.  h may be in
- * the place of x or of the residual; any other overlap is refused.  d up to 40,960. */
+ * the place of x or of the residual; any other overlap is refused.  d up to 20,480. */
 int eg_add_rms_norm(const eg_norm* norm, void* h, int64_t h_stride, void* y, int32_t y_dtype, int64_t y_stride,
                     const eg_fp8_matrix* y8, float* rstd, void* stream);
 
@@ -906,20 +908,20 @@ typedef struct eg_norm_grad {
   const void* d_y;
   const void* h;
   const void* d_residual;
-  const void* weight;
+  const float* weight;
   const float* rstd;
-  int32_t dy_dtype, h_dtype, w_dtype;
+  int32_t dy_dtype, h_dtype;
   int64_t rows, d;
   int64_t dy_stride, h_stride, dr_stride;
 } eg_norm_grad;
 
 /* The gradient of h (of x and of the residual alike) as d_x and, in a second type, as d_x2 (NULL: not
- * wanted), and the weight's, d_weight [d] (NULL: not wanted; then no workspace either).  Sums in 32 bits, in
+ * wanted), and the weight's, d_weight f32 [d] (NULL: not wanted; then no workspace either).  Sums in 32 bits, in
  * a fixed order.  Outputs must not overlap the inputs.  d up to 20,480.  Workspace 16-byte aligned. */
 int64_t eg_add_rms_norm_grad_workspace_size(int64_t rows, int64_t d);
 int eg_add_rms_norm_grad(const eg_norm_grad* grad, void* d_x, int32_t dx_dtype, int64_t dx_stride, void* d_x2,
-                         int32_t dx2_dtype, int64_t dx2_stride, void* d_weight, int32_t dw_dtype, void* workspace,
-                         int64_t workspace_bytes, void* stream);
+                         int32_t dx2_dtype, int64_t dx2_stride, float* d_weight, void* workspace, int64_t workspace_bytes,
+                         void* stream);
 
 /* ---- The norm of all gradients, and their clipping --------------------------------------
  *

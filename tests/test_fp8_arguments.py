@@ -43,7 +43,7 @@ def test_matrices_are_checked(needle, bad):
     a, w = _matrix(5, 300), _matrix(7, 300, 128)
     for name, x in bad.items():
         setattr(a, name, x)
-    _refused(lib.eg_fp8_product(_ref(a), _ref(w), None, 4096, 7, None, 0, 0, None), needle)
+    _refused(lib.eg_fp8_product(_ref(a), _ref(w), None, 4096, 7, None, 0, 0, None, 0, None), needle)
     _refused(lib.eg_fp8_quantize(4096, 0, 300, _ref(a), None), needle)
 
 
@@ -55,14 +55,18 @@ def test_products_are_checked(needle, args):
     lib = _lib().load()
     b = {"k": _matrix(7, 301, 128), None: None, 0: _matrix(7, 300, 128)}[args.get("b", 0)]
     _refused(lib.eg_fp8_product(_ref(_matrix(5, 300)), _ref(b), None, args.get("c", 4096), args.get("ldc", 7), None, 0,
-                                args.get("dtype", 0), None), needle)
+                                args.get("dtype", 0), None, 0, None), needle)
 
 
 def test_linear_is_checked():
     lib = _lib().load()
     w = _matrix(7, 300, 128)
     size = lib.eg_fp8_linear_workspace_size
-    assert size(1, 300) == 0 and size(100, 300) == 100 * (384 + 4) and size(-1, 300) == -1 and size(5, 0) == -1
+    assert size(1, 7, 0, 300) == 0 and size(100, 7, 0, 300) == 100 * (384 + 4) and size(-1, 7, 0, 300) == -1 and size(5, 7, 0, 0) == -1
+    assert size(100, 7, 5, 10_240) > 100 * (10_240 + 80) and lib.eg_fp8_product_workspace_size(100, 7, 5, 10_240) > 0
+    assert lib.eg_fp8_product_workspace_size(1, 7, 0, 10_240) == 0 and lib.eg_fp8_product_workspace_size(1, -7, 0, 10_240) == -1
+    a, b = _matrix(100, 10_240), _matrix(7, 10_240, 128)
+    _refused(lib.eg_fp8_product(_ref(a), _ref(b), None, 4096, 7, None, 0, 0, 4096, 100, None), "workspace", _lib().EG_ERR_WORKSPACE)
     run = lambda x=4096, dtype=0, m=100, ld=300, ws=4096, n=1 << 20: lib.eg_fp8_linear(  # noqa: E731
         x, dtype, m, ld, _ref(w), None, 4096, 7, None, 0, 0, ws, n, None)
     _refused(run(x=None), "NULL")
@@ -101,7 +105,7 @@ def _run_norm(o, h=4 << 20, y=5 << 20, y_dtype=0, y8=None, h_stride=300, y_strid
 @pytest.mark.parametrize("needle,kw,more", [
     ("-1 rows", dict(rows=-1), {}), ("5 rows of 0", dict(d=0), {}), ("eps", dict(eps=-1.0), {}), ("eps", dict(eps=float("nan")), {}),
     ("x: NULL", dict(x=None), {}), ("x: dtype=4", dict(x_dtype=4), {}), ("x: rows", dict(x_stride=299), {}), ("residual: rows", dict(r_stride=10), {}),
-    ("x's type or f32", dict(x_dtype=0, r_dtype=1), {}), ("weight dtype", dict(weight=4096, w_dtype=9), {}), ("misaligned weight", dict(weight=4097), {}),
+    ("x's type or f32", dict(x_dtype=0, r_dtype=1), {}), ("misaligned weight", dict(weight=4097), {}),
     ("h: NULL", {}, dict(h=None)), ("y or y8", {}, dict(y=None)), ("y overlaps x", {}, dict(y=(1 << 20) + 40)),
     ("y overlaps h", {}, dict(y=(4 << 20) + 40)), ("h overlaps x", {}, dict(h=(1 << 20) + 40)), ("h overlaps the residual", {}, dict(h=(2 << 20) + 1200)),
     ("y overlaps the residual", {}, dict(y=(2 << 20) + 400)), ("y: misaligned", {}, dict(y=(5 << 20) + 2)),
@@ -114,7 +118,7 @@ def test_norms_in_blocks_are_checked():
     _refused(_run_norm(_norm(), y=None, y8=_matrix(5, 301)), "y8 is 5 x 301")
     _refused(_run_norm(_norm(), y8=_matrix(5, 300)), "y or y8")
     _refused(_run_norm(_norm(), y=None, y8=_matrix(5, 300, q=1 << 20)), "y overlaps x")
-    _refused(_run_norm(_norm(d=40_961, x_stride=50_000, r_stride=50_000), h_stride=50_000, y_stride=50_000), "at most 40960", _lib().EG_ERR_UNSUPPORTED)
+    _refused(_run_norm(_norm(d=20_481, x_stride=50_000, r_stride=50_000), h_stride=50_000, y_stride=50_000), "at most 20480", _lib().EG_ERR_UNSUPPORTED)
     assert _run_norm(_norm(rows=0, x=None, residual=None), h=None) == 0
 
 
@@ -134,7 +138,7 @@ def _norm_grad(**kw):
 def test_norm_gradients_are_checked(needle, kw, more):
     lib = _lib().load()
     o = _norm_grad(**kw)
-    _refused(lib.eg_add_rms_norm_grad(ctypes.byref(o), more.get("d_x", 6 << 20), 0, 300, more.get("d_x2"), 0, 300, None, 0, None, 0, None), needle)
+    _refused(lib.eg_add_rms_norm_grad(ctypes.byref(o), more.get("d_x", 6 << 20), 0, 300, more.get("d_x2"), 0, 300, None, None, 0, None), needle)
 
 
 def test_norm_gradients_workspace():
@@ -142,11 +146,11 @@ def test_norm_gradients_workspace():
     size = lib.eg_add_rms_norm_grad_workspace_size
     assert size(5, 300) > 0 and size(0, 300) == 0 and size(-1, 300) == -1 and size(5, 20_481) == -1
     o = _norm_grad()
-    args = (ctypes.byref(o), 6 << 20, 0, 300, None, 0, 0, 7 << 20, 0)
+    args = (ctypes.byref(o), 6 << 20, 0, 300, None, 0, 0, 7 << 20)
     _refused(lib.eg_add_rms_norm_grad(*args, 8 << 20, size(5, 300) - 1, None), "workspace", _lib().EG_ERR_WORKSPACE)
     _refused(lib.eg_add_rms_norm_grad(*args, None, size(5, 300), None), "aligned")
     o = _norm_grad(d=20_481, dy_stride=20_481, h_stride=20_481)
-    _refused(lib.eg_add_rms_norm_grad(ctypes.byref(o), 6 << 20, 0, 20_481, None, 0, 0, None, 0, None, 0, None), "at most 20480", _lib().EG_ERR_UNSUPPORTED)
+    _refused(lib.eg_add_rms_norm_grad(ctypes.byref(o), 6 << 20, 0, 20_481, None, 0, 0, None, None, 0, None), "at most 20480", _lib().EG_ERR_UNSUPPORTED)
 
 
 def _clip(*tensors, max_norm=1.0, norm=4096, ws=4096, n=1 << 30):

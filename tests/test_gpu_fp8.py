@@ -105,7 +105,7 @@ def test_weights_and_their_transposes(cuda, n, k, dtype):
 
 SIZES = [(1, 1, 1), (1, 2560, 640), (2, 130, 17), (4, 700, 300), (5, 128, 129), (16, 2560, 272), (17, 1000, 500), (32, 256, 128),
          (33, 640, 200), (64, 2560, 64), (65, 129, 257), (127, 1000, 1111), (300, 384, 2048), (777, 1000, 1111), (1500, 640, 4100),
-         (2047, 2560, 4100)]
+         (2047, 2560, 4100), (70, 5000, 130), (200, 10_240, 2560), (65, 4096, 1)]
 
 
 @pytest.mark.parametrize("m,k,n", SIZES)
@@ -117,11 +117,11 @@ def test_products(cuda, m, k, n, dtype, out):
     y = fp8.product(x, w, out_dtype=out)
     assert y.shape == (m, n) and y.dtype == out
     xv, wv = O.rows(x)[0], w.dequantize().double()
-    exact = out == F32 or m <= 32
+    exact = out == F32
     check_product(y, xv, wv, out, exact)
     # the same from blocks, and the same bits again
     r = fp8.quantize_rows(x)
-    assert torch.equal(fp8.product(r, w, out_dtype=out), y) or m <= 4  # a few rows: other sums' order is not promised
+    assert torch.equal(fp8.product(r, w, out_dtype=out), y) or m <= 32  # few rows take their own blocks in a kernel of its own order
     check_product(fp8.product(r, w, out_dtype=out), xv, wv, out, exact)
     assert torch.equal(fp8.product(x, w, out_dtype=out), y)
 
@@ -137,7 +137,7 @@ def test_gradient(cuda, m, k, n, dtype):
     y = fp8.product(x, w)
     (d_x,) = torch.autograd.grad(y, x, d_y)
     assert d_x.shape == x.shape and d_x.dtype == dtype
-    check_product(d_x, O.rows(d_y)[0], w.dequantize().double().T.contiguous(), dtype, dtype == F32 or m <= 32)
+    check_product(d_x, O.rows(d_y)[0], w.dequantize().double().T.contiguous(), dtype, dtype == F32)
     assert torch.equal(fp8.product_grad(d_y, w), d_x)
 
 
@@ -146,7 +146,7 @@ def test_split_leads_and_strides(cuda):
     from engraft_ngram_amd import fp8
     g = _gen(3)
     w = fp8.quantize_weight(_values(g, 300, 260, F32, 0.02))
-    for m in (3, 40):
+    for m in (3, 20, 40):
         x = _values(g, 2 * m, 260, BF16)
         whole = fp8.product(x, w, out_dtype=F32)
         a, b = fp8.product(x, w, out_dtype=F32, split=128)
@@ -188,11 +188,13 @@ def test_rows_of_views_and_rows_behind(cuda):
     g = _gen(5)
     x, w = _values(g, 90, 384, BF16), fp8.quantize_weight(_values(g, 100, 384, F32, 0.02))
     r = fp8.quantize_rows(x)
-    y = fp8.product(r, w)
-    r.q.view(torch.uint8)[50:] = 0x7F  # NaN
-    r.scales.view(torch.uint8)[50:] = 0xFF
-    part = fp8.Fp8Rows(r.q[10:50], r.scales[10:50], 384)
-    assert torch.equal(fp8.product(part, w), y[10:50])
+    for last in (12, 50, 89):
+        want = fp8.product(fp8.quantize_rows(x[10:last].contiguous()), w)
+        r.q.view(torch.uint8)[last:] = 0x7F  # NaN
+        r.scales.view(torch.uint8)[last:] = 0xFF
+        part = fp8.Fp8Rows(r.q[10:last], r.scales[10:last], 384)
+        assert torch.equal(fp8.product(part, w), want)
+        r = fp8.quantize_rows(x)
 
 
 def test_streams_and_graphs(cuda):

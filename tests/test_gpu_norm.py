@@ -33,7 +33,7 @@ def _reference(x, residual, w, eps):
     return h, v, r, v * r * (1.0 if w is None else w.double())
 
 
-WIDTHS = [(1, 1), (3, 7), (2, 128), (5, 511), (4, 513), (9, 2560), (1200, 2560), (3, 4097), (40, 16_384), (2, 40_960), (2100, 130)]
+WIDTHS = [(1, 1), (3, 7), (2, 128), (5, 511), (4, 513), (9, 2560), (1200, 2560), (3, 4097), (40, 16_384), (2, 20_480), (2100, 130), (3, 1023), (5, 2561), (700, 20_479)]
 
 
 @pytest.mark.parametrize("n,d", WIDTHS)
@@ -81,7 +81,7 @@ def test_norms_in_blocks(cuda, n, d, dtype):
     assert bool((y.q.view(torch.uint8)[:, d:] == 0).all())
 
 
-@pytest.mark.parametrize("n,d", [(1, 1), (3, 7), (5, 511), (9, 2560), (1500, 2560), (3, 4097), (40, 16_384), (2, 20_480), (4100, 130), (0, 64)])
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 7), (5, 511), (9, 2560), (1500, 2560), (3, 4097), (40, 16_384), (2, 20_480), (4100, 130), (0, 64), (1300, 2559), (300, 20_473)])
 @pytest.mark.parametrize("dy_dtype,dtype", [(F32, F32), (BF16, BF16), (F32, F16), (BF16, F32)])
 def test_gradients(cuda, n, d, dy_dtype, dtype):
     from engraft_ngram_amd import norm
