@@ -3,7 +3,7 @@
 //   N = sqrt(sum over all tensors of g^2),   out = g max_norm / N where N > max_norm, g otherwise
 //
 // Bound by its bytes.  Two kinds of launch: every workgroup adds the squares of its tiles (8,192 values
-// of one tensor each) in 64 bits, which neither overflow nor lose small tensors beside large
+// of one tensor each, 2,048 where all tensors are small) in 64 bits, which neither overflow nor lose small tensors beside large
 // ones, and writes its sum; then every workgroup adds all of these sums (a few KB from L2, in one order) and
 // writes its tiles' values, from the last one on: what was read last is in the caches.  The
 // tensors are kernel arguments, 48 a launch, so that nothing is copied to the device.
@@ -17,9 +17,8 @@ namespace eg {
 namespace {
 
 constexpr int kTensors = 48;      // a launch
-constexpr int kTile = 8192;       // values
 constexpr int kThreads = 256;
-constexpr int kMostGroups = 1024; // workgroups a launch
+constexpr int kMostGroups = 2048; // workgroups a launch
 
 struct ClipTensor {
   const void* g;
@@ -90,11 +89,10 @@ __device__ inline void write8(const ClipTensor& t, int64_t i, const float (&v)[8
   }
 }
 
-constexpr int kReads = kTile / (kThreads * 8);  // eight values each, a thread and tile
-
-// A tile's values: all loads are on their way before the first is waited for.
-template <typename T>
-__device__ inline void read_tile(const ClipTensor& t, int64_t tile, float (&v)[kReads][8]) {
+// A tile is READS times eight values a thread; all of its loads are on their way before the first is waited for.
+template <typename T, int READS>
+__device__ inline void read_tile(const ClipTensor& t, int64_t tile, float (&v)[READS][8]) {
+  constexpr int kTile = READS * kThreads * 8, kReads = READS;
   const int64_t i0 = (tile - t.first_tile) * kTile + threadIdx.x * 8;
   if (t.cols == t.g_stride && (tile - t.first_tile + 1) * kTile <= t.values) {
     Raw8<T> r[kReads];
@@ -108,16 +106,17 @@ __device__ inline void read_tile(const ClipTensor& t, int64_t tile, float (&v)[k
   }
 }
 
+template <int READS>
 __global__ __launch_bounds__(kThreads) void squares_kernel(const ClipArgs a) {
   __shared__ double part[kThreads / 64];
   double s = 0.0;
   for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const ClipTensor& t = a.t[tensor_of(a, tile)];
     device_type(t.g_dtype, [&](auto z) {
-      float v[kReads][8];
+      float v[READS][8];
       read_tile<decltype(z)>(t, tile, v);
 #pragma unroll
-      for (int j = 0; j < kReads; ++j)
+      for (int j = 0; j < READS; ++j)
 #pragma unroll
         for (int k = 0; k < 8; ++k) s += (double)v[j][k] * (double)v[j][k];
     });
@@ -144,28 +143,34 @@ __device__ inline double root_of_sums(const double* sums, int64_t count, double*
   return sqrt(s);
 }
 
+template <int READS>
 __global__ __launch_bounds__(kThreads) void scale_kernel(const ClipArgs a, const double* sums, int64_t count, float max_norm, float* norm) {
   __shared__ double part[kThreads / 64];
-  const double root = root_of_sums(sums, count, part);
-  if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)root;
-  const bool clips = root > (double)max_norm && root <= 1.7976931348623157e308;
-  const double factor = clips ? (double)max_norm / root : 1.0;  // as a float it could leave the normal numbers
+  double root = 0.0, factor = 1.0;  // (as a float the factor could leave the normal numbers)
+  bool clips = false;
   for (int64_t k = blockIdx.x; k < a.tiles; k += gridDim.x) {
     const int64_t tile = a.tiles - 1 - k;
     const ClipTensor& t = a.t[tensor_of(a, tile)];
-    if (!clips && t.out == t.g) continue;  // as they are
-    const int64_t i0 = (tile - t.first_tile) * kTile + threadIdx.x * 8;
-    float v[kReads][8];
+    if (k != blockIdx.x && !clips && t.out == t.g) continue;  // as they are
+    float v[READS][8];
     device_type(t.g_dtype, [&](auto z) { read_tile<decltype(z)>(t, tile, v); });
+    if (k == blockIdx.x) {  // (the first tile's loads are on their way meanwhile)
+      root = root_of_sums(sums, count, part);
+      clips = root > (double)max_norm && root <= 1.7976931348623157e308;
+      if (clips) factor = (double)max_norm / root;
+      if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)root;
+      if (!clips && t.out == t.g) continue;
+    }
     if (clips) {
 #pragma unroll
-      for (int j = 0; j < kReads; ++j)
+      for (int j = 0; j < READS; ++j)
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[j][q] = (float)((double)v[j][q] * factor);
     }
+    const int64_t i0 = (tile - t.first_tile) * (READS * kThreads * 8) + threadIdx.x * 8;
     device_type(t.out_dtype, [&](auto y) {
 #pragma unroll
-      for (int j = 0; j < kReads; ++j) write8<decltype(y)>(t, i0 + j * kThreads * 8, v[j]);
+      for (int j = 0; j < READS; ++j) write8<decltype(y)>(t, i0 + j * kThreads * 8, v[j]);
     });
   }
 }
@@ -182,7 +187,14 @@ struct Launch {
   int groups;
 };
 
-int64_t tiles_of(const eg_clip_tensor& t) { return (t.rows * t.cols + kTile - 1) / kTile; }
+// Values of a tile: few, so that more workgroups share them, where there are less than 2^20 in all.
+int tile_of(const eg_clip_tensor* tensors, int64_t count) {
+  int64_t values = 0;
+  for (int64_t i = 0; i < count && values < (1 << 20); ++i) values += std::max<int64_t>(tensors[i].rows * tensors[i].cols, 0);
+  return values < (1 << 20) ? kThreads * 8 : 4 * kThreads * 8;
+}
+
+int64_t tiles_of(const eg_clip_tensor& t, int tile) { return (t.rows * t.cols + tile - 1) / tile; }
 
 int groups_of(int64_t tiles) { return (int)std::min<int64_t>(tiles, kMostGroups); }
 
@@ -212,12 +224,13 @@ using namespace eg;
 extern "C" {
 
 int64_t eg_clip_workspace_size(const eg_clip_tensor* tensors, int64_t count) {
-  if (count < 0 || (tensors == nullptr && count > 0)) return -1;
+  if (check_tensors(tensors, count) != EG_OK) return -1;
+  const int tile = tile_of(tensors, count);
   int64_t sums = 0, tiles = 0;
   int held = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (tensors[i].rows <= 0 || tensors[i].cols <= 0) continue;
-    tiles += tiles_of(tensors[i]);
+    tiles += tiles_of(tensors[i], tile);
     if (++held == kTensors) {
       sums += groups_of(tiles);
       tiles = held = 0;
@@ -257,6 +270,8 @@ int eg_clip_grads(const eg_clip_tensor* tensors, int64_t count, float max_norm, 
       return set_error(EG_ERR_ARG, "clip: %s %lld overlaps %s %lld", name(x), (long long)x->matrix, name(y), (long long)y->matrix);
     }
   }
+  const int tile = tile_of(tensors, count);
+  const bool small = tile == kThreads * 8;
   std::vector<Launch> launches;
   double* at = (double*)workspace;
   for (int64_t i = 0; i < count; ++i) {
@@ -267,14 +282,14 @@ int eg_clip_grads(const eg_clip_tensor* tensors, int64_t count, float max_norm, 
     const bool g_whole = t.rows == 1 || t.g_stride == t.cols, out_whole = t.rows == 1 || t.out_stride == t.cols;
     a.t[a.count++] = {t.g, t.out, t.cols, g_whole ? t.cols : t.g_stride, out_whole ? t.cols : t.out_stride, t.rows * t.cols,
                       t.g_dtype, t.out_dtype, a.tiles};
-    a.tiles += tiles_of(t);
+    a.tiles += tiles_of(t, tile);
   }
   int64_t sums = 0;
   for (Launch& l : launches) {
     l.groups = groups_of(l.args.tiles);
     l.args.sums = at + sums;
     sums += l.groups;
-    squares_kernel<<<l.groups, kThreads, 0, (hipStream_t)stream>>>(l.args);
+    (small ? squares_kernel<1> : squares_kernel<4>)<<<l.groups, kThreads, 0, (hipStream_t)stream>>>(l.args);
     if (const int rc = launch_status("squares_kernel"); rc != EG_OK) return rc;
   }
   if (!scales) {
@@ -282,7 +297,7 @@ int eg_clip_grads(const eg_clip_tensor* tensors, int64_t count, float max_norm, 
     return launch_status("norm_of_sums_kernel");
   }
   for (size_t i = launches.size(); i-- > 0;) {
-    scale_kernel<<<launches[i].groups, kThreads, 0, (hipStream_t)stream>>>(launches[i].args, at, sums, max_norm, i == 0 ? norm : nullptr);
+    (small ? scale_kernel<1> : scale_kernel<4>)<<<launches[i].groups, kThreads, 0, (hipStream_t)stream>>>(launches[i].args, at, sums, max_norm, i == 0 ? norm : nullptr);
     if (const int rc = launch_status("scale_kernel"); rc != EG_OK) return rc;
   }
   return EG_OK;

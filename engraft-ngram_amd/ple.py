@@ -8,9 +8,10 @@ Forward:
   (``gemm_x6``: operands split into three bf16 planes, six products
   accumulated in fp32; or ``gemm_h3``: rows scaled and split into two fp16
   planes, three products), with ``gemm="fp32"`` of the ``gemm_f32`` kernel on
-  the fp32 matrix cores (fp32 products, as the reference's torch matmuls), or
+  the fp32 matrix cores (fp32 products, as the reference's torch matmuls),
   with ``gemm="bf16x3"`` of the ``gemm_x3`` kernel (hi + lo planes, three
-  products: 16 mantissa bits per operand);
+  products: 16 mantissa bits per operand), or with ``gemm="fp8"`` of blocks of
+  8-bit values (``fp8.product``: a quarter of the weights' bytes);
 * ``eg_ple_gate``: per position and stream, the RMS norms of key and hidden,
   the score ``s``, the gate, ``gated = value * gate`` and its RMS norm;
 * ``eg_ple_conv``: the dilated causal depthwise convolution over
@@ -47,7 +48,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, fp8
 
 
 @dataclasses.dataclass
@@ -161,6 +162,7 @@ class _WeightCache:
 _WT = _WeightCache(4)
 _PLANES = _WeightCache(8)
 _HALF = _WeightCache(8)
+_BLOCKS = _WeightCache(8)
 
 
 def _transposed(w: torch.Tensor) -> torch.Tensor:
@@ -521,15 +523,39 @@ WGRAD_MAX_TAPS = 8  # eg_ple_weight_grads' built tap counts (1..8)
 SUMS_MAX_ROWS = 65535 * 63  # eg_ple_conv_backward_sums' rows: one grid row per 63 of them
 
 
+def _weight_blocks(ws: tuple, transposed: bool) -> fp8.Fp8Weight:
+    """The 8-bit blocks of weights with the same columns, one below the other; or of that matrix's
+    transpose alone (blocks of 128 x 128 are the transpose's too)."""
+    def make():
+        w = fp8.quantize_weight(ws[0] if len(ws) == 1 else torch.cat(ws), transpose=transposed)
+        return fp8.Fp8Weight(w.q_t, w.scales_t, w.shape[0]) if transposed else w
+
+    return _BLOCKS.get(ws, make, transposed)
+
+
+def _project_fp8(emb: torch.Tensor, w_key: torch.Tensor, w_value: torch.Tensor):
+    """Key and value from 8-bit blocks, fp32 sums: one product where the value's rows begin a block."""
+    if w_key.shape[0] % 128 == 0:
+        return fp8.product(emb, _weight_blocks((w_key, w_value), False), split=w_key.shape[0])
+    return tuple(fp8.product(emb, _weight_blocks((w,), False)) for w in (w_key, w_value))
+
+
+def _project_backward_fp8(pairs: list) -> torch.Tensor:
+    """``sum d_i w_i`` from the 8-bit blocks of the d_i and of the weights; a pair's weights, several one
+    below the other, have their d side by side."""
+    parts = [fp8.product(d, _weight_blocks(ws if isinstance(ws, tuple) else (ws,), True)) for d, ws in pairs]
+    return parts[0] if len(parts) == 1 else parts[0].add_(parts[1])
+
+
 def _weight_grad(d_y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, gemm: str = "fp32") -> torch.Tensor:
     """``d_y^T x`` (``[out, T]`` x ``[T, in]``), the gradient of ``w`` in
     ``y = x w^T``, with the positions as K: on eg_gemm_f32 (both operands
-    transposed into K-contiguous copies), or with ``gemm="bf16x6"`` on
+    transposed into K-contiguous copies), or with ``gemm="bf16x6"`` or ``"fp8"`` on
     eg_gemm_f16x3 (the same fp32 accuracy, its split reading the transposes in
     place; bf16x3's 16-bit operands are kept to the projections)."""
     if d_y.shape[0] == 0:
         return torch.zeros_like(w)
-    if gemm == "bf16x6":
+    if gemm in ("bf16x6", "fp8"):
         return _gemm_h3((d_y.T,), (x.T,))
     return gemm_f32(d_y.T, x.T)
 
@@ -537,6 +563,8 @@ def _weight_grad(d_y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, gemm: str 
 def _projection_backward(gemm: str, pairs: list) -> torch.Tensor:
     """``d_emb = sum d_i w_i`` over the (d_i, w_i) in ``pairs``, on the
     forward's GEMM."""
+    if gemm == "fp8":
+        return _project_backward_fp8(pairs)
     if gemm == "bf16x6" and pairs[0][0].shape[0] > H3_MIN_ROWS:
         ds, ws = zip(*pairs)
         return _gemm_h3(ds, tuple(w.T for w in ws), planes_b=_half_planes(ws, True))
@@ -579,7 +607,13 @@ class _PleFn(torch.autograd.Function):
         emb32 = emb.to(**f32).contiguous()
         wk32 = w_key.to(**f32)
         wv32 = w_value.to(**f32)
-        if t_len <= FEW_ROWS and _f32_in_place(wk32, wv32):
+        if gemm == "fp8":
+            if any(ctx.needs_input_grad) and not _native_backward_ok(hc, n, conv.shape[1], int(dil),
+                                                                     weights=any(ctx.needs_input_grad[2:8])):
+                raise ValueError(f"gemm='fp8' has gradients up to 4 streams, n_embd 4096 and a convolution reaching back 32 "
+                                 f"rows, got {hc} streams, n_embd {n}, {conv.shape[1]} taps at dilation {int(dil)}")
+            key, value = _project_fp8(emb32, wk32, wv32)
+        elif t_len <= FEW_ROWS and _f32_in_place(wk32, wv32):
             key, value = gemm_f32(emb32, wk32, b_n2=wv32, few_rows=True)
         elif gemm == "bf16x3":
             key, value = gemm_x3(SplitPlanes(emb32), wk32, cache_b=True, b_n2=wv32)
@@ -721,6 +755,19 @@ class _PleFn(torch.autograd.Function):
             d_hist_in = d_full[:h0].reshape(h0, hc, n).to(hist_dt) if need_hist else None
             return (d_emb, d_hidden.to(hidden_dt) if d_hidden is not None else None, None, None, None, None, None,
                     None, d_hist_in, None, None, None, None, None)
+        if (ctx.gemm == "fp8" and need_emb and not detach_gate and not detach_value and n % 256 == 0 and t_len > 0
+                and not (key.data_ptr() | value.data_ptr() | hidden32.data_ptr() | nk32.data_ptr() | nq32.data_ptr()
+                         | nc32.data_ptr() | d_out32.data_ptr() | d_full[h0:].data_ptr()) % 16):
+            # d_key and d_value side by side: their blocks are taken in one launch, and d_emb is one product
+            d_kv = torch.empty((t_len, c_dim + n), **f32)
+            d_s = torch.empty((t_len, hc), **f32)
+            _lib.call("eg_ple_gate_backward_kv", _lib.ptr(key), _lib.ptr(value), _lib.ptr(hidden32), _lib.ptr(nk32),
+                      _lib.ptr(nq32), _lib.ptr(nc32), _lib.ptr(s), _lib.ptr(gate), _lib.ptr(rstd), _lib.ptr(d_out32),
+                      _lib.ptr(d_full[h0:]), t_len, hc, n, _lib.ptr(d_kv), _lib.ptr(d_hidden), _lib.ptr(d_s), st)
+            d_emb = _project_backward_fp8([(d_kv, (wk32, wv32))]).to(emb_dt)
+            d_hist_in = d_full[:h0].reshape(h0, hc, n).to(hist_dt) if need_hist else None
+            return (d_emb, d_hidden.to(hidden_dt) if d_hidden is not None else None, None, None, None, None, None,
+                    None, d_hist_in, None, None, None, None, None)
         d_key = torch.empty((t_len, c_dim), **f32) if (need_emb and not detach_gate) else None
         d_value = torch.empty((t_len, n), **f32) if (need_emb and not detach_value) else None
         if d_key is not None or d_value is not None or d_hidden is not None:
@@ -763,7 +810,7 @@ class _PleFn(torch.autograd.Function):
         need_wk, need_wv, need_nk, need_nq, need_nc, need_cv = need[2:8]
         # both projection weights' gradients: d_key and d_value side by side, so that they
         # are one product with emb (whole rounds of tiles, emb split once)
-        both = (need_wk and need_wv and not detach_gate and not detach_value and ctx.gemm == "bf16x6"
+        both = (need_wk and need_wv and not detach_gate and not detach_value and ctx.gemm in ("bf16x6", "fp8")
                 and n % 256 == 0 and t_len > 0 and not (key.data_ptr() | value.data_ptr() | hidden32.data_ptr()
                                                         | nk32.data_ptr() | nq32.data_ptr() | nc32.data_ptr()
                                                         | d_out32.data_ptr() | d_full[h0:].data_ptr()) % 16)
@@ -784,6 +831,8 @@ class _PleFn(torch.autograd.Function):
         d_emb = None
         if need_emb:
             parts = [(d, w) for d, w in ((d_key, wk32), (d_value, wv32)) if d is not None]
+            if both and ctx.gemm == "fp8":
+                parts = [(d_kv, (wk32, wv32))]
             if parts:  # none: both factors detached, emb has no path to the output
                 d_emb = _projection_backward(ctx.gemm, parts).to(emb_dt)
         wdt = ctx.w_dtypes
@@ -838,10 +887,15 @@ def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w: PleWeights, hist: to
     accuracy), ``"fp32"`` (``gemm_f32``: fp32
     products on the fp32 matrix cores, the reference's torch matmul
     arithmetic) or ``"bf16x3"`` (``gemm_x3``: 16 mantissa bits per operand,
-    about 1e-5 relative per projection).  Up to ``FEW_ROWS`` positions every
-    choice runs ``eg_gemm_f32_rows``."""
-    if gemm not in ("fp32", "bf16x3", "bf16x6"):
-        raise ValueError(f"gemm must be 'fp32', 'bf16x3' or 'bf16x6', got {gemm!r}")
+    about 1e-5 relative per projection).  Up to ``FEW_ROWS`` positions each of these
+    runs ``eg_gemm_f32_rows``.  ``"fp8"``: both projections on 8-bit blocks
+    (``fp8.product``; 4 significant bits an operand, fp32 sums), for serving a block from a
+    quarter of its weights' bytes and training rows through it: the forward and
+    ``d_emb`` take the blocks of ``emb``, of ``d_key`` and ``d_value``, and of the weights, which are kept between calls;
+    the weights' own gradients are those of the rounded block's products, in fp32
+    accuracy from unrounded operands."""
+    if gemm not in ("fp32", "bf16x3", "bf16x6", "fp8"):
+        raise ValueError(f"gemm must be 'fp32', 'bf16x3', 'bf16x6' or 'fp8', got {gemm!r}")
     hc = hparams.hc_mult
     n = hparams.n_embd
     eps = float(hparams.f_norm_rms_eps)
