@@ -94,8 +94,8 @@ def _run(x, weight: Fp8Weight, split: int, code: int):
 class _Product(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, split, code):
-        ctx.weight, ctx.dtype = weight, x.dtype
-        ctx.rows = x.shape[0]
+        ctx.save_for_backward(weight.q_t, weight.scales_t)
+        ctx.shape, ctx.dtype, ctx.split = (x.shape[0], weight.shape[0]), x.dtype, split
         ctx.set_materialize_grads(False)
         y = _run(x, weight, split, code)
         return tuple(y) if split else y[0]
@@ -105,14 +105,17 @@ class _Product(torch.autograd.Function):
     def backward(ctx, *d):
         if all(x is None for x in d):
             return None, None, None, None
-        if len(d) == 2:  # the outputs side by side, as the weight's rows are
+        d_y = d[0]
+        if ctx.split:  # the outputs side by side, as the weight's rows are
+            rows, n = ctx.shape
             like = d[0] if d[0] is not None else d[1]
-            widths = ctx.weight.shape[0] - (d[1].shape[1] if d[1] is not None else 0)
-            first = d[0].shape[1] if d[0] is not None else widths
-            d = [x if x is not None else like.new_zeros((ctx.rows, w))
-                 for x, w in zip(d, (first, ctx.weight.shape[0] - first))]
-            d = [torch.cat(d, 1)]
-        return product_grad(d[0], ctx.weight, dtype=ctx.dtype), None, None, None
+            d_y = torch.cat([like.new_zeros((rows, w)) if x is None else x for x, w in zip(d, (ctx.split, n - ctx.split))], 1)
+        return _grad(d_y, *ctx.saved_tensors, ctx.shape[1], _lib.dtype_code(ctx.dtype)), None, None, None
+
+
+def _grad(d_y, q_t, scales_t, n, code) -> torch.Tensor:
+    """``d_y @ w`` of 2-D rows from the transpose's blocks."""
+    return _lib.autograd_ext().fp8_linear(d_y, q_t, scales_t, n, 0, code, _stream(d_y))[0]
 
 
 def product(x: torch.Tensor | Fp8Rows, weight: Fp8Weight, *, out_dtype: torch.dtype | None = None,
@@ -148,5 +151,5 @@ def product_grad(d_y: torch.Tensor, weight: Fp8Weight, *, dtype: torch.dtype | N
         raise ValueError("the gradient of x needs the weight's transpose: quantize_weight(w, transpose=True)")
     code = _lib.dtype_code(dtype if dtype is not None else d_y.dtype, "dtype")
     rows = d_y if d_y.dim() == 2 else d_y.reshape(-1, d_y.shape[-1])
-    d_x = _lib.autograd_ext().fp8_linear(rows, weight.q_t, weight.scales_t, weight.shape[0], 0, code, _stream(d_y))[0]
+    d_x = _grad(rows, weight.q_t, weight.scales_t, weight.shape[0], code)
     return d_x if d_y.dim() == 2 else d_x.reshape(*d_y.shape[:-1], weight.k)

@@ -63,7 +63,7 @@ def add_rms_norm_grad(d_y: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, we
 
 def _norm_backward(ctx, d_y, d_h):
     """The gradients of x, the residual and the weight; d_y the normed rows' (None: none)."""
-    h, rstd, weight = ctx.saved_tensors
+    h, rstd, weight = ctx.saved_tensors[:3]
     need_x, need_r, need_w = ctx.needs_input_grad[:3]
     x_dtype, r_dtype = ctx.dtypes
     if d_h is not None and d_h.dtype != h.dtype:
@@ -136,8 +136,8 @@ class _NormedProduct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, norm_weight, weight, eps, code):
         rows, h, rstd = _forward(x, residual, norm_weight, eps, -1, True)
-        ctx.save_for_backward(h, rstd, norm_weight)
-        ctx.weight = weight
+        ctx.save_for_backward(h, rstd, norm_weight, weight.q_t, weight.scales_t)
+        ctx.n = weight.shape[0]
         ctx.dtypes = (x.dtype, None if residual is None else residual.dtype)
         ctx.set_materialize_grads(False)
         y = fp8._run(rows, weight, 0, code)[0]
@@ -149,7 +149,7 @@ class _NormedProduct(torch.autograd.Function):
         if d_y is None and d_h is None:
             return None, None, None, None, None, None
         # fp32: the norm's gradients are sums over a row and over all rows of it
-        d_rows = None if d_y is None else fp8.product_grad(d_y, ctx.weight, dtype=torch.float32)
+        d_rows = None if d_y is None else fp8._grad(d_y, *ctx.saved_tensors[3:], ctx.n, 0)
         return (*_norm_backward(ctx, d_rows, d_h), None, None, None)
 
 

@@ -88,6 +88,16 @@ def test_a_norm_that_is_not_finite_leaves_the_values(cuda):
         assert all(torch.equal(torch.nan_to_num(a, nan=5.5), torch.nan_to_num(b, nan=5.5)) for a, b in zip(grads, kept))
 
 
+def test_a_tensor_past_4_gib(cuda):
+    from engraft_ngram_amd import clip
+    x = torch.zeros((1 << 31) + 5, dtype=BF16, device="cuda")
+    x[-3:] = torch.tensor([3.0, -4.0, 12.0])
+    x[0] = 84.0
+    assert float(clip.clip_grads([x], 8.5)) == 85.0
+    assert x[-3:].tolist() == [0.30078125, -0.400390625, 1.203125] and float(x[0]) == 8.375  # the nearest bf16 to 0.3, 0.4, 1.2, 8.4
+    assert float(x[1:-3].abs().max()) == 0.0
+
+
 def test_strides(cuda):
     """Rows of wider buffers, transposes, mixed types; what lies between the rows stays."""
     from engraft_ngram_amd import clip

@@ -223,7 +223,7 @@ def test_streams_and_graphs(cuda):
 
 
 def test_rows_past_4_gib(cuda):
-    """Rows whose bytes lie more than 2^32 apart, and outputs past 2^32 bytes."""
+    """Rows whose bytes lie more than 2^32 apart."""
     from engraft_ngram_amd import fp8
     m, k, n = 1_700_000, 2560, 8
     g = _gen(7)
@@ -236,3 +236,50 @@ def test_rows_past_4_gib(cuda):
     y = fp8.product(r, w, out_dtype=F32)
     assert not bool(y[:-100].any())
     check_product(y[-100:], some.dequantize(F32).double(), w.dequantize().double(), F32, True)
+    # and values and outputs more than 2^32 bytes apart
+    x = torch.zeros((m, k), dtype=BF16, device="cuda")
+    x[-100:] = _values(g, 100, k, BF16)
+    last = fp8.quantize_rows(x[-100:])
+    assert torch.equal(fp8.quantize_rows(x).q[-100:].view(torch.uint8), last.q.view(torch.uint8))
+    w = fp8.quantize_weight(_values(g, 1300, k, F32, 0.02), transpose=False)
+    y = fp8.product(x, w, out_dtype=BF16)
+    assert not bool(y[:-100].any()) and torch.equal(y[-100:], fp8.product(x[-300:], w, out_dtype=BF16)[-100:])
+
+
+def test_a_weight_that_changed_before_the_gradient(cuda):
+    from engraft_ngram_amd import fp8
+    g = _gen(8)
+    w = fp8.quantize_weight(_values(g, 200, 300, F32, 0.02))
+    y = fp8.product(_values(g, 50, 300, F32).requires_grad_(), w)
+    w.q_t.view(torch.uint8).zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_gradients_captured(cuda):
+    """Forward and backward through autograd in one graph: replays see new inputs."""
+    from engraft_ngram_amd import fp8, norm
+    g = _gen(9)
+    w = fp8.quantize_weight(_values(g, 300, 640, F32, 0.02))
+    x, res, d = _values(g, 70, 640, BF16).requires_grad_(), _values(g, 70, 640, BF16), _values(g, 70, 300, BF16)
+    nw = torch.randn(640, generator=g, device="cuda").requires_grad_()
+
+    def step():
+        y, h = norm.normed_product(x, res, nw, w)
+        return (y.detach(), *torch.autograd.grad(y, (x, nw), d))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        with torch.no_grad():
+            x.copy_(_values(g, 70, 640, BF16))
+            d.copy_(_values(g, 70, 300, BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))

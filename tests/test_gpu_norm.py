@@ -215,6 +215,27 @@ def test_rows_of_wider_buffers(cuda):
     assert torch.equal(one[1], norm.add_rms_norm(x[:1].repeat(20, 1), res, None)[1])
 
 
+def test_no_rows_and_rows_past_2_gib(cuda):
+    from engraft_ngram_amd import fp8, norm
+    none = torch.zeros((0, 300), device="cuda")
+    y, h = norm.add_rms_norm(none, none, torch.ones(300, device="cuda"))
+    assert y.shape == (0, 300) and h.shape == (0, 300)
+    y, h = norm.add_rms_norm(none, none, None, out_dtype="fp8")
+    assert y.shape == (0, 300) and y.dequantize().shape == (0, 300)
+    w = fp8.quantize_weight(torch.ones((7, 300), device="cuda"))
+    assert norm.normed_product(none, none, None, w)[0].shape == (0, 7)
+    g = _gen(14)
+    x = torch.zeros((1_700_000, 2560), dtype=BF16, device="cuda")
+    x[-50:] = _values(g, 50, 2560, BF16)
+    want = norm.add_rms_norm_stats(x[-50:], x[-50:], None)
+    y, h, rstd = norm.add_rms_norm_stats(x, x, None)
+    assert torch.equal(y[-50:], want[0]) and torch.equal(h[-50:], want[1]) and not bool(y[:-50].any())
+    d_h, _ = norm.add_rms_norm_grad(y, h, rstd, None)
+    assert torch.equal(d_h[-50:], norm.add_rms_norm_grad(*want, None)[0])
+    y8, _ = norm.add_rms_norm(x, x, None, out_dtype="fp8")
+    assert torch.equal(y8.dequantize()[-50:], norm.add_rms_norm(x[-50:], x[-50:], None, out_dtype="fp8")[0].dequantize())
+
+
 def test_graphs(cuda):
     from engraft_ngram_amd import norm
     g = _gen(13)
