@@ -858,7 +858,7 @@ int eg_fp8_quantize(const void* x, int32_t dtype, int64_t row_stride, const eg_f
   if (out->rows == 0) return EG_OK;
   const int blocks = (int)((out->k + 127) / 128), groups = (blocks + 3) / 4;
   const int64_t units = out->rows * groups;
-  EG_CHECK_ARG((units + 3) / 4 <= INT32_MAX, "fp8_quantize: %lld x %lld is too large", (long long)out->rows, (long long)out->k);
+  EG_CHECK_ARG((units + 3) / 4 < (1 << 24), "fp8_quantize: %lld x %lld is too large", (long long)out->rows, (long long)out->k);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     quantize_kernel<T><<<(unsigned)((units + 3) / 4), 256, 0, (hipStream_t)stream>>>(
@@ -898,7 +898,7 @@ int eg_fp8_dequantize(const eg_fp8_matrix* m, void* out, int32_t dtype, int64_t 
   if (const int rc = check_values(out, dtype, m->rows, m->k, row_stride, "fp8_dequantize"); rc != EG_OK) return rc;
   const int64_t count = m->rows * ((m->k + 7) / 8);
   if (count == 0) return EG_OK;
-  EG_CHECK_ARG((count + 255) / 256 <= INT32_MAX, "fp8_dequantize: %lld x %lld is too large", (long long)m->rows, (long long)m->k);
+  EG_CHECK_ARG((count + 255) / 256 < (1 << 24), "fp8_dequantize: %lld x %lld is too large", (long long)m->rows, (long long)m->k);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     dequantize_kernel<T><<<(unsigned)((count + 255) / 256), 256, 0, (hipStream_t)stream>>>(

@@ -14,6 +14,9 @@ matrix cores of gfx950 take with their operands, and the values are exact in bf1
 infinities become NaN.  The weight is frozen: its gradient is not to be had (the
 ``ple`` block's fp32 weights keep theirs under ``ple_forward(gemm="fp8")``).
 
+The kernel and the order of its sums go by the number of rows: a row's result is the same bits from the same call, and
+may differ in its last ones beside another number of rows.
+
 ``product`` takes the blocks of ``x`` (f32, bf16 or f16) itself; its gradient takes those of the
 output's gradient, along the other axis.  f32 outputs come from exact products and fp32 sums;
 16-bit ones from the fp8 matrix cores, about 1.5e-5 of an output off (bf16 rounds by 2e-3).  The reference's projections are fp32 (``engraft/replica/layers.py:594-606``)."""

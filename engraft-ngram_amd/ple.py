@@ -162,7 +162,6 @@ class _WeightCache:
 _WT = _WeightCache(4)
 _PLANES = _WeightCache(8)
 _HALF = _WeightCache(8)
-_BLOCKS = _WeightCache(8)
 
 
 def _transposed(w: torch.Tensor) -> torch.Tensor:
@@ -523,28 +522,44 @@ WGRAD_MAX_TAPS = 8  # eg_ple_weight_grads' built tap counts (1..8)
 SUMS_MAX_ROWS = 65535 * 63  # eg_ple_conv_backward_sums' rows: one grid row per 63 of them
 
 
-def _weight_blocks(ws: tuple, transposed: bool) -> fp8.Fp8Weight:
-    """The 8-bit blocks of weights with the same columns, one below the other; or of that matrix's
-    transpose alone (blocks of 128 x 128 are the transpose's too)."""
-    def make():
-        w = fp8.quantize_weight(ws[0] if len(ws) == 1 else torch.cat(ws), transpose=transposed)
-        return fp8.Fp8Weight(w.q_t, w.scales_t, w.shape[0]) if transposed else w
+class PleBlocks:
+    """Both projections' weights in 8-bit blocks, for ``ple_forward(gemm="fp8", blocks=...)``: ``parts``, the key's and the
+    value's :class:`fp8.Fp8Weight`, or one of the value's rows below the key's where they begin a block."""
 
-    return _BLOCKS.get(ws, make, transposed)
+    __slots__ = ("parts", "n_key", "n_value")
+
+    def __init__(self, parts: tuple, n_key: int, n_value: int):
+        self.parts, self.n_key, self.n_value = parts, n_key, n_value
+
+    def project(self, emb: torch.Tensor):
+        """Key and value of ``emb``, fp32 sums."""
+        if len(self.parts) == 1:
+            return fp8.product(emb, self.parts[0], split=self.n_key)
+        return tuple(fp8.product(emb, w) for w in self.parts)
+
+    def project_grad(self, d_key: torch.Tensor | None, d_value: torch.Tensor | None, d_kv: torch.Tensor | None = None):
+        """``emb``'s gradient from those of key and value (None: 0), or from both side by side."""
+        if len(self.parts) == 2:
+            parts = [fp8.product_grad(d, w) for d, w in zip((d_key, d_value), self.parts) if d is not None]
+            return parts[0] if len(parts) == 1 else parts[0].add_(parts[1])
+        if d_kv is None:
+            like = d_value if d_key is None else d_key
+            d_kv = torch.cat([like.new_zeros((like.shape[0], n)) if d is None else d
+                              for d, n in ((d_key, self.n_key), (d_value, self.n_value))], 1)
+        return fp8.product_grad(d_kv, self.parts[0])
 
 
-def _project_fp8(emb: torch.Tensor, w_key: torch.Tensor, w_value: torch.Tensor):
-    """Key and value from 8-bit blocks, fp32 sums: one product where the value's rows begin a block."""
+def quantize_projections(w: PleWeights, *, transpose: bool = True) -> PleBlocks:
+    """The blocks of ``w``'s projections, for as long as they stay as they are; ``transpose``: with what ``emb``'s gradient
+    needs (as many bytes again).  Not differentiable."""
+    return _projection_blocks(w.w_key, w.w_value, transpose)
+
+
+def _projection_blocks(w_key: torch.Tensor, w_value: torch.Tensor, transpose: bool) -> PleBlocks:
+    ws = (w_key.detach(), w_value.detach())
     if w_key.shape[0] % 128 == 0:
-        return fp8.product(emb, _weight_blocks((w_key, w_value), False), split=w_key.shape[0])
-    return tuple(fp8.product(emb, _weight_blocks((w,), False)) for w in (w_key, w_value))
-
-
-def _project_backward_fp8(pairs: list) -> torch.Tensor:
-    """``sum d_i w_i`` from the 8-bit blocks of the d_i and of the weights; a pair's weights, several one
-    below the other, have their d side by side."""
-    parts = [fp8.product(d, _weight_blocks(ws if isinstance(ws, tuple) else (ws,), True)) for d, ws in pairs]
-    return parts[0] if len(parts) == 1 else parts[0].add_(parts[1])
+        ws = (torch.cat(ws),)
+    return PleBlocks(tuple(fp8.quantize_weight(w, transpose=transpose) for w in ws), w_key.shape[0], w_value.shape[0])
 
 
 def _weight_grad(d_y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, gemm: str = "fp32") -> torch.Tensor:
@@ -563,8 +578,6 @@ def _weight_grad(d_y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, gemm: str 
 def _projection_backward(gemm: str, pairs: list) -> torch.Tensor:
     """``d_emb = sum d_i w_i`` over the (d_i, w_i) in ``pairs``, on the
     forward's GEMM."""
-    if gemm == "fp8":
-        return _project_backward_fp8(pairs)
     if gemm == "bf16x6" and pairs[0][0].shape[0] > H3_MIN_ROWS:
         ds, ws = zip(*pairs)
         return _gemm_h3(ds, tuple(w.T for w in ws), planes_b=_half_planes(ws, True))
@@ -600,19 +613,16 @@ class _PleFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, emb, hidden, w_key, w_value, nk, nq, nc, conv, hist, eps, dil, detach_value, detach_gate,
-                gemm):
+                gemm, blocks):
         t_len, hc, n = hidden.shape
         dev = hidden.device
         f32 = dict(dtype=torch.float32, device=dev)
         emb32 = emb.to(**f32).contiguous()
-        wk32 = w_key.to(**f32)
-        wv32 = w_value.to(**f32)
+        wk32, wv32 = (x if blocks is not None else x.to(**f32) for x in (w_key, w_value))  # (None: their blocks are given)
         if gemm == "fp8":
-            if any(ctx.needs_input_grad) and not _native_backward_ok(hc, n, conv.shape[1], int(dil),
-                                                                     weights=any(ctx.needs_input_grad[2:8])):
-                raise ValueError(f"gemm='fp8' has gradients up to 4 streams, n_embd 4096 and a convolution reaching back 32 "
-                                 f"rows, got {hc} streams, n_embd {n}, {conv.shape[1]} taps at dilation {int(dil)}")
-            key, value = _project_fp8(emb32, wk32, wv32)
+            if blocks is None:
+                blocks = _projection_blocks(wk32, wv32, ctx.needs_input_grad[0])
+            key, value = blocks.project(emb32)
         elif t_len <= FEW_ROWS and _f32_in_place(wk32, wv32):
             key, value = gemm_f32(emb32, wk32, b_n2=wv32, few_rows=True)
         elif gemm == "bf16x3":
@@ -672,12 +682,13 @@ class _PleFn(torch.autograd.Function):
                                   emb_w)
             ctx.gated = gated
             ctx.dtypes = (emb.dtype, hidden.dtype, hist.dtype)
-            ctx.w_dtypes = tuple(x.dtype for x in (w_key, w_value, nk, nq, nc, conv))
+            ctx.w_dtypes = tuple(x.dtype if x is not None else None for x in (w_key, w_value, nk, nq, nc, conv))
             ctx.tail_rows = new_hist.shape[0]
         else:
             ctx.save_for_backward(emb, hidden, w_key, w_value, nk, nq, nc, conv, hist)
         ctx.cfg = (eps, dil, detach_value, detach_gate)
         ctx.gemm = gemm
+        ctx.blocks = blocks if ctx.needs_input_grad[0] else None
         ctx.mark_non_differentiable(s, gate, value)
         return out.to(hidden.dtype), new_hist, s, gate, value
 
@@ -702,7 +713,7 @@ class _PleFn(torch.autograd.Function):
         # an input the detached graph does not reach keeps autograd's None, as
         # in the reference's own graph (its .grad stays None)
         res = [next(grads) if need else None for need in ctx.needs_input_grad[:9]]
-        return (*res, None, None, None, None, None)
+        return (*res, None, None, None, None, None, None)
 
     @staticmethod
     def _backward_native(ctx, d_out, d_hist):
@@ -754,7 +765,7 @@ class _PleFn(torch.autograd.Function):
                     d_emb = gemm_x3(*[x for part in parts for x in part], cache_b=True).to(emb_dt)
             d_hist_in = d_full[:h0].reshape(h0, hc, n).to(hist_dt) if need_hist else None
             return (d_emb, d_hidden.to(hidden_dt) if d_hidden is not None else None, None, None, None, None, None,
-                    None, d_hist_in, None, None, None, None, None)
+                    None, d_hist_in, None, None, None, None, None, None)
         if (ctx.gemm == "fp8" and need_emb and not detach_gate and not detach_value and n % 256 == 0 and t_len > 0
                 and not (key.data_ptr() | value.data_ptr() | hidden32.data_ptr() | nk32.data_ptr() | nq32.data_ptr()
                          | nc32.data_ptr() | d_out32.data_ptr() | d_full[h0:].data_ptr()) % 16):
@@ -764,10 +775,10 @@ class _PleFn(torch.autograd.Function):
             _lib.call("eg_ple_gate_backward_kv", _lib.ptr(key), _lib.ptr(value), _lib.ptr(hidden32), _lib.ptr(nk32),
                       _lib.ptr(nq32), _lib.ptr(nc32), _lib.ptr(s), _lib.ptr(gate), _lib.ptr(rstd), _lib.ptr(d_out32),
                       _lib.ptr(d_full[h0:]), t_len, hc, n, _lib.ptr(d_kv), _lib.ptr(d_hidden), _lib.ptr(d_s), st)
-            d_emb = _project_backward_fp8([(d_kv, (wk32, wv32))]).to(emb_dt)
+            d_emb = ctx.blocks.project_grad(None, None, d_kv).to(emb_dt)
             d_hist_in = d_full[:h0].reshape(h0, hc, n).to(hist_dt) if need_hist else None
             return (d_emb, d_hidden.to(hidden_dt) if d_hidden is not None else None, None, None, None, None, None,
-                    None, d_hist_in, None, None, None, None, None)
+                    None, d_hist_in, None, None, None, None, None, None)
         d_key = torch.empty((t_len, c_dim), **f32) if (need_emb and not detach_gate) else None
         d_value = torch.empty((t_len, n), **f32) if (need_emb and not detach_value) else None
         if d_key is not None or d_value is not None or d_hidden is not None:
@@ -780,11 +791,13 @@ class _PleFn(torch.autograd.Function):
             # the projections' backward, d_emb = d_key w_key + d_value w_value, as
             # products with the weights' transposes (kept between steps)
             parts = [(d, w) for d, w in ((d_key, wk32), (d_value, wv32)) if d is not None]
-            if parts:  # none: both factors detached, emb has no path to the output
+            if parts and ctx.gemm == "fp8":
+                d_emb = ctx.blocks.project_grad(d_key, d_value).to(emb_dt)
+            elif parts:  # none: both factors detached, emb has no path to the output
                 d_emb = _projection_backward(ctx.gemm, parts).to(emb_dt)
         d_hist_in = d_full[:h0].reshape(h0, hc, n).to(hist_dt) if need_hist else None
         return (d_emb, d_hidden.to(hidden_dt) if d_hidden is not None else None, None, None, None, None, None, None,
-                d_hist_in, None, None, None, None, None)
+                d_hist_in, None, None, None, None, None, None)
 
 
     @staticmethod
@@ -831,9 +844,9 @@ class _PleFn(torch.autograd.Function):
         d_emb = None
         if need_emb:
             parts = [(d, w) for d, w in ((d_key, wk32), (d_value, wv32)) if d is not None]
-            if both and ctx.gemm == "fp8":
-                parts = [(d_kv, (wk32, wv32))]
-            if parts:  # none: both factors detached, emb has no path to the output
+            if parts and ctx.gemm == "fp8":
+                d_emb = ctx.blocks.project_grad(d_key, d_value, d_kv if both else None).to(emb_dt)
+            elif parts:  # none: both factors detached, emb has no path to the output
                 d_emb = _projection_backward(ctx.gemm, parts).to(emb_dt)
         wdt = ctx.w_dtypes
         # the projection weights' gradients d_key^T emb and d_value^T emb (K = the positions); a
@@ -870,12 +883,12 @@ class _PleFn(torch.autograd.Function):
             d_cv = outs[3].to(wdt[5]) if need_cv else None
         d_hist_in = d_full[:h0].reshape(h0, hc, n).to(hist_dt) if need_hist else None
         return (d_emb, d_hidden.to(hidden_dt) if d_hidden is not None else None, d_wk, d_wv, d_nk, d_nq, d_nc, d_cv,
-                d_hist_in, None, None, None, None, None)
+                d_hist_in, None, None, None, None, None, None)
 
 
 def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w: PleWeights, hist: torch.Tensor, hparams,
                 diag: dict | None = None, detach_value: bool = False, detach_gate: bool = False,
-                gemm: str = "bf16x6") -> tuple[torch.Tensor, torch.Tensor]:
+                gemm: str = "bf16x6", blocks: PleBlocks | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``(hidden + gated + conv_out, new history)`` (``engraft/replica/layers.py:
     565-626``).  ``emb [T, n_embd]``, ``hidden [T, hc, n_embd]``, ``hist``
     ``[rows, hc, n_embd]`` (at most ``(K-1)*ple_ngram_size`` rows, empty at a
@@ -891,22 +904,40 @@ def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w: PleWeights, hist: to
     runs ``eg_gemm_f32_rows``.  ``"fp8"``: both projections on 8-bit blocks
     (``fp8.product``; 4 significant bits an operand, fp32 sums), for serving a block from a
     quarter of its weights' bytes and training rows through it: the forward and
-    ``d_emb`` take the blocks of ``emb``, of ``d_key`` and ``d_value``, and of the weights, which are kept between calls;
-    the weights' own gradients are those of the rounded block's products, in fp32
+    ``d_emb`` take the blocks of ``emb``, of ``d_key`` and ``d_value``, and of the weights: ``blocks``, which
+    :func:`quantize_projections` made of them (``w.w_key`` and ``w.w_value`` are not read then and may be None), or
+    taken in the call.  The weights' own gradients are those of the rounded block's products, in fp32
     accuracy from unrounded operands."""
     if gemm not in ("fp32", "bf16x3", "bf16x6", "fp8"):
         raise ValueError(f"gemm must be 'fp32', 'bf16x3', 'bf16x6' or 'fp8', got {gemm!r}")
     hc = hparams.hc_mult
     n = hparams.n_embd
+    if blocks is not None:
+        if gemm != "fp8":
+            raise ValueError(f"blocks are for gemm='fp8', got {gemm!r}")
+        if (blocks.n_key, blocks.n_value, blocks.parts[0].k) != (hc * n, n, n):
+            raise ValueError(f"blocks of [{hc * n}, {n}] and [{n}, {n}] weights expected, got [{blocks.n_key}, "
+                             f"{blocks.parts[0].k}] and [{blocks.n_value}, {blocks.parts[0].k}]")
+        if blocks.parts[0].q_t is None and emb.requires_grad and torch.is_grad_enabled():
+            raise ValueError("emb's gradient needs the weights' transposes: quantize_projections(w, transpose=True)")
+    elif w.w_key is None or w.w_value is None:
+        raise ValueError("w_key and w_value, or their blocks, expected")
     eps = float(hparams.f_norm_rms_eps)
     dil = int(hparams.ple_ngram_size)
     if hidden.dim() != 3 or hidden.shape[1:] != (hc, n) or emb.shape != (hidden.shape[0], n):
         raise ValueError(f"emb [T, {n}] and hidden [T, {hc}, {n}] expected, got {tuple(emb.shape)}, "
                          f"{tuple(hidden.shape)}")
+    if gemm == "fp8" and torch.is_grad_enabled():
+        by_weight = any(x is not None and x.requires_grad for x in (w.w_key, w.w_value, w.norm_key, w.norm_query, w.norm_conv, w.conv1d))
+        if ((by_weight or emb.requires_grad or hidden.requires_grad or hist.requires_grad)
+                and not _native_backward_ok(hc, n, w.conv1d.shape[1], dil, weights=by_weight)):
+            raise ValueError(f"gemm='fp8' has gradients up to 4 streams, n_embd 4096, a convolution reaching back 32 rows and, "
+                             f"for the weights', {WGRAD_MAX_TAPS} taps, got {hc} streams, n_embd {n}, {w.conv1d.shape[1]} taps "
+                             f"at dilation {dil}")
     hist = hist.reshape(-1, hc, n) if hist.numel() else hidden.new_zeros((0, hc, n))
     out, new_hist, s, gate, value = _PleFn.apply(emb, hidden, w.w_key, w.w_value, w.norm_key, w.norm_query,
                                                  w.norm_conv, w.conv1d, hist, eps, dil, detach_value, detach_gate,
-                                                 gemm)
+                                                 gemm, blocks)
     if diag is not None:
         gated_norm = value.norm(dim=-1, keepdim=True) * gate.abs()
         diag["s"] = s.clone()

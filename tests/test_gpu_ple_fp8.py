@@ -99,8 +99,28 @@ def test_gradients_of_rounded_factors(cuda, hc, n, t, weights):
             assert float((got.double() - exact).abs().max()) <= 2e-4 * float(exact.abs().max())
 
 
+@pytest.mark.parametrize("hc,n,t", [(4, 256, 40), (2, 192, 9), (1, 100, 5)])
+@pytest.mark.parametrize("detach", [{}, {"detach_gate": True}, {"detach_value": True}])
+def test_kept_blocks(cuda, hc, n, t, detach):
+    """The same values and gradients as from the weights' own blocks, which are taken in the call; without the weights."""
+    from engraft_ngram_amd import ple
+    _, wd, emb, hidden = _setup(hc, n, t, cuda)
+    hist = torch.zeros(0, hc, n, device=cuda)
+    blocks = ple.quantize_projections(wd)
+    results = []
+    for w, kept in ((wd, None), (wd, blocks), (ple.PleWeights(**dict(vars(wd), w_key=None, w_value=None)), blocks)):
+        e, h = emb.to(cuda).requires_grad_(), hidden.to(cuda).requires_grad_()
+        out, new = ple.ple_forward(e, h, w, hist, _hp(hc, n), gemm="fp8", blocks=kept, **detach)
+        out.square().sum().backward()
+        with torch.no_grad():
+            assert torch.equal(out, ple.ple_forward(e, h, w, hist, _hp(hc, n), gemm="fp8", blocks=kept, **detach)[0])
+        results.append((out.detach(), new, e.grad, h.grad))
+    for got in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, results[0]))
+
+
 def test_weights_modified_in_place_are_taken_again(cuda):
-    """The blocks kept between calls follow the weights, and a captured call takes its own."""
+    """Without kept blocks each call takes the weights' own, a captured one at each replay."""
     from engraft_ngram_amd import ple
     w, wd, emb, hidden = _setup(4, 256, 10, cuda)
     e, h, hist = emb.to(cuda), hidden.to(cuda), torch.zeros(0, 4, 256, device=cuda)
@@ -127,3 +147,20 @@ def test_what_is_refused(cuda):
         ple.ple_forward(emb.to(cuda).requires_grad_(), hidden.to(cuda), wd, hist, _hp(5, 64), gemm="fp8")
     with pytest.raises(ValueError, match="fp8"):
         ple.ple_forward(emb.to(cuda), hidden.to(cuda), wd, hist, _hp(5, 64), gemm="int8")
+    e, h = emb.to(cuda).requires_grad_(), hidden.to(cuda)
+    with torch.no_grad():  # parameters, without a gradient
+        ple.ple_forward(e, h, wd, hist, _hp(5, 64), gemm="fp8")
+    blocks = ple.quantize_projections(wd, transpose=False)
+    ple.ple_forward(e.detach(), h, wd, hist, _hp(5, 64), gemm="fp8", blocks=blocks)
+    with pytest.raises(ValueError, match="blocks"):
+        ple.ple_forward(e.detach(), h, wd, hist, _hp(5, 64), blocks=blocks)
+    none = ple.PleWeights(**dict(vars(wd), w_key=None))
+    with pytest.raises(ValueError, match="blocks"):
+        ple.ple_forward(e.detach(), h, none, hist, _hp(5, 64), gemm="fp8")
+    _, w2, emb2, hidden2 = _setup(2, 64, 4, cuda)
+    with pytest.raises(ValueError, match="blocks"):
+        ple.ple_forward(emb2.to(cuda), hidden2.to(cuda), w2, torch.zeros(0, 2, 64, device=cuda), _hp(2, 64), gemm="fp8", blocks=blocks)
+    half = ple.quantize_projections(w2, transpose=False)
+    with pytest.raises(ValueError, match="transpose"):
+        ple.ple_forward(emb2.to(cuda).requires_grad_(), hidden2.to(cuda), w2, torch.zeros(0, 2, 64, device=cuda), _hp(2, 64),
+                        gemm="fp8", blocks=half)
