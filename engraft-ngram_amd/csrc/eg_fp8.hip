@@ -353,23 +353,32 @@ __device__ inline i32x4 pack_groups(const f32x16& v, int g) {
 // read serves at a time (one chunk of 16 consecutive rows) then touch 16 different 16-byte
 // banks.  A direct-to-LDS load fills 8 rows (1 KB).  Two stages.
 //
+// KH 2 (tiles of which one is in a CU, WN = 1): two such sets of wavefronts, each of which takes one half (64 k) of every block and
+// all of its columns; their sums meet in LDS at the end.  There are two wavefronts a SIMD to fill each other's waits, no fragment of a half is
+// read by more wavefronts than before, and four stages keep the loads of three blocks on their way: 2,047 x 2560 outputs of
+// k 10,240 take 61 us in 128 x 160 tiles, 73 in one set that is PIPED (fp32 outputs 105 either way).  Reading the
+// next block's fragments between the products as well gives nothing more.
+//
 // B's fragment is the MFMA's first operand, so that a lane's registers are consecutive columns of one row of C.
 //
 // PIPED (tiles of which two fit a CU): a block's two halves (64 k) are two sets of fragments; a set is read between
 // the MFMAs of the other one.  In the middle of block kb, once every wavefront has read all of it (the barrier),
 // the loads of block kb + 2 go out into its place, one at a time between the MFMAs of its second half.
-// Otherwise (8 wavefronts, whose second set would not fit the registers) the loads of block kb + 1 go out
+// Otherwise (256-row tiles, 8 wavefronts, whose second set would not fit the registers) the loads of block kb + 1 go out
 // at the start of block kb, and the two wavefronts of a SIMD fill each other's waits.
-template <int BM, int BN, int WM, int WN, bool PIPED, bool EXACT, typename Out>
-__global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void product_kernel(const ProductArgs p) {
+template <int BM, int BN, int WM, int WN, int KH, bool PIPED, bool EXACT, typename Out>
+__global__ __launch_bounds__(WM * WN * KH * 64, WM * WN * KH / 4) void product_kernel(const ProductArgs p) {
   constexpr bool BY_ROW = sizeof(Out) == 2;
-  constexpr int NW = WM * WN, TI = BM / WM / 32, TJ = BN / WN / 32;
-  constexpr int LPW = (BM + BN) / 8 / NW;   // loads a wavefront and stage
+  constexpr int NW = WM * WN * KH, TI = BM / WM / 32, TJ = BN / WN / 32;
+  constexpr int UNITS = (BM + BN) / 8;      // loads of 8 rows a stage
+  constexpr int LPW = (UNITS + NW - 1) / NW, REST = UNITS % NW;  // of a wavefront; the last of those below REST alone
   constexpr int SPW = (BM + BN) / NW;       // rows whose scales a wavefront fetches, 64 a load
   constexpr int SL = (SPW + 63) / 64;
   constexpr int SCALES = (BM + BN) * 128;   // where a stage's scales are
   constexpr int STAGE = (BM + BN) * 132;
-  static_assert((BM / 8) % NW == 0 && (BN / 8) % NW == 0, "a wavefront's j-th load stays in one operand");
+  constexpr int STAGES = KH == 2 ? 4 : 2;
+  static_assert((BM / 8) % NW == 0 && (KH == 2 || REST == 0), "a wavefront's j-th load stays in one operand");
+  static_assert(KH == 1 || (KH == 2 && !PIPED), "halves are not pipelined");
   static_assert(BM % (32 * WM) == 0 && BN % (32 * WN) == 0 && (BM + BN) % NW == 0, "whole fragments");
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -403,15 +412,16 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void product_kernel(cons
     scale_row[i] = e < BM ? p.a_scales + ra * p.lda_scales : p.b_scales[grp] + (rb >> 7) * p.ldb_scales[grp];
   }
   auto load = [&](int kb, int j) {
+    if (REST != 0 && j == LPW - 1 && wave >= REST) return;
     const uint8_t* base = (NW * j < BM / 8 ? a0 : b0) + (int64_t)(first + kb) * 128;
-    __builtin_amdgcn_global_load_lds((const void*)(base + off[j]), (lds_void*)(lds + (kb & 1) * STAGE + (wave + NW * j) * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void*)(base + off[j]), (lds_void*)(lds + (kb & (STAGES - 1)) * STAGE + (wave + NW * j) * 1024), 16, 0, 0);
   };
   auto load_scales = [&](int kb) {
 #pragma unroll
     for (int i = 0; i < SL; ++i)
       if (i * 64 + lane < SPW)
         __builtin_amdgcn_global_load_lds((const void*)(scale_row[i] + ((first + kb) & ~3)),
-                                         (lds_void*)(lds + (kb & 1) * STAGE + SCALES + (wave * SPW + i * 64) * 4), 4, 0, 0);
+                                         (lds_void*)(lds + (kb & (STAGES - 1)) * STAGE + SCALES + (wave * SPW + i * 64) * 4), 4, 0, 0);
   };
   auto load_all = [&](int kb) {  // LPW + SL loads
     load_scales(kb);
@@ -419,7 +429,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void product_kernel(cons
     for (int j = 0; j < LPW; ++j) load(kb, j);
   };
 
-  const int wm = wave / WN, wn = wave % WN;
+  const int kh = KH == 2 ? wave / (WM * WN) : 0, wm = (wave - kh * WM * WN) / WN, wn = wave % WN;
   f32x16 acc[TI][TJ];
 #pragma unroll
   for (int i = 0; i < TI; ++i)
@@ -436,15 +446,15 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void product_kernel(cons
   const int x = (lane >> 1) & 7;
   uint32_t at[2];  // of a lane's first chunk in its row, by half; the other one is 16 away
 #pragma unroll
-  for (int h = 0; h < 2; ++h) at[h] = (lane & 31) * 128 + (((h * 4 + (lane >> 5) * 2) ^ x) << 4);
+  for (int h = 0; h < 2; ++h) at[h] = (lane & 31) * 128 + ((((KH == 2 ? kh : h) * 4 + (lane >> 5) * 2) ^ x) << 4);
   auto row_of = [&](int q) { return q < TI ? (wm * TI + q) * 32 : BM + (wn * TJ + q - TI) * 32; };
   auto read = [&](int kb, int h, int q) {
-    const uint8_t* const st = lds + (kb & 1) * STAGE + row_of(q) * 128;
+    const uint8_t* const st = lds + (kb & (STAGES - 1)) * STAGE + row_of(q) * 128;
     const i32x4 lo = *(const i32x4*)(st + at[h]), hi = *(const i32x4*)(st + (at[h] ^ 16));
     f[SETS == 2 ? h : 0][q] = i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
   auto scale_at = [&](int kb, int q) {
-    return *(const uint32_t*)(lds + (kb & 1) * STAGE + SCALES + (row_of(q) + (lane & 31)) * 4) >> (((first + kb) & 3) * 8);
+    return *(const uint32_t*)(lds + (kb & (STAGES - 1)) * STAGE + SCALES + (row_of(q) + (lane & 31)) * 4) >> (((first + kb) & 3) * 8);
   };
   constexpr int QUARTERS = EXACT ? 4 : 1, PRODUCTS = TI * TJ, STEPS = QUARTERS * PRODUCTS;
   // a half's products, with `between(t)` after the t-th of STEPS
@@ -471,7 +481,31 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void product_kernel(cons
   };
 
   load_all(0);
-  if constexpr (PIPED) {
+  if constexpr (KH == 2) {
+    if (blocks > 1) load_all(1);
+    if (blocks > 2) load_all(2);
+    constexpr int EACH = LPW + SL, LESS = EACH - (REST != 0 ? 1 : 0);
+    for (int kb = 0; kb < blocks; ++kb) {
+      // this wavefront's part of block kb is in LDS (those of the two behind it may be on their way) and its reads of block
+      // kb - 1 are in registers; after the barrier, every wavefront's are
+      if (kb + 2 < blocks) {
+        if (wave < REST || REST == 0) wait_vm<2 * EACH>(); else wait_vm<2 * LESS>();
+      } else if (kb + 1 < blocks) {
+        if (wave < REST || REST == 0) wait_vm<EACH>(); else wait_vm<LESS>();
+      } else {
+        wait_vm<0>();
+      }
+      wait_lgkm0();
+      __builtin_amdgcn_s_barrier();
+      if (kb + 3 < blocks) load_all(kb + 3);
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        sc[q] = scale_at(kb, q);
+        read(kb, 0, q);
+      }
+      half(0, [](int) {});
+    }
+  } else if constexpr (PIPED) {
     if (blocks > 1) {
       load_all(1);
       wait_vm<LPW + SL>();
@@ -547,6 +581,34 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void product_kernel(cons
 #pragma unroll
     for (int j = 0; j < TJ; ++j) asm volatile("" : "+v"(acc[i][j]));
 
+  // the halves' sums: each wavefront ends with those of a part of its columns
+  constexpr int MINE = (TJ + 1) / 2;
+  if constexpr (KH == 2) {
+    static_assert(TI * TJ * WM * WN * 4096 <= STAGES * STAGE, "the halves' sums fit LDS");
+    f32x4* const sums = (f32x4*)lds + (wave - kh * WM * WN) * (TI * TJ * 256) + lane;
+    __syncthreads();  // every wavefront has read all of its last block
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+        if ((j < MINE) != (kh == 0))
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            sums[((i * TJ + j) * 4 + r) * 64] = f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+        if ((j < MINE) == (kh == 0))
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const f32x4 t = sums[((i * TJ + j) * 4 + r) * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * r + e] += t[e];
+          }
+  }
+
   Out* const c = (Out*)p.c[grp] + piece * p.piece_stride;
   const int64_t ldc = p.ldc[grp];
   if constexpr (BY_ROW) {
@@ -558,6 +620,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void product_kernel(cons
       Out* const c_row = c + row * ldc;
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
+        if (KH == 1 || (j < MINE) == (kh == 0))
 #pragma unroll
         for (int g = 0; g < 4; g += 2) {
           typedef Out o8 __attribute__((ext_vector_type(8), aligned(2)));
@@ -578,6 +641,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void product_kernel(cons
     for (int i = 0; i < TI; ++i)
 #pragma unroll
       for (int j = 0; j < TJ; ++j) {
+        if (KH == 2 && (j < MINE) != (kh == 0)) continue;
         const int64_t col = n0 + (wn * TJ + j) * 32 + (lane & 31);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -611,17 +675,17 @@ __global__ __launch_bounds__(256) void piece_sum_kernel(const float* __restrict_
 constexpr int kFewRows = 32;  // of the few-row kernel; 33 rows of 2560 x 10240 take 8.0 us in 64 x 64 tiles, and 15.7 in four groups of 16
 constexpr int64_t kFusedBytes = 64 << 10;
 
-template <int BM, int BN, int WM, int WN, bool PIPED, bool EXACT, typename Out>
+template <int BM, int BN, int WM, int WN, int KH, bool PIPED, bool EXACT, typename Out>
 int launch_tiles(ProductArgs p, hipStream_t st) {
   p.tiles_m = (int)((p.m + BM - 1) / BM);
   p.tiles_n0 = (int)((p.n[0] + BN - 1) / BN);
   p.tiles_n = p.tiles_n0 + (int)((p.n[1] + BN - 1) / BN);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   if (tiles > INT32_MAX) return set_error(EG_ERR_UNSUPPORTED, "fp8 product: %lld tiles", (long long)tiles);
-  const auto kernel = product_kernel<BM, BN, WM, WN, PIPED, EXACT, Out>;
-  constexpr int bytes = 2 * (BM + BN) * 132;
+  const auto kernel = product_kernel<BM, BN, WM, WN, KH, PIPED, EXACT, Out>;
+  constexpr int bytes = (KH == 2 ? 4 : 2) * (BM + BN) * 132;
   EG_CHECK_HIP(allow_lds((const void*)kernel, bytes));
-  kernel<<<(unsigned)(tiles * p.pieces), WM * WN * 64, bytes, st>>>(p);
+  kernel<<<(unsigned)(tiles * p.pieces), WM * WN * KH * 64, bytes, st>>>(p);
   return launch_status("product_kernel");
 }
 
@@ -630,21 +694,25 @@ int launch_tiles(ProductArgs p, hipStream_t st) {
 struct Tile {
   int bm, bn, resident;
   float each, each_exact;
+  bool halves;  // KH 2
 };
 constexpr Tile kTiles[] = {
-    {256, 256, 1, 1.00f, 1.00f},  // fp8 437 us, bf16 816 us of 8192^3
-    {256, 320, 1, 0.92f, 0.93f},  // 507 (205 tiles of 5/4, five rounds for four), 954
-    {256, 192, 1, 1.05f, 1.00f},  // 503, 908
-    {128, 128, 2, 1.17f, 1.09f},  // 514, 887
-    {128, 160, 1, 1.50f, 1.14f},  // 678, 935
-    {64, 128, 3, 1.48f, 1.26f},   // 658, 1024
-    {64, 64, 4, 1.94f, 1.49f},    // 858, 1209
+    {256, 256, 1, 1.00f, 1.00f, false},  // fp8 437 us, bf16 816 us of 8192^3
+    {256, 320, 1, 0.92f, 0.93f, false},  // 507 (205 tiles of 5/4, five rounds for four), 954
+    {256, 192, 1, 1.05f, 1.00f, false},  // 503, 908
+    {128, 128, 2, 1.17f, 1.09f, false},  // 514, 887
+    {128, 160, 1, 1.43f, 1.37f, true},   // 623, 1080
+    {64, 128, 3, 1.48f, 1.26f, false},   // 658, 1024
+    {64, 64, 4, 1.94f, 1.49f, false},    // 858, 1209
+    {64, 160, 1, 1.97f, 1.67f, true},    // 858, 1322
 };
 
-// The tile for m x (n0, n1) outputs: the least time of the CU that gets the most tiles.  A block of a tile of four
-// wavefronts that has its CU to itself takes 14,000 outputs' time (12,000 EXACT) and 0.95 (0.8) an output: its loads' latency.
+// The tile for m x (n0, n1) outputs of `blocks` blocks of k: the least time of the CU that gets the most tiles.  A block of a tile of
+// four wavefronts of whole blocks that has its CU to itself takes 14,000 outputs' time (12,000 EXACT) and 0.95 (0.8) an output, its
+// loads' latency; a halves' tile takes 138,000 (41,000) more, for its first loads and its sums' meeting: 1,024 x 2560 outputs of
+// k 10,240 take 43.6 us (67.2) in 64 x 160 and 50.9 (75.7) in 64 x 64, of k 2560 14.9 and 14.0 (21.7 and 22.3).
 template <bool EXACT>
-int choose_tile(int64_t m, int64_t n0, int64_t n1) {
+int choose_tile(int64_t m, int64_t n0, int64_t n1, int blocks) {
   int best = 0;
   double least = 0;
   for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
@@ -652,9 +720,10 @@ int choose_tile(int64_t m, int64_t n0, int64_t n1) {
     const double area = (double)t.bm * t.bn, each = (EXACT ? t.each_exact : t.each) * area;
     const int64_t tiles = ((m + t.bm - 1) / t.bm) * ((n0 + t.bn - 1) / t.bn + (n1 + t.bn - 1) / t.bn);
     const int64_t a_cu = (tiles + kCUs - 1) / kCUs;
-    const double alone = t.bm == 256 ? 0.0 : EXACT ? 12000 + 0.8 * area : 14000 + 0.95 * area;
+    const double alone = t.bm == 256 || t.halves ? 0.0 : EXACT ? 12000 + 0.8 * area : 14000 + 0.95 * area;
+    const double once = t.halves ? (EXACT ? 41000.0 : 138000.0) / blocks : 0.0;
     auto cost = [&](int64_t count) { return count == 0 ? 0.0 : std::max(alone, count * each); };
-    const double time = (a_cu / t.resident) * cost(t.resident) + cost(a_cu % t.resident);
+    const double time = (a_cu / t.resident) * cost(t.resident) + cost(a_cu % t.resident) + a_cu * once;
     if (i == 0 || time < least) {
       best = i;
       least = time;
@@ -692,7 +761,7 @@ int launch_product(ProductArgs p, float* sums, hipStream_t st) {
     to.c[1] = sums + p.m * p.n[0];
     to.ldc[0] = p.n[0];
     to.ldc[1] = p.n[1];
-    if (const int rc = launch_tiles<64, 64, 2, 2, true, EXACT, float>(to, st); rc != EG_OK) return rc;
+    if (const int rc = launch_tiles<64, 64, 2, 2, 1, true, EXACT, float>(to, st); rc != EG_OK) return rc;
     for (int i = 0; i < 2; ++i) {
       if (p.n[i] == 0) continue;
       const int64_t groups = (p.m * ((p.n[i] + 7) / 8) + 255) / 256;
@@ -701,14 +770,15 @@ int launch_product(ProductArgs p, float* sums, hipStream_t st) {
     }
     return EG_OK;
   }
-  switch (choose_tile<EXACT>(p.m, p.n[0], p.n[1])) {
-    case 0: return launch_tiles<256, 256, 2, 4, false, EXACT, Out>(p, st);
-    case 1: return launch_tiles<256, 320, 4, 2, false, EXACT, Out>(p, st);
-    case 2: return launch_tiles<256, 192, 4, 2, false, EXACT, Out>(p, st);
-    case 3: return launch_tiles<128, 128, 2, 2, true, EXACT, Out>(p, st);
-    case 4: return launch_tiles<128, 160, 4, 1, true, EXACT, Out>(p, st);
-    case 5: return launch_tiles<64, 128, 2, 2, true, EXACT, Out>(p, st);
-    default: return launch_tiles<64, 64, 2, 2, true, EXACT, Out>(p, st);
+  switch (choose_tile<EXACT>(p.m, p.n[0], p.n[1], p.blocks)) {
+    case 0: return launch_tiles<256, 256, 2, 4, 1, false, EXACT, Out>(p, st);
+    case 1: return launch_tiles<256, 320, 4, 2, 1, false, EXACT, Out>(p, st);
+    case 2: return launch_tiles<256, 192, 4, 2, 1, false, EXACT, Out>(p, st);
+    case 3: return launch_tiles<128, 128, 2, 2, 1, true, EXACT, Out>(p, st);
+    case 4: return launch_tiles<128, 160, 4, 1, 2, false, EXACT, Out>(p, st);
+    case 5: return launch_tiles<64, 128, 2, 2, 1, true, EXACT, Out>(p, st);
+    case 6: return launch_tiles<64, 64, 2, 2, 1, true, EXACT, Out>(p, st);
+    default: return launch_tiles<64, 160, 2, 1, 2, false, EXACT, Out>(p, st);
   }
 }
 

@@ -126,6 +126,21 @@ def test_products(cuda, m, k, n, dtype, out):
     assert torch.equal(fp8.product(x, w, out_dtype=out), y)
 
 
+@pytest.mark.parametrize("m,k,n,split", [(2047, 2560, 2560, None), (1900, 2300, 2501, None), (1921, 2433, 2400, 1280),
+                                         (1024, 5248, 2560, None), (1000, 5100, 2500, 640)])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_products_of_long_rows(cuda, m, k, n, split, out):
+    """As many tiles as CUs, whose wavefronts take halves of the blocks: whole and ragged, an even and an odd number of blocks."""
+    from engraft_ngram_amd import fp8
+    g = _gen(m + k)
+    x, w = _values(g, m, k, BF16), fp8.quantize_weight(_values(g, n, k, F32, 0.02), transpose=False)
+    y = fp8.product(x, w, out_dtype=out, split=split)
+    y = torch.cat(y, 1) if split else y
+    check_product(y, O.rows(x)[0], w.dequantize().double(), out, out == F32)
+    again = fp8.product(x, w, out_dtype=out, split=split)
+    assert torch.equal(torch.cat(again, 1) if split else again, y)
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 640, 200), (24, 1000, 300), (130, 300, 700), (600, 2560, 640)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_gradient(cuda, m, k, n, dtype):
