@@ -1,13 +1,14 @@
 // The residual's addition and the RMS norm of the sum, and their gradients.
 //
 //   h = x + residual (rounded to the residual's type: what is kept is what is normed)
-//   r = 1 / sqrt(mean(h^2) + eps),   y = h r w       (in 32 bits; y in 16 or 32 bits, or in blocks of 8)
+//   r = 1 / sqrt(mean(h^2) + eps),   y = h r w       (y in 16 or 32 bits, or in blocks of 8)
 //   d_h = d_residual + r (w d_y) - h r^3 / d sum(w d_y h),   d_w = sum over rows of d_y h r
 //
 // Bound by its bytes: every row is read once, held in registers between its sum and its output, and
 // written once.  A row is w wavefronts' (1 to 16), of which each holds CH pieces of 512 values, eight
 // consecutive ones a lane: a piece is four blocks of the 8-bit output, whose largest values are found
-// within 16 lanes.  One piece a wavefront up to d = 8192 (d = 2560: five wavefronts a row): a wavefront a row
+// within 16 lanes.  A lane's eight squares are added in 32 bits, the lanes' sums and r in 64 (r's error is in all of a row's
+// values), and a value next to a border between two e4m3 numbers is 64 bits: it rounds as the exact one does.  One piece a wavefront up to d = 8192 (d = 2560: five wavefronts a row): a wavefront a row
 // of 2560 held five, and its registers left four wavefronts a SIMD, or spilled; 61 us for 8,188 rows of bf16.
 #include <algorithm>
 
@@ -42,16 +43,70 @@ __device__ inline float wave_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// The sum over a row's W wavefronts; `part`: W floats for each row of the workgroup, of the buffer that
+__device__ inline double wave_sum(double x) {
+#define EG_ROW_ADD(ror)                                                                                                           \
+  {                                                                                                                               \
+    const u32x2 b = __builtin_bit_cast(u32x2, x);                                                                                 \
+    x += __builtin_bit_cast(double, u32x2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)b[0], 0x120 + (ror), 0xf, 0xf, false),     \
+                                          (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b[1], 0x120 + (ror), 0xf, 0xf, false)});   \
+  }
+  EG_ROW_ADD(8)
+  EG_ROW_ADD(4)
+  EG_ROW_ADD(2)
+  EG_ROW_ADD(1)
+#undef EG_ROW_ADD
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// The sum over a row's W wavefronts; `part`: W values for each row of the workgroup, of the buffer that
 // this call's parity names (one barrier a call: the next one uses the other buffer).
-__device__ inline float row_sum(float x, int w, int row_of_block, int wave_of_row, float* part) {
+template <typename T>
+__device__ inline T row_sum(T x, int w, int row_of_block, int wave_of_row, T* part) {
   x = wave_sum(x);
   if (w == 1) return x;
   if ((threadIdx.x & 63) == 0) part[row_of_block * w + wave_of_row] = x;
   __syncthreads();
-  float s = 0.0f;
+  T s = 0;
+#pragma unroll 2
   for (int i = 0; i < w; ++i) s += part[row_of_block * w + i];
   return s;
+}
+
+// 1 / sqrt(a) to about 2^-50: the instruction's approximation and two steps towards it
+__device__ inline double inverse_root(double a) {
+  const double first = __builtin_amdgcn_rsq(a);
+  double r = first;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r *= 1.5 - 0.5 * a * r * r;
+  return r == r ? r : first;  // 0 and infinity, whose steps are NaN
+}
+
+// v g r as floats for the rounding to 8 bits, which round there as the exact products do.  e4m3 values and scales turn at floats
+// with 19 low bits of zeros; 32-bit products are off by 3 units of 2^-24, at most 3 last places, and those within 4
+// of such a float (1.7e-5 of all) are taken again in 64 bits, and beside it if that is where they round to (from more than
+// 2^-48 away, the products' own error).  All of them in 64 bits: 40 us for 8,188 rows of 2560 bf16, 30 so.
+__device__ inline void normed8(const float (&v)[8], const float (&g)[8], double r, float (&y)[8]) {
+  const float rf = (float)r;
+  bool near = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    y[i] = v[i] * rf * g[i];
+    near |= ((__float_as_uint(y[i]) + 4) & 0x7ffffu) <= 8 && y[i] != 0.0f;
+  }
+  if (__builtin_expect(near, 0)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x = v[i], w = g[i];
+      asm volatile("" : "+v"(x), "+v"(w));  // one value after the other: eight at once take the registers of two wavefronts
+      const double a = (double)x * (double)w * r;
+      const uint32_t bits = __float_as_uint((float)a);
+      const double d = fabs((double)(float)a);
+      const bool aside = (bits & 0x7ffffu) == 0 && fabs(d - fabs(a)) > d * 0x1p-48;
+      y[i] = __uint_as_float(!aside ? bits : d < fabs(a) ? bits + 1 : bits - 1);
+      asm volatile("" : "+v"(y[i]));
+    }
+  }
 }
 
 struct NormArgs {
@@ -61,6 +116,7 @@ struct NormArgs {
   int64_t rows;
   int d, w;                   // w: wavefronts a row
   float eps;
+  double inv_d;
   void* h;
   int64_t h_stride;
   void* y;
@@ -80,7 +136,7 @@ __device__ inline float rounded(float x) {
 // R void: no residual (h is x, and not written).
 template <typename X, typename R, int CH, bool RAGGED>
 __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
-  __shared__ float part[2][16];
+  __shared__ double part[2][16];
   constexpr bool ADD = !std::is_same<R, void>::value;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slot = wave / a.w, w = wave - slot * a.w, rows_here = (blockDim.x >> 6) / a.w;
@@ -124,31 +180,33 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) raw_g[c] = load_raw<RAGGED>(a.weight, at[c], a.d);
     }
-    float s = 0.0f;
+    double s = 0.0;
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c) {
+      float part8[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[c][i] * v[c][i];
+      for (int i = 0; i < 4; ++i) part8[i] = v[c][i] * v[c][i] + v[c][i + 4] * v[c][i + 4];
+      s += (double)((part8[0] + part8[1]) + (part8[2] + part8[3]));
+    }
     s = row_sum(s, a.w, slot, w, part[parity]);
     parity ^= 1;
-    const float rstd = 1.0f / sqrtf(s / (float)a.d + a.eps);
+    const double root = inverse_root(s * a.inv_d + (double)a.eps);
+    const float rstd = (float)root;
     if (!live) continue;
     if (a.rstd != nullptr && w == 0 && lane == 0) a.rstd[row] = rstd;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       if constexpr (ADD) store8((R*)a.h + row * a.h_stride + at[c], left[c], v[c]);
-      float y[8];
+      float y[8], g[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = v[c][i] * rstd;
-      if (weighted) {
-        float g[8];
-        values_of<RAGGED, float>(raw_g[c], at[c], a.d, g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] *= g[i];
-      }
+      for (int i = 0; i < 8; ++i) g[i] = 1.0f;
+      if (weighted) values_of<RAGGED, float>(raw_g[c], at[c], a.d, g);
       if (a.y_dtype >= 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = v[c][i] * rstd * g[i];
         store8_any(a.y, a.y_dtype, row * a.y_stride + at[c], left[c], y);
       } else {
+        normed8(v[c], g, root, y);
         const int piece = c * a.w + w;
         if (piece * 4 < blocks)
           store_blocks(y, (uint8_t*)a.y + row * a.y_stride, a.scales + row * a.scale_stride, piece, blocks, lane);
@@ -376,7 +434,7 @@ int eg_add_rms_norm(const eg_norm* o, void* h, int64_t h_stride, void* y, int32_
   const int at_once = rows_at_once(s.w, 4), threads = at_once * s.w * 64;
   const int64_t groups = std::min<int64_t>((o->rows + at_once - 1) / at_once, 1 << 20);
   const NormArgs a = {{o->x, o->x_dtype}, {o->residual, o->r_dtype}, o->weight, o->x_stride, o->r_stride, o->rows,
-                      (int)o->d, s.w, o->eps, h, h_stride, y8 ? y8->q : y, y8 ? -1 : y_dtype, y8 ? y8->stride : y_stride,
+                      (int)o->d, s.w, o->eps, 1.0 / (double)o->d, h, h_stride, y8 ? y8->q : y, y8 ? -1 : y_dtype, y8 ? y8->stride : y_stride,
                       y8 ? y8->scales : nullptr, y8 ? y8->scale_stride : 0, rstd};
   auto launch = [&](auto x, auto r) {
     using X = decltype(x);

@@ -896,7 +896,7 @@ typedef struct eg_norm {
 } eg_norm;
 
 /* h = x + residual, rounded to the residual's type (without a residual h is x and not written);
- * y = h w / sqrt(mean(h^2) + eps) in 32 bits, written as y (y_dtype) or in blocks as y8 (eg_fp8_quantize's):
+ * y = h w / sqrt(mean(h^2) + eps), the root in 64 bits, written as y (y_dtype) or in blocks as y8 (eg_fp8_quantize's):
  * one of the two.  rstd f32 [rows] (NULL: not wanted): 1 / sqrt(...), for the gradient.  h may be in
  * the place of x or of the residual; any other overlap is refused.  d up to 20,480. */
 int eg_add_rms_norm(const eg_norm* norm, void* h, int64_t h_stride, void* y, int32_t y_dtype, int64_t y_stride,

@@ -253,3 +253,21 @@ def test_graphs(cuda):
         e_y, e_h, e_rstd = norm.add_rms_norm_stats(x, res, w)
         e = norm.add_rms_norm_grad(d_y, e_h, e_rstd, w)
         assert torch.equal(y, e_y) and torch.equal(h, e_h) and torch.equal(d_h, e[0]) and torch.equal(d_w, e[1])
+
+
+@pytest.mark.parametrize("value", [1.0, 3.0, 5.0, 7.0, 11.0, 0.375, -13.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [2560, 1000])
+def test_blocks_round_as_the_exact_rows(cuda, value, dtype, d):
+    """Rows of one value are the weight itself (times its sign), however 1 / value rounds: weights on the borders between
+    two e4m3 numbers, the floats beside them, and blocks whose largest is 448 2^e or the float behind it."""
+    from engraft_ngram_amd import fp8, norm
+    g = torch.Generator().manual_seed(3)
+    w = (torch.randint(16, 32, (d,), generator=g) / 16) * 2.0 ** torch.randint(-3, 3, (d,), generator=g)
+    w[::128] = 1.75 * 2.0 ** torch.randint(3, 5, (w[::128].numel(),), generator=g)
+    bits = w.view(torch.int32) + torch.randint(-1, 2, (d,), generator=g, dtype=torch.int32)
+    w = (bits.view(torch.float32) * (1 - 2 * torch.randint(0, 2, (d,), generator=g))).to(cuda)
+    y = norm.rms_norm(torch.full((5, d), value, dtype=dtype, device=cuda), w, eps=0.0, out_dtype="fp8")
+    want = fp8.quantize_rows((w if value > 0 else -w).expand(5, d).contiguous())
+    assert torch.equal(y.q.view(torch.uint8), want.q.view(torch.uint8))
+    assert torch.equal(y.scales.view(torch.uint8), want.scales.view(torch.uint8))
