@@ -453,8 +453,13 @@ __global__ __launch_bounds__(WM * WN * KH * 64, WM * WN * KH / 4) void product_k
     const i32x4 lo = *(const i32x4*)(st + at[h]), hi = *(const i32x4*)(st + (at[h] ^ 16));
     f[SETS == 2 ? h : 0][q] = i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  auto scale_at = [&](int kb, int q) {
-    return *(const uint32_t*)(lds + (kb & (STAGES - 1)) * STAGE + SCALES + (row_of(q) + (lane & 31)) * 4) >> (((first + kb) & 3) * 8);
+  // the dword of four blocks' scales; shifted to the block's own when it is used, so that a read between products is not waited for
+  auto scales_at = [&](int kb, int q) {
+    return *(const uint32_t*)(lds + (kb & (STAGES - 1)) * STAGE + SCALES + (row_of(q) + (lane & 31)) * 4);
+  };
+  auto take_scales = [&](int kb) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) sc[q] = next_sc[q] >> (((first + kb) & 3) * 8);
   };
   constexpr int QUARTERS = EXACT ? 4 : 1, PRODUCTS = TI * TJ, STEPS = QUARTERS * PRODUCTS;
   // a half's products, with `between(t)` after the t-th of STEPS
@@ -500,9 +505,10 @@ __global__ __launch_bounds__(WM * WN * KH * 64, WM * WN * KH / 4) void product_k
       if (kb + 3 < blocks) load_all(kb + 3);
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
-        sc[q] = scale_at(kb, q);
+        next_sc[q] = scales_at(kb, q);
         read(kb, 0, q);
       }
+      take_scales(kb);
       half(0, [](int) {});
     }
   } else if constexpr (PIPED) {
@@ -516,8 +522,9 @@ __global__ __launch_bounds__(WM * WN * KH * 64, WM * WN * KH / 4) void product_k
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       read(0, 0, q);
-      sc[q] = scale_at(0, q);
+      next_sc[q] = scales_at(0, q);
     }
+    take_scales(0);
     // a fragment's reads after each of the first products
     constexpr int PER = (Q + STEPS - 1) / STEPS;
     auto reads_at = [&](int t, auto one) {
@@ -541,7 +548,7 @@ __global__ __launch_bounds__(WM * WN * KH * 64, WM * WN * KH / 4) void product_k
         __builtin_amdgcn_sched_barrier(0);
         reads_at(t, [&](int q) {
           read(kb + 1, 0, q);
-          next_sc[q] = scale_at(kb + 1, q);
+          next_sc[q] = scales_at(kb + 1, q);
         });
         if (more) {
           if (t == 0) load_scales(kb + 2);
@@ -552,8 +559,7 @@ __global__ __launch_bounds__(WM * WN * KH * 64, WM * WN * KH / 4) void product_k
         }
         __builtin_amdgcn_sched_barrier(0);
       });
-#pragma unroll
-      for (int q = 0; q < Q; ++q) sc[q] = next_sc[q];
+      take_scales(kb + 1);
     }
     half(0, [&](int t) { reads_at(t, [&](int q) { read(blocks - 1, 1, q); }); });
     half(1, [](int) {});
@@ -566,7 +572,8 @@ __global__ __launch_bounds__(WM * WN * KH * 64, WM * WN * KH / 4) void product_k
       __builtin_amdgcn_s_barrier();
       if (kb + 1 < blocks) load_all(kb + 1);
 #pragma unroll
-      for (int q = 0; q < Q; ++q) sc[q] = scale_at(kb, q);
+      for (int q = 0; q < Q; ++q) next_sc[q] = scales_at(kb, q);
+      take_scales(kb);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
