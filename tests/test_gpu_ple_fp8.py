@@ -119,6 +119,49 @@ def test_kept_blocks(cuda, hc, n, t, detach):
         assert all(torch.equal(a, b) for a, b in zip(got, results[0]))
 
 
+def test_no_positions(cuda):
+    from engraft_ngram_amd import ple
+    _, wd, _, _ = _setup(2, 128, 1, cuda)
+    for blocks in (None, ple.quantize_projections(wd)):
+        e = torch.zeros(0, 128, device=cuda, requires_grad=True)
+        h = torch.zeros(0, 2, 128, device=cuda, requires_grad=True)
+        hist = torch.randn(9, 2, 128, device=cuda, requires_grad=True)
+        out, new = ple.ple_forward(e, h, wd, hist, _hp(2, 128), gemm="fp8", blocks=blocks)
+        assert out.shape == (0, 2, 128) and torch.equal(new, hist)
+        (out.sum() + new.sum()).backward()
+        assert e.grad.shape == (0, 128) and torch.equal(hist.grad, torch.ones_like(hist))
+
+
+def test_kept_blocks_captured(cuda):
+    """A step with kept blocks, forward and gradient, replayed on other inputs beside eager work."""
+    from engraft_ngram_amd import ple
+    _, wd, emb, hidden = _setup(4, 256, 70, cuda)
+    blocks = ple.quantize_projections(wd)
+    w = ple.PleWeights(**dict(vars(wd), w_key=None, w_value=None))
+    hist = torch.zeros(0, 4, 256, device=cuda)
+    e, h = emb.to(cuda), hidden.to(cuda)
+
+    def step():
+        x = e.detach().requires_grad_()
+        out, _ = ple.ple_forward(x, h, w, hist, _hp(4, 256), gemm="fp8", blocks=blocks)
+        return out.detach(), torch.autograd.grad(out, x, torch.ones_like(out))[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for i in range(3):
+        e.add_(0.01 * (i + 1))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))
+
+
 def test_weights_modified_in_place_are_taken_again(cuda):
     """Without kept blocks each call takes the weights' own, a captured one at each replay."""
     from engraft_ngram_amd import ple
