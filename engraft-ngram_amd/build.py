@@ -53,7 +53,7 @@ def ext_command(out: Path) -> list[str]:
     cmd += ["-o", str(out), *map(str, EXT_SOURCES)]
     for lib_dir in cpp_extension.library_paths():
         cmd += ["-L", lib_dir, f"-Wl,-rpath,{lib_dir}"]
-    return cmd + ["-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    return cmd + ["-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"]
 
 
 def build(verbose: bool = False) -> Path:

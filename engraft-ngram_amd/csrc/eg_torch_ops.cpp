@@ -4,6 +4,7 @@
 // step of 16 matrices) of interpreter time, more than the kernels of a small one.
 // Host code only, in the autograd module; the entry points are the library's own,
 // handed over as addresses.
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
@@ -358,6 +359,11 @@ void muon(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, c
 
 // ---- products of 8-bit blocks --------------------------------------------------------------------
 
+// torch::empty on like's GPU, without the dispatcher's way there (0.3 us of 1.1)
+Tensor fresh(at::IntArrayRef sizes, torch::ScalarType type, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
 std::optional<c10::Device> gpu_of(const Tensor& t) {
   return t.is_cuda() ? std::optional<c10::Device>(t.device()) : std::nullopt;
 }
@@ -396,8 +402,8 @@ eg_fp8_matrix blocks_of(const Tensor& q, const Tensor& scales, int64_t k, int32_
 
 std::pair<Tensor, Tensor> empty_blocks(int64_t rows, int64_t k, int64_t block_rows, const Tensor& like) {
   const int64_t blocks = (k + 127) / 128;
-  return {torch::empty({rows, blocks * 128}, like.options().dtype(torch::kFloat8_e4m3fn)),
-          torch::empty({(rows + block_rows - 1) / block_rows, (blocks + 3) / 4 * 4}, like.options().dtype(torch::kFloat8_e8m0fnu))};
+  return {fresh({rows, blocks * 128}, torch::kFloat8_e4m3fn, like),
+          fresh({(rows + block_rows - 1) / block_rows, (blocks + 3) / 4 * 4}, torch::kFloat8_e8m0fnu, like)};
 }
 
 // (q, scales)
@@ -434,7 +440,7 @@ Tensor fp8_dequantize(const Tensor& q, const Tensor& scales, int64_t k, int64_t 
   const at::AutoDispatchBelowADInplaceOrView no_autograd;
   const c10::OptionalDeviceGuard on(gpu_of(q));
   const eg_fp8_matrix m = blocks_of(q, scales, k, (int32_t)block_rows, "blocks", q.device());
-  const Tensor out = torch::empty({m.rows, k}, q.options().dtype(type_of(dtype, "dtype")));
+  const Tensor out = fresh({m.rows, k}, type_of(dtype, "dtype"), q);
   check(g.fp8_dequantize(&m, rows_of(out, m.rows), (int32_t)dtype, k, (void*)stream));
   return out;
 }
@@ -460,7 +466,7 @@ Outputs outputs(int64_t m, const eg_fp8_matrix& w, int64_t split, int64_t dtype,
     o.b[1].scales = w.scales + split / 128 * w.scale_stride;
   }
   for (int i = 0; i < (o.two ? 2 : 1); ++i) {
-    o.y.push_back(torch::empty({m, o.b[i].rows}, like.options().dtype(type_of(dtype, "out_dtype"))));
+    o.y.push_back(fresh({m, o.b[i].rows}, type_of(dtype, "out_dtype"), like));
     o.at[i] = o.y[i].numel() > 0 ? o.y[i].data_ptr() : nullptr;
     o.ld[i] = o.b[i].rows;
   }
@@ -476,7 +482,7 @@ std::vector<Tensor> fp8_linear(const Tensor& x_, const Tensor& q, const Tensor& 
   Outputs o = outputs(x.size(0), w, split, dtype, x);
   const int64_t need = g.fp8_linear_workspace(x.size(0), o.b[0].rows, o.two ? o.b[1].rows : 0, k);
   if (need < 0) refuse("a product of ", x.sizes(), " values");
-  const Tensor ws = need > 0 ? torch::empty({need}, x.options().dtype(torch::kUInt8)) : Tensor();
+  const Tensor ws = need > 0 ? fresh({need}, torch::kUInt8, x) : Tensor();
   check(g.fp8_linear(rows_of(x, x.size(0)), dtype_code(x), x.size(0), row_stride(x), &o.b[0], o.two ? &o.b[1] : nullptr, o.at[0], o.ld[0],
                      o.at[1], o.ld[1], (int32_t)dtype, need > 0 ? ws.data_ptr() : nullptr, need, (void*)stream));
   return o.y;
@@ -490,7 +496,7 @@ std::vector<Tensor> fp8_product(const Tensor& xq, const Tensor& x_scales, const 
   Outputs o = outputs(a.rows, w, split, dtype, xq);
   const int64_t need = g.fp8_product_workspace(a.rows, o.b[0].rows, o.two ? o.b[1].rows : 0, k);
   if (need < 0) refuse("a product of ", a.rows, " rows of ", k, " values");
-  const Tensor ws = need > 0 ? torch::empty({need}, xq.options().dtype(torch::kUInt8)) : Tensor();
+  const Tensor ws = need > 0 ? fresh({need}, torch::kUInt8, xq) : Tensor();
   check(g.fp8_product(&a, &o.b[0], o.two ? &o.b[1] : nullptr, o.at[0], o.ld[0], o.at[1], o.ld[1], (int32_t)dtype,
                       need > 0 ? ws.data_ptr() : nullptr, need, (void*)stream));
   return o.y;
@@ -520,8 +526,8 @@ std::tuple<Tensor, MaybeTensor, Tensor, MaybeTensor> norm(const Tensor& x_, cons
   }
   check_vector(weight, d, "weight", x.device());
   const Tensor w = weight ? weight->to(torch::kFloat32).contiguous() : Tensor();
-  const Tensor h = residual ? torch::empty({rows, d}, r.options()) : x;
-  const Tensor rstd = stats ? empty_floats(rows, x) : Tensor();
+  const Tensor h = residual ? fresh({rows, d}, r.scalar_type(), r) : x;
+  const Tensor rstd = stats ? fresh({rows}, torch::kFloat32, x) : Tensor();
   eg_norm o = {};
   o.x = rows_of(x, rows);
   o.x_dtype = dtype_code(x);
@@ -543,7 +549,7 @@ std::tuple<Tensor, MaybeTensor, Tensor, MaybeTensor> norm(const Tensor& x_, cons
     check(g.norm(&o, sum, d, nullptr, 0, 0, &y, stat, (void*)stream));
     return {q, scales, h, stats ? MaybeTensor(rstd) : std::nullopt};
   }
-  const Tensor y = torch::empty({rows, d}, x.options().dtype(type_of(dtype, "out_dtype")));
+  const Tensor y = fresh({rows, d}, type_of(dtype, "out_dtype"), x);
   check(g.norm(&o, sum, d, rows_of(y, rows), (int32_t)dtype, d, nullptr, stat, (void*)stream));
   return {y, std::nullopt, h, stats ? MaybeTensor(rstd) : std::nullopt};
 }
@@ -584,11 +590,11 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> norm_grad(const Tensor& d_y_, const
   o.rstd = rows > 0 ? (const float*)rstd.data_ptr() : nullptr;
   o.rows = rows;
   o.d = d;
-  const Tensor d_x = torch::empty({rows, d}, h.options().dtype(type_of(dtype, "the gradient's type")));
-  const Tensor d_x2 = dtype2 >= 0 ? torch::empty({rows, d}, h.options().dtype(type_of(dtype2, "the gradient's type"))) : Tensor();
-  const Tensor d_w = weight_grad ? torch::empty({d}, w.options()) : Tensor();
+  const Tensor d_x = fresh({rows, d}, type_of(dtype, "the gradient's type"), h);
+  const Tensor d_x2 = dtype2 >= 0 ? fresh({rows, d}, type_of(dtype2, "the gradient's type"), h) : Tensor();
+  const Tensor d_w = weight_grad ? fresh({d}, torch::kFloat32, w) : Tensor();
   const int64_t need = weight_grad ? g.norm_grad_workspace(rows, d) : 0;
-  const Tensor ws = need > 0 ? torch::empty({need}, h.options().dtype(torch::kUInt8)) : Tensor();
+  const Tensor ws = need > 0 ? fresh({need}, torch::kUInt8, h) : Tensor();
   check(g.norm_grad(&o, rows_of(d_x, rows), (int32_t)dtype, d, rows_of(d_x2, rows), (int32_t)dtype2, d, weight_grad ? (float*)d_w.data_ptr() : nullptr,
                     need > 0 ? ws.data_ptr() : nullptr, std::max<int64_t>(need, 0), (void*)stream));
   return {d_x, dtype2 >= 0 ? MaybeTensor(d_x2) : std::nullopt, weight_grad ? MaybeTensor(d_w.to(weight->scalar_type())) : std::nullopt};
@@ -648,9 +654,9 @@ Tensor clip(const std::vector<Tensor>& grads, const std::optional<std::vector<Te
     if (o) c.out_dtype = dtype_code(*o);
     tensors.push_back(c);
   }
-  const Tensor result = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
+  const Tensor result = fresh({}, torch::kFloat32, grads[0]);
   const int64_t need = g.clip_workspace(tensors.data(), (int64_t)tensors.size());
-  const Tensor ws = torch::empty({std::max<int64_t>(need, 16)}, grads[0].options().dtype(torch::kUInt8));
+  const Tensor ws = fresh({std::max<int64_t>(need, 16)}, torch::kUInt8, grads[0]);
   check(g.clip(tensors.data(), (int64_t)tensors.size(), (float)max_norm, (float*)result.data_ptr(), ws.data_ptr(), std::max<int64_t>(need, 0),
                (void*)stream));
   if (outs)
