@@ -8,7 +8,7 @@
 // written once.  A row is w wavefronts' (1 to 16), of which each holds CH pieces of 512 values, eight
 // consecutive ones a lane: a piece is four blocks of the 8-bit output, whose largest values are found
 // within 16 lanes.  A lane's eight squares are added in 32 bits, the lanes' sums and r in 64 (r's error is in all of a row's
-// values), and a value next to a border between two e4m3 numbers is 64 bits: it rounds as the exact one does.  One piece a wavefront up to d = 8192 (d = 2560: five wavefronts a row): a wavefront a row
+// values), and a value next to a border between two e4m3 numbers is 64 bits: it rounds as the exact one does (of 3.5 million values none or one otherwise, 2 or 3 in 32 bits).  One piece a wavefront up to d = 8192 (d = 2560: five wavefronts a row): a wavefront a row
 // of 2560 held five, and its registers left four wavefronts a SIMD, or spilled; 61 us for 8,188 rows of bf16.
 #include <algorithm>
 
