@@ -537,6 +537,15 @@ class PleBlocks:
             return fp8.product(emb, self.parts[0], split=self.n_key)
         return tuple(fp8.product(emb, w) for w in self.parts)
 
+    def transposes(self) -> list:
+        """What :meth:`project_grad` reads."""
+        return [t for w in self.parts for t in (w.q_t, w.scales_t)]
+
+    def with_transposes(self, tensors) -> "PleBlocks":
+        """The same with ``tensors`` as its :meth:`transposes`."""
+        parts = tuple(fp8.Fp8Weight(w.q, w.scales, w.k, *tensors[2 * i:2 * i + 2]) for i, w in enumerate(self.parts))
+        return PleBlocks(parts, self.n_key, self.n_value)
+
     def project_grad(self, d_key: torch.Tensor | None, d_value: torch.Tensor | None, d_kv: torch.Tensor | None = None):
         """``emb``'s gradient from those of key and value (None: 0), or from both side by side."""
         if len(self.parts) == 2:
@@ -678,8 +687,9 @@ class _PleFn(torch.autograd.Function):
             rows = full
             if gated:
                 rows = hist32.clone() if any(ctx.needs_input_grad[4:8]) else None
+            # d_emb's blocks as saved tensors: one that is written before the backward is found out
             ctx.save_for_backward(key, value, hidden32, rows, s, gate, rstd, nk32, nq32, nc32, conv32, wk32, wv32, pre,
-                                  emb_w)
+                                  emb_w, *(blocks.transposes() if blocks is not None and ctx.needs_input_grad[0] else ()))
             ctx.gated = gated
             ctx.dtypes = (emb.dtype, hidden.dtype, hist.dtype)
             ctx.w_dtypes = tuple(x.dtype if x is not None else None for x in (w_key, w_value, nk, nq, nc, conv))
@@ -717,7 +727,8 @@ class _PleFn(torch.autograd.Function):
 
     @staticmethod
     def _backward_native(ctx, d_out, d_hist):
-        key, value, hidden32, full, s, gate, rstd, nk32, nq32, nc32, conv32, wk32, wv32, pre, emb32 = ctx.saved_tensors
+        (key, value, hidden32, full, s, gate, rstd, nk32, nq32, nc32, conv32, wk32, wv32, pre, emb32,
+         *transposes) = ctx.saved_tensors
         _eps, dil, detach_value, detach_gate = ctx.cfg
         emb_dt, hidden_dt, hist_dt = ctx.dtypes
         t_len, hc, n = hidden32.shape
@@ -775,7 +786,7 @@ class _PleFn(torch.autograd.Function):
             _lib.call("eg_ple_gate_backward_kv", _lib.ptr(key), _lib.ptr(value), _lib.ptr(hidden32), _lib.ptr(nk32),
                       _lib.ptr(nq32), _lib.ptr(nc32), _lib.ptr(s), _lib.ptr(gate), _lib.ptr(rstd), _lib.ptr(d_out32),
                       _lib.ptr(d_full[h0:]), t_len, hc, n, _lib.ptr(d_kv), _lib.ptr(d_hidden), _lib.ptr(d_s), st)
-            d_emb = ctx.blocks.project_grad(None, None, d_kv).to(emb_dt)
+            d_emb = ctx.blocks.with_transposes(transposes).project_grad(None, None, d_kv).to(emb_dt)
             d_hist_in = d_full[:h0].reshape(h0, hc, n).to(hist_dt) if need_hist else None
             return (d_emb, d_hidden.to(hidden_dt) if d_hidden is not None else None, None, None, None, None, None,
                     None, d_hist_in, None, None, None, None, None, None)
@@ -792,7 +803,7 @@ class _PleFn(torch.autograd.Function):
             # products with the weights' transposes (kept between steps)
             parts = [(d, w) for d, w in ((d_key, wk32), (d_value, wv32)) if d is not None]
             if parts and ctx.gemm == "fp8":
-                d_emb = ctx.blocks.project_grad(d_key, d_value).to(emb_dt)
+                d_emb = ctx.blocks.with_transposes(transposes).project_grad(d_key, d_value).to(emb_dt)
             elif parts:  # none: both factors detached, emb has no path to the output
                 d_emb = _projection_backward(ctx.gemm, parts).to(emb_dt)
         d_hist_in = d_full[:h0].reshape(h0, hc, n).to(hist_dt) if need_hist else None
@@ -809,7 +820,8 @@ class _PleFn(torch.autograd.Function):
         and ``eg_ple_weight_grads`` for the norms and the convolution
         (``eg_ple_weight_sums`` on the partial sums ``sums`` that the convolution's
         backward began)."""
-        key, value, hidden32, full, s, gate, rstd, nk32, nq32, nc32, conv32, wk32, wv32, pre, emb32 = ctx.saved_tensors
+        (key, value, hidden32, full, s, gate, rstd, nk32, nq32, nc32, conv32, wk32, wv32, pre, emb32,
+         *transposes) = ctx.saved_tensors
         _eps, dil, detach_value, detach_gate = ctx.cfg
         emb_dt, hidden_dt, hist_dt = ctx.dtypes
         t_len, hc, n = hidden32.shape
@@ -845,7 +857,7 @@ class _PleFn(torch.autograd.Function):
         if need_emb:
             parts = [(d, w) for d, w in ((d_key, wk32), (d_value, wv32)) if d is not None]
             if parts and ctx.gemm == "fp8":
-                d_emb = ctx.blocks.project_grad(d_key, d_value, d_kv if both else None).to(emb_dt)
+                d_emb = ctx.blocks.with_transposes(transposes).project_grad(d_key, d_value, d_kv if both else None).to(emb_dt)
             elif parts:  # none: both factors detached, emb has no path to the output
                 d_emb = _projection_backward(ctx.gemm, parts).to(emb_dt)
         wdt = ctx.w_dtypes
