@@ -7,8 +7,8 @@
 // Bound by its bytes: every row is read once, held in registers between its sum and its output, and
 // written once.  A row is w wavefronts' (1 to 16), of which each holds CH pieces of 512 values, eight
 // consecutive ones a lane: a piece is four blocks of the 8-bit output, whose largest values are found
-// within 16 lanes.  A lane's eight squares are added in 32 bits, the lanes' sums and r in 64 (r's error is in all of a row's
-// values), and a value next to a border between two e4m3 numbers is 64 bits: it rounds as the exact one does (of 3.5 million values none or one otherwise, 2 or 3 in 32 bits).  One piece a wavefront up to d = 8192 (d = 2560: five wavefronts a row): a wavefront a row
+// within 16 lanes.  A lane's eight squares are added in 32 bits (in 64 where they leave its range), the lanes' sums and r in 64
+// (r's error is in all of a row's values), and a value next to a border between two e4m3 numbers is 64 bits: it rounds as the exact one does (of 3.5 million values none or one otherwise, 2 or 3 in 32 bits).  One piece a wavefront up to d = 8192 (d = 2560: five wavefronts a row): a wavefront a row
 // of 2560 held five, and its registers left four wavefronts a SIMD, or spilled; 61 us for 8,188 rows of bf16.
 #include <algorithm>
 
@@ -85,10 +85,10 @@ __device__ inline double inverse_root(double a) {
 // v g r as floats for the rounding to 8 bits, which round there as the exact products do.  e4m3 values and scales turn at floats
 // with 19 low bits of zeros; 32-bit products are off by 3 units of 2^-24, at most 3 last places, and those within 4
 // of such a float (1.7e-5 of all) are taken again in 64 bits, and beside it if that is where they round to (from more than
-// 2^-48 away, the products' own error).  All of them in 64 bits: 40 us for 8,188 rows of 2560 bf16, 30 so.
-__device__ inline void normed8(const float (&v)[8], const float (&g)[8], double r, float (&y)[8]) {
+// 2^-48 away, the products' own error).  `wide`: all in 64 bits, where r is no normal 32-bit number.  All of them in 64 bits: 40 us for 8,188 rows of 2560 bf16, 30 so.
+__device__ inline void normed8(const float (&v)[8], const float (&g)[8], double r, bool wide, float (&y)[8]) {
   const float rf = (float)r;
-  bool near = false;
+  bool near = wide;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     y[i] = v[i] * rf * g[i];
@@ -107,6 +107,12 @@ __device__ inline void normed8(const float (&v)[8], const float (&g)[8], double 
       asm volatile("" : "+v"(y[i]));
     }
   }
+}
+
+// Whether a mean of squares that were added in 32 bits (eight of them) may be far off: infinite (or NaN), or below 2^-120,
+// where the squares' own roundings, up to 2^-150 each, reach 2^-30 of it.  From its sign and exponent.
+__device__ inline bool leaves_32(double mean) {
+  return __builtin_bit_cast(u32x2, mean)[1] - ((1023u - 120u) << 20) >= (0x7ffu - (1023u - 120u)) << 20;
 }
 
 struct NormArgs {
@@ -133,9 +139,9 @@ __device__ inline float rounded(float x) {
   return (float)(T)x;
 }
 
-// R void: no residual (h is x, and not written).
+// R void: no residual (h is x, and not written).  96 scalar registers: with more a SIMD holds seven wavefronts, not eight.
 template <typename X, typename R, int CH, bool RAGGED>
-__global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
+__global__ __launch_bounds__(1024) __attribute__((amdgpu_num_sgpr(96))) void norm_kernel(const NormArgs a) {
   __shared__ double part[2][16];
   constexpr bool ADD = !std::is_same<R, void>::value;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -189,8 +195,36 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
       s += (double)((part8[0] + part8[1]) + (part8[2] + part8[3]));
     }
     s = row_sum(s, a.w, slot, w, part[parity]);
+    const double eps = (double)a.eps;
+    double mean = fma(s, a.inv_d, eps);
+    // Such a row's squares are added again in 64 bits; the other rows keep their sums.  Where rows share a workgroup's barrier,
+    // every wavefront finds out the same of all of them, from the same sums.
+    const bool wide = __builtin_amdgcn_readfirstlane((int)leaves_32(mean)) != 0;
+    bool again = wide;
+    if (a.w > 1 && rows_here > 1) {
+      again = false;
+      for (int k = 0; k < rows_here; ++k) {
+        double sum = 0.0;
+        for (int i = 0; i < a.w; ++i) sum += part[parity][k * a.w + i];
+        again |= leaves_32(fma(sum, a.inv_d, eps));
+      }
+    }
     parity ^= 1;
-    const double root = inverse_root(s * a.inv_d + (double)a.eps);
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane((int)again) != 0, 0)) {
+      s = 0.0;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float x = v[c][i];
+          asm volatile("" : "+v"(x));
+          s += (double)x * (double)x;
+        }
+      s = row_sum(s, a.w, slot, w, part[parity]);
+      parity ^= 1;
+      if (wide) mean = fma(s, a.inv_d, eps);
+    }
+    const double root = inverse_root(mean);
     const float rstd = (float)root;
     if (!live) continue;
     if (a.rstd != nullptr && w == 0 && lane == 0) a.rstd[row] = rstd;
@@ -201,12 +235,15 @@ __global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) g[i] = 1.0f;
       if (weighted) values_of<RAGGED, float>(raw_g[c], at[c], a.d, g);
-      if (a.y_dtype >= 0) {
+      if (a.y_dtype >= 0 && !wide) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = v[c][i] * rstd * g[i];
+      } else {
+        normed8(v[c], g, root, wide, y);
+      }
+      if (a.y_dtype >= 0) {
         store8_any(a.y, a.y_dtype, row * a.y_stride + at[c], left[c], y);
       } else {
-        normed8(v[c], g, root, y);
         const int piece = c * a.w + w;
         if (piece * 4 < blocks)
           store_blocks(y, (uint8_t*)a.y + row * a.y_stride, a.scales + row * a.scale_stride, piece, blocks, lane);
