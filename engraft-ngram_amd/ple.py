@@ -522,14 +522,29 @@ WGRAD_MAX_TAPS = 8  # eg_ple_weight_grads' built tap counts (1..8)
 SUMS_MAX_ROWS = 65535 * 63  # eg_ple_conv_backward_sums' rows: one grid row per 63 of them
 
 
+def _place(w: torch.Tensor) -> tuple:
+    """Where a tensor's values are, and at which version (inference tensors have none)."""
+    return None if w.is_inference() else w._version, w.data_ptr(), w.shape, w.stride()
+
+
 class PleBlocks:
     """Both projections' weights in 8-bit blocks, for ``ple_forward(gemm="fp8", blocks=...)``: ``parts``, the key's and the
-    value's :class:`fp8.Fp8Weight`, or one of the value's rows below the key's where they begin a block."""
+    value's :class:`fp8.Fp8Weight`, or one of the value's rows below the key's where they begin a block.  ``of``: the
+    weights that they were made of, as weak references and places."""
 
-    __slots__ = ("parts", "n_key", "n_value")
+    __slots__ = ("parts", "n_key", "n_value", "of")
 
-    def __init__(self, parts: tuple, n_key: int, n_value: int):
-        self.parts, self.n_key, self.n_value = parts, n_key, n_value
+    def __init__(self, parts: tuple, n_key: int, n_value: int, of: tuple = ()):
+        self.parts, self.n_key, self.n_value, self.of = parts, n_key, n_value, of
+
+    def check_weights(self, *ws: torch.Tensor | None) -> None:
+        """Raises ValueError for a weight (None: not given) that is not what the blocks were made of: another tensor (a
+        view of all of it is none), or one that was written since."""
+        for name, w, (ref, place) in zip(("w_key", "w_value"), ws, self.of):
+            made_of = ref()
+            if w is not None and (made_of is None or _place(w) != place or _place(made_of) != place):
+                raise ValueError(f"{name} is not the weight that the blocks were made of, or has changed since: take them again "
+                                 f"(quantize_projections), or give None in its place")
 
     def project(self, emb: torch.Tensor):
         """Key and value of ``emb``, fp32 sums."""
@@ -561,7 +576,9 @@ class PleBlocks:
 def quantize_projections(w: PleWeights, *, transpose: bool = True) -> PleBlocks:
     """The blocks of ``w``'s projections, for as long as they stay as they are; ``transpose``: with what ``emb``'s gradient
     needs (as many bytes again).  Not differentiable."""
-    return _projection_blocks(w.w_key, w.w_value, transpose)
+    blocks = _projection_blocks(w.w_key, w.w_value, transpose)
+    blocks.of = tuple((weakref.ref(x), _place(x)) for x in (w.w_key, w.w_value))
+    return blocks
 
 
 def _projection_blocks(w_key: torch.Tensor, w_value: torch.Tensor, transpose: bool) -> PleBlocks:
@@ -917,8 +934,8 @@ def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w: PleWeights, hist: to
     (``fp8.product``; 4 significant bits an operand, fp32 sums), for serving a block from a
     quarter of its weights' bytes and training rows through it: the forward and
     ``d_emb`` take the blocks of ``emb``, of ``d_key`` and ``d_value``, and of the weights: ``blocks``, which
-    :func:`quantize_projections` made of them (``w.w_key`` and ``w.w_value`` are not read then and may be None), or
-    taken in the call.  The weights' own gradients are those of the rounded block's products, in fp32
+    :func:`quantize_projections` made of them (``w.w_key`` and ``w.w_value`` are not read then and may be None; given,
+    they have to be those weights, unchanged), or taken in the call.  The weights' own gradients are those of the rounded block's products, in fp32
     accuracy from unrounded operands."""
     if gemm not in ("fp32", "bf16x3", "bf16x6", "fp8"):
         raise ValueError(f"gemm must be 'fp32', 'bf16x3', 'bf16x6' or 'fp8', got {gemm!r}")
@@ -932,6 +949,7 @@ def ple_forward(emb: torch.Tensor, hidden: torch.Tensor, w: PleWeights, hist: to
                              f"{blocks.parts[0].k}] and [{blocks.n_value}, {blocks.parts[0].k}]")
         if blocks.parts[0].q_t is None and emb.requires_grad and torch.is_grad_enabled():
             raise ValueError("emb's gradient needs the weights' transposes: quantize_projections(w, transpose=True)")
+        blocks.check_weights(w.w_key, w.w_value)
     elif w.w_key is None or w.w_value is None:
         raise ValueError("w_key and w_value, or their blocks, expected")
     eps = float(hparams.f_norm_rms_eps)
