@@ -6,7 +6,7 @@
 * ``clip_grads`` -- the same, with the tensors scaled to a norm of at most ``max_norm``.
 
 Squares are added in 64 bits, in an order that the sizes alone decide, so a norm is the same
-bits every time; nothing is synchronised or copied to the device."""
+bits every time; nothing is synchronised or copied to the device.  Neither is differentiable."""
 from __future__ import annotations
 
 import torch

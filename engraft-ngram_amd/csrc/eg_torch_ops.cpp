@@ -5,6 +5,7 @@
 // Host code only, in the autograd module; the entry points are the library's own,
 // handed over as addresses.
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/extension.h>
 
@@ -364,6 +365,12 @@ Tensor fresh(at::IntArrayRef sizes, torch::ScalarType type, const Tensor& like) 
   return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
 }
 
+// A forward-mode derivative of an input, which requires_grad does not show, would be lost.
+void no_tangent(const Tensor& t) {
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    throw std::runtime_error("forward-mode derivatives are not implemented for this operator");
+}
+
 std::optional<c10::Device> gpu_of(const Tensor& t) {
   return t.is_cuda() ? std::optional<c10::Device>(t.device()) : std::nullopt;
 }
@@ -473,7 +480,10 @@ Outputs outputs(int64_t m, const eg_fp8_matrix& w, int64_t split, int64_t dtype,
   return o;
 }
 
-std::vector<Tensor> fp8_linear(const Tensor& x_, const Tensor& q, const Tensor& scales, int64_t k, int64_t split, int64_t dtype, int64_t stream) {
+// `differentiable`: for a caller whose x may have a derivative
+std::vector<Tensor> fp8_linear(const Tensor& x_, const Tensor& q, const Tensor& scales, int64_t k, int64_t split, int64_t dtype, int64_t stream,
+                               bool differentiable) {
+  if (differentiable) no_tangent(x_);
   const at::AutoDispatchBelowADInplaceOrView no_autograd;
   const c10::OptionalDeviceGuard on(gpu_of(x_));
   const Tensor x = rows_2d(x_, "x");
@@ -509,9 +519,14 @@ void check_vector(const MaybeTensor& w, int64_t d, const char* name, const torch
     refuse(name, " must be f32, bf16 or f16 [", d, "] on ", dev, ", got ", w->scalar_type(), " ", w->sizes(), " on ", w->device());
 }
 
-// (y or its q, y's scales, h, rstd); dtype -1: blocks
+// (y or its q, y's scales, h, rstd); dtype -1: blocks; `differentiable`: for a caller whose inputs may have a derivative
 std::tuple<Tensor, MaybeTensor, Tensor, MaybeTensor> norm(const Tensor& x_, const MaybeTensor& residual, const MaybeTensor& weight, double eps,
-                                                          int64_t dtype, bool stats, int64_t stream) {
+                                                          int64_t dtype, bool stats, int64_t stream, bool differentiable) {
+  if (differentiable) {
+    no_tangent(x_);
+    if (residual) no_tangent(*residual);
+    if (weight) no_tangent(*weight);
+  }
   const at::AutoDispatchBelowADInplaceOrView no_autograd;
   const c10::OptionalDeviceGuard on(gpu_of(x_));
   const Tensor x = rows_2d(x_, "x");

@@ -91,7 +91,7 @@ def _run(x, weight: Fp8Weight, split: int, code: int):
         if x.k != weight.k:
             raise ValueError(f"x must have the weight's {weight.k} columns, got {x.k}")
         return ext.fp8_product(x.q, x.scales, weight.q, weight.scales, weight.k, split, code, _stream(x.q))
-    return ext.fp8_linear(x, weight.q, weight.scales, weight.k, split, code, _stream(x))
+    return ext.fp8_linear(x, weight.q, weight.scales, weight.k, split, code, _stream(x), True)
 
 
 class _Product(torch.autograd.Function):
@@ -118,14 +118,15 @@ class _Product(torch.autograd.Function):
 
 def _grad(d_y, q_t, scales_t, n, code) -> torch.Tensor:
     """``d_y @ w`` of 2-D rows from the transpose's blocks."""
-    return _lib.autograd_ext().fp8_linear(d_y, q_t, scales_t, n, 0, code, _stream(d_y))[0]
+    return _lib.autograd_ext().fp8_linear(d_y, q_t, scales_t, n, 0, code, _stream(d_y), False)[0]
 
 
 def product(x: torch.Tensor | Fp8Rows, weight: Fp8Weight, *, out_dtype: torch.dtype | None = None,
             split: int | None = None):
     """``x @ weight.T`` for ``x`` f32, bf16 or f16 ``[..., k]`` or :class:`Fp8Rows`, as ``out_dtype`` (``x``'s; bf16
     for Fp8Rows).  ``split``: the outputs of the weight's first ``split`` rows (a multiple of 128) and of the others
-    as two tensors.  Differentiable in ``x`` (a tensor) where the weight has its transpose."""
+    as two tensors.  Differentiable in ``x`` (a tensor) where the weight has its transpose, in reverse mode; an ``x`` with a
+    forward-mode derivative is refused."""
     code = _lib.dtype_code(out_dtype if out_dtype is not None else torch.bfloat16 if isinstance(x, Fp8Rows) else x.dtype)
     if split is not None and split < 1:
         raise ValueError(f"split must be a multiple of 128 from 128 on, got {split}")

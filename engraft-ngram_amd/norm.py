@@ -12,7 +12,7 @@ output (or any layer's) and the projections behind it.
 
 ``x`` is f32, bf16 or f16 ``[..., d]``, d up to 20,480; the residual of x's type or f32;
 the weight f32, bf16 or f16 ``[d]`` or None (1).  Eight squares are added in 32 bits, their
-sums and the root in 64, gradients in 32; rows in 8 bits round as the exact ones do, but for one value in millions.  The reference's rms norm is a torch expression
+sums and the root in 64, gradients in 32 and in reverse mode (inputs with a forward-mode derivative are refused); rows in 8 bits round as the exact ones do, but for one value in millions.  The reference's rms norm is a torch expression
 (``engraft/lens.py:282-287``), its additions are apart."""
 from __future__ import annotations
 
@@ -37,11 +37,11 @@ def _code(out_dtype, x: torch.Tensor) -> int:
     return -1 if out_dtype == "fp8" else _lib.dtype_code(x.dtype if out_dtype is None else out_dtype)
 
 
-def _forward(x, residual, weight, eps, code, stats):
+def _forward(x, residual, weight, eps, code, stats, differentiable=True):
     """``(y, h, rstd)`` of 2-D rows, y Fp8Rows for code -1."""
     if not eps >= 0.0:
         raise ValueError(f"eps must be at least 0, got {eps}")
-    y, scales, h, rstd = _lib.autograd_ext().norm(x, residual, weight, eps, code, stats, _stream(x))
+    y, scales, h, rstd = _lib.autograd_ext().norm(x, residual, weight, eps, code, stats, _stream(x), differentiable)
     return (fp8.Fp8Rows(y, scales, x.shape[1]) if code < 0 else y), h, rstd
 
 
@@ -49,7 +49,7 @@ def add_rms_norm_stats(x: torch.Tensor, residual: torch.Tensor | None, weight: t
                        out_dtype: torch.dtype | str | None = None):
     """``(y, h, rstd)`` without autograd: y of ``out_dtype`` (x's; "fp8": ``Fp8Rows``), h in the residual's type (x itself
     without one), rstd f32 ``[rows]`` for :func:`add_rms_norm_grad`.  Rows ``[n, d]``."""
-    return _forward(x, residual, weight, eps, _code(out_dtype, x), True)
+    return _forward(x, residual, weight, eps, _code(out_dtype, x), True, False)
 
 
 def add_rms_norm_grad(d_y: torch.Tensor, h: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None, *,
