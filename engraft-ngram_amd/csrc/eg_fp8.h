@@ -8,7 +8,10 @@
 #include <hip/hip_fp16.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "eg_common.h"
+#include "eg_overlap.h"
 
 namespace eg {
 
@@ -205,6 +208,32 @@ inline int check_values(const void* x, int32_t dtype, int64_t rows, int64_t cols
   EG_CHECK_ARG((uintptr_t)x % item_size(dtype) == 0, "%s: misaligned", what);
   EG_CHECK_ARG(row_stride >= cols || rows <= 1, "%s: rows of %lld values are %lld apart", what, (long long)cols,
                (long long)row_stride);
+  return EG_OK;
+}
+
+// Memory that a call reads or writes.
+struct Area {
+  Extent extent;
+  const char* name;
+};
+inline Area values_area(const void* p, int32_t dtype, int64_t rows, int64_t cols, int64_t stride, const char* name) {
+  return {Extent(p, rows, cols, stride, 1, item_size(dtype)), name};
+}
+inline Area bytes_area(const void* p, int64_t bytes, const char* name) { return {Extent(p, 1, p ? bytes : 0, bytes, 1, 1), name}; }
+inline Area blocks_area(const eg_fp8_matrix& m, const char* name) {
+  return {Extent(m.q, m.rows, (m.k + 127) / 128 * 128, m.stride, 1, 1), name};
+}
+inline Area scales_area(const eg_fp8_matrix& m, const char* name) {
+  return {Extent(m.scales, (m.rows + m.block_rows - 1) / m.block_rows, (m.k + 511) / 512 * 4, m.scale_stride, 1, 1), name};
+}
+
+// Validates that what is written shares no memory with what is read, nor with one another.
+inline int check_areas(const char* what, std::initializer_list<Area> written, std::initializer_list<Area> read) {
+  for (const Area* w = written.begin(); w != written.end(); ++w) {
+    for (const Area* x = w + 1; x != written.end(); ++x)
+      EG_CHECK_ARG(!overlap(w->extent, x->extent), "%s: %s overlaps %s", what, w->name, x->name);
+    for (const Area& x : read) EG_CHECK_ARG(!overlap(w->extent, x.extent), "%s: %s overlaps %s", what, w->name, x.name);
+  }
   return EG_OK;
 }
 

@@ -876,6 +876,18 @@ int check_product(const eg_fp8_matrix* b, const eg_fp8_matrix* b2, void* c, int6
   return EG_OK;
 }
 
+// Validates that outputs and workspace share no memory with the weights, with A (its blocks and scales, or its values) or one another.
+int check_product_areas(const ProductArgs& p, int32_t dtype, const eg_fp8_matrix& b, const eg_fp8_matrix* b2, const void* workspace,
+                        int64_t workspace_bytes, const Area& a, const Area& a_scales, const char* what) {
+  const eg_fp8_matrix none = {nullptr, nullptr, 0, 1, 0, 0, 128}, &second = b2 ? *b2 : none;
+  return check_areas(what,
+                     {values_area(p.c[0], dtype, p.m, p.n[0], p.ldc[0], "an output"),
+                      values_area(p.c[1], dtype, p.m, p.n[1], p.ldc[1], "the second output"),
+                      bytes_area(workspace, workspace_bytes, "the workspace")},
+                     {a, a_scales, blocks_area(b, "b"), scales_area(b, "b's scales"), blocks_area(second, "b2"),
+                      scales_area(second, "b2's scales")});
+}
+
 int run_product(const ProductArgs& p, int32_t dtype, float* sums, hipStream_t st) {
   if (p.m == 0 || p.n[0] == 0) return EG_OK;
   if (p.m <= 16) return launch_few<1, false, float>(p, dtype, st);
@@ -936,6 +948,10 @@ int eg_fp8_quantize(const void* x, int32_t dtype, int64_t row_stride, const eg_f
   const int blocks = (int)((out->k + 127) / 128), groups = (blocks + 3) / 4;
   const int64_t units = out->rows * groups;
   EG_CHECK_ARG((units + 3) / 4 < (1 << 24), "fp8_quantize: %lld x %lld is too large", (long long)out->rows, (long long)out->k);
+  if (const int rc = check_areas("fp8_quantize", {blocks_area(*out, "q"), scales_area(*out, "its scales")},
+                                 {values_area(x, dtype, out->rows, out->k, row_stride, "the values")});
+      rc != EG_OK)
+    return rc;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     quantize_kernel<T><<<(unsigned)((units + 3) / 4), 256, 0, (hipStream_t)stream>>>(
@@ -958,6 +974,13 @@ int eg_fp8_quantize_weight(const void* x, int32_t dtype, int64_t row_stride, int
   if (out->rows == 0) return EG_OK;
   const int64_t by = (out->rows + 127) / 128;
   EG_CHECK_ARG(by <= 65535, "fp8_quantize_weight: %lld rows", (long long)out->rows);
+  const eg_fp8_matrix none = {nullptr, nullptr, 0, 1, 0, 0, 128}, &transpose = out_t ? *out_t : none;
+  if (const int rc = check_areas("fp8_quantize_weight",
+                                 {blocks_area(*out, "q"), scales_area(*out, "its scales"), blocks_area(transpose, "the transpose"),
+                                  scales_area(transpose, "the transpose's scales")},
+                                 {{Extent(x, out->rows, out->k, row_stride, col_stride, item_size(dtype)), "the values"}});
+      rc != EG_OK)
+    return rc;
   const dim3 grid((unsigned)((out->k + 127) / 128), (unsigned)by);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -976,6 +999,10 @@ int eg_fp8_dequantize(const eg_fp8_matrix* m, void* out, int32_t dtype, int64_t 
   const int64_t count = m->rows * ((m->k + 7) / 8);
   if (count == 0) return EG_OK;
   EG_CHECK_ARG((count + 255) / 256 < (1 << 24), "fp8_dequantize: %lld x %lld is too large", (long long)m->rows, (long long)m->k);
+  if (const int rc = check_areas("fp8_dequantize", {values_area(out, dtype, m->rows, m->k, row_stride, "the output")},
+                                 {blocks_area(*m, "q"), scales_area(*m, "its scales")});
+      rc != EG_OK)
+    return rc;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     dequantize_kernel<T><<<(unsigned)((count + 255) / 256), 256, 0, (hipStream_t)stream>>>(
@@ -993,7 +1020,11 @@ int eg_fp8_product(const eg_fp8_matrix* a, const eg_fp8_matrix* b, const eg_fp8_
   if (const int rc = check_fp8(a, 1, "a"); rc != EG_OK) return rc;
   ProductArgs p;
   if (const int rc = check_product(b, b2, c, ldc, c2, ldc2, dtype, a->rows, a->k, &p); rc != EG_OK) return rc;
-  if (const int rc = check_workspace(workspace, workspace_bytes, piece_bytes(p.m, p.n[0], p.n[1], p.k), "fp8_product"); rc != EG_OK) return rc;
+  const int64_t need = piece_bytes(p.m, p.n[0], p.n[1], p.k);
+  if (const int rc = check_workspace(workspace, workspace_bytes, need, "fp8_product"); rc != EG_OK) return rc;
+  if (const int rc = check_product_areas(p, dtype, *b, b2, workspace, need, blocks_area(*a, "a"), scales_area(*a, "a's scales"), "fp8_product");
+      rc != EG_OK)
+    return rc;
   p.a = (const uint8_t*)a->q;
   p.a_scales = a->scales;
   p.lda = a->stride;
@@ -1017,6 +1048,10 @@ int eg_fp8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t x_stride, c
   if (m == 0 || p.n[0] == 0) return EG_OK;
   const int64_t k = b->k, need = eg_fp8_linear_workspace_size(m, b->rows, b2 ? b2->rows : 0, k);
   if (const int rc = check_workspace(workspace, workspace_bytes, need, "fp8_linear"); rc != EG_OK) return rc;
+  if (const int rc = check_product_areas(p, dtype, *b, b2, workspace, need, values_area(x, x_dtype, m, k, x_stride, "x"),
+                                         bytes_area(nullptr, 0, ""), "fp8_linear");
+      rc != EG_OK)
+    return rc;
   if (fused(m, k, p.n[0], p.n[1])) {
     p.x = x;
     p.ldx = x_stride;

@@ -838,7 +838,8 @@ int eg_muon_step(const eg_muon* muon, void* workspace, int64_t workspace_bytes, 
  * (e8m0).  Element (r, c) is q[r * stride + c] * 2^(scales[(r / block_rows) * scale_stride + c / 128] - 127).
  * Strides in bytes: `stride` a multiple of 16, at least k rounded up to 128; scale_stride a
  * multiple of 4, at least the blocks rounded up to 4.  q 16-byte and scales 4-byte aligned.
- * The bytes of q from k to the end of the last block are zeros. */
+ * The bytes of q from k to the end of the last block are zeros.  The calls below refuse outputs and
+ * workspaces that share memory with what they read or with one another (rows may lie between one another's). */
 typedef struct eg_fp8_matrix {
   void* q;
   uint8_t* scales;
