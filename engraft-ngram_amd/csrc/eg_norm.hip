@@ -13,7 +13,6 @@
 #include <algorithm>
 
 #include "eg_fp8.h"
-#include "eg_overlap.h"
 
 namespace eg {
 namespace {
@@ -412,13 +411,6 @@ int64_t grad_groups(int64_t rows, int w) {
   return std::min<int64_t>((rows + at_once - 1) / at_once, 512);
 }
 
-int check_apart(const void* a, int64_t rows, int64_t cols, int64_t stride, int item, const void* b, int64_t b_rows, int64_t b_cols,
-                int64_t b_stride, int b_item, const char* what) {
-  if (a == nullptr || b == nullptr || rows == 0 || b_rows == 0) return EG_OK;
-  EG_CHECK_ARG(!overlap(Extent(a, rows, cols, stride, 1, item), Extent(b, b_rows, b_cols, b_stride, 1, b_item)), "%s", what);
-  return EG_OK;
-}
-
 }  // namespace
 }  // namespace eg
 
@@ -440,33 +432,26 @@ int eg_add_rms_norm(const eg_norm* o, void* h, int64_t h_stride, void* y, int32_
   }
   EG_CHECK_ARG((uintptr_t)o->weight % 4 == 0, "add_rms_norm: misaligned weight");
   EG_CHECK_ARG((y != nullptr) != (y8 != nullptr) || o->rows == 0, "add_rms_norm: y or y8 expected");
-  const int xs = item_size(o->x_dtype);
-  int64_t out_cols = o->d, out_stride = y_stride;
-  int out_item = 1;
-  const void* out = y;
   if (y8 != nullptr) {
     if (const int rc = check_fp8(y8, 1, "add_rms_norm: y8"); rc != EG_OK) return rc;
     EG_CHECK_ARG(y8->rows == o->rows && y8->k == o->d, "add_rms_norm: y8 is %lld x %lld for %lld rows of %lld", (long long)y8->rows,
                  (long long)y8->k, (long long)o->rows, (long long)o->d);
-    out = y8->q;
-    out_cols = (o->d + 127) / 128 * 128;
-    out_stride = y8->stride;
   } else {
     if (const int rc = check_values(y, y_dtype, o->rows, o->d, y_stride, "add_rms_norm: y"); rc != EG_OK) return rc;
-    out_item = item_size(y_dtype);
   }
+  EG_CHECK_ARG((uintptr_t)rstd % 4 == 0, "add_rms_norm: misaligned rstd");
   if (o->rows == 0) return EG_OK;
-  if (const int rc = check_apart(out, o->rows, out_cols, out_stride, out_item, o->x, o->rows, o->d, o->x_stride, xs, "add_rms_norm: y overlaps x"); rc != EG_OK) return rc;
-  if (o->residual != nullptr) {
-    const int rs = item_size(o->r_dtype);
-    if (const int rc = check_apart(out, o->rows, out_cols, out_stride, out_item, o->residual, o->rows, o->d, o->r_stride, rs, "add_rms_norm: y overlaps the residual"); rc != EG_OK) return rc;
-    if (const int rc = check_apart(out, o->rows, out_cols, out_stride, out_item, h, o->rows, o->d, h_stride, rs, "add_rms_norm: y overlaps h"); rc != EG_OK) return rc;
-    // h in the place of x or of the residual: every value is read by the lane that writes it
-    if (!(h == o->residual && h_stride == o->r_stride))
-      if (const int rc = check_apart(h, o->rows, o->d, h_stride, rs, o->residual, o->rows, o->d, o->r_stride, rs, "add_rms_norm: h overlaps the residual"); rc != EG_OK) return rc;
-    if (!(h == o->x && h_stride == o->x_stride && o->x_dtype == o->r_dtype))
-      if (const int rc = check_apart(h, o->rows, o->d, h_stride, rs, o->x, o->rows, o->d, o->x_stride, xs, "add_rms_norm: h overlaps x"); rc != EG_OK) return rc;
-  }
+  const bool add = o->residual != nullptr;
+  const Area none = bytes_area(nullptr, 0, ""), x_area = values_area(o->x, o->x_dtype, o->rows, o->d, o->x_stride, "x"),
+             r_area = add ? values_area(o->residual, o->r_dtype, o->rows, o->d, o->r_stride, "the residual") : none,
+             h_area = add ? values_area(h, o->r_dtype, o->rows, o->d, h_stride, "h") : none,
+             y_area = y8 ? blocks_area(*y8, "y") : values_area(y, y_dtype, o->rows, o->d, y_stride, "y"),
+             scales = y8 ? scales_area(*y8, "y's scales") : none, rstd_area = bytes_area(rstd, o->rows * 4, "rstd"),
+             weight = bytes_area(o->weight, o->d * 4, "the weight");
+  if (const int rc = check_areas("add_rms_norm", {y_area, scales, rstd_area}, {x_area, r_area, h_area, weight}); rc != EG_OK) return rc;
+  // h in the place of x or of the residual: every value is read by the lane that writes it
+  const bool on_x = h == o->x && h_stride == o->x_stride && o->x_dtype == o->r_dtype, on_r = h == o->residual && h_stride == o->r_stride;
+  if (const int rc = check_areas("add_rms_norm", {h_area}, {on_r ? none : r_area, on_x ? none : x_area, weight}); rc != EG_OK) return rc;
   const Split s = split_of(o->d);
   const int at_once = rows_at_once(s.w, 4), threads = at_once * s.w * 64;
   const int64_t groups = std::min<int64_t>((o->rows + at_once - 1) / at_once, 1 << 20);
@@ -511,19 +496,6 @@ int eg_add_rms_norm_grad(const eg_norm_grad* o, void* d_x, int32_t dx_dtype, int
   if (d_x2 != nullptr)
     if (const int rc = check_values(d_x2, dx2_dtype, o->rows, o->d, dx2_stride, "add_rms_norm_grad: d_x2"); rc != EG_OK) return rc;
   EG_CHECK_ARG((uintptr_t)d_weight % 4 == 0, "add_rms_norm_grad: misaligned d_weight");
-  const struct {
-    const void* p;
-    int64_t stride;
-    int item;
-    const char* name;
-  } ins[3] = {{o->d_y, o->dy_stride, item_size(o->dy_dtype), "add_rms_norm_grad: a gradient overlaps d_y"},
-              {o->h, o->h_stride, item_size(o->h_dtype), "add_rms_norm_grad: a gradient overlaps h"},
-              {o->d_residual, o->dr_stride, item_size(o->h_dtype), "add_rms_norm_grad: a gradient overlaps d_residual"}};
-  for (const auto& in : ins) {
-    if (const int rc = check_apart(d_x, o->rows, o->d, dx_stride, item_size(dx_dtype), in.p, o->rows, o->d, in.stride, in.item, in.name); rc != EG_OK) return rc;
-    if (d_x2 != nullptr)
-      if (const int rc = check_apart(d_x2, o->rows, o->d, dx2_stride, item_size(dx2_dtype), in.p, o->rows, o->d, in.stride, in.item, in.name); rc != EG_OK) return rc;
-  }
   const Split s = split_of(o->d);
   const int rows_here = rows_at_once(s.w, 16), threads = rows_here * s.w * 64;
   const int64_t groups = grad_groups(o->rows, s.w);
@@ -533,6 +505,18 @@ int eg_add_rms_norm_grad(const eg_norm_grad* o, void* d_x, int32_t dx_dtype, int
                        (long long)workspace_bytes);
     EG_CHECK_ARG(groups == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "add_rms_norm_grad: the workspace must be 16-byte aligned");
   }
+  const Area none = bytes_area(nullptr, 0, "");
+  if (const int rc = check_areas("add_rms_norm_grad",
+                                 {values_area(d_x, dx_dtype, o->rows, o->d, dx_stride, "d_x"),
+                                  d_x2 ? values_area(d_x2, dx2_dtype, o->rows, o->d, dx2_stride, "d_x2") : none,
+                                  bytes_area(d_weight, o->d * 4, "d_weight"),
+                                  d_weight ? bytes_area(workspace, groups * o->d * 4, "the workspace") : none},
+                                 {values_area(o->d_y, o->dy_dtype, o->rows, o->d, o->dy_stride, "d_y"),
+                                  values_area(o->h, o->h_dtype, o->rows, o->d, o->h_stride, "h"),
+                                  o->d_residual ? values_area(o->d_residual, o->h_dtype, o->rows, o->d, o->dr_stride, "d_residual") : none,
+                                  bytes_area(o->weight, o->d * 4, "the weight"), bytes_area(o->rstd, o->rows * 4, "rstd")});
+      rc != EG_OK)
+    return rc;
   const GradArgs a = {{o->d_y, o->dy_dtype}, {o->h, o->h_dtype}, {o->d_residual, o->h_dtype}, o->weight, o->dy_stride,
                       o->h_stride, o->dr_stride, o->rstd, o->rows, (int)o->d, s.w, d_x, dx_dtype, dx_stride, d_x2, dx2_dtype, dx2_stride,
                       d_weight ? (float*)workspace : nullptr};

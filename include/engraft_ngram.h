@@ -899,7 +899,7 @@ typedef struct eg_norm {
 /* h = x + residual, rounded to the residual's type (without a residual h is x and not written);
  * y = h w / sqrt(mean(h^2) + eps), the root in 64 bits, written as y (y_dtype) or in blocks as y8 (eg_fp8_quantize's):
  * one of the two.  rstd f32 [rows] (NULL: not wanted): 1 / sqrt(...), for the gradient.  h may be in
- * the place of x or of the residual; any other overlap is refused.  d up to 20,480. */
+ * the place of x or of the residual; any other overlap of what is written is refused.  d up to 20,480. */
 int eg_add_rms_norm(const eg_norm* norm, void* h, int64_t h_stride, void* y, int32_t y_dtype, int64_t y_stride,
                     const eg_fp8_matrix* y8, float* rstd, void* stream);
 
@@ -918,7 +918,8 @@ typedef struct eg_norm_grad {
 
 /* The gradient of h (of x and of the residual alike) as d_x and, in a second type, as d_x2 (NULL: not
  * wanted), and the weight's, d_weight f32 [d] (NULL: not wanted; then no workspace either).  Sums in 32 bits, in
- * a fixed order.  Outputs must not overlap the inputs.  d up to 20,480.  Workspace 16-byte aligned. */
+ * a fixed order.  Outputs and workspace must not overlap the inputs or one another (refused).  d up to 20,480.
+ * Workspace 16-byte aligned. */
 int64_t eg_add_rms_norm_grad_workspace_size(int64_t rows, int64_t d);
 int eg_add_rms_norm_grad(const eg_norm_grad* grad, void* d_x, int32_t dx_dtype, int64_t dx_stride, void* d_x2,
                          int32_t dx2_dtype, int64_t dx2_stride, float* d_weight, void* workspace, int64_t workspace_bytes,
