@@ -35,8 +35,8 @@ def grad_norm(grads) -> torch.Tensor:
 def clip_grads(grads, max_norm: float, *, out=None) -> torch.Tensor:
     """:func:`grad_norm`'s value N, with every gradient times ``max_norm / N`` where ``N > max_norm``, in place or as
     ``out`` (tensors of the gradients' shapes, f32, bf16 or f16: all are written, clipped or not).  A norm that is not finite
-    leaves the values as they are.  A gradient given twice is refused, as are outputs that overlap
-    anything else."""
+    leaves the values as they are.  A gradient given twice (or two that share a value) is refused, as are outputs that
+    overlap anything else."""
     grads = _list(grads)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be at least 0, got {max_norm}")

@@ -3,15 +3,15 @@
 //   N = sqrt(sum over all tensors of g^2),   out = g max_norm / N where N > max_norm, g otherwise
 //
 // Bound by its bytes.  Two kinds of launch: every workgroup adds the squares of its tiles (4,096 values
-// of one tensor each, 2,048 where all tensors are small) in 64 bits, which neither overflow nor lose small tensors beside large
+// of one tensor each, 2,048 where there are less than 2^20 in all) in 64 bits, which neither overflow nor lose small tensors beside large
 // ones, and writes its sum; then every workgroup adds all of these sums (a few KB from L2, in one order) and
 // writes its tiles' values, from the last one on: what was read last is in the caches.  The
 // tensors are kernel arguments, 48 a launch, so that nothing is copied to the device.
 #include <algorithm>
+#include <string>
 #include <vector>
 
 #include "eg_fp8.h"
-#include "eg_overlap.h"
 
 namespace eg {
 namespace {
@@ -227,6 +227,20 @@ int check_tensors(const eg_clip_tensor* tensors, int64_t count) {
   return EG_OK;
 }
 
+// The first two gradients (of operands by address) that share a value, which would count twice.
+bool find_twice(const std::vector<Operand>& all, const Operand*& x, const Operand*& y) {
+  for (size_t i = 0; i < all.size(); ++i) {
+    if (all[i].kind != Operand::kGrad) continue;
+    for (size_t j = i + 1; j < all.size() && all[j].extent.at < all[i].extent.end(); ++j) {
+      if (all[j].kind != Operand::kGrad || !overlap(all[i].extent, all[j].extent)) continue;
+      x = &all[i];
+      y = &all[j];
+      return true;
+    }
+  }
+  return false;
+}
+
 }  // namespace
 }  // namespace eg
 
@@ -254,14 +268,16 @@ int eg_clip_grads(const eg_clip_tensor* tensors, int64_t count, float max_norm, 
                   int64_t workspace_bytes, void* stream) try {
   if (const int rc = check_tensors(tensors, count); rc != EG_OK) return rc;
   EG_CHECK_ARG(norm != nullptr, "clip: NULL norm");
+  EG_CHECK_ARG((uintptr_t)norm % 4 == 0, "clip: misaligned norm");
   EG_CHECK_ARG(max_norm >= 0.0f, "clip: max_norm=%g", (double)max_norm);
   const int64_t need = eg_clip_workspace_size(tensors, count);
   if (workspace_bytes < need)
     return set_error(EG_ERR_WORKSPACE, "clip needs %lld bytes of workspace, got %lld", (long long)need, (long long)workspace_bytes);
   EG_CHECK_ARG(need == 0 || (workspace != nullptr && (uintptr_t)workspace % 16 == 0), "clip: the workspace must be 16-byte aligned");
   // a tensor's output is a param here and its gradient a grad: it may be in its own gradient's place, of the
-  // same type and stride, and must not overlap anything else
-  std::vector<Operand> operands;
+  // same type and stride, and must not overlap anything else; the norm and the workspace (as momenta) must not at all
+  std::vector<Operand> operands = {{Operand::kMomentum, (size_t)count, {norm, 1, 1, 1, 1, 4}},
+                                   {Operand::kMomentum, (size_t)count + 1, {workspace, 1, need, need, 1, 1}}};
   bool scales = false;
   for (int64_t i = 0; i < count; ++i) {
     const eg_clip_tensor& t = tensors[i];
@@ -274,12 +290,13 @@ int eg_clip_grads(const eg_clip_tensor* tensors, int64_t count, float max_norm, 
     EG_CHECK_ARG(in_place || !overlap(out, operands.back().extent), "clip: output %lld overlaps its gradient and is not in its place", (long long)i);
     operands.push_back({Operand::kParam, (size_t)i, out});
   }
-  if (scales) {
-    const Operand *x, *y;
-    if (find_overlap(operands, x, y)) {
-      auto name = [](const Operand* o) { return o->kind == Operand::kParam ? "output" : "gradient"; };
-      return set_error(EG_ERR_ARG, "clip: %s %lld overlaps %s %lld", name(x), (long long)x->matrix, name(y), (long long)y->matrix);
-    }
+  const Operand *x, *y;
+  if (find_overlap(operands, x, y) || (scales && find_twice(operands, x, y))) {
+    auto name = [&](const Operand* o) -> std::string {
+      if (o->kind == Operand::kMomentum) return o->matrix == (size_t)count ? "the norm" : "the workspace";
+      return (o->kind == Operand::kParam ? "output " : "gradient ") + std::to_string(o->matrix);
+    };
+    return set_error(EG_ERR_ARG, "clip: %s overlaps %s", name(x).c_str(), name(y).c_str());
   }
   const int tile = tile_of(tensors, count);
   const bool small = tile == kThreads * 8;

@@ -941,8 +941,9 @@ typedef struct eg_clip_tensor {
 
 /* norm f32 [1] = sqrt of the sum of all squares of `count` tensors (a HOST array), added in 64 bits in a fixed
  * order; with an `out`, out = g * max_norm / norm where norm > max_norm, and g otherwise (a norm that is not
- * finite leaves the values as they are).  Either all tensors have an `out` or none.  What is written
- * must not overlap another tensor, nor its own gradient but in place (refused).  Workspace of
+ * finite leaves the values as they are).  Either all tensors have an `out` or none.  What is written (the norm and
+ * the workspace too) must not overlap another tensor, nor its own gradient but in place (refused), and with an
+ * `out` no two gradients may share a value (refused; in a norm alone it counts as often as it is given).  Workspace of
  * eg_clip_workspace_size bytes, 16-byte aligned. */
 int64_t eg_clip_workspace_size(const eg_clip_tensor* tensors, int64_t count);
 int eg_clip_grads(const eg_clip_tensor* tensors, int64_t count, float max_norm, float* norm, void* workspace,
