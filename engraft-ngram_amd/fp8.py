@@ -116,6 +116,14 @@ class _Product(torch.autograd.Function):
         return _grad(d_y, *ctx.saved_tensors, ctx.shape[1], _lib.dtype_code(ctx.dtype)), None, None, None
 
 
+def check_transpose(weight: Fp8Weight) -> None:
+    """Raises ValueError for a weight without its transpose, which the gradient of ``x`` is a product with."""
+    if weight.q_t is None or weight.scales_t is None:
+        raise ValueError("the gradient of x needs the weight's transpose: fp8.quantize_weight(w, transpose=True)")
+    if weight.q_t.shape[0] != weight.k:
+        raise ValueError(f"the transpose of a weight {list(weight.shape)} has {weight.k} rows, got {weight.q_t.shape[0]}")
+
+
 def _grad(d_y, q_t, scales_t, n, code) -> torch.Tensor:
     """``d_y @ w`` of 2-D rows from the transpose's blocks."""
     return _lib.autograd_ext().fp8_linear(d_y, q_t, scales_t, n, 0, code, _stream(d_y), False)[0]
@@ -137,8 +145,7 @@ def product(x: torch.Tensor | Fp8Rows, weight: Fp8Weight, *, out_dtype: torch.dt
         lead = x.shape[:-1]
         x = x.reshape(-1, x.shape[-1])
     if not isinstance(x, Fp8Rows) and x.requires_grad and torch.is_grad_enabled():
-        if weight.q_t is None:
-            raise ValueError("the gradient of x needs the weight's transpose: quantize_weight(w, transpose=True)")
+        check_transpose(weight)
         y = _Product.apply(x, weight, split or 0, code)
         y = list(y) if split else [y]
     else:
@@ -151,8 +158,9 @@ def product(x: torch.Tensor | Fp8Rows, weight: Fp8Weight, *, out_dtype: torch.dt
 def product_grad(d_y: torch.Tensor, weight: Fp8Weight, *, dtype: torch.dtype | None = None) -> torch.Tensor:
     """The gradient of ``x`` in ``product(x, weight)`` from ``d_y`` f32, bf16 or f16 ``[..., n]``: ``d_y @ weight``,
     as ``dtype`` (``d_y``'s)."""
-    if weight.q_t is None:
-        raise ValueError("the gradient of x needs the weight's transpose: quantize_weight(w, transpose=True)")
+    check_transpose(weight)
+    if d_y.dim() == 0:
+        raise ValueError("d_y must be [..., n]")
     code = _lib.dtype_code(dtype if dtype is not None else d_y.dtype, "dtype")
     rows = d_y if d_y.dim() == 2 else d_y.reshape(-1, d_y.shape[-1])
     d_x = _grad(rows, weight.q_t, weight.scales_t, weight.shape[0], code)

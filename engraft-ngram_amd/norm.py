@@ -166,8 +166,7 @@ def normed_product(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: 
     if x2.shape[1] != weight.k:
         raise ValueError(f"x must have the weight's {weight.k} columns, got {list(x.shape)}")
     if _differentiates(x, residual, norm_weight):
-        if weight.q_t is None:
-            raise ValueError("the gradient of x needs the weight's transpose: fp8.quantize_weight(w, transpose=True)")
+        fp8.check_transpose(weight)
         out = _NormedProduct.apply(x2, r2, norm_weight, weight, eps, code)
         y, h = (out, None) if residual is None else out
     else:
