@@ -368,6 +368,7 @@ SIGNATURES = {
     "eg_fp8_dequantize": (c_int32, [POINTER(EgFp8Matrix), c_void_p, c_int32, c_int64, c_void_p]),
     "eg_fp8_product": (c_int32, [POINTER(EgFp8Matrix), POINTER(EgFp8Matrix), POINTER(EgFp8Matrix), c_void_p, c_int64,
                                  c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
+    "eg_fp8_product_tile": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int32, POINTER(c_int32)]),
     "eg_fp8_product_workspace_size": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
     "eg_fp8_linear_workspace_size": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
     "eg_fp8_linear": (c_int32, [c_void_p, c_int32, c_int64, c_int64, POINTER(EgFp8Matrix), POINTER(EgFp8Matrix), c_void_p,

@@ -758,7 +758,7 @@ int64_t piece_bytes(int64_t m, int64_t n0, int64_t n1, int64_t k) {
 
 template <bool EXACT, typename Out>
 int launch_product(ProductArgs p, float* sums, hipStream_t st) {
-  p.pieces = pieces_of(p.m, p.n[0], p.n[1], p.blocks);
+  p.pieces = pieces_of(p.m, p.n[0], p.n[1], p.blocks);  // eg_fp8_product_tile tells of this plan
   p.per = (p.blocks + p.pieces - 1) / p.pieces;
   if (p.pieces > 1) {
     p.pieces = (p.blocks + p.per - 1) / p.per;  // none is empty
@@ -1013,6 +1013,16 @@ int eg_fp8_dequantize(const eg_fp8_matrix* m, void* out, int32_t dtype, int64_t 
 
 int64_t eg_fp8_product_workspace_size(int64_t m, int64_t n, int64_t n2, int64_t k) {
   return known_size(m, n, n2, k) ? piece_bytes(m, n, n2, k) : -1;
+}
+
+int64_t eg_fp8_product_tile(int64_t m, int64_t n, int64_t n2, int64_t k, int32_t dtype, int32_t* pieces) {
+  if (!known_size(m, n, n2, k) || !known_dtype(dtype)) return -1;
+  const int blocks = (int)((k + 127) / 128), cut = pieces_of(m, n, n2, blocks), per = (blocks + cut - 1) / cut;
+  if (pieces != nullptr) *pieces = (blocks + per - 1) / per;
+  if (m <= kFewRows || n + n2 == 0) return 0;
+  if (cut > 1) return (int64_t)64 << 16 | 64;
+  const Tile& t = kTiles[dtype == EG_DTYPE_F32 ? choose_tile<true>(m, n, n2, blocks) : choose_tile<false>(m, n, n2, blocks)];
+  return (int64_t)t.bm << 16 | t.bn;
 }
 
 int eg_fp8_product(const eg_fp8_matrix* a, const eg_fp8_matrix* b, const eg_fp8_matrix* b2, void* c, int64_t ldc, void* c2,

@@ -872,7 +872,11 @@ int64_t eg_fp8_product_workspace_size(int64_t m, int64_t n, int64_t n2, int64_t 
 int eg_fp8_product(const eg_fp8_matrix* a, const eg_fp8_matrix* b, const eg_fp8_matrix* b2, void* c, int64_t ldc,
                    void* c2, int64_t ldc2, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* The same from A's values x [m, b->k] of x_dtype, rows x_stride apart, whose blocks (eg_fp8_quantize's) are taken
+/* The tile of outputs that a workgroup of such a product has, rows << 16 | columns, and the pieces that k is cut into
+ * (NULL: not wanted); 0 for the kernel of few rows and where there are no outputs, -1 for sizes out of range. */
+int64_t eg_fp8_product_tile(int64_t m, int64_t n, int64_t n2, int64_t k, int32_t dtype, int32_t* pieces);
+
+/* The products from A's values x [m, b->k] of x_dtype, rows x_stride apart, whose blocks (eg_fp8_quantize's) are taken
  * on the way. */
 int64_t eg_fp8_linear_workspace_size(int64_t m, int64_t n, int64_t n2, int64_t k);
 int eg_fp8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t x_stride, const eg_fp8_matrix* b,
