@@ -8,8 +8,11 @@
 // written once.  A row is w wavefronts' (1 to 16), of which each holds CH pieces of 512 values, eight
 // consecutive ones a lane: a piece is four blocks of the 8-bit output, whose largest values are found
 // within 16 lanes.  A lane's eight squares are added in 32 bits (in 64 where they leave its range), the lanes' sums and r in 64
-// (r's error is in all of a row's values), and a value next to a border between two e4m3 numbers is 64 bits: it rounds as the exact one does (of 3.5 million values none or one otherwise, 2 or 3 in 32 bits).  One piece a wavefront up to d = 8192 (d = 2560: five wavefronts a row): a wavefront a row
-// of 2560 held five, and its registers left four wavefronts a SIMD, or spilled; 61 us for 8,188 rows of bf16.
+// (r's error is in all of a row's values), and a value next to a border between two e4m3 numbers is 64 bits: it rounds as the
+// exact one does (of 3.5 million values none or one otherwise, 2 or 3 in 32 bits).  One piece a wavefront up to d = 8192
+// (d = 2560: five wavefronts a row): a wavefront a row of 2560 held five, and its registers left four wavefronts a SIMD, or
+// spilled; 61 us for 8,188 rows of bf16.  Longer rows hold two or three pieces a wavefront of 1,024 threads' 128 registers: the
+// forward's ragged kernels and all of the gradient's spill there.
 #include <algorithm>
 
 #include "eg_fp8.h"
@@ -138,9 +141,9 @@ __device__ inline float rounded(float x) {
   return (float)(T)x;
 }
 
-// R void: no residual (h is x, and not written).  96 scalar registers: with more a SIMD holds seven wavefronts, not eight.
+// R void: no residual (h is x, and not written).
 template <typename X, typename R, int CH, bool RAGGED>
-__global__ __launch_bounds__(1024) __attribute__((amdgpu_num_sgpr(96))) void norm_kernel(const NormArgs a) {
+__global__ __launch_bounds__(1024) void norm_kernel(const NormArgs a) {
   __shared__ double part[2][16];
   constexpr bool ADD = !std::is_same<R, void>::value;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_num_sgpr(96))) void nor
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     at[c] = (c * a.w + w) * 512 + lane * 8;
-    left[c] = a.d - at[c];
+    left[c] = RAGGED ? a.d - at[c] : at[c] < a.d ? 8 : 0;
   }
   const int blocks = (a.d + 127) >> 7;
   int parity = 0;
@@ -196,17 +199,13 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_num_sgpr(96))) void nor
     s = row_sum(s, a.w, slot, w, part[parity]);
     const double eps = (double)a.eps;
     double mean = fma(s, a.inv_d, eps);
-    // Such a row's squares are added again in 64 bits; the other rows keep their sums.  Where rows share a workgroup's barrier,
-    // every wavefront finds out the same of all of them, from the same sums.
+    // Such a row's squares are added again in 64 bits; the other rows keep their sums.  Where two rows share a workgroup's barrier
+    // (of two wavefronts each), every wavefront finds out the same of both, from the same sums.  The look costs 1 to 3 %.
     const bool wide = __builtin_amdgcn_readfirstlane((int)leaves_32(mean)) != 0;
     bool again = wide;
-    if (a.w > 1 && rows_here > 1) {
-      again = false;
-      for (int k = 0; k < rows_here; ++k) {
-        double sum = 0.0;
-        for (int i = 0; i < a.w; ++i) sum += part[parity][k * a.w + i];
-        again |= leaves_32(fma(sum, a.inv_d, eps));
-      }
+    if (CH == 1 && a.w == 2) {
+      const double* const other = part[parity] + 2 - 2 * slot;
+      again |= leaves_32(fma(other[0] + other[1], a.inv_d, eps));
     }
     parity ^= 1;
     if (__builtin_expect(__builtin_amdgcn_readfirstlane((int)again) != 0, 0)) {
