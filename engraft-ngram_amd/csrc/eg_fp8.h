@@ -46,7 +46,7 @@ __device__ inline void load8(const T* __restrict__ p, int valid, float (&v)[8]) 
 
 // A lane's eight values of a row of d, from column `at` on, in two steps, so that many loads are on their way before the first
 // is waited for: their bytes, by a load without a branch (a lane past the row's end reads its first or last
-// eight; `tiny`: rows of less than eight, one by one), and their values, zeros in the place of what does not
+// eight; rows of less than eight: one by one), and their values, zeros in the place of what does not
 // exist.  RAGGED: d is no multiple of eight, and the lane at the end reads the row's last eight and moves them.
 template <typename T>
 struct Raw8 {

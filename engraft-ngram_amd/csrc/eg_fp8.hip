@@ -6,9 +6,10 @@
 // arithmetic outside the matrix cores, and a block's values are exact in bf16 (e4m3 has 4 significant
 // bits).  What the fp8 matrix cores do not give is fp32 sums: they align eight products to the
 // largest of the eight and drop what lies 2^-13 below it, before the fp32 addition (seen with
-// 2^16 and 2^3, 2^2 among eight; 1.5e-5 of a product of normal values of any length, without a bias).  That
-// is far below the rounding of a bf16 (2^-8) or fp16 (2^-11) output; an fp32 output takes the
-// bf16 matrix cores instead, at half the rate, on the same bytes: its products are exact and its sums fp32.
+// 2^16 and 2^3, 2^2 among eight): at most 2^-10 of the products' magnitudes, 1.5e-5 of an output of normal
+// values of any length, without a bias, and 4e-5 to 5e-5 where some columns are 20 times the others.  That
+// is below the rounding of a bf16 (2^-8) or fp16 (2^-11; 2.1e-4 on the whole, 2.13e-4 with it) output; an fp32 output takes
+// the bf16 matrix cores instead, at half the rate, on the same bytes: its products are exact and its sums fp32.
 //
 // The scaled MFMA's intrinsic is not convergent: where its result is used in a branch alone, the
 // compiler may move it (with its operands' moves) into the branch, where the lanes that are off keep
@@ -679,7 +680,10 @@ __global__ __launch_bounds__(256) void piece_sum_kernel(const float* __restrict_
 
 // ---- host ----------------------------------------------------------------------------------------
 
-constexpr int kFewRows = 32;  // of the few-row kernel; 33 rows of 2560 x 10240 take 8.0 us in 64 x 64 tiles, and 15.7 in four groups of 16
+// Rows of the few-row kernel.  With the rows' blocks, bf16 outputs: 32 rows of 2560 x 2560 take 8.9 us in it and 33 rows 14.4 in
+// 64 x 64 tiles; 2560 x 640 9.0 and 14.7, 1000 x 1111 8.5 and 9.0.  Where outputs or k are long the tiles are ahead from about
+// 25 rows on: 2560 x 10240 16.1 and 14.5 (24 rows 13.4), 10240 x 2560 21.1 and 15.9 (24 rows 18.7).
+constexpr int kFewRows = 32;
 constexpr int64_t kFusedBytes = 64 << 10;
 
 template <int BM, int BN, int WM, int WN, int KH, bool PIPED, bool EXACT, typename Out>

@@ -19,7 +19,10 @@ may differ in its last ones beside another number of rows.
 
 ``product`` takes the blocks of ``x`` (f32, bf16 or f16) itself; its gradient takes those of the
 output's gradient, along the other axis.  f32 outputs come from exact products and fp32 sums;
-16-bit ones from the fp8 matrix cores, about 1.5e-5 of an output off (bf16 rounds by 2e-3).  The reference's projections are fp32 (``engraft/replica/layers.py:594-606``)."""
+16-bit ones from the fp8 matrix cores, which drop at most 2^-10 of the sum of the products' magnitudes: 1.5e-5 of an
+output with normal operands, up to 5e-5 with activations that have columns far above the others (bf16 rounds by 2^-8,
+f16 by 2^-11; ``out_dtype=torch.float32`` avoids it).  The reference's projections are fp32
+(``engraft/replica/layers.py:594-606``)."""
 from __future__ import annotations
 
 import torch

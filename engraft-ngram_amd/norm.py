@@ -11,8 +11,8 @@ output (or any layer's) and the projections behind it.
                                     bits, differentiable.
 
 ``x`` is f32, bf16 or f16 ``[..., d]``, d up to 20,480; the residual of x's type or f32;
-the weight f32, bf16 or f16 ``[d]`` or None (1).  Eight squares are added in 32 bits, their
-sums and the root in 64, gradients in 32 and in reverse mode (inputs with a forward-mode derivative are refused); rows in 8 bits round as the exact ones do, but for one value in millions.  The reference's rms norm is a torch expression
+the weight f32, bf16 or f16 ``[d]`` or None (1).  Eight squares are added in 32 bits (in 64
+where they leave its range), their sums and the root in 64, gradients in 32 and in reverse mode (inputs with a forward-mode derivative are refused); rows in 8 bits round as the exact ones do, but for one value in millions.  The reference's rms norm is a torch expression
 (``engraft/lens.py:282-287``), its additions are apart."""
 from __future__ import annotations
 

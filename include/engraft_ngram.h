@@ -865,9 +865,12 @@ int eg_fp8_dequantize(const eg_fp8_matrix* m, void* out, int32_t dtype, int64_t 
 
 /* C [m, n] = A B^T and, with b2, C2 [m, n2] = A B2^T: a in blocks of rows (block_rows 1), b and b2
  * weights (block_rows 128) of the same k; C of `dtype`, rows ldc apart.  f32 outputs come from exact products and
- * fp32 sums; bf16 and f16 ones from the fp8 matrix cores, whose sums of eight products drop what lies 2^-13 below
- * the largest of them (about 1.5e-5 of an output, 1 / 100 of bf16's rounding).  The order of a sum depends on m and
- * the outputs' sizes (deterministic for one of each).  Workspace 16-byte aligned. */
+ * fp32 sums of the values as bf16, which holds them but at the ends of its range: below 2^-126 (scales below 2^-124)
+ * they are rounded by up to 2^-134, and from 2^128 on they are infinite.  bf16 and f16 outputs come from the fp8 matrix
+ * cores, whose sums of eight products drop what lies 2^-13 below the largest of them: at most 2^-10 of the sum of the
+ * products' magnitudes, in practice 1.5e-5 of an output (normal operands) to 5e-5 (activations some columns of which
+ * are 20 times the others); bf16 rounds by 2^-8, f16 by 2^-11.  The order of a sum depends on m and the outputs' sizes
+ * (deterministic for one of each).  Workspace 16-byte aligned. */
 int64_t eg_fp8_product_workspace_size(int64_t m, int64_t n, int64_t n2, int64_t k);
 int eg_fp8_product(const eg_fp8_matrix* a, const eg_fp8_matrix* b, const eg_fp8_matrix* b2, void* c, int64_t ldc,
                    void* c2, int64_t ldc2, int32_t dtype, void* workspace, int64_t workspace_bytes, void* stream);
