@@ -530,17 +530,23 @@ def _place(w: torch.Tensor) -> tuple:
 class PleBlocks:
     """Both projections' weights in 8-bit blocks, for ``ple_forward(gemm="fp8", blocks=...)``: ``parts``, the key's and the
     value's :class:`fp8.Fp8Weight`, or one of the value's rows below the key's where they begin a block.  ``of``: the
-    weights that they were made of, as weak references and places."""
+    weights that they were made of, as weak references and places (None: not known, as of copied or pickled blocks)."""
 
     __slots__ = ("parts", "n_key", "n_value", "of")
 
-    def __init__(self, parts: tuple, n_key: int, n_value: int, of: tuple = ()):
+    def __init__(self, parts: tuple, n_key: int, n_value: int, of: tuple | None = None):
         self.parts, self.n_key, self.n_value, self.of = parts, n_key, n_value, of
+
+    def __getstate__(self):
+        return self.parts, self.n_key, self.n_value
+
+    def __setstate__(self, state):
+        self.__init__(*state)
 
     def check_weights(self, *ws: torch.Tensor | None) -> None:
         """Raises ValueError for a weight (None: not given) that is not what the blocks were made of: another tensor (a
-        view of all of it is none), or one that was written since."""
-        for name, w, (ref, place) in zip(("w_key", "w_value"), ws, self.of):
+        view of all of it is none), one that was written since, or any where the blocks' weights are not known."""
+        for name, w, (ref, place) in zip(("w_key", "w_value"), ws, self.of or ((lambda: None, None),) * 2):
             made_of = ref()
             if w is not None and (made_of is None or _place(w) != place or _place(made_of) != place):
                 raise ValueError(f"{name} is not the weight that the blocks were made of, or has changed since: take them again "

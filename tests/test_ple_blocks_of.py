@@ -1,6 +1,8 @@
 """What kept 8-bit blocks take for the weights that they were made of, on the host."""
 from __future__ import annotations
 
+import copy
+import pickle
 import weakref
 
 import pytest
@@ -49,6 +51,17 @@ def test_weights_that_are_gone_or_moved_are_not():
     _refused(blocks, key, value)
 
 
-def test_blocks_that_a_call_takes_itself_know_none():
-    from engraft_ngram_amd import ple
-    ple.PleBlocks((), 8, 4).check_weights(torch.zeros(8, 4), torch.zeros(4, 4))
+@pytest.mark.parametrize("copied", [copy.copy, copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))])
+def test_copied_blocks_know_none(copied):
+    """Their values are the same; which weights they were made of is not known any more, and none has to be given."""
+    from engraft_ngram_amd import fp8, ple
+    key, value = torch.randn(8, 4), torch.randn(4, 4)
+    blocks = _blocks(key, value)
+    blocks.parts = (fp8.Fp8Weight(torch.arange(128, dtype=torch.uint8)[None], torch.full((1, 4), 127, dtype=torch.uint8), 4),)
+    other = copied(blocks)
+    assert (other.n_key, other.n_value, other.parts[0].k) == (8, 4, 4) and torch.equal(other.parts[0].q, blocks.parts[0].q)
+    other.check_weights(None, None)
+    _refused(other, key, None)
+    _refused(other, None, value)
+    _refused(ple.PleBlocks(blocks.parts, 8, 4), key, value)
+    blocks.check_weights(key, value)
